@@ -201,6 +201,60 @@ int ncnn_b200_op_requantize(const int32_t *x, int8_t *y, int64_t count, int64_t 
                             const float *scale_out, int32_t scale_out_count, const float *bias,
                             int32_t bias_count, int32_t relu, void *stream);
 
+/* ---- Operators on device arrays around a network's convolutions: normalisation of feature maps, positions and attention
+ * of their tokens.  The reference's importer has no GroupNorm or RotaryEmbed; its MultiHeadAttention and SDPA lowerings
+ * (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4669) compute the same attention for one image.
+ * All arrays live on one device (which need not be the current one) in memory that kernels reach; a call is asynchronous on
+ * `stream` (a cudaStream_t of that device as void*), allocates nothing, keeps nothing between calls, may be captured into a
+ * graph, and any number of calls may be in flight.  A refused call launches nothing; ncnn_b200_last_error(NULL) says why.
+ * Element types are those of x and y, q, k, v and o; sums and statistics are held in 32 bits, results rounded once. */
+#define NCNN_B200_F32 0
+#define NCNN_B200_F16 1
+#define NCNN_B200_BF16 2
+
+#define NCNN_B200_ACT_NONE 0
+#define NCNN_B200_ACT_RELU 1
+#define NCNN_B200_ACT_SWISH 5 /* y * sigmoid(y) */
+#define NCNN_B200_ACT_GELU 11 /* the erf form */
+
+/* Group norm over channel-last maps, then an activation: x, y [n][pixels][channels],
+ *   y = act((x - m) / sqrt(v + eps) * gamma[c] + beta[c]),
+ * m and v the mean and the biased variance over an image's pixels and the channels of c's group (channels / groups
+ * consecutive ones).  gamma and beta are fp32 [channels] or NULL (1, 0).  x_pitch and y_pitch are the elements from one
+ * pixel to the next (0 = channels), so that a range of a wider tensor's channels can be normalised; images follow one another
+ * at pixels * pitch.  y may be x (same pitches); other overlaps are not allowed.  No images or no pixels: nothing is done. */
+int ncnn_b200_op_group_norm(const void *x, void *y, int32_t type, int64_t n, int64_t pixels, int32_t channels,
+                            int32_t groups, int64_t x_pitch, int64_t y_pitch, const float *gamma, const float *beta,
+                            float eps, int32_t activation, void *stream);
+
+/* Rotary positions with one to four axes (row and column of an image; time, row and column of a video) on the heads of
+ * queries or keys: x, y [tokens][heads][head_dim].  The first 2 * sum(sections) components of a head are pairs: neighbours
+ * (2i, 2i + 1) where `interleaved` is set, else (i, i + sum(sections)).  Axis a owns sections[a] consecutive pairs (`sections`
+ * is host memory), axis 0 the first ones.  Pair (u, v) becomes (u cos t - v sin t, u sin t + v cos t) with
+ * t = positions[token % position_rows][axis] * base^(-j / P): j counts an axis's own pairs and P is its section, or with
+ * `shared_spectrum` j counts all pairs and P is their sum.  The other components are copied.  positions is [position_rows]
+ * [axes] on the device, position_rows 0 = tokens; any 32-bit position, negative ones too, to 2^-32 turns.  strides (host, in
+ * elements: x token, x head, y token, y head) or NULL for dense arrays.  y may be x (same strides); other overlaps are not
+ * allowed.  At most 128 pairs. */
+int ncnn_b200_op_rotary_axes(const void *x, void *y, int32_t type, int64_t tokens, int32_t heads, int32_t head_dim,
+                             const int64_t *strides, const int32_t *positions, int64_t position_rows, int32_t axes,
+                             const int32_t *sections, double base, int32_t interleaved, int32_t shared_spectrum,
+                             void *stream);
+
+/* Attention of lq tokens to lk states of another sequence (or of their own): q, o [batch][lq][heads][head_dim],
+ * k, v [batch][lk][kv_heads][head_dim]; heads is a multiple of kv_heads and query head h reads key head
+ * h / (heads / kv_heads); head_dim 1 to 256.
+ *   o = sum_j softmax_j(scale * q.k_j) v_j   over j < kv_lens[batch] (int32, NULL = lk; held to 0..lk) with
+ *   key_mask[batch][j] != 0 (bytes [batch][lk], NULL = all).
+ * scale 0 = 1 / sqrt(head_dim).  A sequence that is left without a key gets zeros.  Whatever lies at a key that takes no part
+ * is not used, NaN and infinity included.  strides: host, 12 numbers in elements, {batch, row, head} of q, k, v and o in
+ * that order, NULL for dense arrays; components are always next to one another.  o must not overlap an input.
+ * 16-bit types whose rows start at multiples of 16 bytes run on the tensor cores, their probabilities rounded to the type. */
+int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, void *o, int32_t type, int64_t batch,
+                                 int64_t lq, int64_t lk, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                 const int64_t *strides, const int32_t *kv_lens, const uint8_t *key_mask, float scale,
+                                 void *stream);
+
 /* ---- One model on several GPUs of one box (batch sharding).
  * The reference has no counterpart: its entry point takes one image per call and keeps no state between
  * calls (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:48-52), which is what makes the images of a batch

@@ -1,0 +1,110 @@
+// What the stand-alone operators on device arrays share: element types, wide loads and stores, checks of arguments.
+#pragma once
+
+#include "../../include/ncnn_b200.h"
+
+#include <atomic>
+#include <cstdint>
+#include <string>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "engine_impl.h"  // DeviceGuard
+
+namespace nb {
+
+void set_global_error(const std::string& message);  // c_api.cu
+
+// ------------------------------------------------------------------ elements
+// 16-bit elements become fp32 on the way in and are rounded once, to nearest even, on the way out.
+template <class T> __device__ __forceinline__ float op_get(T v);
+template <> __device__ __forceinline__ float op_get<float>(float v) { return v; }
+template <> __device__ __forceinline__ float op_get<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float op_get<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T op_put(float v);
+template <> __device__ __forceinline__ float op_put<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half op_put<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 op_put<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N elements at an address that is a multiple of their size together (N elements of at most 16 bytes).
+template <class T, int N>
+struct alignas(sizeof(T) * N) OpVec {
+  T e[N];
+};
+
+// ------------------------------------------------------------------ host side
+inline int op_elem_bytes(int32_t type) { return type == NCNN_B200_F32 ? 4 : 2; }
+inline bool op_type_ok(int32_t type) { return type == NCNN_B200_F32 || type == NCNN_B200_F16 || type == NCNN_B200_BF16; }
+
+inline int op_fail(int status, const std::string& message) {
+  set_global_error(message);
+  return status;
+}
+
+// The device that `p` lives on; negative where it is no memory that a kernel of this process can reach.
+inline int op_device_of(const void* p) {
+  cudaPointerAttributes a{};
+  if (cudaPointerGetAttributes(&a, p) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged ? a.device : -1;
+}
+
+// Every array of a call on one device: that device, or a message.
+inline int op_common_device(const char* op, std::initializer_list<const void*> arrays, std::string* why) {
+  int device = -1;
+  for (const void* p : arrays) {
+    if (p == nullptr) continue;
+    const int d = op_device_of(p);
+    if (d < 0) {
+      *why = std::string(op) + ": an array is not in device memory";
+      return -1;
+    }
+    if (device >= 0 && d != device) {
+      *why = std::string(op) + ": the arrays are on different devices";
+      return -1;
+    }
+    device = d;
+  }
+  return device;
+}
+
+inline int op_sm_count(int device) {
+  int n = 148;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+  return n;
+}
+
+inline int op_launched(const char* op) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? NCNN_B200_STATUS_SUCCESS : op_fail(NCNN_B200_STATUS_RUNTIME, std::string(op) + ": launch failed: " + cudaGetErrorString(e));
+}
+
+// f(T{}) with the element type that `type` names
+template <class F>
+inline int op_by_type(int32_t type, F&& f) {
+  if (type == NCNN_B200_F32) return f(float{});
+  if (type == NCNN_B200_F16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+
+// No C++ exception leaves an entry point.
+template <class F>
+inline int op_guarded(const char* op, F&& f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    try {
+      set_global_error(std::string(op) + ": internal error: " + e.what());
+    } catch (...) {
+    }
+    return NCNN_B200_STATUS_RUNTIME;
+  } catch (...) {
+    return NCNN_B200_STATUS_RUNTIME;
+  }
+}
+
+}  // namespace nb

@@ -74,6 +74,12 @@ def load_library():
                                           c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p]
     L.ncnn_b200_inner_product_int8_noalloc.argtypes = [c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
                                                        c_int64, c_int32, c_int32, c_int32, c_void_p]
+    L.ncnn_b200_op_group_norm.argtypes = [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int64, c_int64, c_void_p, c_void_p,
+                                          c_float, c_int32, c_void_p]
+    L.ncnn_b200_op_rotary_axes.argtypes = [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_int32,
+                                           c_void_p, ctypes.c_double, c_int32, c_int32, c_void_p]
+    L.ncnn_b200_op_cross_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32,
+                                               c_int32, c_void_p, c_void_p, c_void_p, c_float, c_void_p]
     L.ncnn_b200_multi_load.argtypes = [c_char_p, c_char_p, POINTER(_Options), POINTER(c_int32), c_int32, POINTER(c_void_p)]
     L.ncnn_b200_multi_free.argtypes = [c_void_p]
     L.ncnn_b200_multi_free.restype = None
@@ -335,6 +341,61 @@ def op_requantize(x_ptr, y_ptr, count, inner, channels, scale_in_ptr, scale_in_c
     _op_status(load_library().ncnn_b200_op_requantize(x_ptr, y_ptr, count, inner, channels, scale_in_ptr,
                                                       scale_in_count, scale_out_ptr, scale_out_count, bias_ptr,
                                                       bias_count, 1 if relu else 0, c_void_p(stream)))
+
+
+ELEMENT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+OP_ACTIVATIONS = {"none": 0, "relu": 1, "swish": 5, "gelu": 11}
+
+
+def _op_message(L, st):
+    raise NcnnB200Error(st, L.ncnn_b200_last_error(None).decode())
+
+
+def _of(names, name, what):
+    try:
+        return names[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what} is one of {', '.join(names)}, not {name!r}") from None
+
+
+def op_group_norm(x_ptr, y_ptr, element, n, pixels, channels, groups, gamma_ptr=None, beta_ptr=None, eps=1e-5, activation="none",
+                  x_pitch=0, y_pitch=0, stream=0):
+    """Group norm and an activation ("none", "relu", "swish", "gelu") over channel-last maps [n][pixels][channels] of
+    "f32", "f16" or "bf16" elements; gamma and beta are fp32 [channels] (ncnn_b200_op_group_norm)."""
+    L = load_library()
+    st = L.ncnn_b200_op_group_norm(x_ptr, y_ptr, _of(ELEMENT_TYPES, element, "element"), n, pixels, channels, groups, x_pitch, y_pitch,
+                                   gamma_ptr, beta_ptr, eps, _of(OP_ACTIVATIONS, activation, "activation"), stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_rotary_axes(x_ptr, y_ptr, element, tokens, heads, head_dim, positions_ptr, sections, base=10000.0, interleaved=False,
+                   shared_spectrum=False, position_rows=0, strides=None, stream=0):
+    """Rotary positions with len(sections) axes on [tokens][heads][head_dim]; positions is int32 [position_rows or
+    tokens][axes] on the device, strides (x token, x head, y token, y head) in elements (ncnn_b200_op_rotary_axes)."""
+    L = load_library()
+    if strides is not None and len(strides) != 4:
+        raise ValueError("strides are four numbers: x token, x head, y token, y head")
+    st = L.ncnn_b200_op_rotary_axes(x_ptr, y_ptr, _of(ELEMENT_TYPES, element, "element"), tokens, heads, head_dim,
+                                    None if strides is None else struct.pack("4q", *strides), positions_ptr, position_rows, len(sections),
+                                    struct.pack("%di" % len(sections), *sections), base, 1 if interleaved else 0, 1 if shared_spectrum else 0,
+                                    stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads, kv_heads, head_dim, kv_lens_ptr=None,
+                       key_mask_ptr=None, scale=0.0, strides=None, stream=0):
+    """Attention of q [batch][lq][heads][head_dim] to k, v [batch][lk][kv_heads][head_dim]; kv_lens is int32 [batch], key_mask
+    bytes [batch][lk], strides 12 numbers in elements, {batch, row, head} of q, k, v and o (ncnn_b200_op_cross_attention)."""
+    L = load_library()
+    if strides is not None and len(strides) != 12:
+        raise ValueError("strides are twelve numbers: batch, row and head of q, k, v and o")
+    st = L.ncnn_b200_op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, _of(ELEMENT_TYPES, element, "element"), batch, lq, lk, heads, kv_heads,
+                                        head_dim, None if strides is None else struct.pack("12q", *strides), kv_lens_ptr, key_mask_ptr,
+                                        scale, stream)
+    if st != 0:
+        _op_message(L, st)
 
 
 def inner_product_int8_noalloc(x_ptr, weight_ptr, weight_scales_ptr, input_scale, bias_ptr, y_ptr, m, k, n,
