@@ -255,6 +255,10 @@ int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, vo
                                  const int64_t *strides, const int32_t *kv_lens, const uint8_t *key_mask, float scale,
                                  void *stream);
 
+/* The tensor-core kernel of ncnn_b200_op_cross_attention bounds its waits (2 s each).  This waits for the current device and
+ * returns 7, once, when one of them ran out since the last such call, 0 otherwise. */
+int ncnn_b200_op_check_status(void);
+
 /* ---- One model on several GPUs of one box (batch sharding).
  * The reference has no counterpart: its entry point takes one image per call and keeps no state between
  * calls (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:48-52), which is what makes the images of a batch

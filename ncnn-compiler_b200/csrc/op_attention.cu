@@ -6,6 +6,11 @@
 
 #include "op_attention.h"
 
+#include <cstdlib>
+#include <mutex>
+
+#include "tc_attend.cuh"
+
 namespace nb {
 namespace {
 
@@ -56,8 +61,124 @@ __global__ void __launch_bounds__(256) k_attend_row(const __grid_constant__ Atte
     if (lane + 32 * c < p.d) o[lane + 32 * c] = op_put<T>(total == 0.0f ? 0.0f : sum[c] * scale);
 }
 
+// ------------------------------------------------------------------ tensor cores
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static const EncodeTiledFn fn = [] {
+    cudaDriverEntryPointQueryResult query;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &query) != cudaSuccess || query != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// [sequence][head][row][component] as TMA sees it, boxes of 128 rows of 64 components.  An axis that all heads or sequences
+// share (stride 0) has one entry: `step` says what to multiply its index with.
+bool encode_rows(CUtensorMap* map, bool half, const void* base, int d, long long rows, long long row, int heads, long long head, int batch,
+                 long long seq, int* step) {
+  const int head_extent = head == 0 ? 1 : heads, batch_extent = seq == 0 ? 1 : batch;
+  if (step != nullptr) {
+    step[0] = head == 0 ? 0 : 1;
+    step[1] = seq == 0 ? 0 : 1;
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(head_extent), static_cast<cuuint64_t>(batch_extent)};
+  // an axis of one entry is never stepped over: any valid stride will do
+  const cuuint64_t any = (static_cast<cuuint64_t>(d) * 2 + 15) / 16 * 16;
+  const cuuint64_t strides[3] = {rows == 1 ? any : static_cast<cuuint64_t>(row) * 2, head_extent == 1 ? any : static_cast<cuuint64_t>(head) * 2,
+                                 batch_extent == 1 ? any : static_cast<cuuint64_t>(seq) * 2};
+  const cuuint32_t box[4] = {64, kAttRows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return encode_tiled()(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
+                        ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether rows can be moved 16 bytes at a time (and by TMA): 16-bit types, starts and strides of axes that are stepped over.
+bool rows_of_16_bytes(const AttendParams& p) {
+  auto ok = [](const void* base, std::initializer_list<std::pair<long long, long long>> axes) {
+    if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    for (const auto& a : axes)
+      if (a.second > 1 && a.first % 8 != 0) return false;
+    return true;
+  };
+  return p.d % 8 == 0 && ok(p.q, {{p.q_batch, p.batch}, {p.q_row, p.lq}, {p.q_head, p.heads}}) &&
+         ok(p.k, {{p.k_batch, p.batch}, {p.k_row, p.lk}, {p.k_head, p.kv_heads}}) &&
+         ok(p.v, {{p.v_batch, p.batch}, {p.v_row, p.lk}, {p.v_head, p.kv_heads}}) &&
+         ok(p.o, {{p.o_batch, p.batch}, {p.o_row, p.lq}, {p.o_head, p.heads}});
+}
+
+// Dynamic shared memory above 48 KB is granted to a kernel once per device.  `registers`: what the kernel's roles share out
+// between them; compiled for fewer, their setmaxnreg would wait for ever.
+template <class K>
+cudaError_t grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted, int registers = 0) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (granted->load(std::memory_order_acquire) & bit) return cudaSuccess;
+  if (registers > 0) {
+    cudaFuncAttributes a{};
+    if (const cudaError_t e = cudaFuncGetAttributes(&a, kernel); e != cudaSuccess) return e;
+    if (a.numRegs != registers) return cudaErrorInvalidKernelImage;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) granted->fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
+
+template <class T, int D, int TILES>
+bool launch_tc(const AttendParams& a, int device, cudaStream_t st) {
+  using Shape = TcAttendShape<D, TILES>;
+  TcAttendParams p{};
+  p.a = a;
+  p.scale_log2 = a.scale * 1.44269504088896340736f;
+  p.wait_ns = kTcWaitLimitNs;
+  if (std::getenv("NCNN_B200_TEST_STALL") != nullptr) {
+    p.stall = 1;
+    p.wait_ns = 2000000ull;
+  }
+  alignas(64) CUtensorMap q, k, v;
+  constexpr bool half = std::is_same<T, __half>::value;
+  if (!encode_rows(&q, half, a.q, a.d, a.lq, a.q_row, a.heads, a.q_head, a.batch, a.q_batch, p.q_step) ||
+      !encode_rows(&k, half, a.k, a.d, a.lk, a.k_row, a.kv_heads, a.k_head, a.batch, a.k_batch, p.k_step) ||
+      !encode_rows(&v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p.v_step))
+    return false;
+  static std::atomic<uint64_t> granted{0};
+  if (grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, Shape::kRegsLaunch) != cudaSuccess) return false;
+  const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
+  tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, q, k, v);
+  return true;
+}
+
+template <class T>
+bool attend_tc(const AttendParams& a, int device, cudaStream_t st) {
+  const bool two = a.lq > kAttRows;
+  if (a.d <= 64) return two ? launch_tc<T, 64, 2>(a, device, st) : launch_tc<T, 64, 1>(a, device, st);
+  return two ? launch_tc<T, 128, 2>(a, device, st) : launch_tc<T, 128, 1>(a, device, st);
+}
+
+// Every stride an axis of more than one entry is stepped with has to be a stride that TMA takes: positive and below 2^40 bytes.
+bool tma_strides(const AttendParams& p) {
+  auto ok = [](long long stride, long long extent, bool shared) { return extent == 1 || ((stride > 0 || (shared && stride == 0)) && stride < (1ll << 38)); };
+  return ok(p.q_batch, p.batch, true) && ok(p.q_row, p.lq, false) && ok(p.q_head, p.heads, true) && ok(p.k_batch, p.batch, true) &&
+         ok(p.k_row, p.lk, false) && ok(p.k_head, p.kv_heads, true) && ok(p.v_batch, p.batch, true) && ok(p.v_row, p.lk, false) &&
+         ok(p.v_head, p.kv_heads, true);
+}
+
 }  // namespace
 }  // namespace nb
+
+extern "C" int ncnn_b200_op_check_status(void) {
+  using namespace nb;
+  return op_guarded("op_check_status", [&]() -> int {
+    int status = 0;
+    const int none = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&status, g_attend_status, sizeof status) != cudaSuccess ||
+        (status != 0 && cudaMemcpyToSymbol(g_attend_status, &none, sizeof none) != cudaSuccess))
+      return op_fail(NCNN_B200_STATUS_RUNTIME, std::string("op_check_status: ") + cudaGetErrorString(cudaGetLastError()));
+    return status == 0 ? NCNN_B200_STATUS_SUCCESS
+                       : op_fail(NCNN_B200_STATUS_TIMEOUT, "op_check_status: a wait inside an operator's kernel ran out; its result is not valid");
+  });
+}
 
 extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const void* v, void* o, int32_t type, int64_t batch, int64_t lq,
                                             int64_t lk, int32_t heads, int32_t kv_heads, int32_t head_dim, const int64_t* strides,
@@ -122,6 +243,14 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     DeviceGuard guard(device);
     const long long rows = batch * lq * heads;
     if (rows > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: more than 2^33 rows");
+    if (p.batch * static_cast<long long>(p.heads) > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: too many heads");
+    if (type != NCNN_B200_F32 && p.lk > 0 && p.d <= 128 && rows_of_16_bytes(p) && tma_strides(p)) {
+      if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
+      cudaStream_t st = static_cast<cudaStream_t>(stream);
+      const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, st) : attend_tc<__nv_bfloat16>(p, device, st);
+      if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
+      return op_launched(kOp);
+    }
     op_by_type(type, [&](auto t) {
       using T = decltype(t);
       const unsigned grid = static_cast<unsigned>((rows + 7) / 8);

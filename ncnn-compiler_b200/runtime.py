@@ -80,6 +80,7 @@ def load_library():
                                            c_void_p, ctypes.c_double, c_int32, c_int32, c_void_p]
     L.ncnn_b200_op_cross_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32,
                                                c_int32, c_void_p, c_void_p, c_void_p, c_float, c_void_p]
+    L.ncnn_b200_op_check_status.argtypes = []
     L.ncnn_b200_multi_load.argtypes = [c_char_p, c_char_p, POINTER(_Options), POINTER(c_int32), c_int32, POINTER(c_void_p)]
     L.ncnn_b200_multi_free.argtypes = [c_void_p]
     L.ncnn_b200_multi_free.restype = None
@@ -394,6 +395,14 @@ def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads
     st = L.ncnn_b200_op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, _of(ELEMENT_TYPES, element, "element"), batch, lq, lk, heads, kv_heads,
                                         head_dim, None if strides is None else struct.pack("12q", *strides), kv_lens_ptr, key_mask_ptr,
                                         scale, stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_check_status():
+    """Waits for the current device; raises where a wait inside an operator's kernel ran out since the last call."""
+    L = load_library()
+    st = L.ncnn_b200_op_check_status()
     if st != 0:
         _op_message(L, st)
 

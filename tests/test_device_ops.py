@@ -28,7 +28,8 @@ def normal(g, *shape):
 
 def assert_within(got, want, bound):
     got = got.double()
-    assert not torch.isnan(got).any() and torch.isfinite(got).all()
+    bad = int((~torch.isfinite(got)).sum())
+    assert bad == 0, bad
     over = (got - want).abs() - bound
     worst = int(over.argmax())
     assert over.max() <= 0, (float(got.flatten()[worst]), float(want.flatten()[worst]), float(bound.expand_as(want).flatten()[worst]))
