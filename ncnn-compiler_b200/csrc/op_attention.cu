@@ -9,6 +9,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "attend_few.cuh"
 #include "tc_attend.cuh"
 
 namespace nb {
@@ -156,6 +157,58 @@ bool attend_tc(const AttendParams& a, int device, cudaStream_t st) {
   return two ? launch_tc<T, 128, 2>(a, device, st) : launch_tc<T, 128, 1>(a, device, st);
 }
 
+template <class T, int D, int WARPS, int STAGES, int BLOCKS>
+bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
+  FewParams p{};
+  p.a = a;
+  p.scale_log2 = a.scale * 1.44269504088896340736f;
+  const int shared = a.heads / a.kv_heads;
+  p.row_tiles = (a.lq * shared + kFewRows - 1) / kFewRows;
+  constexpr int smem = sizeof(FewShared<T, D, WARPS, STAGES>);
+  static std::atomic<uint64_t> granted{0};
+  if (grant_smem(k_attend_few<T, D, WARPS, STAGES, BLOCKS>, smem, device, &granted) != cudaSuccess) return false;
+  if (ranks > 8 && cudaFuncSetAttribute(k_attend_few<T, D, WARPS, STAGES, BLOCKS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(ranks, a.kv_heads * p.row_tiles, a.batch);
+  c.blockDim = dim3(WARPS * 32);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = ranks;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  c.attrs = &cluster;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, k_attend_few<T, D, WARPS, STAGES, BLOCKS>, p) == cudaSuccess;
+}
+
+// Whether a call is one of few queries: at most two tiles of 16 to a key head.
+bool few_queries(const AttendParams& p) {
+  const long long rows = static_cast<long long>(p.lq) * (p.heads / p.kv_heads);
+  return rows <= 2 * kFewRows && p.d <= 128 && static_cast<long long>(p.kv_heads) * ((rows + kFewRows - 1) / kFewRows) <= 65535;
+}
+
+template <class T>
+bool attend_few(const AttendParams& a, int device, int sms, cudaStream_t st) {
+  const long long rows = static_cast<long long>(a.lq) * (a.heads / a.kv_heads);
+  const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((rows + kFewRows - 1) / kFewRows);
+  // Few tiles (a cluster of 8 to each leaves SMs idle): CTAs of 8 warps with deep rings, one to an SM, up to 16 to a tile while
+  // each of their warps has two tiles of keys.  4 tiles of 20000 keys: 24.6 us, against 28.7 with CTAs of 4 warps.
+  if (tiles * 8 < sms && a.lk >= 4096) {
+    int ranks = 8;
+    while (ranks < 16 && tiles * ranks * 2 <= sms && a.lk >= ranks * 512) ranks *= 2;
+    return a.d <= 64 ? launch_few<T, 64, 8, 6, 1>(a, device, ranks, st) : launch_few<T, 128, 8, 3, 1>(a, device, ranks, st);
+  }
+  // Otherwise CTAs of 4 warps, two (heads of 64: three) to an SM, and as many to a tile as the device holds at once: a CTA costs
+  // some 3 us of its own (512 tiles of 2048 keys: 103 us with one to a tile, 115 with two, 120 with four; 64 tiles of 8192: 72,
+  // 45, 38 and 49 us with 1, 2, 4 and 8).  Sequences of different lengths even out over four times as many (512 tiles of
+  // ragged lengths: 129, 113, 119 us).
+  const long long most = (a.lens != nullptr ? 8ll : 2ll) * sms;
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= most && a.lk > ranks * 64) ranks *= 2;
+  return a.d <= 64 ? launch_few<T, 64, 4, 4, 3>(a, device, ranks, st) : launch_few<T, 128, 4, 3, 2>(a, device, ranks, st);
+}
+
 // Every stride an axis of more than one entry is stepped with has to be a stride that TMA takes: positive and below 2^40 bytes.
 bool tma_strides(const AttendParams& p) {
   auto ok = [](long long stride, long long extent, bool shared) { return extent == 1 || ((stride > 0 || (shared && stride == 0)) && stride < (1ll << 38)); };
@@ -244,6 +297,15 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     const long long rows = batch * lq * heads;
     if (rows > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: more than 2^33 rows");
     if (p.batch * static_cast<long long>(p.heads) > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: too many heads");
+    if (type != NCNN_B200_F32 && p.lk > 0 && few_queries(p) && rows_of_16_bytes(p)) {
+      cudaStream_t st = static_cast<cudaStream_t>(stream);
+      const int sms = op_sm_count(device);
+      if (!(type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st))) {
+        const int st_code = op_launched(kOp);
+        return st_code != 0 ? st_code : op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: launch failed");
+      }
+      return op_launched(kOp);
+    }
     if (type != NCNN_B200_F32 && p.lk > 0 && p.d <= 128 && rows_of_16_bytes(p) && tma_strides(p)) {
       if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
       cudaStream_t st = static_cast<cudaStream_t>(stream);
