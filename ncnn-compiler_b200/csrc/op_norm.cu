@@ -3,6 +3,8 @@
 // with the mean m and the (biased) variance v over the pixels and the channels of c's group in image i.
 #include <cmath>
 
+#include <cooperative_groups.h>
+
 #include "op_common.cuh"
 
 namespace nb {
@@ -12,15 +14,21 @@ struct NormParams {
   const void* x;
   void* y;
   long long n, pixels, x_pitch, y_pitch;
-  int channels, groups, act;
+  int channels, groups;
   const float *gamma, *beta;
   float eps;
 };
 
-__device__ __forceinline__ float norm_act(float y, int act) {
-  if (act == NCNN_B200_ACT_RELU) return y < 0.0f ? 0.0f : y;  // (a NaN stays one)
-  if (act == NCNN_B200_ACT_SWISH) return __fdividef(y, 1.0f + __expf(-y));
-  if (act == NCNN_B200_ACT_GELU) return 0.5f * y * erfcf(y * -0.70710678118654752f);
+template <int ACT>
+__device__ __forceinline__ float norm_act(float y) {
+  if (ACT == NCNN_B200_ACT_RELU) return y < 0.0f ? 0.0f : y;  // (a NaN stays one)
+  if (ACT == NCNN_B200_ACT_SWISH) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y * -1.44269504088896340736f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));  // (0 where e is infinite)
+    return y * r;
+  }
+  if (ACT == NCNN_B200_ACT_GELU) return 0.5f * y * erfcf(y * -0.70710678118654752f);
   return y;
 }
 
@@ -41,9 +49,220 @@ __device__ float block_sum(float v) {
   return parts[0];
 }
 
-// One CTA to an image's group: mean, variance about it, result; x is read three times.
-template <class T>
-__global__ void __launch_bounds__(512) k_group_norm(const __grid_constant__ NormParams p) {
+// Several groups of an image, `channels` neighbouring channels, belong to a cluster of CTAs, and each CTA has a range of the
+// pixels.  A thread owns V channels (a 16-byte access where addresses allow it) and every ROWS-th pixel of the range, so that
+// scale and offset of the second pass are registers.
+//
+// Statistics.  A thread sums its values and their squares about its own first value of the channel, in fp32, and turns the
+// sums into a mean and a sum of squared deviations from it; from there on those are combined (n, mean, deviations), over the
+// CTA's threads and then over the cluster's CTAs, with the deviations taken about the combined mean.  Sums about zero lose the
+// variance of maps that lie far from it (a mean of 1000 deviations: all of it), and a common shift loses it to one outlier.
+//
+// Bound: HBM, x once and y once, where x stays on the SM or in L2 between the passes.  Every thread has a ring of 16 (or 12) of its own
+// pixels in shared memory, filled by cp.async four at a time (no registers for what is under way: 48 KB a CTA, three CTAs to an
+// SM).  The second pass goes backwards: it begins with what the first one left in the ring and goes on with what L2 saw last.
+// Measured: 8 maps of 64 x 64 x 320, bf16 18 us; 2 of 512 x 512 x 128, fp32 162 us, where two thirds of x have to come from
+// HBM again (5 TB/s in each pass; CTAs of 768 threads, stores that leave L2 first, and whole pixels to a CTA were no faster).
+constexpr int kNormThreads = 256;
+constexpr int kNormMostGroups = 128;
+constexpr int kNormGroup = 4;   // pixels that are asked for together
+
+template <int V>
+constexpr int kNormSlots = V == 8 ? 12 : 16;  // pixels of a thread's ring (three CTAs' rings and statistics fit an SM)
+
+struct NormShape {
+  int channels;       // of a cluster
+  int columns, rows;  // threads: columns of V channels, rows of pixels
+  int slots;          // of a ring: kNormSlots, or fewer where no thread has as many pixels
+};
+
+struct Moments {
+  float mean, m2;
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else if constexpr (BYTES >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_constant__ NormParams p, const __grid_constant__ NormShape s) {
+  namespace cg = cooperative_groups;
+  using Vec = OpVec<T, V>;
+  extern __shared__ __align__(16) uint8_t norm_smem[];
+  // the CTA's, and the cluster's mean and 1 / sqrt(variance + eps), of each group
+  __shared__ Moments group_parts[kNormMostGroups];
+  __shared__ float2 result[kNormMostGroups];
+  Vec* ring = reinterpret_cast<Vec*>(norm_smem) + threadIdx.x;  // [slot][thread]
+  const int size = p.channels / p.groups, groups = s.channels / size;
+  const int ranks = gridDim.x, rank = blockIdx.x;
+  const int blocks = p.channels / s.channels;
+  const long long image = blockIdx.y / blocks;
+  const int c0 = static_cast<int>(blockIdx.y % blocks) * s.channels;
+  // this CTA's pixels, and this thread's
+  const int pixels = static_cast<int>(p.pixels), each = (pixels + ranks - 1) / ranks;
+  const int begin = static_cast<int>(min(static_cast<long long>(each) * rank, p.pixels)), here = min(each, pixels - begin);
+  const int column = threadIdx.x % s.columns, row = threadIdx.x / s.columns;
+  const int count = row < s.rows && row < here ? (here - row + s.rows - 1) / s.rows : 0;
+  const T* x = static_cast<const T*>(p.x) + (image * p.pixels + begin + row) * p.x_pitch + c0 + column * V;
+  T* y = static_cast<T*>(p.y) + (image * p.pixels + begin + row) * p.y_pitch + c0 + column * V;
+  const long long x_step = s.rows * p.x_pitch, y_step = s.rows * p.y_pitch;
+  const int steps = (count + kNormGroup - 1) / kNormGroup;
+  // four pixels of this thread on their way to their slots (2-byte pieces, which cp.async does not take: through registers)
+  auto request = [&](int step) {
+    if (step >= 0 && step < steps) {
+      const T* from = x + step * kNormGroup * x_step;
+      Vec* to = ring + step * kNormGroup % kNormSlots<V> * kNormThreads;
+      if constexpr (sizeof(Vec) >= 4) {
+#pragma unroll
+        for (int u = 0; u < kNormGroup; ++u)
+          if (step * kNormGroup + u < count) copy_async<sizeof(Vec)>(static_cast<uint32_t>(__cvta_generic_to_shared(to + u * kNormThreads)), from + u * x_step);
+      } else {
+        Vec at[kNormGroup];
+#pragma unroll
+        for (int u = 0; u < kNormGroup; ++u)
+          if (step * kNormGroup + u < count) at[u] = *reinterpret_cast<const Vec*>(from + u * x_step);
+#pragma unroll
+        for (int u = 0; u < kNormGroup; ++u)
+          if (step * kNormGroup + u < count) to[u * kNormThreads] = at[u];
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  constexpr int kAhead = kNormSlots<V> / kNormGroup - 1;
+
+  Moments part[V];
+  {
+    float shift[V], s1[V], s2[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) shift[v] = s1[v] = s2[v] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) request(g);
+    for (int g = 0; g < steps; ++g) {
+      request(g + kAhead);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+      const Vec* at = ring + g * kNormGroup % kNormSlots<V> * kNormThreads;
+      if (g == 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) shift[v] = op_get(at->e[v]);
+      }
+#pragma unroll
+      for (int u = 0; u < kNormGroup; ++u)
+        if (g * kNormGroup + u < count) {
+          const Vec in = at[u * kNormThreads];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float d = op_get(in.e[v]) - shift[v];
+            s1[v] += d;
+            s2[v] = fmaf(d, d, s2[v]);
+          }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const float inverse = count > 0 ? 1.0f / static_cast<float>(count) : 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float off = s1[v] * inverse;
+      part[v] = {shift[v] + off, fmaxf(s2[v] - s1[v] * off, 0.0f)};
+    }
+  }
+  // [row][v][column] in shared memory behind the rings
+  Moments* parts = reinterpret_cast<Moments*>(norm_smem + static_cast<size_t>(s.slots) * kNormThreads * sizeof(Vec));
+  if (row < s.rows) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) parts[row * s.channels + v * s.columns + column] = part[v];
+  }
+  __syncthreads();
+  // A warp to a group: lanes over its channels and as many rows as fit; the mean first, the deviations about it second.
+  const int lane = threadIdx.x & 31;
+  const int lane_rows = size < 32 ? 32 / size : 1, lane_row = size < 32 ? lane / size : 0, lane_channel = size < 32 ? lane - lane_row * size : lane;
+  const int whole_rows = here / s.rows, longer = here - whole_rows * s.rows;  // `longer` rows have a pixel more
+  const int rows_in_use = min(s.rows, here);
+  for (int g = threadIdx.x >> 5; g < groups; g += kNormThreads / 32) {
+    auto over = [&](auto&& f) {
+      if (lane_row < lane_rows)
+        for (int i = lane_channel; i < size; i += 32) {
+          const int c = g * size + i;
+          const Moments* of = parts + c % V * s.columns + c / V;
+#pragma unroll 4
+          for (int r = lane_row; r < rows_in_use; r += lane_rows) f(of[r * s.channels], static_cast<float>(whole_rows + (r < longer ? 1 : 0)));
+        }
+    };
+    const float about = parts[g * size % V * s.columns + g * size / V].mean;  // (a group of one value has that for its mean, exactly)
+    float sum = 0.0f, m2 = 0.0f;
+    over([&](const Moments& m, float n) { sum = fmaf(n, m.mean - about, sum); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    const float mean = here > 0 ? about + sum / (static_cast<float>(here) * size) : 0.0f;
+    over([&](const Moments& m, float n) { m2 += fmaf(n * (m.mean - mean), m.mean - mean, m.m2); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o);
+    if (lane == 0) group_parts[g] = {mean, m2};
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (ranks > 1) cluster.sync();
+  else __syncthreads();
+  // the cluster's, the same way: lanes over its CTAs, 16 to a group
+  const float inverse_total = 1.0f / (static_cast<float>(pixels) * size);
+  for (int g0 = threadIdx.x >> 5; g0 * 2 < groups; g0 += kNormThreads / 32) {
+    const int g = g0 * 2 + (lane >> 4), r = lane & 15;
+    Moments m = {0.0f, 0.0f};
+    float n = 0.0f;
+    if (g < groups && r < ranks) {
+      m = ranks > 1 ? *cluster.map_shared_rank(&group_parts[g], r) : group_parts[g];
+      n = static_cast<float>(min(static_cast<long long>(each), max(p.pixels - static_cast<long long>(each) * r, 0ll))) * size;
+    }
+    const float about = __shfl_sync(~0u, m.mean, lane & 16);
+    float sum = n > 0.0f ? n * (m.mean - about) : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    const float mean = fmaf(sum, inverse_total, about);
+    float m2 = n > 0.0f ? fmaf(n * (m.mean - mean), m.mean - mean, m.m2) : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m2 += __shfl_xor_sync(~0u, m2, o);
+    if (g < groups && r == 0) result[g] = make_float2(mean, 1.0f / sqrtf(m2 * inverse_total + p.eps));
+  }
+  __syncthreads();
+  // no CTA's shared memory goes while another reads it: said here, waited for at the end
+  if (ranks > 1) cluster.barrier_arrive();
+  // fp32 keeps the mean apart: x - mean is exact where x is close to it.  A 16-bit x has steps of 2^-8 or 2^-11 of itself, so
+  // that maps which vary at all lie within some 2^12 deviations of their mean, and the one product's rounding (2^-24 of the
+  // mean) stays below that of the result.
+  constexpr bool kFold = sizeof(T) == 2;
+  float mean[kFold ? 1 : V], scale[V], offset[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = column * V + v;
+    const float2 r = result[c / size];
+    scale[v] = r.y * (p.gamma != nullptr ? __ldg(p.gamma + c0 + c) : 1.0f);
+    offset[v] = p.beta != nullptr ? __ldg(p.beta + c0 + c) : 0.0f;
+    if (kFold) offset[v] = fmaf(-r.x, scale[v], offset[v]);
+    else mean[kFold ? 0 : v] = r.x;
+  }
+  for (int g = steps - 1; g >= 0; --g) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+    Vec at[kNormGroup];
+    const Vec* from = ring + g * kNormGroup % kNormSlots<V> * kNormThreads;
+#pragma unroll
+    for (int u = 0; u < kNormGroup; ++u)
+      if (g * kNormGroup + u < count) at[u] = from[u * kNormThreads];
+    request(g - kAhead - 1);
+    T* to = y + g * kNormGroup * y_step;
+#pragma unroll
+    for (int u = 0; u < kNormGroup; ++u)
+      if (g * kNormGroup + u < count) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(kFold ? op_get(at[u].e[v]) : op_get(at[u].e[v]) - mean[kFold ? 0 : v], scale[v], offset[v])));
+        *reinterpret_cast<Vec*>(to + u * y_step) = at[u];
+      }
+  }
+  if (ranks > 1) cluster.barrier_wait();
+}
+
+// Groups of more channels than a CTA has threads for: one CTA to a group, which reads x three times.
+template <class T, int ACT>
+__global__ void __launch_bounds__(kNormThreads) k_group_norm_wide(const __grid_constant__ NormParams p) {
   const int size = p.channels / p.groups;
   const long long image = blockIdx.x / p.groups;
   const int c0 = static_cast<int>(blockIdx.x % p.groups) * size;
@@ -51,19 +270,102 @@ __global__ void __launch_bounds__(512) k_group_norm(const __grid_constant__ Norm
   T* y = static_cast<T*>(p.y) + image * p.pixels * p.y_pitch + c0;
   const long long count = p.pixels * size;
   float sum = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += 512) sum += op_get(x[i / size * p.x_pitch + i % size]);
+  for (long long i = threadIdx.x; i < count; i += kNormThreads) sum += op_get(x[i / size * p.x_pitch + i % size]);
   const float mean = block_sum(sum) / static_cast<float>(count);
   sum = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += 512) {
+  for (long long i = threadIdx.x; i < count; i += kNormThreads) {
     const float d = op_get(x[i / size * p.x_pitch + i % size]) - mean;
     sum = fmaf(d, d, sum);
   }
   const float scale = 1.0f / sqrtf(block_sum(sum) / static_cast<float>(count) + p.eps);
-  for (long long i = threadIdx.x; i < count; i += 512) {
+  for (long long i = threadIdx.x; i < count; i += kNormThreads) {
     const int c = static_cast<int>(i % size);
-    float v = (op_get(x[i / size * p.x_pitch + c]) - mean) * scale;
-    v = fmaf(v, p.gamma ? p.gamma[c0 + c] : 1.0f, p.beta ? p.beta[c0 + c] : 0.0f);
-    y[i / size * p.y_pitch + c] = op_put<T>(norm_act(v, p.act));
+    const float v = fmaf((op_get(x[i / size * p.x_pitch + c]) - mean) * scale, p.gamma ? p.gamma[c0 + c] : 1.0f, p.beta ? p.beta[c0 + c] : 0.0f);
+    y[i / size * p.y_pitch + c] = op_put<T>(norm_act<ACT>(v));
+  }
+}
+
+template <class T, int V, int ACT>
+int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
+  const int size = p.channels / p.groups, sms = op_sm_count(device);
+  NormShape s{};
+  s.channels = take * size;
+  s.columns = s.channels / V;
+  s.rows = kNormThreads / s.columns;
+  const long long items = p.n * (p.groups / take);
+  // CTAs to an item: as many as the device holds, while each thread has four pixels
+  int ranks = 1;
+  while (ranks < 16 && items * ranks * 2 <= 2 * sms && p.pixels > kNormGroup * ranks * static_cast<long long>(s.rows)) ranks *= 2;
+  const long long each = (p.pixels + ranks - 1) / ranks;
+  constexpr int kSlot = static_cast<int>(kNormThreads * sizeof(T) * V);
+  constexpr int kSmem = kNormSlots<V> * kSlot + kNormThreads * V * static_cast<int>(sizeof(Moments));
+  static_assert(kSmem * (3) <= (220 << 10), "shared memory of the CTAs of an SM");
+  s.slots = static_cast<int>(std::min<long long>((each + s.rows - 1) / s.rows, kNormSlots<V>));
+  const int smem = s.slots * kSlot + s.rows * s.channels * static_cast<int>(sizeof(Moments));
+  auto kernel = k_group_norm<T, V, ACT>;
+  static std::atomic<uint64_t> granted{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(granted.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return op_launched("op_group_norm");
+    if (device < 64) granted.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  // blockIdx.y holds 65535: more items go in several launches
+  const long long per_image = p.groups / take, images = std::max<long long>(1, 65535 / per_image);
+  for (long long at = 0; at < p.n; at += images) {
+    NormParams q = p;
+    q.n = std::min(images, p.n - at);
+    q.x = static_cast<const T*>(p.x) + at * p.pixels * p.x_pitch;
+    q.y = static_cast<T*>(p.y) + at * p.pixels * p.y_pitch;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(ranks, static_cast<unsigned>(q.n * per_image));
+    c.blockDim = dim3(kNormThreads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = ranks;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    c.attrs = &cluster;
+    c.numAttrs = 1;
+    if (cudaLaunchKernelEx(&c, kernel, q, s) != cudaSuccess) break;
+  }
+  return op_launched("op_group_norm");
+}
+
+template <class T, int V, int ACT>
+int launch_act(const NormParams& p, int device, cudaStream_t st) {
+  const int size = p.channels / p.groups, sms = op_sm_count(device);
+  // The fewest groups whose channels are whole accesses and 128 bytes of a pixel; 64 to 16 where clusters of 16 CTAs to 128
+  // bytes would be fewer than three quarters of the SMs (2 maps of 512 x 512 x 128: fp32 168, 186 and 397 us with 128, 64 and 32
+  // bytes, bf16 176, 144 and 205).
+  auto pick = [&](int bytes) {
+    int take = 0;
+    for (int g = 1; g <= p.groups; ++g) {
+      if (p.groups % g != 0 || g * size % V != 0) continue;
+      if (g * size / V > kNormThreads || g > kNormMostGroups) break;
+      take = g;
+      if (g * size * static_cast<int>(sizeof(T)) >= bytes) break;
+    }
+    return take;
+  };
+  int take = pick(128);
+  for (int bytes = 64; bytes >= 16 && take > 0 && p.n * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
+  if (take == 0) {
+    k_group_norm_wide<T, ACT><<<static_cast<unsigned>(p.n * p.groups), kNormThreads, 0, st>>>(p);
+    return op_launched("op_group_norm");
+  }
+  return launch_shape<T, V, ACT>(p, take, device, st);
+}
+
+template <class T, int V>
+int launch(const NormParams& p, int activation, int device, cudaStream_t st) {
+  switch (activation) {
+    case NCNN_B200_ACT_RELU: return launch_act<T, V, NCNN_B200_ACT_RELU>(p, device, st);
+    case NCNN_B200_ACT_SWISH: return launch_act<T, V, NCNN_B200_ACT_SWISH>(p, device, st);
+    case NCNN_B200_ACT_GELU: return launch_act<T, V, NCNN_B200_ACT_GELU>(p, device, st);
+    default: return launch_act<T, V, NCNN_B200_ACT_NONE>(p, device, st);
   }
 }
 
@@ -89,17 +391,27 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: a pitch is smaller than a pixel's channels");
     if (x == y && x_pitch != y_pitch) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: in place, both pitches have to be the same");
     if (n == 0 || pixels == 0) return NCNN_B200_STATUS_SUCCESS;
-    if (pixels > (1ll << 40) / std::max(x_pitch, y_pitch) || n > (1ll << 40) / (pixels * std::max(x_pitch, y_pitch)) || n * groups > 0x7fffffffll)
-      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_group_norm: more than 2^40 elements, or 2^31 groups");
+    if (pixels > (1ll << 30) || pixels > (1ll << 40) / std::max(x_pitch, y_pitch) || n > (1ll << 40) / (pixels * std::max(x_pitch, y_pitch)) || n * groups > 0x7fffffffll)
+      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_group_norm: more than 2^30 pixels, 2^40 elements or 2^31 groups");
     std::string why;
     const int device = op_common_device(kOp, {x, y, gamma, beta}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
     DeviceGuard guard(device);
-    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, activation, gamma, beta, eps};
-    op_by_type(type, [&](auto t) {
-      k_group_norm<decltype(t)><<<static_cast<unsigned>(n * groups), 512, 0, static_cast<cudaStream_t>(stream)>>>(p);
-      return 0;
+    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, gamma, beta, eps};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // the widest access that every pixel's and every cluster's channels start and end with
+    auto whole = [&](int v) {
+      const uintptr_t bytes = static_cast<uintptr_t>(v) * op_elem_bytes(type);
+      return reinterpret_cast<uintptr_t>(x) % bytes == 0 && reinterpret_cast<uintptr_t>(y) % bytes == 0 && channels % v == 0 && x_pitch % v == 0 &&
+             y_pitch % v == 0;
+    };
+    const int status = op_by_type(type, [&](auto t) {
+      using T = decltype(t);
+      constexpr int V = 16 / sizeof(T);
+      if (whole(V)) return launch<T, V>(p, activation, device, st);
+      if (whole(2)) return launch<T, 2>(p, activation, device, st);
+      return launch<T, 1>(p, activation, device, st);
     });
-    return op_launched(kOp);
+    return status;
   });
 }
