@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_few(const __grid_
     float s[2][2][4] = {};  // (two sums each: shorter chains)
 #pragma unroll
     for (int c = 0; c < STEPS; ++c) {
+      if (D == 256 && 16 * c >= a.d) break;  // (heads between 128 and 256 share an instantiation)
       uint32_t b[4];
       ldmatrix_x4(b, k_at + (((2 * c + k_piece) ^ (k_row & 7)) << 4));
       mma_16x8x16<T>(s[0][c & 1], q[c], b[0], b[1]);
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_few(const __grid_
     }
 #pragma unroll
     for (int c = 0; c < STEPS; ++c) {
+      if (D == 256 && 16 * c >= a.d) break;
       uint32_t b[4];
       ldmatrix_x4_trans(b, v_at + (((2 * c + v_piece) ^ (v_row & 7)) << 4));
       mma_16x8x16<T>(o[2 * c], lo, b[0], b[1]);

@@ -9,58 +9,12 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "attend_f32.cuh"
 #include "attend_few.cuh"
 #include "tc_attend.cuh"
 
 namespace nb {
 namespace {
-
-// One warp to a query's head, a key at a time: components over the lanes, running maximum and sum.
-template <class T, int PER_LANE>
-__global__ void __launch_bounds__(256) k_attend_row(const __grid_constant__ AttendParams p) {
-  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int h = static_cast<int>(at % p.heads);
-  const long long rest = at / p.heads;
-  const int i = static_cast<int>(rest % p.lq);
-  const int b = static_cast<int>(rest / p.lq);
-  if (b >= p.batch) return;
-  const int kv = h / (p.heads / p.kv_heads);
-  const T* q = static_cast<const T*>(p.q) + b * p.q_batch + i * p.q_row + h * p.q_head;
-  const T* k = static_cast<const T*>(p.k) + b * p.k_batch + kv * p.k_head;
-  const T* v = static_cast<const T*>(p.v) + b * p.v_batch + kv * p.v_head;
-  T* o = static_cast<T*>(p.o) + b * p.o_batch + i * p.o_row + h * p.o_head;
-  const int keys = p.lens == nullptr ? p.lk : min(max(p.lens[b], 0), p.lk);
-  const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + static_cast<long long>(b) * p.lk;
-  float qv[PER_LANE], sum[PER_LANE];
-#pragma unroll
-  for (int c = 0; c < PER_LANE; ++c) {
-    qv[c] = lane + 32 * c < p.d ? op_get(q[lane + 32 * c]) * p.scale : 0.0f;
-    sum[c] = 0.0f;
-  }
-  float top = -INFINITY, total = 0.0f;
-  for (int j = 0; j < keys; ++j) {
-    if (mask != nullptr && mask[j] == 0) continue;
-    float s = 0.0f;
-#pragma unroll
-    for (int c = 0; c < PER_LANE; ++c)
-      if (lane + 32 * c < p.d) s = fmaf(qv[c], op_get(k[j * p.k_row + lane + 32 * c]), s);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(~0u, s, w);
-    const float next = fmaxf(top, s);
-    const float base = next == -INFINITY ? 0.0f : next;
-    const float keep = expf(top - base), e = expf(s - base);
-    total = fmaf(total, keep, e);
-#pragma unroll
-    for (int c = 0; c < PER_LANE; ++c)
-      if (lane + 32 * c < p.d) sum[c] = fmaf(e, op_get(v[j * p.v_row + lane + 32 * c]), sum[c] * keep);
-    top = next;
-  }
-  const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-  for (int c = 0; c < PER_LANE; ++c)
-    if (lane + 32 * c < p.d) o[lane + 32 * c] = op_put<T>(total == 0.0f ? 0.0f : sum[c] * scale);
-}
 
 // ------------------------------------------------------------------ tensor cores
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -96,15 +50,15 @@ bool encode_rows(CUtensorMap* map, bool half, const void* base, int d, long long
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether rows can be moved 16 bytes at a time (and by TMA): 16-bit types, starts and strides of axes that are stepped over.
-bool rows_of_16_bytes(const AttendParams& p) {
-  auto ok = [](const void* base, std::initializer_list<std::pair<long long, long long>> axes) {
-    if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+// Whether `count` elements of `size` bytes can be moved at a time: starts, and strides of the axes that are stepped over.
+bool rows_of(const AttendParams& p, int count, int size) {
+  auto ok = [&](const void* base, std::initializer_list<std::pair<long long, long long>> axes) {
+    if (reinterpret_cast<uintptr_t>(base) % (count * size) != 0) return false;
     for (const auto& a : axes)
-      if (a.second > 1 && a.first % 8 != 0) return false;
+      if (a.second > 1 && a.first % count != 0) return false;
     return true;
   };
-  return p.d % 8 == 0 && ok(p.q, {{p.q_batch, p.batch}, {p.q_row, p.lq}, {p.q_head, p.heads}}) &&
+  return p.d % count == 0 && ok(p.q, {{p.q_batch, p.batch}, {p.q_row, p.lq}, {p.q_head, p.heads}}) &&
          ok(p.k, {{p.k_batch, p.batch}, {p.k_row, p.lk}, {p.k_head, p.kv_heads}}) &&
          ok(p.v, {{p.v_batch, p.batch}, {p.v_row, p.lk}, {p.v_head, p.kv_heads}}) &&
          ok(p.o, {{p.o_batch, p.batch}, {p.o_row, p.lq}, {p.o_head, p.heads}});
@@ -144,7 +98,7 @@ bool launch_tc(const AttendParams& a, int device, cudaStream_t st) {
       !encode_rows(&v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p.v_step))
     return false;
   static std::atomic<uint64_t> granted{0};
-  if (grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, Shape::kRegsLaunch) != cudaSuccess) return false;
+  if (grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, Shape::kShareRegs ? Shape::kRegsLaunch : 0) != cudaSuccess) return false;
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
   tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, q, k, v);
   return true;
@@ -154,7 +108,8 @@ template <class T>
 bool attend_tc(const AttendParams& a, int device, cudaStream_t st) {
   const bool two = a.lq > kAttRows;
   if (a.d <= 64) return two ? launch_tc<T, 64, 2>(a, device, st) : launch_tc<T, 64, 1>(a, device, st);
-  return two ? launch_tc<T, 128, 2>(a, device, st) : launch_tc<T, 128, 1>(a, device, st);
+  if (a.d <= 128) return two ? launch_tc<T, 128, 2>(a, device, st) : launch_tc<T, 128, 1>(a, device, st);
+  return a.d <= 192 ? launch_tc<T, 192, 1>(a, device, st) : launch_tc<T, 256, 1>(a, device, st);
 }
 
 template <class T, int D, int WARPS, int STAGES, int BLOCKS>
@@ -185,7 +140,7 @@ bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
 // Whether a call is one of few queries: at most two tiles of 16 to a key head.
 bool few_queries(const AttendParams& p) {
   const long long rows = static_cast<long long>(p.lq) * (p.heads / p.kv_heads);
-  return rows <= 2 * kFewRows && p.d <= 128 && static_cast<long long>(p.kv_heads) * ((rows + kFewRows - 1) / kFewRows) <= 65535;
+  return rows <= 2 * kFewRows && static_cast<long long>(p.kv_heads) * ((rows + kFewRows - 1) / kFewRows) <= 65535;
 }
 
 template <class T>
@@ -194,7 +149,7 @@ bool attend_few(const AttendParams& a, int device, int sms, cudaStream_t st) {
   const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((rows + kFewRows - 1) / kFewRows);
   // Few tiles (a cluster of 8 to each leaves SMs idle): CTAs of 8 warps with deep rings, one to an SM, up to 16 to a tile while
   // each of their warps has two tiles of keys.  4 tiles of 20000 keys: 24.6 us, against 28.7 with CTAs of 4 warps.
-  if (tiles * 8 < sms && a.lk >= 4096) {
+  if (a.d <= 128 && tiles * 8 < sms && a.lk >= 4096) {
     int ranks = 8;
     while (ranks < 16 && tiles * ranks * 2 <= sms && a.lk >= ranks * 512) ranks *= 2;
     return a.d <= 64 ? launch_few<T, 64, 8, 6, 1>(a, device, ranks, st) : launch_few<T, 128, 8, 3, 1>(a, device, ranks, st);
@@ -206,7 +161,67 @@ bool attend_few(const AttendParams& a, int device, int sms, cudaStream_t st) {
   const long long most = (a.lens != nullptr ? 8ll : 2ll) * sms;
   int ranks = 1;
   while (ranks < 8 && tiles * ranks * 2 <= most && a.lk > ranks * 64) ranks *= 2;
-  return a.d <= 64 ? launch_few<T, 64, 4, 4, 3>(a, device, ranks, st) : launch_few<T, 128, 4, 3, 2>(a, device, ranks, st);
+  if (a.d <= 64) return launch_few<T, 64, 4, 4, 3>(a, device, ranks, st);
+  return a.d <= 128 ? launch_few<T, 128, 4, 3, 2>(a, device, ranks, st) : launch_few<T, 256, 4, 3, 1>(a, device, ranks, st);
+}
+
+// ------------------------------------------------------------------ CUDA cores
+template <class T, int D, int ROWS, bool WIDE>
+cudaError_t launch_split(F32Params& p, int sms, cudaStream_t st) {
+  const AttendParams& a = p.a;
+  const long long rows = static_cast<long long>(a.lq) * (a.heads / a.kv_heads);
+  p.row_tiles = static_cast<int>((rows + ROWS - 1) / ROWS);
+  const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * p.row_tiles;
+  // enough CTAs to a tile to fill the device twice over, while each of their warps has eight keys
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= 4ll * sms && a.lk > ranks * kSplitWarps * 8) ranks *= 2;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(ranks, a.kv_heads * p.row_tiles, a.batch);
+  c.blockDim = dim3(kSplitWarps * 32);
+  c.stream = st;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = ranks;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  c.attrs = &cluster;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, k_attend_split<T, D, ROWS, WIDE>, p);
+}
+
+template <class T, int D, int TM, int KEYS, bool WIDE>
+cudaError_t launch_tile(const F32Params& p, int device, cudaStream_t st) {
+  using Shape = TileShape<D, TM, KEYS>;
+  static std::atomic<uint64_t> granted{0};
+  if (const cudaError_t e = grant_smem(k_attend_tile<T, D, TM, KEYS, WIDE>, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
+  const long long rows = static_cast<long long>(p.a.lq) * (p.a.heads / p.a.kv_heads);
+  const dim3 grid(static_cast<unsigned>((rows + Shape::kRows - 1) / Shape::kRows), p.a.kv_heads, p.a.batch);
+  k_attend_tile<T, D, TM, KEYS, WIDE><<<grid, 256, Shape::kSmem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <class T, bool WIDE>
+cudaError_t attend_f32(const AttendParams& a, int device, int sms, cudaStream_t st) {
+  F32Params p{};
+  p.a = a;
+  p.scale_log2 = a.scale * 1.44269504088896340736f;
+  const long long rows = static_cast<long long>(a.lq) * (a.heads / a.kv_heads);
+  if (rows <= 16 && a.kv_heads * rows <= 65535) {
+    if (rows == 1) {
+      if (a.d <= 64) return launch_split<T, 64, 1, WIDE>(p, sms, st);
+      if (a.d <= 128) return launch_split<T, 128, 1, WIDE>(p, sms, st);
+      return launch_split<T, 256, 1, WIDE>(p, sms, st);
+    }
+    if (a.d <= 64) return launch_split<T, 64, 4, WIDE>(p, sms, st);
+    if (a.d <= 128) return launch_split<T, 128, 4, WIDE>(p, sms, st);
+    return launch_split<T, 256, 2, WIDE>(p, sms, st);
+  }
+  if (a.d <= 64) {
+    // 128 rows to a tile where those fill the device
+    if (a.batch * static_cast<long long>(a.kv_heads) * ((rows + 127) / 128) >= 2 * sms) return launch_tile<T, 64, 8, 64, WIDE>(p, device, st);
+    return launch_tile<T, 64, 4, 64, WIDE>(p, device, st);
+  }
+  if (a.d <= 128) return launch_tile<T, 128, 4, 64, WIDE>(p, device, st);
+  return launch_tile<T, 256, 4, 32, WIDE>(p, device, st);
 }
 
 // Every stride an axis of more than one entry is stepped with has to be a stride that TMA takes: positive and below 2^40 bytes.
@@ -294,10 +309,9 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     const int device = op_common_device(kOp, {q, o, lk > 0 ? k : nullptr, lk > 0 ? v : nullptr, kv_lens, key_mask}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
     DeviceGuard guard(device);
-    const long long rows = batch * lq * heads;
-    if (rows > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: more than 2^33 rows");
+    if (lq > (1ll << 30) / (heads / kv_heads) || batch * lq * heads > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: more than 2^33 rows");
     if (p.batch * static_cast<long long>(p.heads) > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: too many heads");
-    if (type != NCNN_B200_F32 && p.lk > 0 && few_queries(p) && rows_of_16_bytes(p)) {
+    if (type != NCNN_B200_F32 && p.lk > 0 && few_queries(p) && rows_of(p, 8, 2)) {
       cudaStream_t st = static_cast<cudaStream_t>(stream);
       const int sms = op_sm_count(device);
       if (!(type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st))) {
@@ -306,20 +320,19 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
       }
       return op_launched(kOp);
     }
-    if (type != NCNN_B200_F32 && p.lk > 0 && p.d <= 128 && rows_of_16_bytes(p) && tma_strides(p)) {
+    if (type != NCNN_B200_F32 && p.lk > 0 && rows_of(p, 8, 2) && tma_strides(p)) {
       if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
       cudaStream_t st = static_cast<cudaStream_t>(stream);
       const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, st) : attend_tc<__nv_bfloat16>(p, device, st);
       if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
       return op_launched(kOp);
     }
+    const int sms = op_sm_count(device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     op_by_type(type, [&](auto t) {
       using T = decltype(t);
-      const unsigned grid = static_cast<unsigned>((rows + 7) / 8);
-      cudaStream_t st = static_cast<cudaStream_t>(stream);
-      if (p.d <= 64) k_attend_row<T, 2><<<grid, 256, 0, st>>>(p);
-      else if (p.d <= 128) k_attend_row<T, 4><<<grid, 256, 0, st>>>(p);
-      else k_attend_row<T, 8><<<grid, 256, 0, st>>>(p);
+      if (rows_of(p, 4, sizeof(T))) attend_f32<T, true>(p, device, sms, st);
+      else attend_f32<T, false>(p, device, sms, st);
       return 0;
     });
     return op_launched(kOp);

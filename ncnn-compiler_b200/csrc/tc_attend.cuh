@@ -42,13 +42,16 @@ struct TcAttendShape {
   static constexpr int kPanel = kAttRows * 128;  // 128 rows of 64 components
   static constexpr int kTile = kPanel * (D / 64);
   static constexpr int kThreads = 128 + 128 * TILES;
-  static constexpr int kBlocksPerSm = TILES == 2 ? 1 : 2;
-  static constexpr uint32_t kTmemCols = TILES == 2 ? 512 : 256;
+  static constexpr int kBlocksPerSm = TILES == 2 || D > 128 ? 1 : 2;
+  static constexpr uint32_t kTmemCols = TILES == 2 || D > 128 ? 512 : 256;
+  static_assert(TILES * (128 + D) <= static_cast<int>(kTmemCols), "scores and results in tensor memory");
+  // 256 threads alone on an SM have 255 registers each anyway; otherwise the roles share what the CTA was launched with
+  static constexpr bool kShareRegs = D <= 128;
   static constexpr int kRegsLaunch = 65536 / (kThreads * kBlocksPerSm) / 8 * 8;
   static constexpr int kRegsControl = TILES == 2 ? 56 : 40;
   static constexpr int kRegsSoftmax = TILES == 2 ? 224 : 216;
-  static_assert(128 * kRegsControl + 128 * TILES * kRegsSoftmax <= kThreads * kRegsLaunch, "registers of the roles");
-  static constexpr int kSlots = D == 128 ? (TILES == 2 ? 4 : 2) : (TILES == 2 ? 6 : 4);
+  static_assert(!kShareRegs || 128 * kRegsControl + 128 * TILES * kRegsSoftmax <= kThreads * kRegsLaunch, "registers of the roles");
+  static constexpr int kSlots = D > 128 ? 2 : D == 128 ? (TILES == 2 ? 4 : 2) : (TILES == 2 ? 6 : 4);
   static_assert(kSlots % 2 == 0, "values always land in the same slots: `fixed` counts their phases");
   static constexpr int kSmem = 1024 + TILES * kTile + kSlots * kTile;
 };
@@ -165,7 +168,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
   auto o_of = [&](int t) { return tmem + 128u * TILES + static_cast<uint32_t>(D * t); };
 
   if (warp < 4) {
-    reg_dealloc<Shape::kRegsControl>();
+    if constexpr (Shape::kShareRegs) reg_dealloc<Shape::kRegsControl>();
     if (warp == 0 && blocks > 0) {
       if (elect_one()) {
         bool ok = true;
@@ -301,7 +304,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
       if (!ok && lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
     }
   } else {
-    reg_alloc<Shape::kRegsSoftmax>();
+    if constexpr (Shape::kShareRegs) reg_alloc<Shape::kRegsSoftmax>();
     const int t = (warp - 4) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes of tensor memory (lane in the upper half word)
     const int row = row0 + t * kAttRows + (warp & 3) * 32 + lane;
