@@ -12,6 +12,7 @@
 #include "attend_f32.cuh"
 #include "attend_few.cuh"
 #include "tc_attend.cuh"
+#include "tc_attend_short.cuh"
 
 namespace nb {
 namespace {
@@ -30,10 +31,10 @@ EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// [sequence][head][row][component] as TMA sees it, boxes of 128 rows of 64 components.  An axis that all heads or sequences
+// [sequence][head][row][component] as TMA sees it, boxes of 128 rows (results: 32) of 64 components.  An axis that all heads or sequences
 // share (stride 0) has one entry: `step` says what to multiply its index with.
 bool encode_rows(CUtensorMap* map, bool half, const void* base, int d, long long rows, long long row, int heads, long long head, int batch,
-                 long long seq, int* step) {
+                 long long seq, int* step, int box_rows = kAttRows) {
   const int head_extent = head == 0 ? 1 : heads, batch_extent = seq == 0 ? 1 : batch;
   if (step != nullptr) {
     step[0] = head == 0 ? 0 : 1;
@@ -44,7 +45,7 @@ bool encode_rows(CUtensorMap* map, bool half, const void* base, int d, long long
   const cuuint64_t any = (static_cast<cuuint64_t>(d) * 2 + 15) / 16 * 16;
   const cuuint64_t strides[3] = {rows == 1 ? any : static_cast<cuuint64_t>(row) * 2, head_extent == 1 ? any : static_cast<cuuint64_t>(head) * 2,
                                  batch_extent == 1 ? any : static_cast<cuuint64_t>(seq) * 2};
-  const cuuint32_t box[4] = {64, kAttRows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1}, ones[4] = {1, 1, 1, 1};
   return encode_tiled()(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box,
                         ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -80,33 +81,59 @@ cudaError_t grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* g
   return e;
 }
 
+struct TcMaps {
+  alignas(64) CUtensorMap q, k, v, o;
+};
+
+bool fill_tc(const AttendParams& a, bool half, TcAttendParams* p, TcMaps* m) {
+  p->a = a;
+  p->scale_log2 = a.scale * 1.44269504088896340736f;
+  p->wait_ns = kTcWaitLimitNs;
+  if (std::getenv("NCNN_B200_TEST_STALL") != nullptr) {
+    p->stall = 1;
+    p->wait_ns = 2000000ull;
+  }
+  return encode_rows(&m->q, half, a.q, a.d, a.lq, a.q_row, a.heads, a.q_head, a.batch, a.q_batch, p->q_step) &&
+         encode_rows(&m->k, half, a.k, a.d, a.lk, a.k_row, a.kv_heads, a.k_head, a.batch, a.k_batch, p->k_step) &&
+         encode_rows(&m->v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p->v_step) &&
+         encode_rows(&m->o, half, a.o, a.d, a.lq, a.o_row, a.heads, a.o_head, a.batch, a.o_batch, nullptr, 32);
+}
+
+template <class T, int D>
+bool launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
+  using Shape = TcShortShape<D>;
+  TcShortParams p{};
+  TcMaps m;
+  if (!fill_tc(a, std::is_same<T, __half>::value, &p.t, &m)) return false;
+  static std::atomic<uint64_t> granted{0};
+  if (grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch) != cudaSuccess) return false;
+  p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
+  p.tiles = p.row_tiles * a.heads * a.batch;
+  tc_attend_short_kernel<T, D><<<std::min(sms, p.tiles), Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
+  return true;
+}
+
 template <class T, int D, int TILES>
 bool launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   using Shape = TcAttendShape<D, TILES>;
   TcAttendParams p{};
-  p.a = a;
-  p.scale_log2 = a.scale * 1.44269504088896340736f;
-  p.wait_ns = kTcWaitLimitNs;
-  if (std::getenv("NCNN_B200_TEST_STALL") != nullptr) {
-    p.stall = 1;
-    p.wait_ns = 2000000ull;
-  }
-  alignas(64) CUtensorMap q, k, v;
-  constexpr bool half = std::is_same<T, __half>::value;
-  if (!encode_rows(&q, half, a.q, a.d, a.lq, a.q_row, a.heads, a.q_head, a.batch, a.q_batch, p.q_step) ||
-      !encode_rows(&k, half, a.k, a.d, a.lk, a.k_row, a.kv_heads, a.k_head, a.batch, a.k_batch, p.k_step) ||
-      !encode_rows(&v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p.v_step))
-    return false;
+  TcMaps m;
+  if (!fill_tc(a, std::is_same<T, __half>::value, &p, &m)) return false;
   static std::atomic<uint64_t> granted{0};
   if (grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, Shape::kShareRegs ? Shape::kRegsLaunch : 0) != cudaSuccess) return false;
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
-  tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, q, k, v);
+  tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
   return true;
 }
 
 template <class T>
-bool attend_tc(const AttendParams& a, int device, cudaStream_t st) {
+bool attend_tc(const AttendParams& a, int device, int sms, cudaStream_t st) {
   const bool two = a.lq > kAttRows;
+  const long long tiles = static_cast<long long>((a.lq + kAttRows - 1) / kAttRows) * a.heads * a.batch;
+  // one block of keys and a tile for every SM: 4096 queries over 77 keys (8 sequences, 10 heads of 64) 27 us, 55 with a CTA to two
+  // tiles
+  if (a.lk <= kAttRows && a.d <= 128 && tiles >= sms && tiles < (1 << 30))
+    return a.d <= 64 ? launch_short<T, 64>(a, device, sms, st) : launch_short<T, 128>(a, device, sms, st);
   if (a.d <= 64) return two ? launch_tc<T, 64, 2>(a, device, st) : launch_tc<T, 64, 1>(a, device, st);
   if (a.d <= 128) return two ? launch_tc<T, 128, 2>(a, device, st) : launch_tc<T, 128, 1>(a, device, st);
   return a.d <= 192 ? launch_tc<T, 192, 1>(a, device, st) : launch_tc<T, 256, 1>(a, device, st);
@@ -229,7 +256,7 @@ bool tma_strides(const AttendParams& p) {
   auto ok = [](long long stride, long long extent, bool shared) { return extent == 1 || ((stride > 0 || (shared && stride == 0)) && stride < (1ll << 38)); };
   return ok(p.q_batch, p.batch, true) && ok(p.q_row, p.lq, false) && ok(p.q_head, p.heads, true) && ok(p.k_batch, p.batch, true) &&
          ok(p.k_row, p.lk, false) && ok(p.k_head, p.kv_heads, true) && ok(p.v_batch, p.batch, true) && ok(p.v_row, p.lk, false) &&
-         ok(p.v_head, p.kv_heads, true);
+         ok(p.v_head, p.kv_heads, true) && ok(p.o_batch, p.batch, false) && ok(p.o_row, p.lq, false) && ok(p.o_head, p.heads, false);
 }
 
 }  // namespace
@@ -323,7 +350,8 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     if (type != NCNN_B200_F32 && p.lk > 0 && rows_of(p, 8, 2) && tma_strides(p)) {
       if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
       cudaStream_t st = static_cast<cudaStream_t>(stream);
-      const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, st) : attend_tc<__nv_bfloat16>(p, device, st);
+      const int sms = op_sm_count(device);
+      const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
       if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
       return op_launched(kOp);
     }

@@ -108,10 +108,61 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
+               : "memory");
+}
+
+// 2^(x c + from) and 2^(y c + from) packed, and added to a pair of sums: two values to an instruction where there is one
+template <class T>
+__device__ __forceinline__ uint32_t exp_pair(uint32_t x, uint32_t y, uint64_t c2, uint64_t from2, uint64_t& sums) {
+  const float2 t = f32x2_get(f32x2_fma3(f32x2_make(x, y), c2, from2));
+  const float e0 = exp2_fast(t.x), e1 = exp2_fast(t.y);
+  f32x2_add(sums, sums, f32x2_make(__float_as_uint(e0), __float_as_uint(e1)));
+  return pack2<T>(e0, e1);
+}
+
+// A warp's 32 rows of results, scaled, out of tensor memory into a tile of shared memory (panels of 64 components, 128-byte
+// swizzle) and from there to global memory in whole lines (4096 queries over 77 keys: 36 us against 40 with 16-byte stores by
+// rows).  `staged`: the tile; `warp_row`: the warp's first row in it.
+template <class T, int D>
+__device__ __forceinline__ void attend_store(uint32_t o_at, bool any, float total, uint32_t staged, int warp_row, const CUtensorMap* map, int row, int rows,
+                                             int h, int b, int d) {
+  using namespace ptx;
+  const int lane = threadIdx.x & 31, r = warp_row + lane;
+  const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w) {
+    uint32_t o[32];
+    if (any) {
+      tmem_ld32(o_at + 32u * w, o);
+      tmem_ld_wait();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        u[e] = total == 0.0f ? 0u : pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * scale, __uint_as_float(o[8 * i + 2 * e + 1]) * scale);
+      const uint32_t to = staged + (w / 2) * (kAttRows * 128) + r * 128 + (((w % 2 * 4 + i) ^ (r & 7)) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && row + warp_row < rows) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+      if (64 * c < d) tma_store_4d(map, staged + c * (kAttRows * 128) + warp_row * 128, 64 * c, row + warp_row, h, b);
+    bulk_commit();
+  }
+}
+
 template <class T, int D, int TILES>
 __global__ void __launch_bounds__(TcAttendShape<D, TILES>::kThreads, TcAttendShape<D, TILES>::kBlocksPerSm)
 tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v) {
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o) {
   using namespace ptx;
   using Shape = TcAttendShape<D, TILES>;
   constexpr int kTile = Shape::kTile, kPanel = Shape::kPanel, kSlots = Shape::kSlots;
@@ -307,7 +358,6 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
     if constexpr (Shape::kShareRegs) reg_alloc<Shape::kRegsSoftmax>();
     const int t = (warp - 4) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes of tensor memory (lane in the upper half word)
-    const int row = row0 + t * kAttRows + (warp & 3) * 32 + lane;
     if (t < tiles) {
       const uint32_t s_at = s_of(t) + lanes, o_at = o_of(t) + lanes;
       const float c = p.scale_log2;
@@ -362,21 +412,18 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
           }
         }
         const float from = base == -INFINITY ? 0.0f : -base;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t c2 = f32x2_make(__float_as_uint(c), __float_as_uint(c)), from2 = f32x2_make(__float_as_uint(from), __float_as_uint(from));
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e0 = exp2_fast(fmaf(__uint_as_float(s[32 * w + 2 * i]), c, from));
-            const float e1 = exp2_fast(fmaf(__uint_as_float(s[32 * w + 2 * i + 1]), c, from));
-            sum[(2 * i) & 3] += e0;
-            sum[(2 * i + 1) & 3] += e1;
-            packed[i] = pack2<T>(e0, e1);
-          }
+          for (int i = 0; i < 16; ++i) packed[i] = exp_pair<T>(s[32 * w + 2 * i], s[32 * w + 2 * i + 1], c2, from2, sums[i & 1]);
           tmem_st16(s_at + 16u * w, packed);
         }
-        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        f32x2_add(sums[0], sums[0], sums[1]);
+        const float2 sum = f32x2_get(sums[0]);
+        total += sum.x + sum.y;
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
@@ -389,27 +436,9 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
       if (!ok) {
         if (lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
       } else {
-        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-        T* out = static_cast<T*>(p.a.o) + batch * p.a.o_batch + row * p.a.o_row + head * p.a.o_head;
-#pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-          uint32_t o[32];
-          if (blocks > 0) {
-            tmem_ld32(o_at + 32u * w, o);
-            tmem_ld_wait();
-          }
-          if (row < p.a.lq) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (32 * w + 8 * i >= p.a.d) break;
-              uint32_t u[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u[e] = total == 0.0f ? 0u : pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * scale, __uint_as_float(o[8 * i + 2 * e + 1]) * scale);
-              *reinterpret_cast<uint4*>(out + 32 * w + 8 * i) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
-        }
+        // (every product is done: the queries' tile is free)
+        attend_store<T, D>(o_at, blocks > 0, total, q_at + t * kTile, (warp & 3) * 32, &map_o, row0 + t * kAttRows, p.a.lq, head, batch, p.a.d);
+        if (lane == 0) bulk_wait_read();
       }
       tc_fence_before_sync();
     }

@@ -414,6 +414,18 @@ def test_cross_attention_masks(pkg, element, d, lq, b, lk):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("d,lk", [(64, 77), (40, 128), (128, 100), (72, 33), (64, 16), (128, 1)])
+def test_cross_attention_text(pkg, element, d, lk):
+    """Many queries over few keys, more tiles than SMs: whole sequences, ragged ones, one without keys, masks with holes."""
+    check_attend(pkg, element, 4, 700, lk, 8, 4, d)
+    check_attend(pkg, element, 5, 650, lk, 8, 8, d, lens=[lk, 0, 1, lk // 2 + 1, 0])
+    mask = torch.rand(5, lk, generator=torch.Generator().manual_seed(lk)) < 0.5
+    mask[3] = False
+    check_attend(pkg, element, 5, 650, lk, 8, 2, d, mask=mask, lens=[lk, lk, lk // 2 + 1, lk, lk - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
 @pytest.mark.parametrize("lq", [1, 150])
 def test_cross_attention_layouts(pkg, element, lq):
     """Head-major arrays, slices of a joint projection, keys that all heads or all sequences share, one element's alignment."""
