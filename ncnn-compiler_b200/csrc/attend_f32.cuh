@@ -27,6 +27,7 @@ struct F32Params {
   AttendParams a;
   float scale_log2;
   int row_tiles;
+  int ranks;  // CTAs to a tile of many queries
 };
 
 // ------------------------------------------------------------------ few queries
@@ -169,37 +170,40 @@ __global__ void __launch_bounds__(kSplitWarps * 32) k_attend_split(const __grid_
 }
 
 // ------------------------------------------------------------------ many queries
-// A tile of 16 TM rows (query, head of the key head) against blocks of KEYS keys, all in shared memory as fp32; 256 threads, 16 to
-// a row.  A thread computes TM rows by KEYS / 16 keys of scores, then TM rows by D / 16 components of results out of the
+// A tile of rows (query, head of the key head) against blocks of KEYS keys, all in shared memory as fp32; 16 threads to TM rows.  A thread computes TM rows by KEYS / 16 keys of scores, then TM rows by D / 16 components of results out of the
 // probabilities, which its own half warp wrote.  Every 4 x 4 products take two 16-byte loads of which one is a broadcast.
-// Bound: the FMA pipe.
-template <int D, int TM, int KEYS>
+// Bound: the FMA pipe (32 of 74 TFLOP/s over 1024 x 1024, 64 heads of 64: half the issue slots are loads, addresses and the softmax).
+// Where the tiles are fewer than the device holds, a tile's blocks of keys are dealt to the CTAs of a cluster, which join their
+// results over distributed shared memory (2394 queries over 1768 keys, two heads of 128 on one key head: 498 us without).
+template <int D, int TM, int KEYS, int THREADS>
 struct TileShape {
-  static constexpr int kRows = 16 * TM;
+  static constexpr int kRows = THREADS / 16 * TM;
   static constexpr int kPitch = D + 4;  // floats: rows start in different banks
   static constexpr int kSmem = (kRows * kPitch + KEYS * kPitch + KEYS * D + kRows * (KEYS + 4)) * 4;
 };
 
-template <class T, int D, int TM, int KEYS, bool WIDE>
-__global__ void __launch_bounds__(256) k_attend_tile(const __grid_constant__ F32Params p) {
-  using Shape = TileShape<D, TM, KEYS>;
+template <class T, int D, int TM, int KEYS, int THREADS, bool WIDE>
+__global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1) k_attend_tile(const __grid_constant__ F32Params p) {
+  namespace cg = cooperative_groups;
+  using Shape = TileShape<D, TM, KEYS, THREADS>;
   constexpr int ROWS = Shape::kRows, PITCH = Shape::kPitch, TN = KEYS / 16, PER = D / 64;
   extern __shared__ __align__(16) float tile_smem[];
   float* qs = tile_smem;                // [row][component]
   float* ks = qs + ROWS * PITCH;        // [key][component]
   float* vs = ks + KEYS * PITCH;        // [key][component]
   float* ps = vs + KEYS * D;            // [row][key]
-  __shared__ uint8_t takes[KEYS];
+  __shared__ uint8_t takes[2][KEYS];
   const AttendParams& a = p.a;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int kv_head = blockIdx.y, batch = blockIdx.z, shared = a.heads / a.kv_heads;
-  const int all_rows = a.lq * shared, row0 = blockIdx.x * ROWS;
+  const int ranks = p.ranks, rank = blockIdx.x % ranks;
+  const int all_rows = a.lq * shared, row0 = blockIdx.x / ranks * ROWS;
   const int keys = a.lens == nullptr ? a.lk : min(max(__ldg(a.lens + batch), 0), a.lk);
   const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + static_cast<long long>(batch) * a.lk;
   const T* k = static_cast<const T*>(a.k) + batch * a.k_batch + kv_head * a.k_head;
   const T* v = static_cast<const T*>(a.v) + batch * a.v_batch + kv_head * a.v_head;
   const int pieces = (a.d + 3) / 4;  // of four components; the others stay zero
-  for (int i = threadIdx.x; i < ROWS * (D / 4); i += 256) {
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += THREADS) {
     const int r = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (row < all_rows)
@@ -215,25 +219,37 @@ __global__ void __launch_bounds__(256) k_attend_tile(const __grid_constant__ F32
 #pragma unroll
     for (int c = 0; c < PER; ++c) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
-  for (int j0 = 0; j0 < keys; j0 += KEYS) {
-    __syncthreads();
+  // A block's keys are asked for when the last block's scores are done, its values when the last block's products are: fp32 rows
+  // come by cp.async meanwhile.
+  auto flag = [&](int at, int j0) {
     if (threadIdx.x < KEYS) {
       const int j = j0 + threadIdx.x;
-      takes[threadIdx.x] = j < keys && (mask == nullptr || __ldg(mask + j) != 0);
+      takes[at][threadIdx.x] = j < keys && (mask == nullptr || __ldg(mask + j) != 0);
     }
-    __syncthreads();
-    // eight lanes or more to a key: whole sectors
-    for (int i = threadIdx.x; i < KEYS * (D / 4); i += 256) {
-      const int r = i / (D / 4), c = i % (D / 4) * 4;
-      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-      if (takes[r]) {
-        x = four_of<T, WIDE>(k + (j0 + r) * a.k_row, c, a.d);
-        y = four_of<T, WIDE>(v + (j0 + r) * a.v_row, c, a.d);
+  };
+  auto fetch = [&](float* to, int pitch, const T* from, long long stride, int j0, const uint8_t* part) {
+    if (j0 < keys)
+      for (int i = threadIdx.x; i < KEYS * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4;
+        const bool used = part[r] != 0 && c < a.d;
+        if constexpr (WIDE && sizeof(T) == 4)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to + r * pitch + c))),
+                       "l"(used ? from + (j0 + r) * stride + c : from), "r"(used ? 16 : 0)
+                       : "memory");
+        else
+          *reinterpret_cast<float4*>(to + r * pitch + c) = used ? four_of<T, WIDE>(from + (j0 + r) * stride, c, a.d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
-      *reinterpret_cast<float4*>(ks + r * PITCH + c) = x;
-      *reinterpret_cast<float4*>(vs + r * D + c) = y;
-    }
-    __syncthreads();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int step = ranks * KEYS;
+  int now = 0;
+  flag(0, rank * KEYS);
+  __syncthreads();
+  fetch(ks, PITCH, k, a.k_row, rank * KEYS, takes[0]);
+  fetch(vs, D, v, a.v_row, rank * KEYS, takes[0]);
+  for (int j0 = rank * KEYS; j0 < keys; j0 += step, now ^= 1) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();  // the keys are there
     float s[TM][TN] = {};
 #pragma unroll 2
     for (int c = 0; c < pieces; ++c) {
@@ -247,9 +263,13 @@ __global__ void __launch_bounds__(256) k_attend_tile(const __grid_constant__ F32
 #pragma unroll
         for (int n = 0; n < TN; ++n) s[i][n] = dot4(x[i], y[n], s[i][n]);
     }
+    flag(now ^ 1, j0 + step);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the values are there, nobody needs the keys
+    fetch(ks, PITCH, k, a.k_row, j0 + step, takes[now ^ 1]);
     uint32_t out = 0;  // this thread's keys without a part
 #pragma unroll
-    for (int n = 0; n < TN; ++n) out |= (takes[tx + 16 * n] ? 0u : 1u) << n;
+    for (int n = 0; n < TN; ++n) out |= (takes[now][tx + 16 * n] ? 0u : 1u) << n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       float m = top[i];
@@ -291,6 +311,54 @@ __global__ void __launch_bounds__(256) k_attend_tile(const __grid_constant__ F32
           }
         }
     }
+    __syncthreads();  // nobody needs the values
+    fetch(vs, D, v, a.v_row, j0 + step, takes[now ^ 1]);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (ranks > 1) {
+    // a CTA's results take the place of its queries, and each CTA joins its share of the rows
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ float tops[ROWS], totals[ROWS];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float all = total[i];
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) all += __shfl_xor_sync(~0u, all, w);
+      const int r = ty * TM + i;
+      if (tx == 0) {
+        tops[r] = top[i];
+        totals[r] = all;
+      }
+#pragma unroll
+      for (int c = 0; c < PER; ++c) *reinterpret_cast<float4*>(qs + r * PITCH + 64 * c + 4 * tx) = o[i][c];
+    }
+    cluster.sync();
+    const int share = ROWS / ranks, from = rank * share;
+    for (int i = threadIdx.x; i < share * (D / 4); i += THREADS) {
+      const int r = from + i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
+      if (row >= all_rows || c >= a.d) continue;
+      float m = -INFINITY;
+      for (int n = 0; n < ranks; ++n) m = fmaxf(m, *cluster.map_shared_rank(&tops[r], n));
+      const float base = m == -INFINITY ? 0.0f : m;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, all = 0.0f;
+      for (int n = 0; n < ranks; ++n) {
+        const float f = exp2f(*cluster.map_shared_rank(&tops[r], n) - base);
+        const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(qs + r * PITCH + c, n));
+        all = fmaf(f, *cluster.map_shared_rank(&totals[r], n), all);
+        x[0] = fmaf(f, y.x, x[0]);
+        x[1] = fmaf(f, y.y, x[1]);
+        x[2] = fmaf(f, y.z, x[2]);
+        x[3] = fmaf(f, y.w, x[3]);
+      }
+      const float scale = all == 0.0f ? 0.0f : 1.0f / all;
+      T* to = static_cast<T*>(a.o) + batch * a.o_batch + row / shared * a.o_row + (kv_head * shared + row % shared) * a.o_head + c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.d) to[e] = op_put<T>(all == 0.0f ? 0.0f : x[e] * scale);
+    }
+    cluster.sync();  // no CTA's shared memory goes while another reads it
+    return;
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i) {

@@ -215,15 +215,29 @@ cudaError_t launch_split(F32Params& p, int sms, cudaStream_t st) {
   return cudaLaunchKernelEx(&c, k_attend_split<T, D, ROWS, WIDE>, p);
 }
 
-template <class T, int D, int TM, int KEYS, bool WIDE>
-cudaError_t launch_tile(const F32Params& p, int device, cudaStream_t st) {
-  using Shape = TileShape<D, TM, KEYS>;
+template <class T, int D, int TM, int KEYS, int THREADS, bool WIDE>
+cudaError_t launch_tile(F32Params p, int device, int sms, cudaStream_t st) {
+  using Shape = TileShape<D, TM, KEYS, THREADS>;
   static std::atomic<uint64_t> granted{0};
-  if (const cudaError_t e = grant_smem(k_attend_tile<T, D, TM, KEYS, WIDE>, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
+  auto kernel = k_attend_tile<T, D, TM, KEYS, THREADS, WIDE>;
+  if (const cudaError_t e = grant_smem(kernel, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
   const long long rows = static_cast<long long>(p.a.lq) * (p.a.heads / p.a.kv_heads);
-  const dim3 grid(static_cast<unsigned>((rows + Shape::kRows - 1) / Shape::kRows), p.a.kv_heads, p.a.batch);
-  k_attend_tile<T, D, TM, KEYS, WIDE><<<grid, 256, Shape::kSmem, st>>>(p);
-  return cudaGetLastError();
+  const long long row_tiles = (rows + Shape::kRows - 1) / Shape::kRows, tiles = row_tiles * p.a.kv_heads * p.a.batch;
+  // CTAs to a tile: what the device holds at once (two to an SM for heads up to 64), while each has two blocks of keys
+  p.ranks = 1;
+  while (p.ranks < 8 && tiles * p.ranks * 2 <= (D == 64 ? 2 : 1) * sms && p.a.lk > p.ranks * 2 * KEYS) p.ranks *= 2;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(static_cast<unsigned>(row_tiles * p.ranks), p.a.kv_heads, p.a.batch);
+  c.blockDim = dim3(THREADS);
+  c.dynamicSmemBytes = Shape::kSmem;
+  c.stream = st;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = p.ranks;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  c.attrs = &cluster;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, p);
 }
 
 template <class T, bool WIDE>
@@ -244,11 +258,11 @@ cudaError_t attend_f32(const AttendParams& a, int device, int sms, cudaStream_t 
   }
   if (a.d <= 64) {
     // 128 rows to a tile where those fill the device
-    if (a.batch * static_cast<long long>(a.kv_heads) * ((rows + 127) / 128) >= 2 * sms) return launch_tile<T, 64, 8, 64, WIDE>(p, device, st);
-    return launch_tile<T, 64, 4, 64, WIDE>(p, device, st);
+    if (a.batch * static_cast<long long>(a.kv_heads) * ((rows + 127) / 128) >= 2 * sms) return launch_tile<T, 64, 8, 64, 256, WIDE>(p, device, sms, st);
+    return launch_tile<T, 64, 4, 64, 256, WIDE>(p, device, sms, st);
   }
-  if (a.d <= 128) return launch_tile<T, 128, 4, 64, WIDE>(p, device, st);
-  return launch_tile<T, 256, 4, 32, WIDE>(p, device, st);
+  if (a.d <= 128) return launch_tile<T, 128, 4, 64, 512, WIDE>(p, device, sms, st);
+  return launch_tile<T, 256, 4, 32, 512, WIDE>(p, device, sms, st);
 }
 
 // Every stride an axis of more than one entry is stepped with has to be a stride that TMA takes: positive and below 2^40 bytes.
