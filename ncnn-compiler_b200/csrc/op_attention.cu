@@ -164,10 +164,15 @@ bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   return cudaLaunchKernelEx(&c, k_attend_few<T, D, WARPS, STAGES, BLOCKS>, p) == cudaSuccess;
 }
 
-// Whether a call is one of few queries: at most two tiles of 16 to a key head.
-bool few_queries(const AttendParams& p) {
-  const long long rows = static_cast<long long>(p.lq) * (p.heads / p.kv_heads);
-  return rows <= 2 * kFewRows && static_cast<long long>(p.kv_heads) * ((rows + kFewRows - 1) / kFewRows) <= 65535;
+// Whether a call is one of few queries.  At most two tiles of 16 to a key head always are.  So are up to 160 tiles over 512 keys or
+// more where the tensor-core kernel, which gives a head's 128 queries to one CTA from the first key to the last, would use less
+// than half of the SMs: 8 heads of 64 queries over 4096 keys 12 us against 46, of 128 queries 24 against 52, of 256 over 8192
+// (128 tiles) 75 against 112; 32 heads of 64 over 1024 (128 tiles) 15 against 16.
+bool few_queries(const AttendParams& p, int sms) {
+  const long long rows = static_cast<long long>(p.lq) * (p.heads / p.kv_heads), row_tiles = (rows + kFewRows - 1) / kFewRows;
+  if (p.kv_heads * row_tiles > 65535) return false;
+  const long long ctas = static_cast<long long>(p.batch) * p.heads * ((p.lq + kAttRows - 1) / kAttRows);
+  return rows <= 2 * kFewRows || (p.batch * p.kv_heads * row_tiles <= 160 && p.lk >= 512 && 2 * ctas <= sms);
 }
 
 template <class T>
@@ -352,25 +357,23 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     DeviceGuard guard(device);
     if (lq > (1ll << 30) / (heads / kv_heads) || batch * lq * heads > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: more than 2^33 rows");
     if (p.batch * static_cast<long long>(p.heads) > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_cross_attention: too many heads");
-    if (type != NCNN_B200_F32 && p.lk > 0 && few_queries(p) && rows_of(p, 8, 2)) {
-      cudaStream_t st = static_cast<cudaStream_t>(stream);
-      const int sms = op_sm_count(device);
-      if (!(type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st))) {
-        const int st_code = op_launched(kOp);
-        return st_code != 0 ? st_code : op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: launch failed");
-      }
-      return op_launched(kOp);
-    }
-    if (type != NCNN_B200_F32 && p.lk > 0 && rows_of(p, 8, 2) && tma_strides(p)) {
-      if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
-      cudaStream_t st = static_cast<cudaStream_t>(stream);
-      const int sms = op_sm_count(device);
-      const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
-      if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
-      return op_launched(kOp);
-    }
     const int sms = op_sm_count(device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (type != NCNN_B200_F32 && p.lk > 0 && rows_of(p, 8, 2)) {
+      if (few_queries(p, sms)) {
+        if (!(type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st))) {
+          const int failed = op_launched(kOp);
+          return failed != 0 ? failed : op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the kernel could not be launched");
+        }
+        return op_launched(kOp);
+      }
+      if (tma_strides(p)) {
+        if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
+        const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
+        if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
+        return op_launched(kOp);
+      }
+    }
     op_by_type(type, [&](auto t) {
       using T = decltype(t);
       if (rows_of(p, 4, sizeof(T))) attend_f32<T, true>(p, device, sms, st);
