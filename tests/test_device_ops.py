@@ -507,6 +507,116 @@ def test_cross_attention_is_the_same_every_time(pkg, element):
         assert all(torch.equal(o[0], t) for t in o[1:])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f16", "f32"])
+@pytest.mark.parametrize("b,lq,lk,heads,kv_heads,d", [(1, 6, 1399, 16, 2, 128), (1, 64, 600, 8, 8, 64), (2, 100, 777, 4, 4, 160), (1, 700, 513, 2, 1, 96),
+                                                      (1, 1, 9000, 2, 2, 64), (1, 20, 5000, 1, 1, 128), (1, 1, 4100, 1, 1, 256), (1, 300, 2000, 1, 1, 200)])
+def test_cross_attention_split_keys(pkg, element, b, lq, lk, heads, kv_heads, d):
+    """Calls whose keys are cut over warps, CTAs and clusters: with masks, and lengths that leave some of them nothing."""
+    mask = torch.rand(b, lk, generator=torch.Generator().manual_seed(lk)) < 0.3
+    check_attend(pkg, element, b, lq, lk, heads, kv_heads, d, mask=mask)
+    check_attend(pkg, element, b, lq, lk, heads, kv_heads, d, lens=[9] * b)
+    check_attend(pkg, element, b, lq, lk, heads, kv_heads, d, lens=[lk - 7] * b, mask=mask)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(pkg):
+    """Rows 2^21 elements apart, 1100 of them: offsets in elements pass 2^31."""
+    rows, pitch = 1100, 1 << 21
+    for element in ("bf16", "f32"):
+        kind = KIND[element]
+        big = torch.empty(rows * pitch, device="cuda", dtype=kind)
+        view = torch.as_strided(big, (rows, 256), (pitch, 1))
+        view.copy_(normal(gen(4), rows, 256))
+        size = big.element_size()
+        for lq in (1, 200):
+            q = normal(gen(5), 1, lq, 1, 128).to(kind)
+            o = torch.empty_like(q)
+            strides = (lq * 128, 128, 128, 0, pitch, 128, 0, pitch, 128, lq * 128, 128, 128)
+            pkg.op_cross_attention(q.data_ptr(), big.data_ptr(), big.data_ptr() + 128 * size, o.data_ptr(), element, 1, lq, rows, 1, 1, 128, strides=strides)
+            k, v = view[:, :128].reshape(1, rows, 1, 128), view[:, 128:].reshape(1, rows, 1, 128)
+            assert_within(o, *attend_want(q, k, v, torch.ones(1, rows, dtype=torch.bool, device="cuda"), 128 ** -0.5, element))
+        y = torch.empty(rows, 256, device="cuda", dtype=kind)
+        pkg.op_group_norm(big.data_ptr(), y.data_ptr(), element, 1, rows, 256, 8, None, None, 1e-5, "none", pitch, 0)
+        want, off = norm_want(view.reshape(1, rows, 256), 8, None, None, 1e-5, "none")
+        assert_within(y.view(1, rows, 256), want, off + U[element] * (want.abs() + off) + TINY[element])
+        positions = torch.arange(rows, device="cuda", dtype=torch.int32).view(rows, 1).contiguous()
+        want, mag = rotary_want(view.reshape(rows, 2, 128), positions, [64], 10000.0, False, False)
+        pkg.op_rotary_axes(big.data_ptr(), big.data_ptr(), element, rows, 2, 128, positions.data_ptr(), [64], strides=(pitch, 128, pitch, 128))
+        assert_within(view.reshape(rows, 2, 128), want, 10 * F * mag + U[element] * (want.abs() + 10 * F * mag) + TINY[element])
+        del big, view
+
+
+@pytest.mark.gpu
+def test_calls_at_once(pkg):
+    """Different calls in flight on several streams, and replays of two captured graphs at once, share nothing."""
+    def make(n):
+        lq, lk = ((1, 2000), (200, 700), (1500, 60), (40, 900))[n % 4]
+        element = ("bf16", "f32")[n // 4]
+        q, k, v = (normal(gen(10 * n + i), 2, l, 4, 64).to(KIND[element]) for i, l in enumerate((lq, lk, lk)))
+        x = normal(gen(n), 2, 3000 + n, 64).to(KIND[element])
+        return element, lq, lk, q, k, v, x, torch.empty_like(q), torch.empty_like(x)
+
+    def run(c, stream):
+        element, lq, lk, q, k, v, x, o, y = c
+        pkg.op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), element, 2, lq, lk, 4, 4, 64, stream=stream)
+        pkg.op_group_norm(x.data_ptr(), y.data_ptr(), element, 2, x.shape[1], 64, 8, None, None, 1e-5, "swish", stream=stream)
+
+    calls = [make(n) for n in range(8)]
+    for c in calls:
+        run(c, 0)
+    torch.cuda.synchronize()
+    alone = [(c[-2].clone(), c[-1].clone()) for c in calls]
+    for c in calls:
+        c[-2].zero_()
+        c[-1].zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for c, s in zip(calls, streams):
+            run(c, s.cuda_stream)
+    torch.cuda.synchronize()
+    for c, (o, y) in zip(calls, alone):
+        assert torch.equal(c[-2], o) and torch.equal(c[-1], y)
+    graphs = []
+    for c in calls[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(c, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+        c[-2].zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for c, (o, y) in zip(calls[:2], alone):
+        assert torch.equal(c[-2], o) and torch.equal(c[-1], y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,heads", [(200, 300, 2), (100, 300, 64), (2000, 100, 16)])
+def test_a_wait_that_runs_out_is_reported(pkg, monkeypatch, lq, lk, heads):
+    """NCNN_B200_TEST_STALL leaves the first block of keys unloaded and shortens the waits to 2 ms: the call's kernel gives up,
+    ncnn_b200_op_check_status says so once, and later calls are right."""
+    q, k, v = (normal(gen(n), 1, l, heads, 64).half() for n, l in ((0, lq), (1, lk), (2, lk)))
+    o = torch.empty_like(q)
+
+    def call():
+        pkg.op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), "f16", 1, lq, lk, heads, heads, 64)
+
+    pkg.op_check_status()
+    monkeypatch.setenv("NCNN_B200_TEST_STALL", "1")
+    call()
+    monkeypatch.delenv("NCNN_B200_TEST_STALL")
+    assert status_of(pkg.op_check_status) == 7
+    pkg.op_check_status()
+    call()
+    pkg.op_check_status()
+    assert_within(o, *attend_want(q, k, v, torch.ones(1, lk, dtype=torch.bool, device="cuda"), 0.125, "f16"))
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
