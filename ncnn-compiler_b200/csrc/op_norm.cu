@@ -72,6 +72,8 @@ constexpr int kNormSlots = V == 8 ? 12 : 16;  // pixels of a thread's ring (thre
 
 struct NormShape {
   int channels;       // of a cluster
+  int size, groups;   // channels of a group, groups of a cluster
+  int each;           // pixels of a CTA (the last ones may have fewer)
   int columns, rows;  // threads: columns of V channels, rows of pixels
   int slots;          // of a ring: kNormSlots, or fewer where no thread has as many pixels
 };
@@ -95,16 +97,16 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
   __shared__ Moments group_parts[kNormMostGroups];
   __shared__ float2 result[kNormMostGroups];
   Vec* ring = reinterpret_cast<Vec*>(norm_smem) + threadIdx.x;  // [slot][thread]
-  const int size = p.channels / p.groups, groups = s.channels / size;
+  const int size = s.size, groups = s.groups;
   const int ranks = gridDim.x, rank = blockIdx.x;
-  const int blocks = p.channels / s.channels;
-  const long long image = blockIdx.y / blocks;
-  const int c0 = static_cast<int>(blockIdx.y % blocks) * s.channels;
-  // this CTA's pixels, and this thread's
-  const int pixels = static_cast<int>(p.pixels), each = (pixels + ranks - 1) / ranks;
+  const long long image = blockIdx.z;
+  const int c0 = blockIdx.y * s.channels;
+  // this CTA's pixels, and this thread's: `longer` rows of threads have a pixel more
+  const int pixels = static_cast<int>(p.pixels), each = s.each;
   const int begin = static_cast<int>(min(static_cast<long long>(each) * rank, p.pixels)), here = min(each, pixels - begin);
-  const int column = threadIdx.x % s.columns, row = threadIdx.x / s.columns;
-  const int count = row < s.rows && row < here ? (here - row + s.rows - 1) / s.rows : 0;
+  const int row = static_cast<int>(threadIdx.x / static_cast<unsigned>(s.columns)), column = static_cast<int>(threadIdx.x) - row * s.columns;
+  const int whole_rows = here / s.rows, longer = here - whole_rows * s.rows;
+  const int count = row < s.rows ? whole_rows + (row < longer ? 1 : 0) : 0;
   const T* x = static_cast<const T*>(p.x) + (image * p.pixels + begin + row) * p.x_pitch + c0 + column * V;
   T* y = static_cast<T*>(p.y) + (image * p.pixels + begin + row) * p.y_pitch + c0 + column * V;
   const long long x_step = s.rows * p.x_pitch, y_step = s.rows * p.y_pitch;
@@ -173,11 +175,19 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
 #pragma unroll
     for (int v = 0; v < V; ++v) parts[row * s.channels + v * s.columns + column] = part[v];
   }
+  float scale[V], offset[V];  // asked for here, needed behind the statistics
+  int to_group = column * V / size, in_group = column * V - to_group * size;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = c0 + column * V + v;
+    const bool mine = row < s.rows;
+    scale[v] = p.gamma != nullptr && mine ? __ldg(p.gamma + c) : 1.0f;
+    offset[v] = p.beta != nullptr && mine ? __ldg(p.beta + c) : 0.0f;
+  }
   __syncthreads();
   // A warp to a group: lanes over its channels and as many rows as fit; the mean first, the deviations about it second.
   const int lane = threadIdx.x & 31;
   const int lane_rows = size < 32 ? 32 / size : 1, lane_row = size < 32 ? lane / size : 0, lane_channel = size < 32 ? lane - lane_row * size : lane;
-  const int whole_rows = here / s.rows, longer = here - whole_rows * s.rows;  // `longer` rows have a pixel more
   const int rows_in_use = min(s.rows, here);
   for (int g = threadIdx.x >> 5; g < groups; g += kNormThreads / 32) {
     auto over = [&](auto&& f) {
@@ -226,19 +236,16 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
   __syncthreads();
   // no CTA's shared memory goes while another reads it: said here, waited for at the end
   if (ranks > 1) cluster.barrier_arrive();
-  // fp32 keeps the mean apart: x - mean is exact where x is close to it.  A 16-bit x has steps of 2^-8 or 2^-11 of itself, so
-  // that maps which vary at all lie within some 2^12 deviations of their mean, and the one product's rounding (2^-24 of the
-  // mean) stays below that of the result.
-  constexpr bool kFold = sizeof(T) == 2;
-  float mean[kFold ? 1 : V], scale[V], offset[V];
+  float mean[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int c = column * V + v;
-    const float2 r = result[c / size];
-    scale[v] = r.y * (p.gamma != nullptr ? __ldg(p.gamma + c0 + c) : 1.0f);
-    offset[v] = p.beta != nullptr ? __ldg(p.beta + c0 + c) : 0.0f;
-    if (kFold) offset[v] = fmaf(-r.x, scale[v], offset[v]);
-    else mean[kFold ? 0 : v] = r.x;
+    const float2 r = row < s.rows ? result[to_group] : make_float2(0.0f, 0.0f);
+    mean[v] = r.x;
+    scale[v] *= r.y;
+    if (++in_group == size) {
+      in_group = 0;
+      ++to_group;
+    }
   }
   for (int g = steps - 1; g >= 0; --g) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
@@ -252,8 +259,9 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
 #pragma unroll
     for (int u = 0; u < kNormGroup; ++u)
       if (g * kNormGroup + u < count) {
+        // (x - mean is exact where x is close to the mean)
 #pragma unroll
-        for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(kFold ? op_get(at[u].e[v]) : op_get(at[u].e[v]) - mean[kFold ? 0 : v], scale[v], offset[v])));
+        for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(op_get(at[u].e[v]) - mean[v], scale[v], offset[v])));
         *reinterpret_cast<Vec*>(to + u * y_step) = at[u];
       }
   }
@@ -290,16 +298,20 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   const int size = p.channels / p.groups, sms = op_sm_count(device);
   NormShape s{};
   s.channels = take * size;
+  s.size = size;
+  s.groups = take;
   s.columns = s.channels / V;
   s.rows = kNormThreads / s.columns;
   const long long items = p.n * (p.groups / take);
-  // CTAs to an item: as many as the device holds, while each thread has four pixels
+  // CTAs to an item: two to an SM at most, while each thread has four pixels; a power of two (clusters of 9 or 13 leave SMs of a
+  // GPC idle: 8 maps of 64 x 64 x 320 18 us with 8, 22 with 9)
   int ranks = 1;
   while (ranks < 16 && items * ranks * 2 <= 2 * sms && p.pixels > kNormGroup * ranks * static_cast<long long>(s.rows)) ranks *= 2;
   const long long each = (p.pixels + ranks - 1) / ranks;
   constexpr int kSlot = static_cast<int>(kNormThreads * sizeof(T) * V);
   constexpr int kSmem = kNormSlots<V> * kSlot + kNormThreads * V * static_cast<int>(sizeof(Moments));
   static_assert(kSmem * (3) <= (220 << 10), "shared memory of the CTAs of an SM");
+  s.each = static_cast<int>(each);
   s.slots = static_cast<int>(std::min<long long>((each + s.rows - 1) / s.rows, kNormSlots<V>));
   const int smem = s.slots * kSlot + s.rows * s.channels * static_cast<int>(sizeof(Moments));
   auto kernel = k_group_norm<T, V, ACT>;
@@ -311,15 +323,14 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
       return op_launched("op_group_norm");
     if (device < 64) granted.fetch_or(bit, std::memory_order_acq_rel);
   }
-  // blockIdx.y holds 65535: more items go in several launches
-  const long long per_image = p.groups / take, images = std::max<long long>(1, 65535 / per_image);
+  const long long images = 65535;  // blockIdx.z holds that many: more go in several launches
   for (long long at = 0; at < p.n; at += images) {
     NormParams q = p;
     q.n = std::min(images, p.n - at);
     q.x = static_cast<const T*>(p.x) + at * p.pixels * p.x_pitch;
     q.y = static_cast<T*>(p.y) + at * p.pixels * p.y_pitch;
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3(ranks, static_cast<unsigned>(q.n * per_image));
+    c.gridDim = dim3(ranks, p.groups / take, static_cast<unsigned>(q.n));
     c.blockDim = dim3(kNormThreads);
     c.dynamicSmemBytes = smem;
     c.stream = st;
@@ -391,8 +402,8 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: a pitch is smaller than a pixel's channels");
     if (x == y && x_pitch != y_pitch) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: in place, both pitches have to be the same");
     if (n == 0 || pixels == 0) return NCNN_B200_STATUS_SUCCESS;
-    if (pixels > (1ll << 30) || pixels > (1ll << 40) / std::max(x_pitch, y_pitch) || n > (1ll << 40) / (pixels * std::max(x_pitch, y_pitch)) || n * groups > 0x7fffffffll)
-      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_group_norm: more than 2^30 pixels, 2^40 elements or 2^31 groups");
+    if (groups > 65535 || pixels > (1ll << 30) || pixels > (1ll << 40) / std::max(x_pitch, y_pitch) || n > (1ll << 40) / (pixels * std::max(x_pitch, y_pitch)) || n * groups > 0x7fffffffll)
+      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_group_norm: more than 2^30 pixels, 2^40 elements, 65535 groups of an image or 2^31 in all");
     std::string why;
     const int device = op_common_device(kOp, {x, y, gamma, beta}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
