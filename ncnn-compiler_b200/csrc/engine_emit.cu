@@ -1,6 +1,7 @@
 // Nodes -> kernel launches: every node of a plan becomes one Step (a closure that enqueues its kernel), and the
 // edges between the caller's CHW arrays and the channel-last arena.
 #include "engine_impl.h"
+#include "op_norm.h"
 
 namespace nb {
 
@@ -913,6 +914,16 @@ bool EngineImpl::emit_node(std::vector<Step>& steps, const Node& node, int64_t n
       else launch_plain(k_unary<1>, grid, 256, 0, st, in, out, count, up);
       return launch_ok();
     };
+    steps.push_back(std::move(s));
+    return true;
+  }
+  if (node.kind == N_NORM) {
+    const ActRef in = ref(node.in[0], n);
+    const long long pixels = static_cast<long long>(to.h) * to.w;
+    const int channels = to.c, groups = node.norm_groups, act = node.act, device = device_;
+    const float *gamma = node.d_scale, *beta = node.d_offset, eps = node.norm_eps;
+    s.kernel = "k_group_norm";
+    s.run = [=](cudaStream_t st) { return launch_group_norm(in, out, n, pixels, channels, groups, gamma, beta, eps, act, device, st); };
     steps.push_back(std::move(s));
     return true;
   }

@@ -23,7 +23,7 @@
 
 namespace nb {
 
-enum NodeKind { N_CONV, N_DW, N_IP, N_GEMM, N_POOL, N_BINARY, N_UNARY, N_RELAYOUT, N_SOFTMAX, N_CONCAT, N_REMAP, N_REDUCE, N_DECONV };
+enum NodeKind { N_CONV, N_DW, N_IP, N_GEMM, N_POOL, N_BINARY, N_UNARY, N_RELAYOUT, N_SOFTMAX, N_CONCAT, N_REMAP, N_REDUCE, N_DECONV, N_NORM };
 enum Impl { IMPL_NONE, IMPL_TC, IMPL_DIRECT };
 
 struct Tensor {
@@ -92,6 +92,8 @@ struct Node {
   std::vector<ConcatParams> concat;  // one per input
   RemapParams remap{};
   ReduceParams reduce{};
+  int norm_groups = 0;  // N_NORM: gamma and beta are un_scale and un_offset, the activation behind it `act`
+  float norm_eps = 0.0f;
   bool broadcast = false;  // N_BINARY whose operands differ in shape
   // N_CONV (tensor-core path) that writes straight into a channel Concat's result: its output
   // rows are `out_ld` channels long and start `out_ch_off` channels in (0 = dense, its own tensor)

@@ -1,5 +1,6 @@
 // ncnn layers -> nodes of the executor: one importer per layer type, with the checks of the reference's importers.
 #include "engine_impl.h"
+#include "op_norm.h"
 
 namespace nb {
 
@@ -964,6 +965,37 @@ bool EngineImpl::import_layers(std::string* err) {
         volatile float sm = scale * mean[c];
         n.un_scale[c] = scale;
         n.un_offset[c] = bias[c] - sm;
+      }
+      n.in = {in};
+      n.out = new_tensor(l.tops[0]);
+      Tensor& to = tensors_[n.out];
+      const std::string keep = to.name;
+      to = ti;
+      to.name = keep;
+      to.alias = -1;
+      to.is_input = false;
+      nodes_.push_back(std::move(n));
+    } else if (t == "GroupNorm") {
+      // not in the reference's importer: ncnn's layer on [c,h,w], statistics over each group's channels and all pixels
+      if (l.bottoms.size() != 1 || l.tops.size() != 1) return fail(err, where + "expects one input and one output");
+      const int in = by_name_.at(l.bottoms[0]);
+      const Tensor ti = tensors_[resolve(in)];
+      const int64_t groups = l.params.get_int(0, 1), ch = l.params.get_int(1, 0), affine = l.params.get_int(3, 1);
+      const float eps = l.params.get_float(2, 0.001f);
+      if (ti.i8 || ti.rank != 3 || ti.c != ch) return fail(err, where + "GroupNorm takes an f32 [c,h,w] tensor of its channel count");
+      if (groups <= 0 || groups > ch || ch % groups != 0) return fail(err, where + "channels must be a positive multiple of group");
+      if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(err, where + "eps must be finite and not negative");
+      if (!group_norm_fits(ti.c, static_cast<int>(groups))) return fail(err, where + "groups of so many channels are not supported");
+      if (affine == 1 && l.weights.size() != 2) return fail(err, where + "weights are missing (was a .bin supplied?)");
+      Node n;
+      n.kind = N_NORM;
+      n.name = l.name;
+      n.type = t;
+      n.norm_groups = static_cast<int>(groups);
+      n.norm_eps = eps;
+      if (affine == 1) {
+        n.un_scale = l.weights[0].as_f32();
+        n.un_offset = l.weights[1].as_f32();
       }
       n.in = {in};
       n.out = new_tensor(l.tops[0]);

@@ -70,12 +70,13 @@ void EngineImpl::fuse() {
       Node& p = nodes_[pj];
       const bool contraction = p.kind == N_CONV || p.kind == N_DW || p.kind == N_IP;
       const bool binary = p.kind == N_BINARY;
-      if (!(contraction || binary)) continue;
-      if (contraction && p.act != ACT_NONE) continue;
+      const bool norm = p.kind == N_NORM && (u.un.act == ACT_RELU || u.un.act == ACT_SWISH || u.un.act == ACT_GELU);
+      if (!(contraction || binary || norm)) continue;
+      if ((contraction || norm) && p.act != ACT_NONE) continue;
       if (binary && p.bin.act != ACT_NONE) continue;
       if (tensors_[src].i8 && u.un.act != ACT_RELU) continue;
       if (p.kind == N_GEMM) continue;
-      if (contraction) {
+      if (contraction || norm) {
         p.act = u.un.act;
         p.act_a = u.un.act_a;
         p.act_b = u.un.act_b;

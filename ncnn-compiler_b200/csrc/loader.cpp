@@ -629,6 +629,17 @@ bool load_layer_weights(LayerDef& l, BinCursor& c, std::string* err) {
       if (!push(l, c, ch, 1, {ch}, name, err)) return false;
     return true;
   }
+  if (t == "GroupNorm") {  // not in the reference; ncnn's own layer: 0=group 1=channels 2=eps 3=affine
+    int64_t ch, affine;
+    if (!int_param(l.params, 1, 0, "channels", &ch, err) || !int_param(l.params, 3, 1, "affine", &affine, err)) return false;
+    if (ch <= 0 || (affine != 0 && affine != 1)) {
+      *err = "GroupNorm channels must be positive and affine 0 or 1";
+      return false;
+    }
+    for (const char* name : {"GroupNorm gamma", "GroupNorm beta"})
+      if (affine == 1 && !push(l, c, ch, 1, {ch}, name, err)) return false;
+    return true;
+  }
   if (t == "Quantize") {
     static const char* n[] = {"scale"};
     return load_counts(l, c, {{0, 1}}, n, false, err);
@@ -682,7 +693,7 @@ bool load_layer_weights(LayerDef& l, BinCursor& c, std::string* err) {
   // their payload cannot be skipped reliably, so the file is rejected.
   for (const char* w : {"MemoryData", "LayerNorm", "Embed",
                         "MultiHeadAttention", "Scale", "DeconvolutionDepthWise", "InstanceNorm",
-                        "GroupNorm", "RNN", "LSTM", "GRU"}) {
+                        "RNN", "LSTM", "GRU"}) {
     if (t == w) {
       *err = "layer type " + t + " carries weights and is not supported by this runtime";
       return false;

@@ -6,6 +6,7 @@
 #include <cooperative_groups.h>
 
 #include "op_common.cuh"
+#include "op_norm.h"
 
 namespace nb {
 namespace {
@@ -17,6 +18,8 @@ struct NormParams {
   int channels, groups;
   const float *gamma, *beta;
   float eps;
+  ActRef in, out;  // a graph's tensors, in place of x and y
+  long long first_image;
 };
 
 template <int ACT>
@@ -82,13 +85,19 @@ struct Moments {
   float mean, m2;
 };
 
+__device__ __forceinline__ void graph_load(const ActRef& a, long long i, OpVec<float, 4>& v) { *reinterpret_cast<float4*>(&v) = act_load4(a, i); }
+__device__ __forceinline__ void graph_load(const ActRef& a, long long i, OpVec<float, 1>& v) { v.e[0] = act_load(a, i); }
+__device__ __forceinline__ void graph_store(const ActRef& a, long long i, const OpVec<float, 4>& v) { act_store4(a, i, *reinterpret_cast<const float4*>(&v)); }
+__device__ __forceinline__ void graph_store(const ActRef& a, long long i, const OpVec<float, 1>& v) { act_store(a, i, v.e[0]); }
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
   else if constexpr (BYTES >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 
-template <class T, int V, int ACT>
+// GRAPH: the tensors of a loaded graph, in whatever format their other readers and writers want.
+template <class T, int V, int ACT, bool GRAPH>
 __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_constant__ NormParams p, const __grid_constant__ NormShape s) {
   namespace cg = cooperative_groups;
   using Vec = OpVec<T, V>;
@@ -110,13 +119,20 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
   const T* x = static_cast<const T*>(p.x) + (image * p.pixels + begin + row) * p.x_pitch + c0 + column * V;
   T* y = static_cast<T*>(p.y) + (image * p.pixels + begin + row) * p.y_pitch + c0 + column * V;
   const long long x_step = s.rows * p.x_pitch, y_step = s.rows * p.y_pitch;
+  const long long element = GRAPH ? ((p.first_image + image) * p.pixels + begin + row) * p.x_pitch + c0 + column * V : 0;
   const int steps = (count + kNormGroup - 1) / kNormGroup;
   // four pixels of this thread on their way to their slots (2-byte pieces, which cp.async does not take: through registers)
   auto request = [&](int step) {
     if (step >= 0 && step < steps) {
       const T* from = x + step * kNormGroup * x_step;
       Vec* to = ring + step * kNormGroup % kNormSlots<V> * kNormThreads;
-      if constexpr (sizeof(Vec) >= 4) {
+      if (GRAPH && p.in.fmt != FMT_F32) {
+        if constexpr (GRAPH) {
+#pragma unroll
+          for (int u = 0; u < kNormGroup; ++u)
+            if (step * kNormGroup + u < count) graph_load(p.in, element + (step * kNormGroup + u) * x_step, to[u * kNormThreads]);
+        }
+      } else if constexpr (sizeof(Vec) >= 4) {
 #pragma unroll
         for (int u = 0; u < kNormGroup; ++u)
           if (step * kNormGroup + u < count) copy_async<sizeof(Vec)>(static_cast<uint32_t>(__cvta_generic_to_shared(to + u * kNormThreads)), from + u * x_step);
@@ -262,7 +278,8 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
         // (x - mean is exact where x is close to the mean)
 #pragma unroll
         for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(op_get(at[u].e[v]) - mean[v], scale[v], offset[v])));
-        *reinterpret_cast<Vec*>(to + u * y_step) = at[u];
+        if constexpr (GRAPH) graph_store(p.out, element + (g * kNormGroup + u) * x_step, at[u]);
+        else *reinterpret_cast<Vec*>(to + u * y_step) = at[u];
       }
   }
   if (ranks > 1) cluster.barrier_wait();
@@ -293,7 +310,7 @@ __global__ void __launch_bounds__(kNormThreads) k_group_norm_wide(const __grid_c
   }
 }
 
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool GRAPH>
 int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   const int size = p.channels / p.groups, sms = op_sm_count(device);
   NormShape s{};
@@ -302,7 +319,8 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   s.groups = take;
   s.columns = s.channels / V;
   s.rows = kNormThreads / s.columns;
-  const long long items = p.n * (p.groups / take);
+  // (a graph's images are cut alike whatever the batch: a batch equals its images run alone, bit for bit)
+  const long long items = (GRAPH ? 1 : p.n) * (p.groups / take);
   // CTAs to an item: two to an SM at most, while each thread has four pixels; a power of two (clusters of 9 or 13 leave SMs of a
   // GPC idle: 8 maps of 64 x 64 x 320 18 us with 8, 22 with 9)
   int ranks = 1;
@@ -314,7 +332,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   s.each = static_cast<int>(each);
   s.slots = static_cast<int>(std::min<long long>((each + s.rows - 1) / s.rows, kNormSlots<V>));
   const int smem = s.slots * kSlot + s.rows * s.channels * static_cast<int>(sizeof(Moments));
-  auto kernel = k_group_norm<T, V, ACT>;
+  auto kernel = k_group_norm<T, V, ACT, GRAPH>;
   static std::atomic<uint64_t> granted{0};
   const uint64_t bit = 1ull << (device & 63);
   if (!(granted.load(std::memory_order_acquire) & bit)) {
@@ -329,6 +347,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
     q.n = std::min(images, p.n - at);
     q.x = static_cast<const T*>(p.x) + at * p.pixels * p.x_pitch;
     q.y = static_cast<T*>(p.y) + at * p.pixels * p.y_pitch;
+    q.first_image = at;
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(ranks, p.groups / take, static_cast<unsigned>(q.n));
     c.blockDim = dim3(kNormThreads);
@@ -345,7 +364,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   return op_launched("op_group_norm");
 }
 
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool GRAPH>
 int launch_act(const NormParams& p, int device, cudaStream_t st) {
   const int size = p.channels / p.groups, sms = op_sm_count(device);
   // The fewest groups whose channels are whole accesses and 128 bytes of a pixel; 64 to 16 where clusters of 16 CTAs to 128
@@ -362,25 +381,41 @@ int launch_act(const NormParams& p, int device, cudaStream_t st) {
     return take;
   };
   int take = pick(128);
-  for (int bytes = 64; bytes >= 16 && take > 0 && p.n * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
+  for (int bytes = 64; bytes >= 16 && take > 0 && (GRAPH ? 1 : p.n) * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
   if (take == 0) {
+    if (GRAPH) return NCNN_B200_STATUS_CONSTRAINT_VIOLATION;  // (the import refuses such groups)
     k_group_norm_wide<T, ACT><<<static_cast<unsigned>(p.n * p.groups), kNormThreads, 0, st>>>(p);
     return op_launched("op_group_norm");
   }
-  return launch_shape<T, V, ACT>(p, take, device, st);
+  return launch_shape<T, V, ACT, GRAPH>(p, take, device, st);
 }
 
-template <class T, int V>
+template <class T, int V, bool GRAPH = false>
 int launch(const NormParams& p, int activation, int device, cudaStream_t st) {
   switch (activation) {
-    case NCNN_B200_ACT_RELU: return launch_act<T, V, NCNN_B200_ACT_RELU>(p, device, st);
-    case NCNN_B200_ACT_SWISH: return launch_act<T, V, NCNN_B200_ACT_SWISH>(p, device, st);
-    case NCNN_B200_ACT_GELU: return launch_act<T, V, NCNN_B200_ACT_GELU>(p, device, st);
-    default: return launch_act<T, V, NCNN_B200_ACT_NONE>(p, device, st);
+    case NCNN_B200_ACT_RELU: return launch_act<T, V, NCNN_B200_ACT_RELU, GRAPH>(p, device, st);
+    case NCNN_B200_ACT_SWISH: return launch_act<T, V, NCNN_B200_ACT_SWISH, GRAPH>(p, device, st);
+    case NCNN_B200_ACT_GELU: return launch_act<T, V, NCNN_B200_ACT_GELU, GRAPH>(p, device, st);
+    default: return launch_act<T, V, NCNN_B200_ACT_NONE, GRAPH>(p, device, st);
   }
 }
 
 }  // namespace
+
+bool group_norm_fits(int channels, int groups) {
+  const int size = channels / groups, v = channels % 4 == 0 ? 4 : 1;
+  int take = 1;  // groups that are whole accesses together
+  while (take <= groups && (groups % take != 0 || take * size % v != 0)) ++take;
+  return take <= kNormMostGroups && take * size / v <= kNormThreads;
+}
+
+cudaError_t launch_group_norm(const ActRef& in, const ActRef& out, long long images, long long pixels, int channels, int groups, const float* gamma,
+                              const float* beta, float eps, int act, int device, cudaStream_t st) {
+  NormParams p{in.p0, out.p0, images, pixels, channels, channels, channels, groups, gamma, beta, eps, in, out, 0};
+  const int status = channels % 4 == 0 ? launch<float, 4, true>(p, act, device, st) : launch<float, 1, true>(p, act, device, st);
+  return status == NCNN_B200_STATUS_SUCCESS ? cudaSuccess : cudaErrorLaunchFailure;
+}
+
 }  // namespace nb
 
 extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int64_t n, int64_t pixels, int32_t channels, int32_t groups,
@@ -408,7 +443,7 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
     const int device = op_common_device(kOp, {x, y, gamma, beta}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
     DeviceGuard guard(device);
-    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, gamma, beta, eps};
+    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, gamma, beta, eps, {}, {}, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // the widest access that every pixel's and every cluster's channels start and end with
     auto whole = [&](int v) {

@@ -160,6 +160,31 @@ def residual_block(prefix, seed=600, h=16, w=16, c=64, cout=96, k=3):
     return wr.save(prefix)
 
 
+def group_norm_block(prefix, seed=620, h=16, w=16, c=64, cout=96, groups=32, act="Swish", eps=1e-5, affine=True):
+    """The residual block of an image generator: Input -> [GroupNorm -> act -> 3x3 conv to `cout` -> GroupNorm -> act -> 3x3
+    conv] + a 1x1 conv of the input.  A group norm here reads the block's input (which a convolution reads, too) or a
+    convolution's plain result, and writes a convolution's operand."""
+    net = _Net(seed)
+    wr = net.w
+
+    def norm(name, bottom, top, ch):
+        wr.layer("GroupNorm", name, [bottom], [top + "_n"], f"0={groups} 1={ch} 2={eps:e} 3={1 if affine else 0}")
+        if affine:
+            wr.f32(1 + 0.3 * net.rng.standard_normal(ch))
+            wr.f32(0.3 * net.rng.standard_normal(ch))
+        wr.layer(act, name + "_act", [top + "_n"], [top], "0=0" if act == "GELU" else "")
+
+    wr.layer("Input", "input", [], ["data"], f"0={w} 1={h} 2={c}")
+    wr.layer("Split", "split", ["data"], ["a", "b"])
+    norm("norm1", "a", "n1", c)
+    net.conv("conv1", "n1", "c1", c, cout, 3, 1, 1, act=0, zero_bias=False)
+    norm("norm2", "c1", "n2", cout)
+    net.conv("conv2", "n2", "c2", cout, cout, 3, 1, 1, act=0, zero_bias=False)
+    net.conv("skip", "b", "s", c, cout, 1, 1, 0, act=0, zero_bias=False)
+    wr.layer("Eltwise", "add", ["c2", "s"], ["output"], "0=1")
+    return wr.save(prefix)
+
+
 def fire_classifier(prefix, seed=700, size=32, classes=10, act="ReLU"):
     """SqueezeNet-style stand-in for the operators next to the hot path: stem convolution, two
     fire modules (1x1 squeeze, 1x1 and 3x3 expand joined by a channel Concat), Dropout, a 1x1

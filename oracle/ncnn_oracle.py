@@ -223,6 +223,9 @@ def _load_weights(layer: Layer, b: _Bin):
     elif t == "BatchNorm":
         for _ in range(4):
             layer.weights.append(b.read(layer.geti(0), 1))
+    elif t == "GroupNorm":  # not in the reference: ncnn's layer, gamma and beta where affine (default 1)
+        for _ in range(2 if layer.geti(3, 1) else 0):
+            layer.weights.append(b.read(layer.geti(1), 1))
     elif t == "Gemm":
         # graph.cpp:1858-1926: constant B [N,K] (transB=1), optional row bias C, int8 scale
         if layer.geti(5) and layer.geti(6):
@@ -742,6 +745,20 @@ def op_softmax(layer: Layer, x):
     return (e * (F32(1) / s).astype(F32)).astype(F32)
 
 
+def op_group_norm(layer: Layer, x):
+    """ncnn's GroupNorm on [h][w][c] (the reference has none): (x - mean) / sqrt(var + eps) * gamma + beta over the pixels and
+    channels of a group, evaluated in 64 bits and rounded once."""
+    groups, ch, eps = layer.geti(0, 1), layer.geti(1), layer.getf(2, 0.001)
+    if x.ndim != 3 or x.shape[2] != ch or groups <= 0 or ch % groups:
+        raise ValueError("GroupNorm takes a [c,h,w] tensor of its channel count, a multiple of its groups")
+    t = x.astype(np.float64).reshape(-1, groups, ch // groups)
+    mean = t.mean((0, 2), keepdims=True)
+    t = ((t - mean) / np.sqrt(((t - mean) ** 2).mean((0, 2), keepdims=True) + eps)).reshape(x.shape)
+    if layer.weights:
+        t = t * layer.weights[0].astype(np.float64) + layer.weights[1].astype(np.float64)
+    return t.astype(F32)
+
+
 def op_concat(layer: Layer, ins):
     """import_concat (ImportTensor.cpp:48-96) + ConvertConcat (NCNNToTosa.cpp:2012-2045)."""
     if len(ins) < 2:
@@ -995,6 +1012,8 @@ class Model:
                 out = op_dropout(l, ins[0])
             elif t == "Softmax":
                 out = op_softmax(l, ins[0])
+            elif t == "GroupNorm":
+                out = op_group_norm(l, ins[0])
             elif t == "Concat":
                 out = op_concat(l, ins)
             elif t == "UnaryOp":
