@@ -15,6 +15,7 @@
 #include <sstream>
 
 #include "conv_f32.cuh"
+#include "device_guard.h"
 #include "host_stage.h"
 #include "ip_rows.cuh"
 #include "kernels.cuh"
@@ -222,27 +223,6 @@ inline int host_quantize(float x, float s) {
   r = std::max(std::min(r, 127.0f), -127.0f);
   return static_cast<int>(r);
 }
-
-
-// Makes the model's device current for the duration of a call and puts the caller's device back:
-// a process may hold one handle per GPU and call them in any order from one thread.
-struct DeviceGuard {
-  int previous = -1;
-  bool switched = false;
-  explicit DeviceGuard(int device) {
-    if (device < 0) return;
-    if (cudaGetDevice(&previous) != cudaSuccess) {
-      previous = -1;
-      cudaGetLastError();
-    }
-    if (previous != device) switched = cudaSetDevice(device) == cudaSuccess && previous >= 0;
-  }
-  ~DeviceGuard() {
-    if (switched) cudaSetDevice(previous);
-  }
-  DeviceGuard(const DeviceGuard&) = delete;
-  DeviceGuard& operator=(const DeviceGuard&) = delete;
-};
 
 class EngineImpl {
  public:

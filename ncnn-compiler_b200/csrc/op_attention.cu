@@ -376,8 +376,14 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     }
     op_by_type(type, [&](auto t) {
       using T = decltype(t);
-      if (rows_of(p, 4, sizeof(T))) attend_f32<T, true>(p, device, sms, st);
-      else attend_f32<T, false>(p, device, sms, st);
+      // (16-bit rows come here when they are not aligned: element by element)
+      if constexpr (sizeof(T) == 4) {
+        if (rows_of(p, 4, sizeof(T))) {
+          attend_f32<T, true>(p, device, sms, st);
+          return 0;
+        }
+      }
+      attend_f32<T, false>(p, device, sms, st);
       return 0;
     });
     return op_launched(kOp);

@@ -3,8 +3,11 @@
 
 #include "../../include/ncnn_b200.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <exception>
+#include <initializer_list>
 #include <string>
 
 #include <cuda.h>
@@ -12,7 +15,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include "engine_impl.h"  // DeviceGuard
+#include "device_guard.h"
 
 namespace nb {
 

@@ -17,14 +17,16 @@ struct NormParams {
   long long n, pixels, x_pitch, y_pitch;
   int channels, groups;
   const float *gamma, *beta;
-  float eps;
-  ActRef in, out;  // a graph's tensors, in place of x and y
+  float eps, floor;
+  ActRef in, out;  // fp32: x and y, or a graph's tensors
   long long first_image;
+  int by_image;  // cut images alike whatever their number
 };
 
+// No activation and ReLU are one kernel: the line above a floor of minus infinity or 0.
 template <int ACT>
-__device__ __forceinline__ float norm_act(float y) {
-  if (ACT == NCNN_B200_ACT_RELU) return y < 0.0f ? 0.0f : y;  // (a NaN stays one)
+__device__ __forceinline__ float norm_act(float y, float floor) {
+  if (ACT == NCNN_B200_ACT_NONE) return y < floor ? floor : y;  // (a NaN stays one)
   if (ACT == NCNN_B200_ACT_SWISH) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y * -1.44269504088896340736f));
@@ -96,11 +98,12 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
   else if constexpr (BYTES >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 
-// GRAPH: the tensors of a loaded graph, in whatever format their other readers and writers want.
-template <class T, int V, int ACT, bool GRAPH>
+// fp32 tensors are those of a loaded graph, too, in whatever format their other readers and writers want.
+template <class T, int V, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_constant__ NormParams p, const __grid_constant__ NormShape s) {
   namespace cg = cooperative_groups;
   using Vec = OpVec<T, V>;
+  constexpr bool GRAPH = sizeof(T) == 4;
   extern __shared__ __align__(16) uint8_t norm_smem[];
   // the CTA's, and the cluster's mean and 1 / sqrt(variance + eps), of each group
   __shared__ Moments group_parts[kNormMostGroups];
@@ -119,7 +122,9 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
   const T* x = static_cast<const T*>(p.x) + (image * p.pixels + begin + row) * p.x_pitch + c0 + column * V;
   T* y = static_cast<T*>(p.y) + (image * p.pixels + begin + row) * p.y_pitch + c0 + column * V;
   const long long x_step = s.rows * p.x_pitch, y_step = s.rows * p.y_pitch;
-  const long long element = GRAPH ? ((p.first_image + image) * p.pixels + begin + row) * p.x_pitch + c0 + column * V : 0;
+  // (fp32) elements from the tensors' starts
+  const long long pixel0 = GRAPH ? (p.first_image + image) * p.pixels + begin + row : 0;
+  const long long x_element = GRAPH ? pixel0 * p.x_pitch + c0 + column * V : 0, y_element = GRAPH ? pixel0 * p.y_pitch + c0 + column * V : 0;
   const int steps = (count + kNormGroup - 1) / kNormGroup;
   // four pixels of this thread on their way to their slots (2-byte pieces, which cp.async does not take: through registers)
   auto request = [&](int step) {
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
         if constexpr (GRAPH) {
 #pragma unroll
           for (int u = 0; u < kNormGroup; ++u)
-            if (step * kNormGroup + u < count) graph_load(p.in, element + (step * kNormGroup + u) * x_step, to[u * kNormThreads]);
+            if (step * kNormGroup + u < count) graph_load(p.in, x_element + (step * kNormGroup + u) * x_step, to[u * kNormThreads]);
         }
       } else if constexpr (sizeof(Vec) >= 4) {
 #pragma unroll
@@ -277,8 +282,8 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
       if (g * kNormGroup + u < count) {
         // (x - mean is exact where x is close to the mean)
 #pragma unroll
-        for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(op_get(at[u].e[v]) - mean[v], scale[v], offset[v])));
-        if constexpr (GRAPH) graph_store(p.out, element + (g * kNormGroup + u) * x_step, at[u]);
+        for (int v = 0; v < V; ++v) at[u].e[v] = op_put<T>(norm_act<ACT>(fmaf(op_get(at[u].e[v]) - mean[v], scale[v], offset[v]), p.floor));
+        if constexpr (GRAPH) graph_store(p.out, y_element + (g * kNormGroup + u) * y_step, at[u]);
         else *reinterpret_cast<Vec*>(to + u * y_step) = at[u];
       }
   }
@@ -306,11 +311,11 @@ __global__ void __launch_bounds__(kNormThreads) k_group_norm_wide(const __grid_c
   for (long long i = threadIdx.x; i < count; i += kNormThreads) {
     const int c = static_cast<int>(i % size);
     const float v = fmaf((op_get(x[i / size * p.x_pitch + c]) - mean) * scale, p.gamma ? p.gamma[c0 + c] : 1.0f, p.beta ? p.beta[c0 + c] : 0.0f);
-    y[i / size * p.y_pitch + c] = op_put<T>(norm_act<ACT>(v));
+    y[i / size * p.y_pitch + c] = op_put<T>(norm_act<ACT>(v, p.floor));
   }
 }
 
-template <class T, int V, int ACT, bool GRAPH>
+template <class T, int V, int ACT>
 int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   const int size = p.channels / p.groups, sms = op_sm_count(device);
   NormShape s{};
@@ -320,7 +325,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   s.columns = s.channels / V;
   s.rows = kNormThreads / s.columns;
   // (a graph's images are cut alike whatever the batch: a batch equals its images run alone, bit for bit)
-  const long long items = (GRAPH ? 1 : p.n) * (p.groups / take);
+  const long long items = (p.by_image ? 1 : p.n) * (p.groups / take);
   // CTAs to an item: two to an SM at most, while each thread has four pixels; a power of two (clusters of 9 or 13 leave SMs of a
   // GPC idle: 8 maps of 64 x 64 x 320 18 us with 8, 22 with 9)
   int ranks = 1;
@@ -332,7 +337,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   s.each = static_cast<int>(each);
   s.slots = static_cast<int>(std::min<long long>((each + s.rows - 1) / s.rows, kNormSlots<V>));
   const int smem = s.slots * kSlot + s.rows * s.channels * static_cast<int>(sizeof(Moments));
-  auto kernel = k_group_norm<T, V, ACT, GRAPH>;
+  auto kernel = k_group_norm<T, V, ACT>;
   static std::atomic<uint64_t> granted{0};
   const uint64_t bit = 1ull << (device & 63);
   if (!(granted.load(std::memory_order_acquire) & bit)) {
@@ -364,7 +369,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   return op_launched("op_group_norm");
 }
 
-template <class T, int V, int ACT, bool GRAPH>
+template <class T, int V, int ACT>
 int launch_act(const NormParams& p, int device, cudaStream_t st) {
   const int size = p.channels / p.groups, sms = op_sm_count(device);
   // The fewest groups whose channels are whole accesses and 128 bytes of a pixel; 64 to 16 where clusters of 16 CTAs to 128
@@ -381,22 +386,22 @@ int launch_act(const NormParams& p, int device, cudaStream_t st) {
     return take;
   };
   int take = pick(128);
-  for (int bytes = 64; bytes >= 16 && take > 0 && (GRAPH ? 1 : p.n) * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
+  for (int bytes = 64; bytes >= 16 && take > 0 && (p.by_image ? 1 : p.n) * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
   if (take == 0) {
-    if (GRAPH) return NCNN_B200_STATUS_CONSTRAINT_VIOLATION;  // (the import refuses such groups)
+    if (p.by_image) return NCNN_B200_STATUS_CONSTRAINT_VIOLATION;  // (the import refuses such groups)
     k_group_norm_wide<T, ACT><<<static_cast<unsigned>(p.n * p.groups), kNormThreads, 0, st>>>(p);
     return op_launched("op_group_norm");
   }
-  return launch_shape<T, V, ACT, GRAPH>(p, take, device, st);
+  return launch_shape<T, V, ACT>(p, take, device, st);
 }
 
-template <class T, int V, bool GRAPH = false>
-int launch(const NormParams& p, int activation, int device, cudaStream_t st) {
+template <class T, int V>
+int launch(NormParams p, int activation, int device, cudaStream_t st) {
+  p.floor = activation == NCNN_B200_ACT_RELU ? 0.0f : -INFINITY;
   switch (activation) {
-    case NCNN_B200_ACT_RELU: return launch_act<T, V, NCNN_B200_ACT_RELU, GRAPH>(p, device, st);
-    case NCNN_B200_ACT_SWISH: return launch_act<T, V, NCNN_B200_ACT_SWISH, GRAPH>(p, device, st);
-    case NCNN_B200_ACT_GELU: return launch_act<T, V, NCNN_B200_ACT_GELU, GRAPH>(p, device, st);
-    default: return launch_act<T, V, NCNN_B200_ACT_NONE, GRAPH>(p, device, st);
+    case NCNN_B200_ACT_SWISH: return launch_act<T, V, NCNN_B200_ACT_SWISH>(p, device, st);
+    case NCNN_B200_ACT_GELU: return launch_act<T, V, NCNN_B200_ACT_GELU>(p, device, st);
+    default: return launch_act<T, V, NCNN_B200_ACT_NONE>(p, device, st);
   }
 }
 
@@ -411,8 +416,8 @@ bool group_norm_fits(int channels, int groups) {
 
 cudaError_t launch_group_norm(const ActRef& in, const ActRef& out, long long images, long long pixels, int channels, int groups, const float* gamma,
                               const float* beta, float eps, int act, int device, cudaStream_t st) {
-  NormParams p{in.p0, out.p0, images, pixels, channels, channels, channels, groups, gamma, beta, eps, in, out, 0};
-  const int status = channels % 4 == 0 ? launch<float, 4, true>(p, act, device, st) : launch<float, 1, true>(p, act, device, st);
+  NormParams p{in.p0, out.p0, images, pixels, channels, channels, channels, groups, gamma, beta, eps, 0.0f, in, out, 0, 1};
+  const int status = channels % 4 == 0 ? launch<float, 4>(p, act, device, st) : launch<float, 1>(p, act, device, st);
   return status == NCNN_B200_STATUS_SUCCESS ? cudaSuccess : cudaErrorLaunchFailure;
 }
 
@@ -443,7 +448,7 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
     const int device = op_common_device(kOp, {x, y, gamma, beta}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
     DeviceGuard guard(device);
-    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, gamma, beta, eps, {}, {}, 0};
+    NormParams p{x, y, n, pixels, x_pitch, y_pitch, channels, groups, gamma, beta, eps, 0.0f, {}, {}, 0, 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // the widest access that every pixel's and every cluster's channels start and end with
     auto whole = [&](int v) {
@@ -454,8 +459,13 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
     const int status = op_by_type(type, [&](auto t) {
       using T = decltype(t);
       constexpr int V = 16 / sizeof(T);
+      if constexpr (sizeof(T) == 4) {
+        p.in.p0 = const_cast<float*>(static_cast<const float*>(x));
+        p.out.p0 = static_cast<float*>(y);
+      }
       if (whole(V)) return launch<T, V>(p, activation, device, st);
-      if (whole(2)) return launch<T, 2>(p, activation, device, st);
+      if constexpr (sizeof(T) == 2)
+        if (whole(2)) return launch<T, 2>(p, activation, device, st);
       return launch<T, 1>(p, activation, device, st);
     });
     return status;

@@ -1,7 +1,7 @@
 // Group norm as the layers of a loaded graph have it (op_norm.cu).
 #pragma once
 
-#include "kernels.cuh"
+#include "act_ref.cuh"
 
 namespace nb {
 
