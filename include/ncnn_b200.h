@@ -204,7 +204,8 @@ int ncnn_b200_op_requantize(const int32_t *x, int8_t *y, int64_t count, int64_t 
 /* ---- Operators on device arrays around a network's convolutions: normalisation of feature maps, positions and attention
  * of their tokens.  The reference's importer has no GroupNorm or RotaryEmbed; its MultiHeadAttention and SDPA lowerings
  * (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:3859-4669) compute the same attention for one image.
- * All arrays live on one device (which need not be the current one) in memory that kernels reach; a call is asynchronous on
+ * All arrays live in device (or managed) memory of one device, which need not be the current one, and start at multiples of
+ * their elements' size; a call is asynchronous on
  * `stream` (a cudaStream_t of that device as void*), allocates nothing, keeps nothing between calls, may be captured into a
  * graph, and any number of calls may be in flight.  A refused call launches nothing; ncnn_b200_last_error(NULL) says why.
  * Element types are those of x and y, q, k, v and o; sums and statistics are held in 32 bits, results rounded once. */

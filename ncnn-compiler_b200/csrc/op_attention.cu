@@ -70,7 +70,7 @@ bool rows_of(const AttendParams& p, int count, int size) {
 template <class K>
 cudaError_t grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted, int registers = 0) {
   const uint64_t bit = 1ull << (device & 63);
-  if (granted->load(std::memory_order_acquire) & bit) return cudaSuccess;
+  if (device < 64 && (granted->load(std::memory_order_acquire) & bit)) return cudaSuccess;
   if (registers > 0) {
     cudaFuncAttributes a{};
     if (const cudaError_t e = cudaFuncGetAttributes(&a, kernel); e != cudaSuccess) return e;
@@ -309,6 +309,9 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     if (batch == 0 || lq == 0) return NCNN_B200_STATUS_SUCCESS;
     if (q == nullptr || o == nullptr || (lk > 0 && (k == nullptr || v == nullptr)))
       return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_cross_attention: NULL argument");
+    const int size = op_elem_bytes(type);
+    if (!op_starts(q, size) || !op_starts(k, size) || !op_starts(v, size) || !op_starts(o, size) || !op_starts(kv_lens, 4))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_cross_attention: an array does not start at a multiple of its elements' size");
     if (o == q || o == k || o == v) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_cross_attention: the result must not lie over an input");
     AttendParams p{};
     p.q = q;

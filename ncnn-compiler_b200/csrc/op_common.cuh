@@ -72,6 +72,9 @@ inline int op_device_of(const void* p) {
   return a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged ? a.device : -1;
 }
 
+// Whether an array starts where its elements can: a kernel would fault on one that does not.
+inline bool op_starts(const void* p, int elem_bytes) { return reinterpret_cast<uintptr_t>(p) % elem_bytes == 0; }
+
 // Every array of a call on one device: that device, or a message.
 inline int op_common_device(const char* op, std::initializer_list<const void*> arrays, std::string* why) {
   int device = -1;

@@ -340,7 +340,7 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   auto kernel = k_group_norm<T, V, ACT>;
   static std::atomic<uint64_t> granted{0};
   const uint64_t bit = 1ull << (device & 63);
-  if (!(granted.load(std::memory_order_acquire) & bit)) {
+  if (device >= 64 || !(granted.load(std::memory_order_acquire) & bit)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return op_launched("op_group_norm");
@@ -441,6 +441,8 @@ extern "C" int ncnn_b200_op_group_norm(const void* x, void* y, int32_t type, int
     if (x_pitch < channels || y_pitch < channels)
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: a pitch is smaller than a pixel's channels");
     if (x == y && x_pitch != y_pitch) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: in place, both pitches have to be the same");
+    if (!op_starts(x, op_elem_bytes(type)) || !op_starts(y, op_elem_bytes(type)) || !op_starts(gamma, 4) || !op_starts(beta, 4))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_group_norm: an array does not start at a multiple of its elements' size");
     if (n == 0 || pixels == 0) return NCNN_B200_STATUS_SUCCESS;
     if (groups > 65535 || pixels > (1ll << 30) || pixels > (1ll << 40) / std::max(x_pitch, y_pitch) || n > (1ll << 40) / (pixels * std::max(x_pitch, y_pitch)) || n * groups > 0x7fffffffll)
       return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_group_norm: more than 2^30 pixels, 2^40 elements, 65535 groups of an image or 2^31 in all");

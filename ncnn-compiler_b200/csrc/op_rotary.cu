@@ -142,6 +142,8 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
     if (x == nullptr || y == nullptr || positions == nullptr || sections == nullptr)
       return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_rotary_axes: NULL argument");
     if (!op_type_ok(type)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: unknown element type");
+    if (!op_starts(x, op_elem_bytes(type)) || !op_starts(y, op_elem_bytes(type)) || !op_starts(positions, 4))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: an array does not start at a multiple of its elements' size");
     if (tokens < 0 || tokens > (1ll << 31) || heads <= 0 || heads > 65536 || head_dim <= 0 || head_dim > 65536 || axes <= 0 || axes > kMaxAxes)
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: tokens must be 0 to 2^31, heads and head_dim 1 to 65536, axes 1 to 4");
     if (!(base >= 1.0) || !(base <= 1e30)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: base must be 1 to 1e30");
@@ -167,6 +169,8 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
     p.x_token = p.y_token = static_cast<long long>(heads) * head_dim;
     p.x_head = p.y_head = head_dim;
     if (strides != nullptr) {
+      for (int i = 0; i < 4; ++i)
+        if (strides[i] > (1ll << 50) / std::max<int64_t>(tokens, heads)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_rotary_axes: a stride is too large");
       p.x_token = strides[0];
       p.x_head = strides[1];
       p.y_token = strides[2];

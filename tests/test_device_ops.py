@@ -47,6 +47,22 @@ def host(n=64):
     return a, a.ctypes.data
 
 
+def test_arrays_that_start_between_elements_are_refused(pkg):
+    keep = [host() for _ in range(4)]
+    a, b, c, d = (x[1] for x in keep)
+    for at in range(4):
+        p = [a, b, c, d]
+        p[at] += 1 if at < 2 else 2
+        assert status_of(lambda: pkg.op_group_norm(p[0], p[1], "bf16", 1, 2, 4, 2, p[2], p[3])) == 2
+        with pytest.raises(pkg.NcnnB200Error, match="start"):
+            pkg.op_cross_attention(*[x + (1 if n == at else 0) for n, x in enumerate((a, b, c, d))], "f16", 1, 1, 1, 1, 1, 8)
+    with pytest.raises(pkg.NcnnB200Error, match="start"):
+        pkg.op_cross_attention(a, b, c, d, "f16", 1, 1, 1, 1, 1, 8, kv_lens_ptr=a + 2)
+    for x, y, p in ((a + 2, b, c), (a, b + 2, c), (a, b, c + 2)):
+        with pytest.raises(pkg.NcnnB200Error, match="start"):
+            pkg.op_rotary_axes(x, y, "f32", 1, 1, 8, p, [2])
+
+
 def test_group_norm_refuses(pkg):
     a, p = host()
     b, r = host()
@@ -83,6 +99,8 @@ def test_rotary_refuses(pkg):
                 dict(strides=(8, 8, 7, 8)), dict(strides=(-8, 8, 8, 8)), dict(heads=2, strides=(16, 8, 16, 4)), dict(x=p, y=p, strides=(16, 8, 8, 8))):
         assert status_of(call(**bad)) == 2, bad
     assert status_of(call(tokens=1 << 31, heads=1 << 10)) == 4
+    for at in range(4):
+        assert status_of(call(strides=[1 << 62 if n == at else 8 for n in range(4)])) == 4
     assert status_of(call(strides=(1, 2, 3))) == "ValueError"
     with pytest.raises(pkg.NcnnB200Error) as err:
         call()()
@@ -477,6 +495,12 @@ def test_cross_attention_nan_stays_in_its_row(pkg, element, lq):
     q[0, 0, 0, 3] = math.nan
     v[0, 7, 1, 5] = math.nan
     o = torch.empty_like(q)
+    bad = k.clone()
+    for key in (15, 46, 299):
+        bad[0, key, 1, 2] = math.nan
+        pkg.op_cross_attention(q.data_ptr(), bad.data_ptr(), v.data_ptr(), o.data_ptr(), element, 1, lq, 300, 2, 2, 64)
+        assert torch.isnan(o[0, :, 1]).all() and torch.isfinite(o[0, 1:, 0]).all()
+        bad[0, key, 1, 2] = 0
     pkg.op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), element, 1, lq, 300, 2, 2, 64)
     assert torch.isnan(o[0, 0, 0]).all() and torch.isfinite(o[0, 1:, 0]).all()
     assert torch.isnan(o[0, :, 1, 5]).all() and torch.isfinite(o[0, :, 1, :5]).all() and torch.isfinite(o[0, :, 1, 6:]).all()
