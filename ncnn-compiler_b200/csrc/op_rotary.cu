@@ -125,8 +125,10 @@ void launch(RotaryParams& p, bool in_place, int sms, cudaStream_t st) {
   constexpr int PAIRS = NEIGHBOURS ? (V > 1 ? V / 2 : 1) : V;
   p.tail_units = in_place ? 0 : (p.head_dim - 2 * p.pairs) / V;
   const long long units = p.pairs / PAIRS + p.tail_units;
-  // several heads to a thread where that leaves enough threads to fill the device
-  if (p.heads >= 4 && p.tokens * ((p.heads + 3) / 4) * units >= sms * 2048ll) launch_heads<T, V, NEIGHBOURS, 4>(p, units, sms, st);
+  // Several heads to a thread where that leaves enough threads to fill the device: four accesses under way.  32760 tokens of 24
+  // heads of 128, one, two, four, eight heads: neighbours 153, 95, 74, 82 us, halves apart (two accesses a head) 129, 91, 108, 165.
+  constexpr int HEADS = NEIGHBOURS ? 4 : 2;
+  if (p.heads >= HEADS && p.tokens * ((p.heads + HEADS - 1) / HEADS) * units >= sms * 2048ll / 4 * HEADS) launch_heads<T, V, NEIGHBOURS, HEADS>(p, units, sms, st);
   else launch_heads<T, V, NEIGHBOURS, 1>(p, units, sms, st);
 }
 
