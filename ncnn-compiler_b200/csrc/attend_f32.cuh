@@ -23,6 +23,8 @@ __device__ __forceinline__ float4 four_of(const T* row, int c, int d) {
 
 __device__ __forceinline__ float dot4(float4 a, float4 b, float c) { return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c)))); }
 
+constexpr int kF32Ranks = 8;  // CTAs of a cluster at most
+
 struct F32Params {
   AttendParams a;
   float scale_log2;
@@ -153,15 +155,26 @@ __global__ void __launch_bounds__(kSplitWarps * 32) k_attend_split(const __grid_
   else __syncthreads();
   for (int i = rank * kSplitWarps * 32 + threadIdx.x; i < rows * a.d; i += ranks * kSplitWarps * 32) {
     const int r = i / a.d, c = i % a.d;
-    float m = -INFINITY;
-    for (int n = 0; n < ranks; ++n) m = fmaxf(m, *cluster.map_shared_rank(&cta_top[r], n));
+    // (loads of other CTAs' memory are asked for together)
+    float tops[kF32Ranks], totals[kF32Ranks], x[kF32Ranks], m = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < kF32Ranks; ++n) {
+      const int from = min(n, ranks - 1);
+      tops[n] = *cluster.map_shared_rank(&cta_top[r], from);
+      totals[n] = *cluster.map_shared_rank(&cta_total[r], from);
+      x[n] = *cluster.map_shared_rank(&part[0][r][c], from);
+    }
+#pragma unroll
+    for (int n = 0; n < kF32Ranks; ++n) m = fmaxf(m, tops[n]);
     const float base = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f, all = 0.0f;
-    for (int n = 0; n < ranks; ++n) {
-      const float f = exp2f(*cluster.map_shared_rank(&cta_top[r], n) - base);
-      sum = fmaf(f, *cluster.map_shared_rank(&part[0][r][c], n), sum);
-      all = fmaf(f, *cluster.map_shared_rank(&cta_total[r], n), all);
-    }
+#pragma unroll
+    for (int n = 0; n < kF32Ranks; ++n)
+      if (n < ranks) {
+        const float f = exp2f(tops[n] - base);
+        sum = fmaf(f, x[n], sum);
+        all = fmaf(f, totals[n], all);
+      }
     const int row = row0 + r;
     static_cast<T*>(a.o)[batch * a.o_batch + row / shared * a.o_row + (kv_head * shared + row % shared) * a.o_head + c] =
         op_put<T>(all == 0.0f ? 0.0f : sum / all);
@@ -338,19 +351,29 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1) k_attend_tile(const 
     for (int i = threadIdx.x; i < share * (D / 4); i += THREADS) {
       const int r = from + i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
       if (row >= all_rows || c >= a.d) continue;
-      float m = -INFINITY;
-      for (int n = 0; n < ranks; ++n) m = fmaxf(m, *cluster.map_shared_rank(&tops[r], n));
+      float4 y[kF32Ranks];
+      float their_top[kF32Ranks], their_total[kF32Ranks], m = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < kF32Ranks; ++n) {
+        const int of = min(n, ranks - 1);
+        their_top[n] = *cluster.map_shared_rank(&tops[r], of);
+        their_total[n] = *cluster.map_shared_rank(&totals[r], of);
+        y[n] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(qs + r * PITCH + c, of));
+      }
+#pragma unroll
+      for (int n = 0; n < kF32Ranks; ++n) m = fmaxf(m, their_top[n]);
       const float base = m == -INFINITY ? 0.0f : m;
       float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, all = 0.0f;
-      for (int n = 0; n < ranks; ++n) {
-        const float f = exp2f(*cluster.map_shared_rank(&tops[r], n) - base);
-        const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(qs + r * PITCH + c, n));
-        all = fmaf(f, *cluster.map_shared_rank(&totals[r], n), all);
-        x[0] = fmaf(f, y.x, x[0]);
-        x[1] = fmaf(f, y.y, x[1]);
-        x[2] = fmaf(f, y.z, x[2]);
-        x[3] = fmaf(f, y.w, x[3]);
-      }
+#pragma unroll
+      for (int n = 0; n < kF32Ranks; ++n)
+        if (n < ranks) {
+          const float f = exp2f(their_top[n] - base);
+          all = fmaf(f, their_total[n], all);
+          x[0] = fmaf(f, y[n].x, x[0]);
+          x[1] = fmaf(f, y[n].y, x[1]);
+          x[2] = fmaf(f, y[n].z, x[2]);
+          x[3] = fmaf(f, y[n].w, x[3]);
+        }
       const float scale = all == 0.0f ? 0.0f : 1.0f / all;
       T* to = static_cast<T*>(a.o) + batch * a.o_batch + row / shared * a.o_row + (kv_head * shared + row % shared) * a.o_head + c;
 #pragma unroll

@@ -20,6 +20,7 @@
 namespace nb {
 
 constexpr int kFewRows = 16;
+constexpr int kFewRanks = 16;  // CTAs of a cluster at most
 
 struct FewParams {
   AttendParams a;
@@ -278,23 +279,46 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_few(const __grid_
   const int pieces = a.d / 8;
   for (int i = rank * WARPS * 32 + threadIdx.x; i < rows * pieces; i += ranks * WARPS * 32) {
     const int row = i / pieces, at = i % pieces * 8;
-    float m = -INFINITY;
-    for (int c = 0; c < ranks; ++c) m = fmaxf(m, *cluster.map_shared_rank(&sh.cta_top[row], c));
+    // (every load of another CTA's memory takes some 700 clocks: they are asked for together)
+    float tops[kFewRanks], factor[kFewRanks], m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kFewRanks; ++c) tops[c] = c < ranks ? *cluster.map_shared_rank(&sh.cta_top[row], c) : -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kFewRanks; ++c) {
+      factor[c] = c < ranks ? *cluster.map_shared_rank(&sh.cta_total[row], c) : 0.0f;
+      m = fmaxf(m, tops[c]);
+    }
     const float base = m == -INFINITY ? 0.0f : m;
     float sum[8] = {}, all = 0.0f;
-    for (int c = 0; c < ranks; ++c) {
-      const float f = exp2f(*cluster.map_shared_rank(&sh.cta_top[row], c) - base);
-      all = fmaf(f, *cluster.map_shared_rank(&sh.cta_total[row], c), all);
-      const float4* x = reinterpret_cast<const float4*>(cluster.map_shared_rank(&sh.part[0][row][at], c));
-      const float4 x0 = x[0], x1 = x[1];
-      sum[0] = fmaf(f, x0.x, sum[0]);
-      sum[1] = fmaf(f, x0.y, sum[1]);
-      sum[2] = fmaf(f, x0.z, sum[2]);
-      sum[3] = fmaf(f, x0.w, sum[3]);
-      sum[4] = fmaf(f, x1.x, sum[4]);
-      sum[5] = fmaf(f, x1.y, sum[5]);
-      sum[6] = fmaf(f, x1.z, sum[6]);
-      sum[7] = fmaf(f, x1.w, sum[7]);
+#pragma unroll
+    for (int c = 0; c < kFewRanks; ++c) {
+      const float f = exp2f(tops[c] - base);
+      all = fmaf(f, factor[c], all);
+      factor[c] = f;
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < kFewRanks; c0 += 4) {
+      if (c0 >= ranks) break;
+      float4 x[4][2];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4* from = reinterpret_cast<const float4*>(cluster.map_shared_rank(&sh.part[0][row][at], min(c0 + c, ranks - 1)));
+        x[c][0] = from[0];
+        x[c][1] = from[1];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c0 + c >= ranks) break;
+        const float f = factor[c0 + c];
+        sum[0] = fmaf(f, x[c][0].x, sum[0]);
+        sum[1] = fmaf(f, x[c][0].y, sum[1]);
+        sum[2] = fmaf(f, x[c][0].z, sum[2]);
+        sum[3] = fmaf(f, x[c][0].w, sum[3]);
+        sum[4] = fmaf(f, x[c][1].x, sum[4]);
+        sum[5] = fmaf(f, x[c][1].y, sum[5]);
+        sum[6] = fmaf(f, x[c][1].z, sum[6]);
+        sum[7] = fmaf(f, x[c][1].w, sum[7]);
+      }
     }
     const float scale = all == 0.0f ? 0.0f : 1.0f / all;
     OpVec<T, 8> out;
