@@ -187,16 +187,17 @@ __global__ void __launch_bounds__(kSplitWarps * 32) k_attend_split(const __grid_
 // probabilities, which its own half warp wrote.  Every 4 x 4 products take two 16-byte loads of which one is a broadcast.
 // Bound: the FMA pipe (32 of 74 TFLOP/s over 1024 x 1024, 64 heads of 64: half the issue slots are loads, addresses and the softmax).
 // Where the tiles are fewer than the device holds, a tile's blocks of keys are dealt to the CTAs of a cluster, which join their
-// results over distributed shared memory (2394 queries over 1768 keys, two heads of 128 on one key head: 498 us without).
+// results over distributed shared memory (2394 queries over 1768 keys, two heads of 128 on one key head: 498 us without, 176 so).
 template <int D, int TM, int KEYS, int THREADS>
 struct TileShape {
   static constexpr int kRows = THREADS / 16 * TM;
+  static constexpr int kBlocksPerSm = D > 64 ? 1 : 2;  // (three, of 80 registers a thread, are slower)
   static constexpr int kPitch = D + 4;  // floats: rows start in different banks
   static constexpr int kSmem = (kRows * kPitch + KEYS * kPitch + KEYS * D + kRows * (KEYS + 4)) * 4;
 };
 
 template <class T, int D, int TM, int KEYS, int THREADS, bool WIDE>
-__global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1) k_attend_tile(const __grid_constant__ F32Params p) {
+__global__ void __launch_bounds__(THREADS, TileShape<D, TM, KEYS, THREADS>::kBlocksPerSm) k_attend_tile(const __grid_constant__ F32Params p) {
   namespace cg = cooperative_groups;
   using Shape = TileShape<D, TM, KEYS, THREADS>;
   constexpr int ROWS = Shape::kRows, PITCH = Shape::kPitch, TN = KEYS / 16, PER = D / 64;
@@ -347,10 +348,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1) k_attend_tile(const 
       for (int c = 0; c < PER; ++c) *reinterpret_cast<float4*>(qs + r * PITCH + 64 * c + 4 * tx) = o[i][c];
     }
     cluster.sync();
-    const int share = ROWS / ranks, from = rank * share;
+    const int share = (ROWS + ranks - 1) / ranks, from = rank * share;
     for (int i = threadIdx.x; i < share * (D / 4); i += THREADS) {
       const int r = from + i / (D / 4), c = i % (D / 4) * 4, row = row0 + r;
-      if (row >= all_rows || c >= a.d) continue;
+      if (r >= ROWS || row >= all_rows || c >= a.d) continue;
       float4 y[kF32Ranks];
       float their_top[kF32Ranks], their_total[kF32Ranks], m = -INFINITY;
 #pragma unroll

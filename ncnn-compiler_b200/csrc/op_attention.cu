@@ -228,9 +228,11 @@ cudaError_t launch_tile(F32Params p, int device, int sms, cudaStream_t st) {
   if (const cudaError_t e = grant_smem(kernel, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
   const long long rows = static_cast<long long>(p.a.lq) * (p.a.heads / p.a.kv_heads);
   const long long row_tiles = (rows + Shape::kRows - 1) / Shape::kRows, tiles = row_tiles * p.a.kv_heads * p.a.batch;
-  // CTAs to a tile: what the device holds at once (two to an SM for heads up to 64), while each has two blocks of keys
-  p.ranks = 1;
-  while (p.ranks < 8 && tiles * p.ranks * 2 <= (D == 64 ? 2 : 1) * sms && p.a.lk > p.ranks * 2 * KEYS) p.ranks *= 2;
+  // CTAs to a tile: what the device holds at once, while each has a block of keys; no more than the blocks are dealt evenly to
+  const long long blocks = (p.a.lk + KEYS - 1) / KEYS, most = std::max<long long>(1, std::min<long long>({kF32Ranks, Shape::kBlocksPerSm * sms / tiles, blocks}));
+  const long long deal = (blocks + most - 1) / most;  // blocks of the busiest CTA
+  p.ranks = static_cast<int>((blocks + deal - 1) / std::max<long long>(1, deal));
+  p.ranks = std::max(p.ranks, 1);
   cudaLaunchConfig_t c{};
   c.gridDim = dim3(static_cast<unsigned>(row_tiles * p.ranks), p.a.kv_heads, p.a.batch);
   c.blockDim = dim3(THREADS);
