@@ -247,9 +247,10 @@ int ncnn_b200_op_rotary_axes(const void *x, void *y, int32_t type, int64_t token
  * h / (heads / kv_heads); head_dim 1 to 256.
  *   o = sum_j softmax_j(scale * q.k_j) v_j   over j < kv_lens[batch] (int32, NULL = lk; held to 0..lk) with
  *   key_mask[batch][j] != 0 (bytes [batch][lk], NULL = all).
- * scale 0 = 1 / sqrt(head_dim).  A sequence that is left without a key gets zeros.  Whatever lies at a key that takes no part
- * is not used, NaN and infinity included.  strides: host, 12 numbers in elements, {batch, row, head} of q, k, v and o in
- * that order, NULL for dense arrays; components are always next to one another.  o must not overlap an input.
+ * scale 0 = 1 / sqrt(head_dim).  A sequence that is left without a key gets zeros, and so does a query whose every score is minus
+ * infinity.  Whatever lies at a key that takes no part is not used, NaN and infinity included.  strides: host, 12 numbers in
+ * elements, {batch, row, head} of q, k, v and o in that order, NULL for dense arrays; components are always next to one
+ * another.  o must not overlap an input.
  * 16-bit types whose rows start at multiples of 16 bytes run on the tensor cores, their probabilities rounded to the type. */
 int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, void *o, int32_t type, int64_t batch,
                                  int64_t lq, int64_t lk, int32_t heads, int32_t kv_heads, int32_t head_dim,

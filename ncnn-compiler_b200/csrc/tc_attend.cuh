@@ -127,13 +127,14 @@ __device__ __forceinline__ uint32_t exp_pair(uint32_t x, uint32_t y, uint64_t c2
 // 4500 keys, 16 heads of 128: 209 us, 215 without, 208 with every fourth pair, 234 with every second).
 // 2^x = 2^n 2^f with n the nearest whole number (out of the sum with 1.5 2^23, whose last bits it is) and f in [-1/2, 1/2];
 // 2^f by a polynomial through the Chebyshev points of that range, of relative error: degree 3 is good to 2^-13.3, an
-// eighteenth of bf16's half step, degree 4 to 2^-18.  x is held to -120 (2^-120 of the row's largest term); a NaN stays one.
+// eighteenth of bf16's half step, degree 4 to 2^-18.  x is held to -127, where the exponent's bits are 0 and the term is exactly 0,
+// as ex2 has it for a term below 2^-126: keys of score minus infinity add nothing, and a row of them has the sum 0.  A NaN stays one.
 template <class T>
 __device__ __forceinline__ uint32_t exp_pair_fma(uint32_t x, uint32_t y, uint64_t c2, uint64_t from2, uint64_t& sums) {
   auto both = [](float v) { return f32x2_make(__float_as_uint(v), __float_as_uint(v)); };
   float2 t = f32x2_get(f32x2_fma3(f32x2_make(x, y), c2, from2));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.x) : "f"(-120.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.y) : "f"(-120.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.x) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.y) : "f"(-127.0f));
   const uint64_t at = f32x2_make(__float_as_uint(t.x), __float_as_uint(t.y));
   uint64_t whole, n;
   f32x2_add(whole, at, both(12582912.0f));
