@@ -290,29 +290,82 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
   if (ranks > 1) cluster.barrier_wait();
 }
 
-// Groups of more channels than a CTA has threads for: one CTA to a group, which reads x three times.
+// Moves the shift of n values' sums (s1 of their differences from it, s2 of the squares) to their mean.
+__device__ __forceinline__ void recentre(float n, float& shift, float& s1, float& s2) {
+  const float to = shift + s1 / n, off = to - shift;
+  s2 = fmaxf(fmaf(-off, fmaf(-n, off, 2.0f * s1), s2), 0.0f);
+  s1 = fmaf(-n, off, s1);
+  shift = to;
+}
+
+// Groups of more channels than a CTA has threads for: one CTA to a group, which reads x twice, four elements of a thread at a time.
+//
+// Statistics.  A thread may have tens of thousands of values: a sum about zero drifts by deviations there (a map of 128 x 128 x 1028
+// with a mean of 1003 deviations: by 0.18).  So they are summed as in k_group_norm, about the thread's first value, and the shift
+// follows the mean after 4, 8, 16, ... values: a first value far from the others would otherwise stand in every difference.
 template <class T, int ACT>
 __global__ void __launch_bounds__(kNormThreads) k_group_norm_wide(const __grid_constant__ NormParams p) {
+  constexpr int kTogether = 4;
   const int size = p.channels / p.groups;
   const long long image = blockIdx.x / p.groups;
   const int c0 = static_cast<int>(blockIdx.x % p.groups) * size;
   const T* x = static_cast<const T*>(p.x) + image * p.pixels * p.x_pitch + c0;
   T* y = static_cast<T*>(p.y) + image * p.pixels * p.y_pitch + c0;
-  const long long count = p.pixels * size;
-  float sum = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += kNormThreads) sum += op_get(x[i / size * p.x_pitch + i % size]);
-  const float mean = block_sum(sum) / static_cast<float>(count);
-  sum = 0.0f;
-  for (long long i = threadIdx.x; i < count; i += kNormThreads) {
-    const float d = op_get(x[i / size * p.x_pitch + i % size]) - mean;
-    sum = fmaf(d, d, sum);
-  }
-  const float scale = 1.0f / sqrtf(block_sum(sum) / static_cast<float>(count) + p.eps);
-  for (long long i = threadIdx.x; i < count; i += kNormThreads) {
-    const int c = static_cast<int>(i % size);
-    const float v = fmaf((op_get(x[i / size * p.x_pitch + c]) - mean) * scale, p.gamma ? p.gamma[c0 + c] : 1.0f, p.beta ? p.beta[c0 + c] : 0.0f);
-    y[i / size * p.y_pitch + c] = op_put<T>(norm_act<ACT>(v, p.floor));
-  }
+  // this thread's elements, every 256th of the group's: f gets pixels (from p.pixels on: none) and channels
+  auto over = [&](auto&& f) {
+    long long pixel = static_cast<int>(threadIdx.x) / size;
+    int c = static_cast<int>(threadIdx.x) % size;
+    while (pixel < p.pixels) {
+      long long at_pixel[kTogether];
+      int at_c[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        at_pixel[u] = pixel;
+        at_c[u] = c;
+        for (c += kNormThreads; c >= size; c -= size) ++pixel;
+      }
+      f(at_pixel, at_c);
+    }
+  };
+  float shift = 0.0f, s1 = 0.0f, s2 = 0.0f;
+  int n = 0;
+  over([&](const long long (&pixel)[kTogether], const int (&c)[kTogether]) {
+    T in[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      if (pixel[u] < p.pixels) in[u] = x[pixel[u] * p.x_pitch + c[u]];
+    if (n == 0) shift = op_get(in[0]);
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      if (pixel[u] < p.pixels) {
+        const float d = op_get(in[u]) - shift;
+        s1 += d;
+        s2 = fmaf(d, d, s2);
+        ++n;
+      }
+    if ((n & (n - 1)) == 0) recentre(static_cast<float>(n), shift, s1, s2);
+  });
+  if (n > 0) recentre(static_cast<float>(n), shift, s1, s2);
+  // the CTA's, about its first thread's mean (a group of one value has that for its mean, exactly)
+  __shared__ float first;
+  if (threadIdx.x == 0) first = shift;
+  __syncthreads();
+  const float about = first, count = static_cast<float>(p.pixels * size);
+  const float mean = about + block_sum(n > 0 ? n * (shift - about) + s1 : 0.0f) / count;
+  const float m2 = block_sum(n > 0 ? fmaf(n * (shift - mean), shift - mean, s2) : 0.0f);
+  const float scale = 1.0f / sqrtf(m2 / count + p.eps);
+  over([&](const long long (&pixel)[kTogether], const int (&c)[kTogether]) {
+    T in[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      if (pixel[u] < p.pixels) in[u] = x[pixel[u] * p.x_pitch + c[u]];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      if (pixel[u] < p.pixels) {
+        const float v = fmaf((op_get(in[u]) - mean) * scale, p.gamma ? p.gamma[c0 + c[u]] : 1.0f, p.beta ? p.beta[c0 + c[u]] : 0.0f);
+        y[pixel[u] * p.y_pitch + c[u]] = op_put<T>(norm_act<ACT>(v, p.floor));
+      }
+  });
 }
 
 template <class T, int V, int ACT>

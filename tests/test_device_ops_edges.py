@@ -9,7 +9,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_device_ops import KIND, TYPES, U, assert_within, gen, normal
+from test_device_ops import F, KIND, TYPES, U, assert_within, check_norm, gen, normal
 
 
 def attend(pkg, q, k, v, element, scale=0.0, lens=None):
@@ -57,3 +57,67 @@ def test_shares_below_the_smallest_number_are_zero(pkg, element, lq, lk, heads):
     v[:, 0] = 1
     o = attend(pkg, q, k, v, element, 1.0)
     assert torch.equal(o, torch.ones_like(o))
+
+
+# ------------------------------------------------------------------------------------------------ group norm
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_groups_wider_than_a_cta(pkg, element, in_place):
+    """Groups of more than 256 accesses of channels (16-byte ones, or what the address and the channels allow), one and several of
+    them, whole tensors and ranges of a wider one's channels; at most 2^9 values to a thread, as norm_want counts."""
+    wide = 2056 if element != "f32" else 1028
+    check_norm(pkg, element, 1, 60, wide, 1, "none", in_place=in_place)
+    check_norm(pkg, element, 3, 41, 2 * wide, 2, "swish", in_place=in_place)
+    check_norm(pkg, element, 2, 1, wide, 1, "relu", in_place=in_place)
+    check_norm(pkg, element, 2, 7, 5140, 1, "gelu", affine=False, in_place=in_place)
+    check_norm(pkg, element, 2, 130, 300, 1, "gelu", shift=1, in_place=in_place)
+    check_norm(pkg, element, 1, 90, 771, 3, "swish", x_pitch=773, y_pitch=773 if in_place else 771, in_place=in_place)
+
+
+def check_statistics(pkg, x, groups, terms):
+    """Against the formula in 64 bits; `terms`: the values of a thread.  A thread's sums of differences from a shift near the mean
+    are off by `terms` F of the sum of their sizes (two deviations a value at most), its squares' likewise; joining 256 threads
+    and 16 CTAs adds 2^8 F of six deviations and the mean's own rounding, 3 F of its size."""
+    n, p, c = x.shape
+    y = torch.empty_like(x)
+    pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", n, p, c, groups, None, None, 1e-5, "none")
+    t = x.double().view(n, p, groups, c // groups)
+    mean = t.mean((1, 3), keepdim=True)
+    sd = torch.sqrt((t - mean).square().mean((1, 3), keepdim=True) + 1e-5)
+    z = (t - mean) / sd
+    dm = (2 * terms + 6 * 2.0 ** 8) * F + 3 * F * mean.abs() / sd
+    assert_within(y, z.reshape(n, p, c), (dm + z.abs() * ((terms + 64) * F + dm * dm + 8 * F)).reshape(n, p, c))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pixels,mean", [(16384, 1003.0), (65536, 1003.0), (4096, 0.0)])
+def test_groups_wider_than_a_cta_far_from_zero(pkg, pixels, mean):
+    """Sums of so many values about zero would put the mean off by 0.2 (16384 pixels) and 2 deviations (65536)."""
+    x = normal(gen(1), 1, pixels, 1028) + mean
+    check_statistics(pkg, x, 1, pixels * 1028 // 256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("outlier", [1e3, 1e5])
+def test_groups_wider_than_a_cta_with_an_outlier(pkg, outlier):
+    """The first value of a thread far from all others."""
+    x = normal(gen(1), 1, 4096, 1028)
+    x[0, 0, 0] = outlier
+    check_statistics(pkg, x, 1, 4096 * 1028 // 256)
+
+
+@pytest.mark.gpu
+def test_groups_wider_than_a_cta_constant_and_nonfinite(pkg):
+    """A group of one value is beta; a NaN or an infinity stays in its own group of its own image."""
+    x = torch.full((2, 37, 2060), 3.0, device="cuda")
+    x[1] = normal(gen(1), 37, 2060)
+    x[1, 5, 2] = math.nan
+    y = torch.empty_like(x)
+    beta = torch.arange(2060, device="cuda", dtype=torch.float32)
+    pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", 2, 37, 2060, 2, None, beta.data_ptr(), 1e-5, "relu")
+    assert torch.equal(y[0], beta.expand(37, 2060))
+    assert torch.isnan(y[1, :, :1030]).all() and torch.isfinite(y[1, :, 1030:]).all()
+    x[1, 5, 2] = math.inf
+    pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", 2, 37, 2060, 2, None, beta.data_ptr(), 1e-5, "relu")
+    assert torch.isnan(y[1, 5, 2]) and torch.isfinite(y[1, :, 1030:]).all()
