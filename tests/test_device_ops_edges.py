@@ -77,8 +77,9 @@ def test_groups_wider_than_a_cta(pkg, element, in_place):
 
 def check_statistics(pkg, x, groups, terms):
     """Against the formula in 64 bits; `terms`: the values of a thread.  A thread's sums of differences from a shift near the mean
-    are off by `terms` F of the sum of their sizes (two deviations a value at most), its squares' likewise; joining 256 threads
-    and 16 CTAs adds 2^8 F of six deviations and the mean's own rounding, 3 F of its size."""
+    are off by `terms` F of the sum of their sizes (two deviations a value at most), its squares' likewise; its first 64 may stand
+    about an outlier, whose square their sums then lose 64 * 64 / 2 F of.  Joining 256 threads and 16 CTAs adds 2^8 F of six
+    deviations and the mean's own rounding, 3 F of its size."""
     n, p, c = x.shape
     y = torch.empty_like(x)
     pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", n, p, c, groups, None, None, 1e-5, "none")
@@ -87,7 +88,7 @@ def check_statistics(pkg, x, groups, terms):
     sd = torch.sqrt((t - mean).square().mean((1, 3), keepdim=True) + 1e-5)
     z = (t - mean) / sd
     dm = (2 * terms + 6 * 2.0 ** 8) * F + 3 * F * mean.abs() / sd
-    assert_within(y, z.reshape(n, p, c), (dm + z.abs() * ((terms + 64) * F + dm * dm + 8 * F)).reshape(n, p, c))
+    assert_within(y, z.reshape(n, p, c), (dm + z.abs() * ((terms + 2.0 ** 11) * F + dm * dm + 8 * F)).reshape(n, p, c))
 
 
 @pytest.mark.gpu
@@ -121,3 +122,13 @@ def test_groups_wider_than_a_cta_constant_and_nonfinite(pkg):
     x[1, 5, 2] = math.inf
     pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", 2, 37, 2060, 2, None, beta.data_ptr(), 1e-5, "relu")
     assert torch.isnan(y[1, 5, 2]) and torch.isfinite(y[1, :, 1030:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("outlier", [1e2, 1e3, 1e4, 1e5])
+@pytest.mark.parametrize("pixels,channels,terms", [(65536, 255, 4096), (262144, 32, 512)])
+def test_group_norm_with_an_outlier(pkg, outlier, pixels, channels, terms):
+    """The first value of a thread far from all others (16 CTAs to the group, one or 32 rows of threads)."""
+    x = normal(gen(1), 1, pixels, channels)
+    x[0, 0, 0] = outlier
+    check_statistics(pkg, x, 1, terms)
