@@ -261,6 +261,12 @@ int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, vo
  * returns 7, once, when one of them ran out since the last such call, 0 otherwise. */
 int ncnn_b200_op_check_status(void);
 
+/* For tests of failures, not for production: what later calls of ncnn_b200_op_cross_attention on the tensor cores do, in all
+ * threads.  stall 1: their first block of keys never arrives, so that their waits run out.  wait_ns: the limit of a wait (0 = the
+ * usual one).  registers: as if the kernels had been compiled for so many (0 = as they are); other than the count that their roles
+ * share out, a call is refused.  All 0: as usual. */
+int ncnn_b200_op_test_hooks(int32_t stall, uint64_t wait_ns, int32_t registers);
+
 /* ---- One model on several GPUs of one box (batch sharding).
  * The reference has no counterpart: its entry point takes one image per call and keeps no state between
  * calls (lib/Conversion/NCNNToTosa/NCNNToTosa.cpp:48-52), which is what makes the images of a batch

@@ -6,8 +6,6 @@
 
 #include "op_attention.h"
 
-#include <cstdlib>
-#include <mutex>
 
 #include "attend_f32.cuh"
 #include "attend_few.cuh"
@@ -16,6 +14,12 @@
 
 namespace nb {
 namespace {
+
+// What ncnn_b200_op_test_hooks asked for.
+struct {
+  std::atomic<int> stall{0}, registers{0};
+  std::atomic<unsigned long long> wait_ns{0};
+} g_hooks;
 
 // ------------------------------------------------------------------ tensor cores
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -70,6 +74,8 @@ bool rows_of(const AttendParams& p, int count, int size) {
 template <class K>
 cudaError_t grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted, int registers = 0) {
   const uint64_t bit = 1ull << (device & 63);
+  const int as_if = registers > 0 ? g_hooks.registers.load(std::memory_order_relaxed) : 0;
+  if (as_if != 0 && as_if != registers) return cudaErrorInvalidKernelImage;
   if (device < 64 && (granted->load(std::memory_order_acquire) & bit)) return cudaSuccess;
   if (registers > 0) {
     cudaFuncAttributes a{};
@@ -89,10 +95,8 @@ bool fill_tc(const AttendParams& a, bool half, TcAttendParams* p, TcMaps* m) {
   p->a = a;
   p->scale_log2 = a.scale * 1.44269504088896340736f;
   p->wait_ns = kTcWaitLimitNs;
-  if (std::getenv("NCNN_B200_TEST_STALL") != nullptr) {
-    p->stall = 1;
-    p->wait_ns = 2000000ull;
-  }
+  p->stall = g_hooks.stall.load(std::memory_order_relaxed);
+  if (const unsigned long long ns = g_hooks.wait_ns.load(std::memory_order_relaxed); ns != 0) p->wait_ns = ns;
   return encode_rows(&m->q, half, a.q, a.d, a.lq, a.q_row, a.heads, a.q_head, a.batch, a.q_batch, p->q_step) &&
          encode_rows(&m->k, half, a.k, a.d, a.lk, a.k_row, a.kv_heads, a.k_head, a.batch, a.k_batch, p->k_step) &&
          encode_rows(&m->v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p->v_step) &&
@@ -282,6 +286,13 @@ bool tma_strides(const AttendParams& p) {
 
 }  // namespace
 }  // namespace nb
+
+extern "C" int ncnn_b200_op_test_hooks(int32_t stall, uint64_t wait_ns, int32_t registers) {
+  nb::g_hooks.stall.store(stall != 0 ? 1 : 0);
+  nb::g_hooks.wait_ns.store(wait_ns);
+  nb::g_hooks.registers.store(registers);
+  return NCNN_B200_STATUS_SUCCESS;
+}
 
 extern "C" int ncnn_b200_op_check_status(void) {
   using namespace nb;

@@ -81,6 +81,7 @@ def load_library():
     L.ncnn_b200_op_cross_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32,
                                                c_int32, c_void_p, c_void_p, c_void_p, c_float, c_void_p]
     L.ncnn_b200_op_check_status.argtypes = []
+    L.ncnn_b200_op_test_hooks.argtypes = [c_int32, ctypes.c_uint64, c_int32]
     L.ncnn_b200_multi_load.argtypes = [c_char_p, c_char_p, POINTER(_Options), POINTER(c_int32), c_int32, POINTER(c_void_p)]
     L.ncnn_b200_multi_free.argtypes = [c_void_p]
     L.ncnn_b200_multi_free.restype = None
@@ -385,6 +386,20 @@ def op_rotary_axes(x_ptr, y_ptr, element, tokens, heads, head_dim, positions_ptr
         _op_message(L, st)
 
 
+# Tests set NCNN_B200_TEST_STALL between calls.  The library does not read the environment for that: another thread of the host
+# may be changing it.  (os.environ's lookup of a name that is not there takes 0.6 us of a call's 6, its dict's 0.02.)
+_ENVIRON = getattr(os.environ, "_data", None)
+_stalled = False
+
+
+def _stall_as_asked(L):
+    global _stalled
+    asked = b"NCNN_B200_TEST_STALL" in _ENVIRON if _ENVIRON is not None else "NCNN_B200_TEST_STALL" in os.environ
+    if asked != _stalled:
+        L.ncnn_b200_op_test_hooks(1 if asked else 0, 2000000 if asked else 0, 0)
+        _stalled = asked
+
+
 def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads, kv_heads, head_dim, kv_lens_ptr=None,
                        key_mask_ptr=None, scale=0.0, strides=None, stream=0):
     """Attention of q [batch][lq][heads][head_dim] to k, v [batch][lk][kv_heads][head_dim]; kv_lens is int32 [batch], key_mask
@@ -392,6 +407,7 @@ def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads
     L = load_library()
     if strides is not None and len(strides) != 12:
         raise ValueError("strides are twelve numbers: batch, row and head of q, k, v and o")
+    _stall_as_asked(L)
     st = L.ncnn_b200_op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, _of(ELEMENT_TYPES, element, "element"), batch, lq, lk, heads, kv_heads,
                                         head_dim, None if strides is None else struct.pack("12q", *strides), kv_lens_ptr, key_mask_ptr,
                                         scale, stream)

@@ -59,6 +59,20 @@ def test_shares_below_the_smallest_number_are_zero(pkg, element, lq, lk, heads):
     assert torch.equal(o, torch.ones_like(o))
 
 
+@pytest.mark.gpu
+def test_the_environment_of_the_host_is_not_read_by_a_call(pkg, monkeypatch):
+    """Another thread may be changing it.  The Python binding passes NCNN_B200_TEST_STALL on through ncnn_b200_op_test_hooks."""
+    q, k, v = (normal(gen(n), 1, l, 2, 64).half() for n, l in ((0, 200), (1, 300), (2, 300)))
+    o = torch.empty_like(q)
+    pkg.op_check_status()
+    monkeypatch.setenv("NCNN_B200_TEST_STALL", "1")
+    L = pkg.load_library()
+    assert L.ncnn_b200_op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), 1, 1, 200, 300, 2, 2, 64, None, None, None, 0.0, None) == 0
+    monkeypatch.delenv("NCNN_B200_TEST_STALL")
+    pkg.op_check_status()
+    assert torch.isfinite(o).all()
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
