@@ -103,35 +103,43 @@ bool fill_tc(const AttendParams& a, bool half, TcAttendParams* p, TcMaps* m) {
          encode_rows(&m->o, half, a.o, a.d, a.lq, a.o_row, a.heads, a.o_head, a.batch, a.o_batch, nullptr, 32);
 }
 
+// A launch that did not happen because of the kernel itself.
+int refused_kernel(cudaError_t e) {
+  cudaGetLastError();
+  return op_fail(NCNN_B200_STATUS_RUNTIME, std::string("op_cross_attention: the kernel was not granted its registers and shared memory: ") + cudaGetErrorString(e));
+}
+int no_maps() { return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made"); }
+
 template <class T, int D>
-bool launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
+int launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
   using Shape = TcShortShape<D>;
   TcShortParams p{};
   TcMaps m;
-  if (!fill_tc(a, std::is_same<T, __half>::value, &p.t, &m)) return false;
+  if (!fill_tc(a, std::is_same<T, __half>::value, &p.t, &m)) return no_maps();
   static std::atomic<uint64_t> granted{0};
-  if (grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch) != cudaSuccess) return false;
+  if (const cudaError_t e = grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
   p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
   p.tiles = p.row_tiles * a.heads * a.batch;
   tc_attend_short_kernel<T, D><<<std::min(sms, p.tiles), Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
-  return true;
+  return op_launched("op_cross_attention");
 }
 
 template <class T, int D, int TILES>
-bool launch_tc(const AttendParams& a, int device, cudaStream_t st) {
+int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   using Shape = TcAttendShape<D, TILES>;
   TcAttendParams p{};
   TcMaps m;
-  if (!fill_tc(a, std::is_same<T, __half>::value, &p, &m)) return false;
+  if (!fill_tc(a, std::is_same<T, __half>::value, &p, &m)) return no_maps();
   static std::atomic<uint64_t> granted{0};
-  if (grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, Shape::kShareRegs ? Shape::kRegsLaunch : 0) != cudaSuccess) return false;
+  const int registers = Shape::kShareRegs ? Shape::kRegsLaunch : 0;
+  if (const cudaError_t e = grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
   tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
-  return true;
+  return op_launched("op_cross_attention");
 }
 
 template <class T>
-bool attend_tc(const AttendParams& a, int device, int sms, cudaStream_t st) {
+int attend_tc(const AttendParams& a, int device, int sms, cudaStream_t st) {
   const bool two = a.lq > kAttRows;
   const long long tiles = static_cast<long long>((a.lq + kAttRows - 1) / kAttRows) * a.heads * a.batch;
   // one block of keys and a tile for every SM: 4096 queries over 77 keys (8 sequences, 10 heads of 64) 27 us, 55 with a CTA to two
@@ -144,7 +152,7 @@ bool attend_tc(const AttendParams& a, int device, int sms, cudaStream_t st) {
 }
 
 template <class T, int D, int WARPS, int STAGES, int BLOCKS>
-bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
+int launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   FewParams p{};
   p.a = a;
   p.scale_log2 = a.scale * 1.44269504088896340736f;
@@ -152,8 +160,10 @@ bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   p.row_tiles = (a.lq * shared + kFewRows - 1) / kFewRows;
   constexpr int smem = sizeof(FewShared<T, D, WARPS, STAGES>);
   static std::atomic<uint64_t> granted{0};
-  if (grant_smem(k_attend_few<T, D, WARPS, STAGES, BLOCKS>, smem, device, &granted) != cudaSuccess) return false;
-  if (ranks > 8 && cudaFuncSetAttribute(k_attend_few<T, D, WARPS, STAGES, BLOCKS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  const auto kernel = k_attend_few<T, D, WARPS, STAGES, BLOCKS>;
+  if (const cudaError_t e = grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return refused_kernel(e);
+  if (ranks > 8)
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return refused_kernel(e);
   cudaLaunchConfig_t c{};
   c.gridDim = dim3(ranks, a.kv_heads * p.row_tiles, a.batch);
   c.blockDim = dim3(WARPS * 32);
@@ -165,7 +175,8 @@ bool launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   c.attrs = &cluster;
   c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, k_attend_few<T, D, WARPS, STAGES, BLOCKS>, p) == cudaSuccess;
+  cudaLaunchKernelEx(&c, kernel, p);
+  return op_launched("op_cross_attention");
 }
 
 // Whether a call is one of few queries.  At most two tiles of 16 to a key head always are.  So are up to 160 tiles over 512 keys or
@@ -180,7 +191,7 @@ bool few_queries(const AttendParams& p, int sms) {
 }
 
 template <class T>
-bool attend_few(const AttendParams& a, int device, int sms, cudaStream_t st) {
+int attend_few(const AttendParams& a, int device, int sms, cudaStream_t st) {
   const long long rows = static_cast<long long>(a.lq) * (a.heads / a.kv_heads);
   const long long tiles = static_cast<long long>(a.batch) * a.kv_heads * ((rows + kFewRows - 1) / kFewRows);
   // Few tiles (a cluster of 8 to each leaves SMs idle): CTAs of 8 warps with deep rings, one to an SM, up to 16 to a tile while
@@ -376,18 +387,10 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
     const int sms = op_sm_count(device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (type != NCNN_B200_F32 && p.lk > 0 && rows_of(p, 8, 2)) {
-      if (few_queries(p, sms)) {
-        if (!(type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st))) {
-          const int failed = op_launched(kOp);
-          return failed != 0 ? failed : op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the kernel could not be launched");
-        }
-        return op_launched(kOp);
-      }
+      if (few_queries(p, sms)) return type == NCNN_B200_F16 ? attend_few<__half>(p, device, sms, st) : attend_few<__nv_bfloat16>(p, device, sms, st);
       if (tma_strides(p)) {
         if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: cuTensorMapEncodeTiled is not available from this driver");
-        const bool done = type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
-        if (!done) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_cross_attention: the tensor maps could not be made");
-        return op_launched(kOp);
+        return type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
       }
     }
     op_by_type(type, [&](auto t) {

@@ -73,6 +73,26 @@ def test_the_environment_of_the_host_is_not_read_by_a_call(pkg, monkeypatch):
     assert torch.isfinite(o).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,heads", [(200, 300, 2), (100, 300, 80), (700, 100, 64)])
+def test_a_kernel_of_other_registers_is_refused_by_its_name(pkg, lq, lk, heads):
+    """setmaxnreg would wait without a limit there.  The message speaks of registers, nothing is launched, later calls are right."""
+    q, k, v = (normal(gen(n), 1, l, heads, 64).half() for n, l in ((0, lq), (1, lk), (2, lk)))
+    want = attend(pkg, q, k, v, "f16")
+    o = torch.full_like(q, 5.0)
+    L = pkg.load_library()
+    L.ncnn_b200_op_test_hooks(0, 0, 24)
+    try:
+        with pytest.raises(pkg.NcnnB200Error, match="registers") as err:
+            pkg.op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), "f16", 1, lq, lk, heads, heads, 64)
+    finally:
+        L.ncnn_b200_op_test_hooks(0, 0, 0)
+    assert err.value.status == 6
+    torch.cuda.synchronize()
+    assert (o == 5.0).all()
+    assert torch.equal(attend(pkg, q, k, v, "f16"), want)
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
