@@ -120,8 +120,8 @@ int launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
   if (const cudaError_t e = grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
   p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
   p.tiles = p.row_tiles * a.heads * a.batch;
-  tc_attend_short_kernel<T, D><<<std::min(sms, p.tiles), Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
-  return op_launched("op_cross_attention");
+  return op_launched("op_cross_attention",
+                     op_launch(tc_attend_short_kernel<T, D>, dim3(std::min(sms, p.tiles)), Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
 
 template <class T, int D, int TILES>
@@ -134,8 +134,7 @@ int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   const int registers = Shape::kShareRegs ? Shape::kRegsLaunch : 0;
   if (const cudaError_t e = grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
-  tc_attend_kernel<T, D, TILES><<<grid, Shape::kThreads, Shape::kSmem, st>>>(p, m.q, m.k, m.v, m.o);
-  return op_launched("op_cross_attention");
+  return op_launched("op_cross_attention", op_launch(tc_attend_kernel<T, D, TILES>, grid, Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
 
 template <class T>
@@ -164,19 +163,7 @@ int launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   if (const cudaError_t e = grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return refused_kernel(e);
   if (ranks > 8)
     if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return refused_kernel(e);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(ranks, a.kv_heads * p.row_tiles, a.batch);
-  c.blockDim = dim3(WARPS * 32);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = ranks;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  c.attrs = &cluster;
-  c.numAttrs = 1;
-  cudaLaunchKernelEx(&c, kernel, p);
-  return op_launched("op_cross_attention");
+  return op_launched("op_cross_attention", op_launch(kernel, dim3(ranks, a.kv_heads * p.row_tiles, a.batch), WARPS * 32, smem, st, ranks, p));
 }
 
 // Whether a call is one of few queries.  At most two tiles of 16 to a key head always are.  So are up to 160 tiles over 512 keys or
@@ -222,17 +209,7 @@ cudaError_t launch_split(F32Params& p, int sms, cudaStream_t st) {
   // enough CTAs to a tile to fill the device twice over, while each of their warps has eight keys
   int ranks = 1;
   while (ranks < 8 && tiles * ranks * 2 <= 4ll * sms && a.lk > ranks * kSplitWarps * 8) ranks *= 2;
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(ranks, a.kv_heads * p.row_tiles, a.batch);
-  c.blockDim = dim3(kSplitWarps * 32);
-  c.stream = st;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = ranks;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  c.attrs = &cluster;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, k_attend_split<T, D, ROWS, WIDE>, p);
+  return op_launch(k_attend_split<T, D, ROWS, WIDE>, dim3(ranks, a.kv_heads * p.row_tiles, a.batch), kSplitWarps * 32, 0, st, ranks, p);
 }
 
 template <class T, int D, int TM, int KEYS, int THREADS, bool WIDE>
@@ -248,18 +225,7 @@ cudaError_t launch_tile(F32Params p, int device, int sms, cudaStream_t st) {
   const long long deal = (blocks + most - 1) / most;  // blocks of the busiest CTA
   p.ranks = static_cast<int>((blocks + deal - 1) / std::max<long long>(1, deal));
   p.ranks = std::max(p.ranks, 1);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(static_cast<unsigned>(row_tiles * p.ranks), p.a.kv_heads, p.a.batch);
-  c.blockDim = dim3(THREADS);
-  c.dynamicSmemBytes = Shape::kSmem;
-  c.stream = st;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = p.ranks;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  c.attrs = &cluster;
-  c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, p);
+  return op_launch(kernel, dim3(static_cast<unsigned>(row_tiles * p.ranks), p.a.kv_heads, p.a.batch), THREADS, Shape::kSmem, st, p.ranks, p);
 }
 
 template <class T, bool WIDE>
@@ -393,18 +359,12 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
         return type == NCNN_B200_F16 ? attend_tc<__half>(p, device, sms, st) : attend_tc<__nv_bfloat16>(p, device, sms, st);
       }
     }
-    op_by_type(type, [&](auto t) {
+    return op_by_type(type, [&](auto t) {
       using T = decltype(t);
       // (16-bit rows come here when they are not aligned: element by element)
-      if constexpr (sizeof(T) == 4) {
-        if (rows_of(p, 4, sizeof(T))) {
-          attend_f32<T, true>(p, device, sms, st);
-          return 0;
-        }
-      }
-      attend_f32<T, false>(p, device, sms, st);
-      return 0;
+      if constexpr (sizeof(T) == 4)
+        if (rows_of(p, 4, sizeof(T))) return op_launched(kOp, attend_f32<T, true>(p, device, sms, st));
+      return op_launched(kOp, attend_f32<T, false>(p, device, sms, st));
     });
-    return op_launched(kOp);
   });
 }

@@ -100,9 +100,29 @@ inline int op_sm_count(int device) {
   return n;
 }
 
-inline int op_launched(const char* op) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? NCNN_B200_STATUS_SUCCESS : op_fail(NCNN_B200_STATUS_RUNTIME, std::string(op) + ": launch failed: " + cudaGetErrorString(e));
+// The status of a launch: what the launch itself answered.  (cudaGetLastError holds errors of earlier calls, too: a model that
+// could not be laid out would make the next operator fail.)
+inline int op_launched(const char* op, cudaError_t e) {
+  if (e == cudaSuccess) return NCNN_B200_STATUS_SUCCESS;
+  cudaGetLastError();  // said here, and not to be met by another call
+  return op_fail(NCNN_B200_STATUS_RUNTIME, std::string(op) + ": launch failed: " + cudaGetErrorString(e));
+}
+
+// CTAs of `cluster` along x, if any
+template <class... P, class... A>
+inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, int cluster, const A&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute size{};
+  size.id = cudaLaunchAttributeClusterDimension;
+  size.val.clusterDim.x = cluster;
+  size.val.clusterDim.y = size.val.clusterDim.z = 1;
+  c.attrs = &size;
+  c.numAttrs = cluster > 0 ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 // f(T{}) with the element type that `type` names

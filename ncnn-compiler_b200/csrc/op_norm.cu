@@ -406,9 +406,9 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   static std::atomic<uint64_t> granted{0};
   const uint64_t bit = 1ull << (device & 63);
   if (device >= 64 || !(granted.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return op_launched("op_group_norm");
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return op_launched("op_group_norm", e);
     if (device < 64) granted.fetch_or(bit, std::memory_order_acq_rel);
   }
   const long long images = 65535;  // blockIdx.z holds that many: more go in several launches
@@ -418,20 +418,10 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
     q.x = static_cast<const T*>(p.x) + at * p.pixels * p.x_pitch;
     q.y = static_cast<T*>(p.y) + at * p.pixels * p.y_pitch;
     q.first_image = at;
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(ranks, p.groups / take, static_cast<unsigned>(q.n));
-    c.blockDim = dim3(kNormThreads);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = ranks;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    c.attrs = &cluster;
-    c.numAttrs = 1;
-    if (cudaLaunchKernelEx(&c, kernel, q, s) != cudaSuccess) break;
+    const dim3 grid(ranks, p.groups / take, static_cast<unsigned>(q.n));
+    if (const cudaError_t e = op_launch(kernel, grid, kNormThreads, smem, st, ranks, q, s); e != cudaSuccess) return op_launched("op_group_norm", e);
   }
-  return op_launched("op_group_norm");
+  return NCNN_B200_STATUS_SUCCESS;
 }
 
 template <class T, int V, int ACT>
@@ -454,8 +444,7 @@ int launch_act(const NormParams& p, int device, cudaStream_t st) {
   for (int bytes = 64; bytes >= 16 && take > 0 && (p.by_image ? 1 : p.n) * (p.groups / take) * 16 * 4 < 3 * sms; bytes /= 2) take = pick(bytes);
   if (take == 0) {
     if (p.by_image) return NCNN_B200_STATUS_CONSTRAINT_VIOLATION;  // (the import refuses such groups)
-    k_group_norm_wide<T, ACT><<<static_cast<unsigned>(p.n * p.groups), kNormThreads, 0, st>>>(p);
-    return op_launched("op_group_norm");
+    return op_launched("op_group_norm", op_launch(k_group_norm_wide<T, ACT>, dim3(static_cast<unsigned>(p.n * p.groups)), kNormThreads, 0, st, 0, p));
   }
   return launch_shape<T, V, ACT>(p, take, device, st);
 }

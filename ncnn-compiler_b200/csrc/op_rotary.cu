@@ -107,29 +107,31 @@ __global__ void __launch_bounds__(256) k_rotary_axes(const __grid_constant__ Rot
 }
 
 template <class T, int V, bool NEIGHBOURS, int HEADS>
-void launch_heads(RotaryParams p, long long units, int sms, cudaStream_t st) {
+cudaError_t launch_heads(RotaryParams p, long long units, int sms, cudaStream_t st) {
   p.head_groups = (p.heads + HEADS - 1) / HEADS;
   const long long tokens = p.tokens, a_token = p.head_groups * units;
   const long long most = std::max<long long>(1, (1ll << 30) / a_token);  // tokens of a launch: thread numbers have 32 bits
   for (p.first_token = 0; p.first_token < tokens; p.first_token += most) {
     p.tokens = std::min(most, tokens - p.first_token);
     const long long blocks = (p.tokens * a_token + 255) / 256;
-    k_rotary_axes<T, V, NEIGHBOURS, HEADS><<<static_cast<unsigned>(std::min<long long>(blocks, sms * 16ll)), 256, 0, st>>>(p);
+    const dim3 grid(static_cast<unsigned>(std::min<long long>(blocks, sms * 16ll)));
+    if (const cudaError_t e = op_launch(k_rotary_axes<T, V, NEIGHBOURS, HEADS>, grid, 256, 0, st, 0, p); e != cudaSuccess) return e;
     p.x = static_cast<const T*>(p.x) + most * p.x_token;
     p.y = static_cast<T*>(p.y) + most * p.y_token;
   }
+  return cudaSuccess;
 }
 
 template <class T, int V, bool NEIGHBOURS>
-void launch(RotaryParams& p, bool in_place, int sms, cudaStream_t st) {
+cudaError_t launch(RotaryParams& p, bool in_place, int sms, cudaStream_t st) {
   constexpr int PAIRS = NEIGHBOURS ? (V > 1 ? V / 2 : 1) : V;
   p.tail_units = in_place ? 0 : (p.head_dim - 2 * p.pairs) / V;
   const long long units = p.pairs / PAIRS + p.tail_units;
   // Several heads to a thread where that leaves enough threads to fill the device: four accesses under way.  32760 tokens of 24
   // heads of 128, one, two, four, eight heads: neighbours 153, 95, 74, 82 us, halves apart (two accesses a head) 129, 91, 108, 165.
   constexpr int HEADS = NEIGHBOURS ? 4 : 2;
-  if (p.heads >= HEADS && p.tokens * ((p.heads + HEADS - 1) / HEADS) * units >= sms * 2048ll / 4 * HEADS) launch_heads<T, V, NEIGHBOURS, HEADS>(p, units, sms, st);
-  else launch_heads<T, V, NEIGHBOURS, 1>(p, units, sms, st);
+  if (p.heads >= HEADS && p.tokens * ((p.heads + HEADS - 1) / HEADS) * units >= sms * 2048ll / 4 * HEADS) return launch_heads<T, V, NEIGHBOURS, HEADS>(p, units, sms, st);
+  return launch_heads<T, V, NEIGHBOURS, 1>(p, units, sms, st);
 }
 
 }  // namespace
@@ -216,20 +218,13 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
              p.y_token % v == 0 && p.y_head % v == 0 && p.pairs % pairs_a_unit == 0 && (interleaved ? 2 * p.pairs : p.pairs) % v == 0 && head_dim % v == 0;
     };
     const int v = all_multiples(wide) ? wide : all_multiples(2) ? 2 : 1;  // elements of an access
-    op_by_type(type, [&](auto t) {
+    return op_by_type(type, [&](auto t) {
       using T = decltype(t);
       constexpr int V = 16 / sizeof(T);
-      if (interleaved) {
-        if (v == V) launch<T, V, true>(p, in_place, sms, st);
-        else if (v == 2) launch<T, 2, true>(p, in_place, sms, st);
-        else launch<T, 1, true>(p, in_place, sms, st);
-      } else {
-        if (v == V) launch<T, V, false>(p, in_place, sms, st);
-        else if (v == 2) launch<T, 2, false>(p, in_place, sms, st);
-        else launch<T, 1, false>(p, in_place, sms, st);
-      }
-      return 0;
+      cudaError_t e;
+      if (interleaved) e = v == V ? launch<T, V, true>(p, in_place, sms, st) : v == 2 ? launch<T, 2, true>(p, in_place, sms, st) : launch<T, 1, true>(p, in_place, sms, st);
+      else e = v == V ? launch<T, V, false>(p, in_place, sms, st) : v == 2 ? launch<T, 2, false>(p, in_place, sms, st) : launch<T, 1, false>(p, in_place, sms, st);
+      return op_launched(kOp, e);
     });
-    return op_launched(kOp);
   });
 }

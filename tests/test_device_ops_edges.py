@@ -21,6 +21,30 @@ def attend(pkg, q, k, v, element, scale=0.0, lens=None):
     return o
 
 
+# ------------------------------------------------------------------------------------------------ whose error it is
+@pytest.mark.gpu
+@pytest.mark.parametrize("earlier", ["no such device", "no room"])
+def test_an_earlier_error_is_not_this_call_s(pkg, tmp_path, earlier):
+    """A load that asks for a device that is not there, and a batch that no device has room for, fail; operators afterwards run."""
+    param, bin_ = pkg.zoo.single_conv(str(tmp_path / "conv"))
+    x = normal(gen(1), 2, 64, 4, 64)
+    positions = torch.zeros(128, 1, device="cuda", dtype=torch.int32)
+    calls = [lambda y: pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", 2, 64, 256, 8),
+             lambda y: pkg.op_rotary_axes(x.data_ptr(), y.data_ptr(), "f32", 128, 4, 64, positions.data_ptr(), [32]),
+             lambda y: pkg.op_cross_attention(x.data_ptr(), x.data_ptr(), x.data_ptr(), y.data_ptr(), "f32", 2, 64, 64, 4, 4, 64),
+             lambda y: pkg.op_cross_attention(x.data_ptr(), x.data_ptr(), x.data_ptr(), y.data_ptr(), "bf16", 1, 64, 64, 4, 4, 64),
+             lambda y: pkg.op_cross_attention(x.data_ptr(), x.data_ptr(), x.data_ptr(), y.data_ptr(), "bf16", 2, 1, 64, 4, 4, 64)]
+    model = pkg.Model(param, bin_)
+    for call in calls:
+        if earlier == "no room":
+            assert model.launch_count(1 << 20) < 0
+        else:
+            with pytest.raises(pkg.NcnnB200Error):
+                pkg.Model(param, bin_, device=99)
+        call(torch.empty_like(x))
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 # queries, keys, heads: a few queries; many over whole blocks of 128 keys, over a last block that is not whole; at most 128 keys
 SHAPES = [(1, 512, 2), (200, 512, 80), (100, 640, 80), (200, 500, 80), (700, 128, 64)]
