@@ -257,8 +257,9 @@ int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, vo
                                  const int64_t *strides, const int32_t *kv_lens, const uint8_t *key_mask, float scale,
                                  void *stream);
 
-/* The tensor-core kernel of ncnn_b200_op_cross_attention bounds its waits (2 s each).  This waits for the current device and
- * returns 7, once, when one of them ran out since the last such call, 0 otherwise. */
+/* The tensor-core kernels of ncnn_b200_op_cross_attention bound their waits (2 s each).  This waits for the current device and
+ * for every device that such a call went to, and returns 7, once to each thread, when one of the waits ran out, on any of them and
+ * in any thread's call, since that thread's last such call (its first: since the library was loaded); 0 otherwise. */
 int ncnn_b200_op_check_status(void);
 
 /* For tests of failures, not for production: what later calls of ncnn_b200_op_cross_attention on the tensor cores do, in all

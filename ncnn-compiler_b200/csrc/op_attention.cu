@@ -21,6 +21,14 @@ struct {
   std::atomic<unsigned long long> wait_ns{0};
 } g_hooks;
 
+// The devices that calls on the tensor cores went to (as bits).
+std::atomic<uint64_t> g_waited_on{0};
+
+void will_wait_on(int device) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(g_waited_on.load(std::memory_order_relaxed) & bit)) g_waited_on.fetch_or(bit, std::memory_order_relaxed);
+}
+
 // ------------------------------------------------------------------ tensor cores
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -120,6 +128,7 @@ int launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
   if (const cudaError_t e = grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
   p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
   p.tiles = p.row_tiles * a.heads * a.batch;
+  will_wait_on(device);
   return op_launched("op_cross_attention",
                      op_launch(tc_attend_short_kernel<T, D>, dim3(std::min(sms, p.tiles)), Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
@@ -134,6 +143,7 @@ int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   const int registers = Shape::kShareRegs ? Shape::kRegsLaunch : 0;
   if (const cudaError_t e = grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
+  will_wait_on(device);
   return op_launched("op_cross_attention", op_launch(tc_attend_kernel<T, D, TILES>, grid, Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
 
@@ -274,13 +284,23 @@ extern "C" int ncnn_b200_op_test_hooks(int32_t stall, uint64_t wait_ns, int32_t 
 extern "C" int ncnn_b200_op_check_status(void) {
   using namespace nb;
   return op_guarded("op_check_status", [&]() -> int {
-    int status = 0;
-    const int none = 0;
-    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&status, g_attend_status, sizeof status) != cudaSuccess ||
-        (status != 0 && cudaMemcpyToSymbol(g_attend_status, &none, sizeof none) != cudaSuccess))
-      return op_fail(NCNN_B200_STATUS_RUNTIME, std::string("op_check_status: ") + cudaGetErrorString(cudaGetLastError()));
-    return status == 0 ? NCNN_B200_STATUS_SUCCESS
-                       : op_fail(NCNN_B200_STATUS_TIMEOUT, "op_check_status: a wait inside an operator's kernel ran out; its result is not valid");
+    // The kernels count for ever, and each thread remembers what it has been told: no thread takes an answer from another, and no
+    // count is lost between being read and being cleared.
+    static thread_local unsigned told[64] = {};
+    bool ran_out = false;
+    auto failed = [] { return op_fail(NCNN_B200_STATUS_RUNTIME, std::string("op_check_status: ") + cudaGetErrorString(cudaGetLastError())); };
+    if (cudaDeviceSynchronize() != cudaSuccess) return failed();
+    const uint64_t devices = g_waited_on.load();
+    for (int d = 0; d < 64; ++d) {
+      if (!(devices >> d & 1u)) continue;
+      DeviceGuard guard(d);
+      unsigned count = 0;
+      if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&count, g_attend_gave_up, sizeof count) != cudaSuccess) return failed();
+      ran_out = ran_out || count != told[d];
+      told[d] = count;
+    }
+    return !ran_out ? NCNN_B200_STATUS_SUCCESS
+                    : op_fail(NCNN_B200_STATUS_TIMEOUT, "op_check_status: a wait inside an operator's kernel ran out; its result is not valid");
   });
 }
 

@@ -24,7 +24,7 @@
 
 namespace nb {
 
-__device__ int g_attend_status;  // a wait that ran out: ncnn_b200_op_check_status
+__device__ unsigned g_attend_gave_up;  // CTAs in which a wait ran out, ever: ncnn_b200_op_check_status
 
 constexpr int kAttRows = 128;  // queries of a tile, and keys of a block
 
@@ -256,8 +256,8 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
-  auto gave_up = [&](int code) {
-    if (atomicCAS(&abort_flag, 0, 1) == 0) atomicCAS(&g_attend_status, 0, code);
+  auto gave_up = [&] {
+    if (atomicCAS(&abort_flag, 0, 1) == 0) atomicAdd(&g_attend_gave_up, 1u);
   };
   auto s_of = [&](int t) { return tmem + 128u * t; };
   auto o_of = [&](int t) { return tmem + 128u * TILES + static_cast<uint32_t>(D * t); };
@@ -286,7 +286,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
           for (int c = 0; c < D / 64; ++c) tma_load_4d(to + c * kPanel, value ? &map_v : &map_k, bar, c * 64, (j >> 1) * kAttRows, h, b);
           used = j + 1;
         }
-        if (!ok) gave_up(TC_TIMEOUT_PRODUCER);
+        if (!ok) gave_up();
         // no copy may be under way when the CTA's shared memory is given back
         auto landed = [](uint32_t bar, uint32_t parity) {
           for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(bar, parity); ++tries) {
@@ -361,7 +361,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
           }
         }
         if (!ok) {
-          gave_up(TC_TIMEOUT_MMA);
+          gave_up();
           tc_commit(smem_u32(&drained));  // nor may MMAs be under way
           for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&drained), 0); ++tries) {
           }
@@ -401,7 +401,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&fixed[slot]));
       }
-      if (!ok && lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
+      if (!ok && lane == 0) gave_up();
     }
   } else {
     if constexpr (Shape::kShareRegs) reg_alloc<Shape::kRegsSoftmax>();
@@ -495,7 +495,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
         tc_fence_after_sync();
       }
       if (!ok) {
-        if (lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
+        if (lane == 0) gave_up();
       } else {
         // (every product is done: the queries' tile is free)
         attend_store<T, D>(o_at, blocks > 0, total, q_at + t * kTile, (warp & 3) * 32, &map_o, row0 + t * kAttRows, p.a.lq, head, batch, p.a.d);

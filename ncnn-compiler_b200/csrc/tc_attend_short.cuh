@@ -77,8 +77,8 @@ tc_attend_short_kernel(const __grid_constant__ TcShortParams p, const __grid_con
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
-  auto gave_up = [&](int code) {
-    if (atomicCAS(&abort_flag, 0, 1) == 0) atomicCAS(&g_attend_status, 0, code);
+  auto gave_up = [&] {
+    if (atomicCAS(&abort_flag, 0, 1) == 0) atomicAdd(&g_attend_gave_up, 1u);
   };
   auto wait = [&](uint64_t& bar, int parity) { return mbar_wait_bounded(smem_u32(&bar), parity & 1, abort_ptr, p.t.wait_ns); };
   auto s_of = [&](int t) { return tmem + 128u * t; };
@@ -137,7 +137,7 @@ tc_attend_short_kernel(const __grid_constant__ TcShortParams p, const __grid_con
           queries = n + 1;
           return true;
         });
-        if (!ok) gave_up(TC_TIMEOUT_PRODUCER);
+        if (!ok) gave_up();
         // no copy may be under way when the CTA's shared memory is given back
         auto landed = [](uint32_t bar, int parity) {
           for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(bar, parity & 1); ++tries) {
@@ -190,7 +190,7 @@ tc_attend_short_kernel(const __grid_constant__ TcShortParams p, const __grid_con
         });
         if (ok && before.n >= 0) ok = products(before);
         if (!ok) {
-          gave_up(TC_TIMEOUT_MMA);
+          gave_up();
           tc_commit(smem_u32(&drained));  // nor may MMAs be under way
           for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&drained), 0); ++tries) {
           }
@@ -221,7 +221,7 @@ tc_attend_short_kernel(const __grid_constant__ TcShortParams p, const __grid_con
         if (lane == 0) mbar_arrive(smem_u32(&kv_fixed[half]));
         return true;
       });
-      if (!ok && lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
+      if (!ok && lane == 0) gave_up();
     }
   } else {
     reg_alloc<Shape::kRegsSoftmax>();
@@ -310,7 +310,7 @@ tc_attend_short_kernel(const __grid_constant__ TcShortParams p, const __grid_con
       return true;
     });
     left();
-    if (!ok && lane == 0) gave_up(TC_TIMEOUT_EPILOGUE);
+    if (!ok && lane == 0) gave_up();
   }
   __syncthreads();
   if (warp == 1) {

@@ -416,7 +416,7 @@ def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads
 
 
 def op_check_status():
-    """Waits for the current device; raises where a wait inside an operator's kernel ran out since the last call."""
+    """Waits for the devices of earlier calls; raises where a wait inside an operator's kernel ran out since this thread's last call."""
     L = load_library()
     st = L.ncnn_b200_op_check_status()
     if st != 0:

@@ -4,6 +4,7 @@ infinity, shares too small for a type, values far from zero, outliers, errors th
 Tolerances as in test_device_ops.py: derived from the arithmetic, F = 2^-24, U[t] half a step of type t.
 """
 import math
+import threading
 
 import pytest
 
@@ -43,6 +44,51 @@ def test_an_earlier_error_is_not_this_call_s(pkg, tmp_path, earlier):
                 pkg.Model(param, bin_, device=99)
         call(torch.empty_like(x))
     torch.cuda.synchronize()
+
+
+def stalled_call(pkg, device="cuda"):
+    """A call whose first block of keys never arrives: its waits run out after 2 ms."""
+    q, k, v = (torch.randn(1, l, 2, 64, device=device).half() for l in (200, 300, 300))
+    o = torch.empty_like(q)
+    L = pkg.load_library()
+    L.ncnn_b200_op_test_hooks(1, 2000000, 0)
+    try:
+        pkg.op_cross_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), "f16", 1, 200, 300, 2, 2, 64)
+    finally:
+        L.ncnn_b200_op_test_hooks(0, 0, 0)
+    torch.cuda.synchronize(device)
+
+
+def status(pkg):
+    try:
+        pkg.op_check_status()
+    except pkg.NcnnB200Error as e:
+        return e.status
+    return 0
+
+
+@pytest.mark.gpu
+def test_every_thread_is_told_of_a_wait_that_ran_out(pkg):
+    """A thread that asks first takes the answer from no other; each gets it once."""
+    status(pkg)
+    stalled_call(pkg)
+    others = []
+    t = threading.Thread(target=lambda: others.extend([status(pkg), status(pkg)]))
+    t.start()
+    t.join()
+    assert others == [7, 0]
+    assert [status(pkg), status(pkg)] == [7, 0]
+    stalled_call(pkg)
+    assert [status(pkg), status(pkg)] == [7, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_wait_that_ran_out_on_another_device_is_told(pkg):
+    status(pkg)
+    stalled_call(pkg, "cuda:1")
+    assert torch.cuda.current_device() == 0
+    assert [status(pkg), status(pkg)] == [7, 0]
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
