@@ -212,7 +212,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
   extern __shared__ uint8_t attend_smem[];
   __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], fixed[kSlots], s_full[TILES], p_half[TILES], p_full[TILES], o_full[TILES], drained, to_fix;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_flag;
+  __shared__ int abort_flag, walked;  // walked: blocks of keys that the MMAs have begun with
 
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -229,9 +229,11 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
   const uint32_t smem = (smem_u32(attend_smem) + 1023u) & ~1023u;
   const uint32_t q_at = smem, ring = smem + TILES * kTile;
   volatile int* abort_ptr = &abort_flag;
+  volatile int* walked_ptr = &walked;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    walked = 0;
     mbar_init(smem_u32(&q_full), 1);
     mbar_init(smem_u32(&drained), 1);
     mbar_init(smem_u32(&to_fix), 1);
@@ -336,6 +338,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
             if (t == 0) {
               ok = wait_slot(v_use);
               const bool last = !fix_all && fix_last && j == blocks - 1;
+              *walked_ptr = j + 1;
               if (ok && last) mbar_arrive(smem_u32(&to_fix));
               if (ok && (fix_all || last))
                 ok = mbar_wait_bounded(smem_u32(&fixed[v_use % kSlots]), fix_all ? (v_use / kSlots) & 1 : 0, abort_ptr, p.wait_ns);
@@ -380,9 +383,16 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
           clear[w] = __ballot_sync(~0u, !part && r < rows);
         }
         // Under a mask the MMAs wait for this warp in every block, so that it sees every phase of the ring's barriers.  Without
-        // one the ring runs ahead of it, and the issuing thread says when the last block has landed.
-        ok = __all_sync(~0u, fix_all ? mbar_wait_bounded(smem_u32(&full[slot]), (use / kSlots) & 1, abort_ptr, p.wait_ns)
-                                     : mbar_wait_bounded(smem_u32(&to_fix), 0, abort_ptr, p.wait_ns));
+        // one the ring runs ahead of it, and the issuing thread says when the last block has landed.  That is a wait for the whole
+        // walk over the keys, whose time has no bound: its limit begins anew as long as the walk gets on.
+        auto last_landed = [&] {
+          while (true) {
+            const int seen = *walked_ptr;
+            if (mbar_wait_bounded(smem_u32(&to_fix), 0, abort_ptr, p.wait_ns)) return true;
+            if (*abort_ptr != 0 || *walked_ptr == seen) return false;
+          }
+        };
+        ok = __all_sync(~0u, fix_all ? mbar_wait_bounded(smem_u32(&full[slot]), (use / kSlots) & 1, abort_ptr, p.wait_ns) : last_landed());
         if (!ok) break;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {

@@ -163,6 +163,26 @@ def test_a_kernel_of_other_registers_is_refused_by_its_name(pkg, lq, lk, heads):
     assert torch.equal(attend(pkg, q, k, v, "f16"), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [100, 200])
+def test_a_walk_over_the_keys_may_take_longer_than_a_wait(pkg, lq):
+    """2^20 keys take some 10 ms, each step a microsecond; the limit of a wait is 2 ms here.  The sequence ends before the array and
+    inside a step of 16 keys: one warp waits for the last block from the start."""
+    lk, heads = 1 << 20, 80
+    q, k, v = (normal(gen(n), 1, l, h, 64).to(torch.bfloat16) for n, l, h in ((0, lq, heads), (1, lk, 1), (2, lk, 1)))
+    lens = torch.tensor([lk - 3], device="cuda", dtype=torch.int32)
+    status(pkg)
+    want = attend(pkg, q, k, v, "bf16", lens=lens)
+    L = pkg.load_library()
+    L.ncnn_b200_op_test_hooks(0, 2000000, 0)
+    try:
+        got = attend(pkg, q, k, v, "bf16", lens=lens)
+    finally:
+        L.ncnn_b200_op_test_hooks(0, 0, 0)
+    assert status(pkg) == 0
+    assert torch.isfinite(got).all() and torch.equal(got, want)
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
