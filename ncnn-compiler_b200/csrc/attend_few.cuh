@@ -5,11 +5,11 @@
 // result of its own.  tcgen05 has no use here: it would take 128 rows for the one to 16 that there are, and HBM is the bound
 // (the products of a tile take a fifth of the time that its 8 KB take to arrive).
 //
-// Each warp has a ring of two or three tiles in shared memory that its own lanes fill with cp.async, whole rows at a time (HBM
+// Each warp has a ring of three to six tiles in shared memory that its own lanes fill with cp.async, whole rows at a time (HBM
 // needs some 60 KB under way on each SM), 16-byte pieces exchanged by the row's number so that ldmatrix, which brings both
 // operands into fragments, reads all banks; values are transposed by it on the way.
-// Probabilities are split into two terms of the type, so that nothing of their 32 bits' first 16 (bf16) is lost: the
-// products have room for it.
+// Probabilities are split into two terms of the type, for which the products have room: 16 of their bits are kept in bf16, 22 in
+// fp16 (fewer below 2^-14, none below 2^-25, of 2^-7 of the running maximum: kProbabilityLift).
 // The warps' results are joined in shared memory, the CTAs' over distributed shared memory, in a fixed order.
 #pragma once
 
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_few(const __grid_
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float from = base[r] == -INFINITY ? 0.0f : base[r];
+      const float from = base[r] == -INFINITY ? 0.0f : base[r] - kProbabilityLift<T>;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float e0 = exp2_approx(x[n][2 * r] - from), e1 = exp2_approx(x[n][2 * r + 1] - from);

@@ -3,6 +3,7 @@
 
 #include <array>
 #include <tuple>
+#include <type_traits>
 
 #include "op_common.cuh"
 
@@ -17,5 +18,11 @@ struct AttendParams {
   const uint8_t* mask;  // [batch][lk], or null
   float scale;
 };
+
+// Probabilities of long keys and their sum are held this many powers of two higher.  fp16 has nothing below 2^-24 (2^-25 rounds to
+// 0), and many keys of little weight behind one of much would be in the sum but not in the products (131071 keys of 2^-25.07 each:
+// 0 instead of 0.0037).  With the slack of 2^8 that the running maximum has, probabilities stay at 2^15 or less, and weights from
+// 2^-32 of a row's largest on are there.  bf16 has fp32's range.
+template <class T> constexpr float kProbabilityLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 }  // namespace nb

@@ -3,7 +3,7 @@
 // A CTA holds TILES tiles of 128 queries of one head and walks the keys in blocks of 128 with a running maximum and sum:
 //   S = Q K^T        tcgen05.mma, both operands in shared memory, 128 x 128 fp32 in tensor memory
 //   P = 2^(S c - m)  c = scale / ln 2; a thread owns a query's row: it loads the 128 scores, takes their maximum, and writes P,
-//                    rounded to the type, over S (64 columns of packed pairs)
+//                    rounded to the type, over S (64 columns of packed pairs); fp16 times 2^7 (kProbabilityLift)
 //   O += P V         tcgen05.mma with P out of tensor memory; V as TMA brings it is [key][component], the keys being the
 //                    contraction: the descriptor's MN-major form
 // O is divided by the sum of the unrounded P at the end.  When a row's maximum rises, O has to be scaled; up to 2^8 the old
@@ -470,7 +470,7 @@ tc_attend_kernel(const __grid_constant__ TcAttendParams p, const __grid_constant
             }
           }
         }
-        const float from = base == -INFINITY ? 0.0f : -base;
+        const float from = base == -INFINITY ? 0.0f : kProbabilityLift<T> - base;
         const uint64_t c2 = f32x2_make(__float_as_uint(c), __float_as_uint(c)), from2 = f32x2_make(__float_as_uint(from), __float_as_uint(from));
         uint64_t sums[2] = {0, 0};
         // P leaves in halves: the first one's products begin while the second one's exponentials are taken

@@ -183,6 +183,29 @@ def test_a_walk_over_the_keys_may_take_longer_than_a_wait(pkg, lq):
     assert torch.isfinite(got).all() and torch.equal(got, want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+@pytest.mark.parametrize("lq,lk,heads,sinks", [(130, 131072, 80, 1), (1, 1 << 22, 1, 128)])
+def test_many_keys_of_little_weight_behind_few_of_much(pkg, element, lq, lk, heads, sinks):
+    """Key 0 (or the first keys of 128 tiles of 16, one to each warp of the cluster that shares out a query's keys) at a score of 0 and
+    value 0, all others at -17.375 (2^-25.07) and value 1: the result is their share.  Scores are exact.  Sums: up to lk / 16 steps of
+    the products, which truncate (2 F each), and lk / 64 additions of a thread.  An fp16 probability is off by 2^-32 of a sink at
+    most, a bf16 one by its rounding; the result's own rounding."""
+    q = torch.zeros(1, lq, heads, 64, device="cuda", dtype=KIND[element])
+    q[..., 0] = 1
+    k = torch.zeros(1, lk, 1, 64, device="cuda", dtype=KIND[element])
+    k[..., 0] = -17.375
+    v = torch.ones_like(k)
+    k[0, 0:16 * sinks:16, 0, 0] = 0
+    v[0, 0:16 * sinks:16] = 0
+    o = attend(pkg, q, k, v, element, 1.0)
+    weak = (lk - sinks) * math.exp(-17.375)
+    want = torch.full_like(o, weak / (weak + sinks), dtype=torch.float64)
+    off = (lk / 16 * 2 + lk / 64) * F + 2.0 ** -20 + U[element]
+    lost = 2.0 ** -32 * lk / sinks if element == "f16" else U[element] * want
+    assert_within(o, want, off * want + lost)
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
