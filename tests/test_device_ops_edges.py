@@ -279,3 +279,36 @@ def test_group_norm_with_an_outlier(pkg, outlier, pixels, channels, terms):
     x = normal(gen(1), 1, pixels, channels)
     x[0, 0, 0] = outlier
     check_statistics(pkg, x, 1, terms)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels", [64, 1028])
+def test_swish_of_fp32_is_good_to_fp32(pkg, channels):
+    """Against the formula on the values without an activation, which are the same.  2^t is off by 4 F of itself (the instruction's
+    2^-22), its correction, 1 + e, the reciprocal after a Newton step and the product by F each, the reciprocal's remainder by less
+    than F: 9 F.  (An argument rounded once would add F for every unit of it.)  Above -80 nothing leaves fp32's range."""
+    x = normal(gen(1), 1, 2000, channels)
+    gamma = torch.full((channels,), 15.0, device="cuda")
+    line, got = torch.empty_like(x), torch.empty_like(x)
+    for y, act in ((line, "none"), (got, "swish")):
+        pkg.op_group_norm(x.data_ptr(), y.data_ptr(), "f32", 1, 2000, channels, 1, gamma.data_ptr(), None, 1e-5, act)
+    line = line.double()
+    assert -80 < line.min() < -50
+    want = line * torch.sigmoid(line)
+    assert_within(got, want, 9 * F * want.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+def test_swish_at_the_ends_of_the_numbers(pkg, element):
+    """A gamma of 0 leaves beta: far negative values give 0, far positive ones themselves, minus infinity and NaN a NaN."""
+    values = [math.inf, 3e38, 1e30, 200.0, 100.0, 88.5, 0.0, -0.0, -88.5, -100.0, -200.0, -1e30, -3e38, -math.inf, math.nan, 1.0]
+    x = normal(gen(1), 1, 50, 16).to(KIND[element])
+    y = torch.empty_like(x)
+    gamma, beta = torch.zeros(16, device="cuda"), torch.tensor(values, device="cuda")
+    pkg.op_group_norm(x.data_ptr(), y.data_ptr(), element, 1, 50, 16, 4, gamma.data_ptr(), beta.data_ptr(), 1e-5, "swish")
+    got = y[0].float()
+    assert torch.equal(got[:, :13], got[:1, :13].expand(50, 13))
+    assert torch.equal(y[0, 0, :6], beta[:6].to(KIND[element]))
+    assert (got[:, 6:13].abs() < 1e-35).all()
+    assert torch.isnan(got[:, 13:15]).all()
