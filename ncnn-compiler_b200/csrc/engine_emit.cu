@@ -908,7 +908,7 @@ bool EngineImpl::emit_node(std::vector<Step>& steps, const Node& node, int64_t n
       return true;
     }
     const int grid = grid_for(vec ? count / 4 : count);
-    s.kernel = "k_unary";
+    s.kernel = up.op == UN_COPY ? "k_unary:copy" : "k_unary";
     s.run = [=](cudaStream_t st) {
       if (vec) launch_plain(k_unary<4>, grid, 256, 0, st, in, out, count, up);
       else launch_plain(k_unary<1>, grid, 256, 0, st, in, out, count, up);

@@ -474,6 +474,38 @@ bool EngineImpl::prepare_weights(std::string* err) {
     nodes_.insert(nodes_.begin() + k, std::move(q));
     ++k;
   }
+  // A group norm subtracts the mean: in a map far from zero, what its operand loses to a contraction's format (a bf16 pair has 16
+  // bits, tf32 11) is a part of the deviations that are left.  A tensor that both read stays fp32, and the contractions read a copy
+  // of it in their format.
+  for (size_t k = 0; k < nodes_.size(); ++k) {
+    if (nodes_[k].kind != N_NORM) continue;
+    const int src = resolve(nodes_[k].in[0]);
+    int copy = -1;
+    for (size_t j = 0; j < nodes_.size(); ++j) {
+      const bool contraction = nodes_[j].kind == N_CONV || nodes_[j].kind == N_IP || nodes_[j].kind == N_GEMM;
+      if (!contraction || nodes_[j].impl != IMPL_TC || nodes_[j].term != 0 || resolve(nodes_[j].in[0]) != src) continue;
+      if (copy < 0) {
+        Node c;
+        c.kind = N_UNARY;
+        c.name = tensors_[src].name + ":operand";
+        c.type = "Split";
+        c.un.op = UN_COPY;
+        c.in = {src};
+        c.out = copy = new_tensor(c.name);
+        Tensor& to = tensors_[copy];
+        const std::string keep = to.name;
+        to = tensors_[src];
+        to.name = keep;
+        to.alias = -1;
+        to.is_input = false;
+        to.input_index = -1;
+        nodes_.insert(nodes_.begin() + j, std::move(c));
+        if (j <= k) ++k;
+        ++j;
+      }
+      nodes_[j].in[0] = copy;
+    }
+  }
   // formats: an fp32 tensor is kept as hi/lo planes (or tf32-rounded in the fast mode) only
   // when a tensor-core contraction reads it as its operand; everything else stays one
   // plain fp32 plane, which halves the traffic of the memory-bound layers around it
