@@ -179,14 +179,17 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
       p.x_head = strides[1];
       p.y_token = strides[2];
       p.y_head = strides[3];
-      // heads (and tokens) of the result that overlap would be written twice
-      const bool heads_inside = p.y_head >= head_dim && p.y_token >= (heads - 1) * p.y_head + head_dim;
-      const bool tokens_inside = p.y_token >= head_dim && (heads == 1 || p.y_head >= (tokens - 1) * p.y_token + head_dim);
-      if (p.x_token < 0 || p.x_head < 0 || !(heads_inside || tokens_inside || (heads == 1 && p.y_token >= head_dim)))
-        return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: negative strides, or results that overlap");
+      // heads (and tokens) of the result that overlap would be written twice; an axis of one entry is never stepped over
+      bool apart = p.x_token >= 0 && p.x_head >= 0 && p.y_token >= 0 && p.y_head >= 0;
+      if (apart) {
+        const bool heads_inside = (heads == 1 || p.y_head >= head_dim) && (tokens == 1 || p.y_token >= (heads - 1) * p.y_head + head_dim);
+        const bool tokens_inside = (tokens == 1 || p.y_token >= head_dim) && (heads == 1 || p.y_head >= (tokens - 1) * p.y_token + head_dim);
+        apart = heads_inside || tokens_inside;
+      }
+      if (!apart) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: negative strides, or results that overlap");
     }
     const bool in_place = x == y;
-    if (in_place && (p.x_token != p.y_token || p.x_head != p.y_head))
+    if (in_place && ((tokens > 1 && p.x_token != p.y_token) || (heads > 1 && p.x_head != p.y_head)))
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: in place, both sides need the same strides");
     p.positions = positions;
     // the frequencies of an axis are powers of one ratio; 64-bit mantissas keep the 53 bits that double would round to

@@ -10,7 +10,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_device_ops import F, KIND, TYPES, U, assert_within, check_norm, gen, normal
+from test_device_ops import F, KIND, TYPES, U, assert_within, check_norm, check_rotary, gen, normal
 
 
 def attend(pkg, q, k, v, element, scale=0.0, lens=None):
@@ -312,3 +312,45 @@ def test_swish_at_the_ends_of_the_numbers(pkg, element):
     assert torch.equal(y[0, 0, :6], beta[:6].to(KIND[element]))
     assert (got[:, 6:13].abs() < 1e-35).all()
     assert torch.isnan(got[:, 13:15]).all()
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+ONE_OF = [(1, 4, (0, 64, 0, 64)), (1, 4, (64, 64, 8, 80)), (1, 4, (7, 65, 3, 66)), (5, 1, (64, 0, 64, 0)), (5, 1, (80, 8, 72, 3)), (1, 1, (0, 0, 0, 0)),
+          (1, 4, (0, 0, 0, 64))]
+
+
+@pytest.mark.parametrize("tokens,heads,strides", ONE_OF)
+def test_the_stride_of_an_axis_of_one_entry_says_nothing(pkg, tokens, heads, strides):
+    """One token's, or one head's, step is never taken: host memory is what is refused here, not strides."""
+    import numpy as np
+
+    keep = [np.zeros(1024, np.float32) for _ in range(3)]
+    x, y, positions = (a.ctypes.data for a in keep)
+    with pytest.raises(pkg.NcnnB200Error, match="device memory"):
+        pkg.op_rotary_axes(x, y, "f32", tokens, heads, 64, positions, [32], strides=strides)
+    with pytest.raises(pkg.NcnnB200Error, match="device memory"):  # in place: strides that are stepped with have to agree
+        pkg.op_rotary_axes(x, x, "f32", tokens, heads, 64, positions, [32],
+                           strides=(strides[2] + (8 if tokens == 1 else 0), strides[3] + (8 if heads == 1 else 0), *strides[2:]))
+
+
+def test_strides_that_are_stepped_with_are_still_refused(pkg):
+    import numpy as np
+
+    keep = [np.zeros(1024, np.float32) for _ in range(3)]
+    x, y, positions = (a.ctypes.data for a in keep)
+    for tokens, heads, strides in ((1, 4, (0, 64, 0, 63)), (5, 1, (64, 0, 63, 0)), (2, 2, (128, 64, 64, 64)), (1, 4, (-1, 64, 0, 64)), (5, 1, (64, 0, 64, -1)),
+                                   (2, 2, (128, 64, 100, 64))):
+        with pytest.raises(pkg.NcnnB200Error, match="strides"):
+            pkg.op_rotary_axes(x, y, "f32", tokens, heads, 64, positions, [32], strides=strides)
+    for tokens, heads, strides in ((2, 1, (64, 64, 72, 64)), (1, 2, (64, 64, 64, 72))):
+        with pytest.raises(pkg.NcnnB200Error, match="in place"):
+            pkg.op_rotary_axes(x, x, "f32", tokens, heads, 64, positions, [32], strides=strides)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_of_one_token_or_one_head(pkg, element, interleaved):
+    for tokens, heads, strides in ONE_OF[:-1]:
+        check_rotary(pkg, element, tokens, heads, 64, [10, 16], interleaved, False, strides=strides)
+    check_rotary(pkg, element, 1, 4, 64, [10, 16], interleaved, True, strides=(0, 64, 0, 64), in_place=True)
