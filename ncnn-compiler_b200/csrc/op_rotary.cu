@@ -150,6 +150,7 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: an array does not start at a multiple of its elements' size");
     if (tokens < 0 || tokens > (1ll << 31) || heads <= 0 || heads > 65536 || head_dim <= 0 || head_dim > 65536 || axes <= 0 || axes > kMaxAxes)
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: tokens must be 0 to 2^31, heads and head_dim 1 to 65536, axes 1 to 4");
+    if (position_rows < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: position_rows must not be negative");
     if (!(base >= 1.0) || !(base <= 1e30)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: base must be 1 to 1e30");
     RotaryParams p{};
     int64_t pairs = 0;
@@ -159,7 +160,7 @@ extern "C" int ncnn_b200_op_rotary_axes(const void* x, void* y, int32_t type, in
     }
     if (pairs <= 0 || pairs > kMaxPairs || 2 * pairs > head_dim)
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_rotary_axes: the sections must hold 1 to 128 pairs, and head_dim twice as many components");
-    if (position_rows <= 0 || position_rows > tokens) position_rows = tokens;
+    if (position_rows == 0 || position_rows > tokens) position_rows = tokens;
     if (tokens == 0) return NCNN_B200_STATUS_SUCCESS;
     p.x = x;
     p.y = y;

@@ -354,3 +354,15 @@ def test_rotary_of_one_token_or_one_head(pkg, element, interleaved):
     for tokens, heads, strides in ONE_OF[:-1]:
         check_rotary(pkg, element, tokens, heads, 64, [10, 16], interleaved, False, strides=strides)
     check_rotary(pkg, element, 1, 4, 64, [10, 16], interleaved, True, strides=(0, 64, 0, 64), in_place=True)
+
+
+def test_a_negative_number_of_positions_is_refused(pkg):
+    """0 stands for one to each token; below that is a mistake of the caller, whose array may have any size."""
+    import numpy as np
+
+    keep = [np.zeros(1024, np.float32) for _ in range(3)]
+    x, y, positions = (a.ctypes.data for a in keep)
+    for rows, says in ((-1, "position_rows"), (-(1 << 40), "position_rows"), (0, "device memory"), (2, "device memory"), (1 << 40, "device memory")):
+        with pytest.raises(pkg.NcnnB200Error, match=says) as err:
+            pkg.op_rotary_axes(x, y, "f32", 2, 1, 64, positions, [32], position_rows=rows)
+        assert err.value.status == 2
