@@ -315,7 +315,9 @@ extern "C" int ncnn_b200_op_cross_attention(const void* q, const void* k, const 
         heads % kv_heads != 0 || head_dim <= 0 || head_dim > 256)
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE,
                      "op_cross_attention: batch 0 to 65535, lengths 0 to 2^30, heads a multiple of kv_heads up to 65535, head_dim 1 to 256");
-    if (!(scale >= 0.0f) || std::isinf(scale)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_cross_attention: scale must be finite and not negative");
+    // (the kernels' exponentials are powers of two: scale / ln 2 has to be a number, too)
+    if (!(scale >= 0.0f) || std::isinf(scale * 1.44269504088896340736f))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_cross_attention: scale must not be negative, and scale / ln 2 finite");
     if (batch == 0 || lq == 0) return NCNN_B200_STATUS_SUCCESS;
     if (q == nullptr || o == nullptr || (lk > 0 && (k == nullptr || v == nullptr)))
       return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_cross_attention: NULL argument");

@@ -206,6 +206,18 @@ def test_many_keys_of_little_weight_behind_few_of_much(pkg, element, lq, lk, hea
     assert_within(o, want, off * want + lost)
 
 
+def test_a_scale_past_the_largest_number_is_refused(pkg):
+    """The kernels multiply scores by scale / ln 2; infinite, it would make a NaN of a score of 0."""
+    import numpy as np
+
+    keep = [np.zeros(64, np.float32) for _ in range(4)]
+    q, k, v, o = (a.ctypes.data for a in keep)
+    for scale, says in ((2.4e38, "scale"), (3.4e38, "scale"), (2.3e38, "device memory"), (1e-45, "device memory")):
+        with pytest.raises(pkg.NcnnB200Error, match=says) as err:
+            pkg.op_cross_attention(q, k, v, o, "f32", 1, 1, 1, 1, 1, 8, scale=scale)
+        assert err.value.status == 2
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 @pytest.mark.gpu
 @pytest.mark.parametrize("element", TYPES)
