@@ -234,9 +234,10 @@ int ncnn_b200_op_group_norm(const void *x, void *y, int32_t type, int64_t n, int
  * is host memory), axis 0 the first ones.  Pair (u, v) becomes (u cos t - v sin t, u sin t + v cos t) with
  * t = positions[token % position_rows][axis] * base^(-j / P): j counts an axis's own pairs and P is its section, or with
  * `shared_spectrum` j counts all pairs and P is their sum.  The other components are copied.  positions is [position_rows]
- * [axes] on the device, position_rows 0 = tokens; any 32-bit position, negative ones too, to 2^-32 turns.  strides (host, in
- * elements: x token, x head, y token, y head) or NULL for dense arrays.  y may be x (same strides); other overlaps are not
- * allowed.  At most 128 pairs. */
+ * [axes] on the device, position_rows 0 = tokens; any 32-bit position, negative ones too: angles are good to 2^-25 of a turn
+ * (fp32's rounding of half turns; the frequencies add up to 2^-30 at a position of 2^31).  strides (host, in
+ * elements: x token, x head, y token, y head) or NULL for dense arrays; that of an axis of one entry may be anything.  y may be x
+ * (same strides); other overlaps are not allowed.  At most 128 pairs. */
 int ncnn_b200_op_rotary_axes(const void *x, void *y, int32_t type, int64_t tokens, int32_t heads, int32_t head_dim,
                              const int64_t *strides, const int32_t *positions, int64_t position_rows, int32_t axes,
                              const int32_t *sections, double base, int32_t interleaved, int32_t shared_spectrum,
@@ -247,7 +248,7 @@ int ncnn_b200_op_rotary_axes(const void *x, void *y, int32_t type, int64_t token
  * h / (heads / kv_heads); head_dim 1 to 256.
  *   o = sum_j softmax_j(scale * q.k_j) v_j   over j < kv_lens[batch] (int32, NULL = lk; held to 0..lk) with
  *   key_mask[batch][j] != 0 (bytes [batch][lk], NULL = all).
- * scale 0 = 1 / sqrt(head_dim).  A sequence that is left without a key gets zeros, and so does a query whose every score is minus
+ * scale 0 = 1 / sqrt(head_dim); scale / ln 2 has to be finite.  A sequence that is left without a key gets zeros, and so does a query whose every score is minus
  * infinity.  Whatever lies at a key that takes no part is not used, NaN and infinity included.  strides: host, 12 numbers in
  * elements, {batch, row, head} of q, k, v and o in that order, NULL for dense arrays; components are always next to one
  * another.  o must not overlap an input.

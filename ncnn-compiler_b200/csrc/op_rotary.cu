@@ -5,8 +5,9 @@
 //
 // Angles.  fp32 products lose a far position's angle (position 100 000: 0.008 rad).  A frequency is held as turns
 // per position in 64-bit fixed point, F = frequency / 2 pi * 2^64; position * F modulo 2^64 is the fraction of a turn:
-// the wrap of the integer product is the range reduction, exact to position * 2^-65 turns for every 32-bit position,
-// negative ones too.  The signed product over 2^63 is in half turns, which sincospif takes.
+// the wrap of the integer product is the range reduction, exact for every 32-bit position, negative ones too.  F itself is off by
+// its rounding and by those of the powers before it (up to 127 products of 64-bit mantissas): 2^-30 of a turn at a position of 2^31.
+// The signed product over 2^63 is in half turns, which sincospif takes as fp32: off by 2^-26 of a turn.
 //
 // Bound: HBM, each element read and written once.  A thread turns the same pairs of several heads of a token, so
 // that angles are computed once per `heads_per_thread` heads.

@@ -378,3 +378,27 @@ def test_a_negative_number_of_positions_is_refused(pkg):
         with pytest.raises(pkg.NcnnB200Error, match=says) as err:
             pkg.op_rotary_axes(x, y, "f32", 2, 1, 64, positions, [32], position_rows=rows)
         assert err.value.status == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("base", [1.01, 2.0, 10000.0])
+def test_angles_of_far_positions_of_slow_spectra(pkg, base):
+    """Frequencies close to one another and positions at the ends of their type, against 60 digits: 2^-25 of a turn, sincospif's own
+    2 F, and F for each product with (1, 0)."""
+    from decimal import Decimal, getcontext
+
+    getcontext().prec = 60
+    turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    at = [0, 1, -1, (1 << 31) - 1, -(1 << 31), 2000000011, -1999999973, 123456789]
+    positions = torch.tensor(at, dtype=torch.int32, device="cuda").view(-1, 1).contiguous()
+    x = torch.zeros(len(at), 1, 256, device="cuda")
+    x[..., :128] = 1
+    y = torch.empty_like(x)
+    pkg.op_rotary_axes(x.data_ptr(), y.data_ptr(), "f32", len(at), 1, 256, positions.data_ptr(), [128], base)
+    want = torch.empty(len(at), 256, dtype=torch.float64)
+    for i, p in enumerate(at):
+        for j in range(128):
+            part = p * (-Decimal(base).ln() * j / 128).exp() / turn
+            angle = 2 * math.pi * float(part - part.to_integral_value())
+            want[i, j], want[i, 128 + j] = math.cos(angle), math.sin(angle)
+    assert_within(y.view(len(at), 256), want.cuda(), torch.full((len(at), 256), 2 * math.pi * 2.0 ** -25 + 4 * F, device="cuda"))
