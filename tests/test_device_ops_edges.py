@@ -10,7 +10,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_device_ops import F, KIND, TYPES, U, assert_within, check_norm, check_rotary, gen, normal
+from test_device_ops import F, KIND, TYPES, U, assert_within, attend_want, check_norm, check_rotary, gen, normal
 
 
 def attend(pkg, q, k, v, element, scale=0.0, lens=None):
@@ -216,6 +216,18 @@ def test_a_scale_past_the_largest_number_is_refused(pkg):
         with pytest.raises(pkg.NcnnB200Error, match=says) as err:
             pkg.op_cross_attention(q, k, v, o, "f32", 1, 1, 1, 1, 1, 8, scale=scale)
         assert err.value.status == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("lq,lk,heads,kv_heads", [(1, 3000, 8, 2), (20, 5000, 2, 1), (150, 700, 4, 4), (600, 100, 40, 40)])
+def test_a_sequence_alone_has_its_value_of_a_batch(pkg, element, lq, lk, heads, kv_heads):
+    """Keys may be cut over other CTAs than in a batch: the same value within the arithmetic's bound, not always the same bits."""
+    q, k, v = (normal(gen(n), 3, l, h, 64).to(KIND[element]) for n, l, h in ((0, lq, heads), (1, lk, kv_heads), (2, lk, kv_heads)))
+    batch, alone = attend(pkg, q, k, v, element), attend(pkg, q[1:2], k[1:2], v[1:2], element)
+    want, bound = attend_want(q[1:2], k[1:2], v[1:2], torch.ones(1, lk, dtype=torch.bool, device="cuda"), 0.125, element)
+    assert_within(alone, want, bound)
+    assert_within(batch[1:2], want, bound)
 
 
 # ------------------------------------------------------------------------------------------------ group norm

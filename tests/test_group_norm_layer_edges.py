@@ -3,9 +3,21 @@ import numpy as np
 import pytest
 
 from conftest import rel_l2
-from test_group_norm_layer import TOL
+from test_group_norm_layer import TOL, graph, refusal
 
 F = 2.0 ** -24
+
+
+def test_groups_that_no_cta_holds_are_refused_at_load(pkg, tmp_path):
+    """256 threads of four channels each (of one, where the channels are no multiple of four), over whole accesses."""
+    for channels, groups in ((1028, 1), (257, 1), (2056, 2), (514, 2), (1028, 4)):  # (the last: only all four groups are whole accesses)
+        status, message = refusal(pkg, tmp_path, f"0={groups} 1={channels}", f"0=2 1=2 2={channels}", (np.ones(channels), np.zeros(channels)))
+        assert status == 8 and "so many channels" in message, (channels, groups)
+    for channels, groups in ((1024, 1), (255, 1), (2048, 2), (510, 2), (1024, 4)):
+        weights = (np.ones(channels), np.zeros(channels))
+        param, bin_ = graph(pkg, tmp_path / "m", [("Input", "input", [], ["data"], f"0=2 1=2 2={channels}"),
+                                                  ("GroupNorm", "norm", ["data"], ["output"], f"0={groups} 1={channels}")], weights)
+        assert pkg.Model(param, bin_, plan_only=True).output_shapes == [(channels, 2, 2)]
 
 
 @pytest.mark.gpu
