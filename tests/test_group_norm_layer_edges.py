@@ -57,3 +57,13 @@ def test_an_operand_that_a_convolution_reads_too(pkg, oracle, tmp_path, mode, fi
     plain = pkg.Model(param, bin_, accuracy_mode=mode, use_cuda_graph=False)
     for name, alone, value in zip(model.output_names, model.run(x[2]), plain.run(x)):
         assert np.array_equal(got[name][2], alone) and np.array_equal(got[name], value)
+
+
+@pytest.mark.gpu
+def test_a_batch_that_is_uploaded_in_pieces(pkg, tmp_path, monkeypatch):
+    """16 MB of inputs: the first layers run piece by piece while the next piece is on its way, with the bits of the whole batch."""
+    param, bin_ = pkg.zoo.group_norm_block(str(tmp_path / "block"), h=64, w=64, c=64, cout=32, groups=8)
+    x = (np.random.default_rng(1).standard_normal((16, 64, 64, 64)) + 3).astype(np.float32)
+    got = pkg.Model(param, bin_).run(x)[0]
+    monkeypatch.setenv("NCNN_B200_PIPELINE", "0")
+    assert np.array_equal(got, pkg.Model(param, bin_).run(x)[0])
