@@ -94,6 +94,7 @@ __device__ __forceinline__ void recentre(float n, float inverse, float& shift, f
 constexpr int kNormThreads = 256;
 constexpr int kNormMostGroups = 128;
 constexpr int kNormGroup = 4;   // pixels that are asked for together
+constexpr int kNormFirstMove = 64;  // pixels of a thread before its shift moves
 
 template <int V>
 constexpr int kNormSlots = V == 8 ? 12 : 16;  // pixels of a thread's ring (three CTAs' rings and statistics fit an SM)
@@ -121,8 +122,9 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
   else if constexpr (BYTES >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 
+// LONG: ranges of more than 64 pixels to a thread.
 // fp32 tensors are those of a loaded graph, too, in whatever format their other readers and writers want.
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool LONG>
 __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_constant__ NormParams p, const __grid_constant__ NormShape s) {
   namespace cg = cooperative_groups;
   using Vec = OpVec<T, V>;
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  constexpr int kAhead = kNormSlots<V> / kNormGroup - 1, kFirstMove = 64 / kNormGroup;
+  constexpr int kAhead = kNormSlots<V> / kNormGroup - 1;
 
   Moments part[V];
   {
@@ -205,15 +207,16 @@ __global__ void __launch_bounds__(kNormThreads, 3) k_group_norm(const __grid_con
           }
         }
     };
-    // (two loops: short ranges need no move of the shift and pay little for it; 8 maps of 64 x 64 x 320 take 20.2 us, 20.6 with one loop)
+    // (ranges that need no move of the shift have a kernel without one: code that they only pass cost 8 maps of 64 x 64 x 320 0.6 of 20 us)
     int g = 0;
-    for (const int until = min(kFirstMove, steps); g < until; ++g) add(g);
-    for (int until = kFirstMove; g < steps;) {
-      const float n = static_cast<float>(g * kNormGroup), inverse = 1.0f / n;
+    for (int until = LONG ? min(kNormFirstMove / kNormGroup, steps) : steps; g < steps;) {
+      for (; g < until; ++g) add(g);
+      if (LONG && g < steps) {
+        const float n = static_cast<float>(g * kNormGroup), inverse = 1.0f / n;
 #pragma unroll
-      for (int v = 0; v < V; ++v) recentre(n, inverse, shift[v], s1[v], s2[v]);
-      until *= 4;
-      for (const int to = min(until, steps); g < to; ++g) add(g);
+        for (int v = 0; v < V; ++v) recentre(n, inverse, shift[v], s1[v], s2[v]);
+        until = min(4 * until, steps);
+      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const float inverse = count > 0 ? 1.0f / static_cast<float>(count) : 0.0f;
@@ -415,8 +418,10 @@ int launch_shape(const NormParams& p, int take, int device, cudaStream_t st) {
   s.each = static_cast<int>(each);
   s.slots = static_cast<int>(std::min<long long>((each + s.rows - 1) / s.rows, kNormSlots<V>));
   const int smem = s.slots * kSlot + s.rows * s.channels * static_cast<int>(sizeof(Moments));
-  auto kernel = k_group_norm<T, V, ACT>;
-  static std::atomic<uint64_t> granted{0};
+  const bool far = (each + s.rows - 1) / s.rows > kNormFirstMove;
+  auto kernel = far ? k_group_norm<T, V, ACT, true> : k_group_norm<T, V, ACT, false>;
+  static std::atomic<uint64_t> grants[2];
+  std::atomic<uint64_t>& granted = grants[far ? 1 : 0];
   const uint64_t bit = 1ull << (device & 63);
   if (device >= 64 || !(granted.load(std::memory_order_acquire) & bit)) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
