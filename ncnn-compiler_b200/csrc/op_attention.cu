@@ -149,10 +149,14 @@ int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
 
 template <class T>
 int attend_tc(const AttendParams& a, int device, int sms, cudaStream_t st) {
+  // Two tiles to a CTA, whose MMAs and softmaxes take turns, or one, and two CTAs to an SM (heads above 128: one).  Device times, bf16,
+  // two and one: 2048 queries over 2048 keys, 16 heads of 128 37 and 40 us (of 64: 30 and 32); 4096 over 4096, 40 heads of 128 360 and
+  // 363; but 4096 over 4096, 10 heads of 128 118 and 114, and grids that do not fill the device: 1024 over 1024, 10 heads of 64
+  // 16.8 and 14.3, 300 over 3000, 16 heads of 128 44 and 38.  Full grids decide.
   const bool two = a.lq > kAttRows;
   const long long tiles = static_cast<long long>((a.lq + kAttRows - 1) / kAttRows) * a.heads * a.batch;
-  // one block of keys and a tile for every SM: 4096 queries over 77 keys (8 sequences, 10 heads of 64) 27 us, 55 with a CTA to two
-  // tiles
+  // one block of keys and a tile for every SM: 4096 queries over 77 keys (8 sequences, 10 heads of 64) 28.6 us of device time, 57 with
+  // a CTA to two tiles
   if (a.lk <= kAttRows && a.d <= 128 && tiles >= sms && tiles < (1 << 30))
     return a.d <= 64 ? launch_short<T, 64>(a, device, sms, st) : launch_short<T, 128>(a, device, sms, st);
   if (a.d <= 64) return two ? launch_tc<T, 64, 2>(a, device, st) : launch_tc<T, 64, 1>(a, device, st);
@@ -178,8 +182,9 @@ int launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
 
 // Whether a call is one of few queries.  At most two tiles of 16 to a key head always are.  So are up to 160 tiles over 512 keys or
 // more where the tensor-core kernel, which gives a head's 128 queries to one CTA from the first key to the last, would use less
-// than half of the SMs: 8 heads of 64 queries over 4096 keys 12 us against 46, of 128 queries 24 against 52, of 256 over 8192
-// (128 tiles) 75 against 112; 32 heads of 64 over 1024 (128 tiles) 15 against 16.
+// than half of the SMs.  Device times, bf16, this kernel and that one: 8 heads of 64 (128) of 64 queries over 4096 keys 12 (16) us
+// against 46 (49), of 128 queries 16 (24) against 47 (49), of 256 over 8192 keys (128 tiles) 46 (74) against 104 (108); 32 heads
+// of 64 queries over 1024 keys (128 tiles) 10.6 (15.3) against 14.2 (15.4).
 bool few_queries(const AttendParams& p, int sms) {
   const long long rows = static_cast<long long>(p.lq) * (p.heads / p.kv_heads), row_tiles = (rows + kFewRows - 1) / kFewRows;
   if (p.kv_heads * row_tiles > 65535) return false;
@@ -244,6 +249,10 @@ cudaError_t attend_f32(const AttendParams& a, int device, int sms, cudaStream_t 
   p.a = a;
   p.scale_log2 = a.scale * 1.44269504088896340736f;
   const long long rows = static_cast<long long>(a.lq) * (a.heads / a.kv_heads);
+  // Up to 16 rows to a key head in tiles of a few rows over split keys, more in tiles of 64 or 128 rows.  Device times of split and
+  // tiled keys over 4096 keys, one key head of 128: 23 and 135 us with 16 rows, 23 and 136 with 48; eight: 81 and 136 with 16, 106
+  // and 136 with 24, 148 and 137 with 48; 64 key heads of 64 over 1024 keys: 35 and 42 with 8, 57 and 42 with 16, 92 and 43 with 17.
+  // (The crossing lies at 8 rows where key heads fill the device and above 48 where there are few: 16 is between them.)
   if (rows <= 16 && a.kv_heads * rows <= 65535) {
     if (rows == 1) {
       if (a.d <= 64) return launch_split<T, 64, 1, WIDE>(p, sms, st);

@@ -89,8 +89,9 @@ __device__ __forceinline__ void recentre(float n, float inverse, float& shift, f
 // Bound: HBM, x once and y once, where x stays on the SM or in L2 between the passes.  Every thread has a ring of 16 (or 12) of its own
 // pixels in shared memory, filled by cp.async four at a time (no registers for what is under way: 48 KB a CTA, three CTAs to an
 // SM).  The second pass goes backwards: it begins with what the first one left in the ring and goes on with what L2 saw last.
-// Measured: 8 maps of 64 x 64 x 320, bf16 18 us; 2 of 512 x 512 x 128, fp32 162 us, where two thirds of x have to come from
-// HBM again (5 TB/s in each pass; CTAs of 768 threads, stores that leave L2 first, and whole pixels to a CTA were no faster).
+// Device times of captured calls: 8 maps of 64 x 64 x 320, bf16 19.5 us; 2 of 512 x 512 x 128, fp32 162 us, where two thirds of x have
+// to come from HBM again (5 TB/s in each pass; CTAs of 768 threads, stores that leave L2 first, and whole pixels to a CTA were no
+// faster).
 constexpr int kNormThreads = 256;
 constexpr int kNormMostGroups = 128;
 constexpr int kNormGroup = 4;   // pixels that are asked for together

@@ -5,7 +5,7 @@
 // shared memory for its tiles, the next head's are loaded into the other half meanwhile, queries come through a ring.  The two
 // groups of softmax warps take the tiles in turn: while one has its exponentials and its stores, the other's MMAs run, and the
 // CTA's start (barriers, tensor memory, first loads: some 2 us) is paid once an SM instead of once for every two tiles.
-// Measured (8 sequences of 4096 queries over 77 keys, 10 heads of 64, fp16): 27 us, 3.2 TB/s; HBM would allow 13.  A tile takes
+// Measured (8 sequences of 4096 queries over 77 keys, 10 heads of 64, fp16): 28.6 us of device time, 3.0 TB/s; HBM would allow 13.  A tile takes
 // a group some 4000 clocks, of which 1100 are exponentials and the rest the chain scores - maximum - products - results, of
 // which the two groups hide half.
 #pragma once
