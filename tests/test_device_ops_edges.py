@@ -10,7 +10,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_device_ops import F, KIND, TYPES, U, assert_within, attend_want, check_norm, check_rotary, gen, normal
+from test_device_ops import F, KIND, TYPES, U, assert_within, attend_want, check_attend, check_norm, check_rotary, gen, normal, rotary_want
 
 
 def attend(pkg, q, k, v, element, scale=0.0, lens=None):
@@ -414,3 +414,55 @@ def test_angles_of_far_positions_of_slow_spectra(pkg, base):
             angle = 2 * math.pi * float(part - part.to_integral_value())
             want[i, j], want[i, 128 + j] = math.cos(angle), math.sin(angle)
     assert_within(y.view(len(at), 256), want.cuda(), torch.full((len(at), 256), 2 * math.pi * 2.0 ** -25 + 4 * F, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------------ the ends of the ranges
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+def test_more_images_than_a_grid_has_rows(pkg, element):
+    check_norm(pkg, element, 70000, 3, 4, 2, "swish")
+    check_norm(pkg, element, 66000, 2, 6, 2, "none", in_place=True, x_pitch=7, y_pitch=7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+def test_the_most_sequences_and_heads(pkg, element):
+    q, k, v = (normal(gen(n), 65535, l, 1, 8).to(KIND[element]) for n, l in ((0, 1), (1, 3), (2, 3)))
+    o = attend(pkg, q, k, v, element)
+    p = torch.softmax((q.double() * k.double()).sum(-1)[:, :, 0] * 8 ** -0.5, 1)
+    want, spread = (p[..., None] * v[:, :, 0].double()).sum(1), (p[..., None] * v[:, :, 0].double().abs()).sum(1)
+    # attend_want's bound for 8 components and 3 keys of sizes up to 6: scores to 24 F * 6 * 6 * 8 / sqrt(8), the probability's rounding
+    rel = 2 * 24 * F * 6 * 6 * 8 ** 0.5 + 28 * F + (U[element] if element != "f32" else 0)
+    assert_within(o[:, 0, 0], want, rel * spread + U[element] * (want.abs() + rel * spread) + 2.0 ** -23 * v.abs().max() * (element == "f16") + 2.0 ** -25)
+    q = normal(gen(0), 1, 1, 65535, 8).to(KIND[element])
+    k, v = (normal(gen(n), 1, 40, 1, 8).to(KIND[element]) for n in (1, 2))
+    o = attend(pkg, q, k, v, element)
+    # every head reads the same keys: heads are queries of one head
+    want, bound = attend_want(q.view(1, 65535, 1, 8), k, v, torch.ones(1, 40, dtype=torch.bool, device="cuda"), 8 ** -0.5, element)
+    assert_within(o.view(1, 65535, 1, 8), want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("lq", [1, 140])
+def test_keys_and_values_that_overlap_in_memory(pkg, element, lq):
+    """Windows of one signal: rows of 64 components, 8 (and 4) elements from one to the next."""
+    for step in (8, 4):
+        check_attend(pkg, element, 1, lq, 300, 2, 1, 64, strides=(lq * 128, 128, 64, 0, step, 64, 0, step, 64, lq * 128, 128, 64))
+
+
+@pytest.mark.gpu
+def test_rotary_of_more_threads_than_a_launch(pkg):
+    """2^23 + 70 tokens of 128 pairs at an odd address, 2^30 pairs to a launch: the last tokens belong to a second one, and positions
+    repeat through both."""
+    tokens, rows, d = (1 << 23) + 70, 1000, 256
+    x = torch.empty(tokens * d + 1, device="cuda", dtype=torch.float16)
+    view = x[1:].view(tokens, d)
+    some = torch.cat([torch.arange(0, 40), torch.arange((1 << 23) - 40, tokens)]).cuda()
+    view.zero_()
+    view[some] = normal(gen(1), some.numel(), d).half()
+    positions = torch.randint(-1000, 1000, (rows, 2), generator=gen(2), device="cuda", dtype=torch.int64).to(torch.int32)
+    want, mag = rotary_want(view[some].view(-1, 1, d), positions[some % rows], [64, 64], 10000.0, True, False)
+    pkg.op_rotary_axes(x.data_ptr() + 2, x.data_ptr() + 2, "f16", tokens, 1, d, positions.data_ptr(), [64, 64], 10000.0, True, False, rows)
+    assert_within(view[some].view(-1, 1, d), want, 10 * F * mag + U["f16"] * (want.abs() + 10 * F * mag) + 2.0 ** -25)
+    assert not view[1 << 20].any()
