@@ -258,6 +258,87 @@ int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, vo
                                  const int64_t *strides, const int32_t *kv_lens, const uint8_t *key_mask, float scale,
                                  void *stream);
 
+/* ---- A decoder in 8-bit integers: products whose activations are quantised token by token, a paged cache of keys and values, and
+ * attention over it.  (The reference quantises with scales known ahead; these find them in the data.)  What is said above of arrays,
+ * streams and refusals holds here too.
+ *
+ * A row of numbers becomes 8-bit integers and a step:  top = max |x|, step = top / 127, q = 127 x / top rounded to the nearest whole
+ * number, halves away from zero (exactly: the integers are those of real arithmetic).  A row whose top is below 2^-100 is held as
+ * zeros with step 0; one with an infinity or NaN as zeros with step NaN, so that what is computed from it says so. */
+
+/* Rows x [rows][columns] as integers q and steps [rows].  Pitches are the elements from one row to the next (0 = columns); bytes of q
+ * between rows are left as they are.  Also what weights for the products below are laid out with: a row to a channel. */
+int ncnn_b200_op_quantize_rows(const void *x, int32_t type, int64_t rows, int32_t columns, int64_t x_pitch, int8_t *q,
+                               int64_t q_pitch, float *steps, void *stream);
+
+/* InnerProduct of tokens in 8-bit integers with a scale for each token and each channel:
+ *   y[t][c] = act(steps[t] * weight_steps[c] * sum_i q[t][i] weight[c][i] + bias[c]),
+ * q and steps the rows of x [tokens][k] as above, the sum exact.  weight is int8 [n] rows of k at weight_pitch bytes (0 = k),
+ * weight_steps and bias fp32 [n] (bias may be NULL), y [tokens][n] of x's type; pitches of x and y in elements (0 = k, n).
+ * Weights that start at a multiple of 16 bytes with a pitch that is one run on the tensor cores.  k up to 131072 (so that no sum
+ * passes 32 bits).  The integers of x pass through `workspace`: device memory, at a multiple of 16 bytes, of as many bytes as
+ * ncnn_b200_op_inner_product_tokens_workspace says (negative for sizes that a call refuses); calls that may overlap need one each. */
+int64_t ncnn_b200_op_inner_product_tokens_workspace(int64_t tokens, int32_t k);
+int ncnn_b200_op_inner_product_tokens(const void *x, void *y, int32_t type, int64_t tokens, int32_t k, int32_t n,
+                                      int64_t x_pitch, int64_t y_pitch, const int8_t *weight, int64_t weight_pitch,
+                                      const float *weight_steps, const float *bias, int32_t activation, void *workspace,
+                                      int64_t workspace_bytes, void *stream);
+
+/* Keys and values of many sequences in pages: integers k, v [pages][kv_heads][page_size][row], a row being head_dim rounded up to a
+ * multiple of 16 bytes, and k_steps, v_steps [pages][kv_heads][page_size].  page_size is a power of two from 16 to 1024, head_dim
+ * 1 to 256; k and v start at multiples of 16 bytes, steps at multiples of 16, too. */
+typedef struct ncnn_b200_cache {
+  int8_t *k;
+  int8_t *v;
+  float *k_steps;
+  float *v_steps;
+  int64_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+} ncnn_b200_cache;
+
+/* Which tokens a call is about: the last ones of each sequence.  Sequence s has lens[s] tokens with these (int32 on the device; held
+ * to 0..max_len), and rows starts[s] to starts[s + 1] - 1 of the call's arrays are its last ones, in order (int32 [sequences + 1] on the
+ * device, ascending, held to 0..tokens; NULL: one row to each sequence).  Position p of sequence s lies in row p % page_size of page
+ * table[s * table_width + p / page_size] (int32 on the device).  A page outside the cache is not there: nothing is written to it, and
+ * keys in it take no part.  A row before a sequence's first position (more rows than lens) has no place, either.  Rows of the arrays
+ * behind the last sequence's are left as they are.
+ * max_tokens: no sequence has more rows than this (0 = tokens); rows above it are left as they are.  max_len: no sequence is longer
+ * (0 = table_width * page_size, which is the most).  Both are limits that the host knows: launches are sized by them. */
+typedef struct ncnn_b200_cache_batch {
+  const int32_t *table;
+  const int32_t *lens;
+  const int32_t *starts;
+  int64_t sequences;
+  int64_t tokens;
+  int32_t table_width;
+  int32_t max_tokens;
+  int64_t max_len;
+} ncnn_b200_cache_batch;
+
+/* Quantises keys and values [tokens][kv_heads][head_dim] into the pages of their positions.  strides: host, four numbers in elements,
+ * {token, head} of k and of v, NULL for dense arrays.  Pages that a call writes to belong to one sequence each. */
+int ncnn_b200_op_cache_write(const ncnn_b200_cache *cache, const ncnn_b200_cache_batch *batch, const void *k, const void *v,
+                             int32_t type, const int64_t *strides, void *stream);
+/* The same tokens' values, integer times step, rounded to the type.  k or v may be NULL.  Rows without a place get zeros. */
+int ncnn_b200_op_cache_read(const ncnn_b200_cache *cache, const ncnn_b200_cache_batch *batch, void *k, void *v, int32_t type,
+                            const int64_t *strides, void *stream);
+
+/* Causal attention of the batch's tokens to their sequences' pages: q, o [tokens][heads][head_dim]; a token at position p of its
+ * sequence has the keys 0 to p, its own among them (write before): o = sum_j softmax_j(scale * q.k_j) v_j.  heads is a multiple of
+ * kv_heads and query head h reads key head h / (heads / kv_heads); scale 0 = 1 / sqrt(head_dim); strides as above, of q and of o.
+ * shared: the first `shared` positions (a multiple of page_size) of every sequence lie in the pages that the table's first row names;
+ * they are read once for all sequences.  0: none.  A token that has no key gets zeros.  Results do not depend on which other
+ * sequences are in the batch beyond the order of sums.  Values of tokens should be below 2^110.
+ * workspace: device memory at a multiple of 16 bytes, of as many bytes as ncnn_b200_op_cache_attention_workspace says for the same
+ * cache, batch, heads and shared (0: none is needed; negative: the call would be refused); calls that may overlap need one each. */
+int64_t ncnn_b200_op_cache_attention_workspace(const ncnn_b200_cache *cache, const ncnn_b200_cache_batch *batch, int32_t heads,
+                                               int64_t shared);
+int ncnn_b200_op_cache_attention(const ncnn_b200_cache *cache, const ncnn_b200_cache_batch *batch, const void *q, void *o,
+                                 int32_t type, int32_t heads, const int64_t *strides, int64_t shared, float scale,
+                                 void *workspace, int64_t workspace_bytes, void *stream);
+
 /* The tensor-core kernels of ncnn_b200_op_cross_attention bound their waits (2 s each).  This waits for the current device and
  * for every device that such a call went to, and returns 7, once to each thread, when one of the waits ran out, on any of them and
  * in any thread's call, since that thread's last such call (its first: since the library was loaded); 0 otherwise. */

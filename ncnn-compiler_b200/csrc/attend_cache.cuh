@@ -1,0 +1,482 @@
+// Attention over a paged cache of 8-bit integers for few rows: a pass over the pages at HBM speed.
+//
+// A CTA has a tile of 16 rows that read one key head (a row is a token and one of the head's query heads) and a range of keys; its
+// warps take blocks of 16 keys in turn, each with a running maximum, sum and result.  The products are mma.sync m16n8k16: HBM is the
+// bound, not the tensor cores, and tcgen05 would want 128 rows.
+//
+// Integers are exact in either 16-bit type (|q| is at most 127), so the steps stay out of the products: a key's multiplies its scores,
+// a value's its probabilities.  No integer is exchanged between lanes.  The contraction's order is free: a lane takes 16 neighbouring
+// bytes of "its" keys as the operands of four products, and the queries are permuted to match; for values it takes the same
+// components of four keys and picks one byte of each.  So a lane copies (cp.async) only what it reads itself, into a queue
+// of its own in shared memory: no barriers, and every access of shared memory takes neighbouring 16 bytes for neighbouring lanes.
+//
+// Roundings: scores of 16-bit queries are exact products (f32 queries: three bf16 terms, 24 bits); probabilities times steps are
+// split into two bf16 terms (16 bits), f32 three.
+//
+// The ranges' results go to the caller's workspace with their maximum (of scores in powers of two) and sum, and k_attend_cache_join
+// puts them together in the order of the keys; one range alone writes its result itself.
+#pragma once
+
+#include "attend_few.cuh"
+#include "op_cache.h"
+
+namespace nb {
+
+constexpr int kCacheRows = 16;
+
+struct AttendCacheParams {
+  CacheParams c;
+  const void* q;
+  void* o;
+  long long q_token, q_head, o_token, o_head;
+  int heads, rows_a_head;  // query heads; those of one key head
+  float scale_log2;
+  int shared;              // keys 0..shared-1 are the first table row's for all sequences
+  int prefix;              // 1: this launch is about those keys, its rows are all tokens'
+  int chunk;               // keys of a range
+  int first_range;         // number of this launch's first range
+  int prefix_ranges, prefix_chunk, own_ranges, own_chunk;  // for joining
+  float* part;             // [range][token][head][part_width], or null: one range, results go to o
+  float2* part_top;        // [range][token][head]: maximum, sum
+  int part_width;
+  int o_wide;              // four components of o can be stored at a time
+};
+
+// four int8 as two pairs of T (the first in the lower half)
+template <class T> __device__ __forceinline__ uint32_t int8_pair(uint32_t spread);  // integers in bytes 0 and 2
+template <> __device__ __forceinline__ uint32_t int8_pair<__nv_bfloat16>(uint32_t x) {
+  // 128 + the low seven bits, less 128 or 256
+  uint32_t a, b, r;
+  asm("lop3.b32 %0, %1, 0x007f007f, 0x43004300, 0xea;" : "=r"(a) : "r"(x));
+  asm("lop3.b32 %0, %1, 0x00800080, 0x43004300, 0xea;" : "=r"(b) : "r"(x));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void int8_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    // 1024 + (q + 128), less 1152
+    const uint32_t u = w ^ 0x80808080u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+  } else {
+    lo = int8_pair<__nv_bfloat16>(__byte_perm(w, 0u, 0x4140));
+    hi = int8_pair<__nv_bfloat16>(__byte_perm(w, 0u, 0x4342));
+  }
+}
+
+__device__ __forceinline__ void queue_16(uint32_t to, const void* from, bool take) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void queue_8(uint32_t to, const void* from, bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(take ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
+template <class T, int D, int WARPS, int STAGES>
+struct CacheFewShared {
+  static constexpr int kQTerms = sizeof(T) == 4 ? 3 : 1;
+  static constexpr int kValueBytes = D / 8;                    // of a key that a lane takes
+  static constexpr int kKeyBytes = 2 * (D / 64) * 512;         // of a block, a warp
+  static constexpr int kValues = 4 * kValueBytes * 32;
+  static constexpr int kStage = kKeyBytes + kValues + 4 * 256;  // and the steps
+  uint4 q[kQTerms][D / 16][32];                                // fragments by lane
+  union {
+    uint8_t ring[WARPS][STAGES][kStage];
+    struct {
+      float part[WARPS][kCacheRows][D + 4];
+      float top[WARPS][kCacheRows], total[WARPS][kCacheRows];
+    };
+  };
+};
+
+template <class T, int D, int WARPS, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const __grid_constant__ AttendCacheParams p) {
+  using Shared = CacheFewShared<T, D, WARPS, STAGES>;
+  using KT = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
+  using VT = __nv_bfloat16;
+  constexpr int STEPS = D / 16, QTERMS = Shared::kQTerms, PTERMS = sizeof(T) == 4 ? 3 : 2;
+  constexpr int VB = Shared::kValueBytes;
+  extern __shared__ __align__(128) uint8_t cache_few_smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(cache_few_smem);
+  const CacheParams& c = p.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane >> 2, quad = lane & 3;
+  const int range = blockIdx.z, kv_head = blockIdx.y, G = p.rows_a_head;
+  // rows of this tile: 16 from row0 on, of a sequence or of all
+  int sequence = 0;
+  long long row0 = static_cast<long long>(blockIdx.x) * kCacheRows, first = 0, rows;
+  int before = 0;  // position of a sequence's first row
+  if (p.prefix) {
+    rows = c.tokens * G;
+  } else {
+    const int tiles = static_cast<int>((static_cast<long long>(c.max_tokens) * G + kCacheRows - 1) / kCacheRows);
+    sequence = blockIdx.x / tiles;
+    row0 = static_cast<long long>(blockIdx.x % tiles) * kCacheRows;
+    first = cache_start(c, sequence);
+    const long long count = max(cache_start(c, sequence + 1) - first, 0ll);
+    rows = min(count, static_cast<long long>(c.max_tokens)) * G;
+    before = static_cast<int>(max(cache_len(c, sequence) - count, -(1ll << 30)));
+  }
+  if (row0 >= rows) return;
+  // a lane's row: its token and position (lanes 16 to 31 repeat lanes 0 to 15)
+  const long long my_row = row0 + (lane & 15);
+  int my_position = -2;  // -2: no row
+  if (my_row < rows) {
+    if (p.prefix) {
+      const CachePlace place = cache_place(c, my_row / G);
+      my_position = place.sequence < 0 ? -2 : place.position;
+    } else {
+      my_position = max(before + static_cast<int>(my_row / G), -1);
+    }
+  }
+  const int last = __reduce_max_sync(~0u, my_position);
+  const int least = __reduce_min_sync(~0u, my_position < -1 ? 0x7fffffff : my_position);
+  const int from = p.prefix ? range * p.chunk : p.shared + range * p.chunk;
+  const int end = p.prefix ? min(p.shared, last + 1) : last + 1;
+  const int to = min(from + p.chunk, end);
+  if (from >= to && p.part != nullptr) return;  // (whoever joins knows)
+  int position[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) position[r] = __shfl_sync(~0u, my_position, group + 8 * r);
+
+  const long long table_row = p.prefix ? 0 : sequence;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.ring[warp][0][0])) + lane * 16;
+  const uint32_t ring8 = ring - lane * 8;
+  // pages of this warp's next 32 blocks, one to a lane
+  int ahead = 0;
+  auto look_ahead = [&](int i) {
+    const int key = from + (warp + (i + lane) * WARPS) * 16;
+    ahead = key < to ? cache_page(c, static_cast<int>(table_row), key) : -1;
+  };
+  uint32_t held = 0;  // of the blocks under way, the last one lowest: whether their page is there
+  auto request = [&](int stage, int i) {
+    if ((i & 31) == 0) look_ahead(i);
+    const int key = from + (warp + i * WARPS) * 16;
+    const int page = __shfl_sync(~0u, ahead, i & 31);
+    held = held << 1 | (page >= 0 ? 1u : 0u);
+    if (key < to) {
+      const bool take = page >= 0;
+      const int in_page = key & ((1 << c.page_shift) - 1);
+      const long long line = ((take ? static_cast<long long>(page) * c.kv_heads + kv_head : 0) << c.page_shift) + (take ? in_page : 0);
+      const int8_t* k = c.k + line * c.row;
+      const int8_t* v = c.v + line * c.row;
+      const uint32_t at = ring + stage * Shared::kStage;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int cc = 0; cc < D / 64; ++cc) {
+          const int byte = cc * 64 + quad * 16;
+          const bool use = take && byte < c.row;
+          queue_16(at + (n * (D / 64) + cc) * 512, k + (use ? (group + 8 * n) * c.row + byte : 0), use);
+        }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int key_of = 2 * quad + (n & 1) + 8 * (n >> 1);
+        if constexpr (VB == 8) {
+          const bool use = take && group * 8 < c.row;
+          queue_8(ring8 + stage * Shared::kStage + Shared::kKeyBytes + n * 256, v + (use ? key_of * c.row + group * 8 : 0), use);
+        } else {
+#pragma unroll
+          for (int h = 0; h < VB / 16; ++h) {
+            const int byte = group * VB + h * 16;
+            const bool use = take && byte < c.row;
+            queue_16(at + Shared::kKeyBytes + (n * (VB / 16) + h) * 512, v + (use ? key_of * c.row + byte : 0), use);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const uint32_t steps_at = ring8 + stage * Shared::kStage + Shared::kKeyBytes + Shared::kValues + n * 256;
+        queue_8(steps_at, c.k_steps + line + (take ? 2 * quad + 8 * n : 0), take);
+        queue_8(steps_at + 512, c.v_steps + line + (take ? 2 * quad + 8 * n : 0), take);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int blocks = from < to ? ((to - from + 15) / 16 - warp + WARPS - 1) / WARPS : 0;
+#pragma unroll
+  for (int n = 0; n < STAGES - 1; ++n) request(n, n);
+
+  // the queries as A fragments in the order of the keys' bytes: a warp makes every WARPS-th product's
+  for (int s = warp; s < STEPS; s += WARPS) {
+    uint32_t f[QTERMS][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const long long row = row0 + group + 8 * r;
+      const long long token = first + row / G;
+      const int head = kv_head * G + static_cast<int>(row % G);
+      const T* q = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = (s / 4) * 64 + quad * 16 + (s % 4) * 4 + 2 * e;
+        const float x = position[r] > -2 && at < c.d ? op_get(q[at]) : 0.0f, y = position[r] > -2 && at + 1 < c.d ? op_get(q[at + 1]) : 0.0f;
+        if constexpr (QTERMS == 1) {
+          const OpVec<KT, 2> pair{{op_put<KT>(x), op_put<KT>(y)}};
+          f[0][r + 2 * e] = *reinterpret_cast<const uint32_t*>(&pair);
+        } else {
+          uint32_t rest;
+          split_pair<__nv_bfloat16>(x, y, f[0][r + 2 * e], rest);
+          const float x1 = x - __bfloat162float(op_put<__nv_bfloat16>(x)), y1 = y - __bfloat162float(op_put<__nv_bfloat16>(y));
+          split_pair<__nv_bfloat16>(x1, y1, f[1][r + 2 * e], f[2][r + 2 * e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QTERMS; ++t) sh.q[t][s][lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
+  }
+  __syncthreads();
+
+  float o[D / 8][4] = {};
+  float base[2] = {-INFINITY, -INFINITY}, total[2] = {0.0f, 0.0f};
+  const uint32_t q_at = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.q[0][0][0])) + lane * 16;
+  int stage = 0;
+  for (int i = 0; i < blocks; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    const bool there = held >> (STAGES - 2) & 1u;  // (before the next request's shift)
+    request(stage == 0 ? STAGES - 1 : stage - 1, i + STAGES - 1);
+    const uint32_t at = ring + stage * Shared::kStage, at8 = ring8 + stage * Shared::kStage + Shared::kKeyBytes;
+    const int key = from + (warp + i * WARPS) * 16;
+    float s[2][4] = {};
+#pragma unroll
+    for (int cc = 0; cc < D / 64; ++cc) {
+      const uint4 k0 = lds_16(at + cc * 512), k1 = lds_16(at + (D / 64 + cc) * 512);
+      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t b[4];
+        int8_quad<KT>(w0[j], b[0], b[1]);
+        int8_quad<KT>(w1[j], b[2], b[3]);
+#pragma unroll
+        for (int t = QTERMS - 1; t >= 0; --t) {  // (small terms first)
+          const uint4 f = lds_16(q_at + (t * STEPS + cc * 4 + j) * 512);
+          const uint32_t a[4] = {f.x, f.y, f.z, f.w};
+          mma_16x8x16<KT>(s[0], a, b[0], b[1]);
+          mma_16x8x16<KT>(s[1], a, b[2], b[3]);
+        }
+      }
+    }
+    // s[n][e]: row group + 8 (e / 2), key 8 n + 2 quad + e % 2
+    float x[2][4], m[2], value_step[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const uint2 ks = lds_8(at8 + Shared::kValues + n * 256), vs = lds_8(at8 + Shared::kValues + 512 + n * 256);
+      const float f0 = __uint_as_float(ks.x) * p.scale_log2, f1 = __uint_as_float(ks.y) * p.scale_log2;
+      value_step[n][0] = __uint_as_float(vs.x);
+      value_step[n][1] = __uint_as_float(vs.y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] = s[n][e] * (e & 1 ? f1 : f0);
+    }
+    const bool whole = there && key + 15 <= least && key + 15 < to;
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at_key = key + 8 * n + 2 * quad + (e & 1);
+          if (!there || at_key > position[e >> 1] || at_key >= to) x[n][e] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      m[r] = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
+      m[r] = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 1));
+      m[r] = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 2));
+    }
+    // the base of the exponentials follows the maximum when that is 2^8 or more above it
+    if (__any_sync(~0u, m[0] > base[0] + 8.0f || m[1] > base[1] + 8.0f)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float next = fmaxf(base[r], m[r]);
+        const float keep = next == -INFINITY ? 1.0f : exp2_approx(base[r] - next);
+        base[r] = next;
+        total[r] *= keep;
+#pragma unroll
+        for (int t = 0; t < D / 8; ++t) {
+          o[t][2 * r] *= keep;
+          o[t][2 * r + 1] *= keep;
+        }
+      }
+    }
+    uint32_t prob[PTERMS][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float zero = base[r] == -INFINITY ? 0.0f : base[r];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float e0 = exp2_approx(x[n][2 * r] - zero), e1 = exp2_approx(x[n][2 * r + 1] - zero);
+        total[r] += e0 + e1;
+        // (the step of a key that takes no part may be anything)
+        const float y0 = !whole && x[n][2 * r] == -INFINITY ? 0.0f : e0 * value_step[n][0];
+        const float y1 = !whole && x[n][2 * r + 1] == -INFINITY ? 0.0f : e1 * value_step[n][1];
+        split_pair<VT>(y0, y1, prob[0][2 * n + r], prob[1][2 * n + r]);
+        if constexpr (PTERMS == 3) {
+          const float r0 = y0 - __bfloat162float(op_put<VT>(y0)), r1 = y1 - __bfloat162float(op_put<VT>(y1));
+          split_pair<VT>(r0, r1, prob[1][2 * n + r], prob[2][2 * n + r]);
+        }
+      }
+    }
+    constexpr int WORDS = VB / 4;
+    uint32_t v[4][WORDS];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if constexpr (VB == 8) {
+        const uint2 w = lds_8(at8 + n * 256);
+        v[n][0] = w.x;
+        v[n][1] = w.y;
+      } else {
+#pragma unroll
+        for (int h = 0; h < VB / 16; ++h) {
+          const uint4 w = lds_16(at + Shared::kKeyBytes + (n * (VB / 16) + h) * 512);
+          v[n][4 * h] = w.x;
+          v[n][4 * h + 1] = w.y;
+          v[n][4 * h + 2] = w.z;
+          v[n][4 * h + 3] = w.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < D / 8; ++t) {
+      // byte t % 4 of two keys' words, in bytes 0 and 2
+      const uint32_t b0 = int8_pair<VT>(__byte_perm(v[0][t / 4], v[1][t / 4], 0x0400u + (t % 4) * 0x0101u));
+      const uint32_t b1 = int8_pair<VT>(__byte_perm(v[2][t / 4], v[3][t / 4], 0x0400u + (t % 4) * 0x0101u));
+#pragma unroll
+      for (int w = PTERMS - 1; w >= 0; --w) mma_16x8x16<VT>(o[t], prob[w], b0, b1);
+    }
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();  // the results take the ring's place
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    total[r] += __shfl_xor_sync(~0u, total[r], 1);
+    total[r] += __shfl_xor_sync(~0u, total[r], 2);
+    if (quad == 0) {
+      sh.top[warp][group + 8 * r] = base[r];
+      sh.total[warp][group + 8 * r] = total[r];
+    }
+    // o[t][e]: row group + 8 (e / 2), component (2 quad + e % 2) (D / 8) + t
+    if (position[r] > -2)
+#pragma unroll
+      for (int t = 0; t < D / 8; t += 4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float4*>(&sh.part[warp][group + 8 * r][(2 * quad + e) * (D / 8) + t]) =
+              make_float4(o[t][2 * r + e], o[t + 1][2 * r + e], o[t + 2][2 * r + e], o[t + 3][2 * r + e]);
+  }
+  __syncthreads();
+  const long long all_rows = c.tokens * p.heads;
+  for (int i = threadIdx.x; i < kCacheRows * (D / 4); i += WARPS * 32) {
+    const int r = i / (D / 4), at = i % (D / 4) * 4;
+    const int where = __shfl_sync(~0u, my_position, r);
+    if (where < -1 || at >= c.d) continue;
+    float top = sh.top[0][r];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sh.top[w][r]);
+    const float zero = top == -INFINITY ? 0.0f : top;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = exp2f(sh.top[w][r] - zero);
+      const float4 y = *reinterpret_cast<const float4*>(&sh.part[w][r][at]);
+      sum = make_float4(fmaf(f, y.x, sum.x), fmaf(f, y.y, sum.y), fmaf(f, y.z, sum.z), fmaf(f, y.w, sum.w));
+      all = fmaf(f, sh.total[w][r], all);
+    }
+    const long long row = row0 + r, token = first + row / G;
+    const int head = kv_head * G + static_cast<int>(row % G);
+    if (p.part != nullptr) {
+      const long long line = (p.first_range + range) * all_rows + token * p.heads + head;
+      *reinterpret_cast<float4*>(p.part + line * p.part_width + at) = sum;
+      if (at == 0) p.part_top[line] = make_float2(top, all);
+    } else {
+      const float scale = all == 0.0f ? 0.0f : 1.0f / all;
+      T* out = static_cast<T*>(p.o) + token * p.o_token + head * p.o_head + at;
+      const float y[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
+      if (p.o_wide) {
+        OpVec<T, 4> w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.e[e] = op_put<T>(all == 0.0f ? 0.0f : y[e]);
+        *reinterpret_cast<OpVec<T, 4>*>(out) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at + e < c.d) out[e] = op_put<T>(all == 0.0f ? 0.0f : y[e]);
+      }
+    }
+  }
+}
+
+// The ranges' results of a row, joined: a warp to a row, ranges in the order of the keys.
+template <class T>
+__global__ void __launch_bounds__(256) k_attend_cache_join(const __grid_constant__ AttendCacheParams p) {
+  const CacheParams& c = p.c;
+  const int lane = threadIdx.x & 31;
+  const long long rows = c.tokens * p.heads, row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const long long token = row / p.heads;
+  const int head = static_cast<int>(row - token * p.heads);
+  const CachePlace place = cache_place(c, token);
+  if (place.sequence < 0) return;
+  // the ranges that hold keys of this row
+  const int of_prefix = place.position < 0 || p.shared == 0 ? 0 : min(place.position, p.shared - 1) / p.prefix_chunk + 1;
+  const int own = place.position < p.shared ? 0 : (place.position - p.shared) / p.own_chunk + 1;
+  const int ranges = of_prefix + own;
+  auto line_of = [&](int n) { return (n < of_prefix ? n : p.prefix_ranges + n - of_prefix) * rows + row; };
+  float top = -INFINITY;
+  for (int n = lane; n < ranges; n += 32) top = fmaxf(top, p.part_top[line_of(n)].x);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
+  const float zero = top == -INFINITY ? 0.0f : top;
+  float all = 0.0f;
+  float4 sum[2] = {};
+  for (int n0 = 0; n0 < ranges; n0 += 32) {
+    float2 mine = make_float2(-INFINITY, 0.0f);
+    if (n0 + lane < ranges) mine = p.part_top[line_of(n0 + lane)];
+    const float factor = exp2f(mine.x - zero);
+    const int here = min(32, ranges - n0);
+#pragma unroll 4
+    for (int n = 0; n < here; ++n) {
+      const float f = __shfl_sync(~0u, factor, n);
+      all = fmaf(f, __shfl_sync(~0u, mine.y, n), all);
+      const float* from = p.part + line_of(n0 + n) * p.part_width;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = h * 128 + lane * 4;
+        if (at < c.d) {
+          const float4 y = *reinterpret_cast<const float4*>(from + at);
+          sum[h] = make_float4(fmaf(f, y.x, sum[h].x), fmaf(f, y.y, sum[h].y), fmaf(f, y.z, sum[h].z), fmaf(f, y.w, sum[h].w));
+        }
+      }
+    }
+  }
+  const float scale = all == 0.0f ? 0.0f : 1.0f / all;
+  T* out = static_cast<T*>(p.o) + token * p.o_token + head * p.o_head;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = h * 128 + lane * 4;
+    const float y[4] = {sum[h].x * scale, sum[h].y * scale, sum[h].z * scale, sum[h].w * scale};
+    if (at >= c.d) continue;
+    if (p.o_wide) {
+      OpVec<T, 4> w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.e[e] = op_put<T>(all == 0.0f ? 0.0f : y[e]);
+      *reinterpret_cast<OpVec<T, 4>*>(out + at) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at + e < c.d) out[at + e] = op_put<T>(all == 0.0f ? 0.0f : y[e]);
+    }
+  }
+}
+
+}  // namespace nb

@@ -1,0 +1,391 @@
+// A paged cache of keys and values in 8-bit integers on device arrays: quantised as they are written (ncnn_b200_op_cache_write),
+// read back (ncnn_b200_op_cache_read), and attention over it (ncnn_b200_op_cache_attention).
+#include <array>
+#include <cmath>
+
+#include "attend_cache.cuh"
+#include "op_cache.h"
+#include "row_int8.cuh"
+
+namespace nb {
+namespace {
+
+struct CacheRowsParams {
+  CacheParams c;
+  void *k, *v;  // the call's arrays (writing: read only)
+  long long k_token, k_head, v_token, v_head;
+  int kinds;    // 2: keys and values; 1: those that are not null
+};
+
+// A row (keys or values of a token's head) to LANES lanes, eight components to each: what a lane reads is one or two accesses of 16
+// bytes (WIDE) or eight elements.  Bound: HBM for many tokens, the chain of loads (starts, lens, table, row) for few.
+template <class T, int LANES, bool WIDE, bool READ>
+__global__ void __launch_bounds__(256) k_cache_rows(const __grid_constant__ CacheRowsParams p) {
+  const CacheParams& c = p.c;
+  constexpr int ROWS = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const long long rows = c.tokens * p.kinds * c.kv_heads;
+  const long long line = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / LANES;
+  const bool there = line < rows;
+  const long long rest = (there ? line : 0) / c.kv_heads, token = rest / p.kinds;
+  const int head = static_cast<int>((there ? line : 0) - rest * c.kv_heads);
+  const bool value = p.kinds == 2 ? rest % 2 == 1 : p.k == nullptr;
+  T* row = static_cast<T*>(value ? p.v : p.k) + token * (value ? p.v_token : p.k_token) + head * (value ? p.v_head : p.k_head);
+  const int at = lane * 8;
+  float x[8];
+  uint32_t top = 0;
+  if constexpr (!READ) {
+    // (asked for before the row's place is known)
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      if constexpr (WIDE) {
+        OpVec<T, V> w{};
+        if (there && at + i < c.d) w = *reinterpret_cast<const OpVec<T, V>*>(row + at + i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i + e] = at + i < c.d ? op_get(w.e[e]) : 0.0f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i + e] = there && at + i + e < c.d ? op_get(row[at + i + e]) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(x[e]));
+#pragma unroll
+    for (int w = LANES / 2; w > 0; w >>= 1) top = max(top, __shfl_xor_sync(~0u, top, w));
+  }
+  if (!there) return;
+  const CachePlace place = cache_place(c, token);
+  if (place.sequence < 0) return;
+  const int page = place.position < 0 ? -1 : cache_page(c, place.sequence, place.position);
+  const long long slot = (((page < 0 ? 0ll : page) * c.kv_heads + head) << c.page_shift) + (place.position & ((1 << c.page_shift) - 1));
+  int8_t* ints = (value ? c.v : c.k) + slot * c.row + at;
+  float* steps = (value ? c.v_steps : c.k_steps) + slot;
+  if constexpr (READ) {
+    OpVec<T, 8> out{};
+    if (page >= 0 && at < c.row) {
+      const float step = *steps;
+      const uint2 w = *reinterpret_cast<const uint2*>(ints);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out.e[e] = op_put<T>(static_cast<float>(static_cast<int8_t>((e < 4 ? w.x : w.y) >> (8 * (e % 4)))) * step);
+    }
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      if constexpr (WIDE) {
+        if (at + i < c.d) *reinterpret_cast<OpVec<T, V>*>(row + at + i) = *reinterpret_cast<const OpVec<T, V>*>(&out.e[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (at + i + e < c.d) row[at + i + e] = out.e[i + e];
+      }
+    }
+  } else {
+    if (page < 0 || at >= c.row) return;
+    const RowScale scale = row_scale<T>(top);
+    uint32_t w[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      w[g] = low_bytes(row_integer<T>(x[4 * g], scale), row_integer<T>(x[4 * g + 1], scale), row_integer<T>(x[4 * g + 2], scale),
+                       row_integer<T>(x[4 * g + 3], scale));
+    *reinterpret_cast<uint2*>(ints) = make_uint2(w[0], w[1]);
+    if (lane == 0) *steps = scale.step;
+  }
+}
+
+template <class T, bool READ>
+cudaError_t cache_rows(const CacheRowsParams& p, bool wide, cudaStream_t st) {
+  const long long rows = p.c.tokens * p.kinds * p.c.kv_heads;
+  const int pieces = p.c.row / 8;
+  auto go = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    const dim3 grid(static_cast<unsigned>((rows + 256 / LANES - 1) / (256 / LANES)));
+    return wide ? op_launch(k_cache_rows<T, LANES, true, READ>, grid, 256, 0, st, 0, p) : op_launch(k_cache_rows<T, LANES, false, READ>, grid, 256, 0, st, 0, p);
+  };
+  if (pieces <= 8) return go(std::integral_constant<int, 8>{});
+  return pieces <= 16 ? go(std::integral_constant<int, 16>{}) : go(std::integral_constant<int, 32>{});
+}
+
+// ------------------------------------------------------------------ arguments
+// What a cache and a batch say, checked: 0, or a status (the message is set).  `device`: -1 asks for no check of memory.
+int cache_params(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, CacheParams* p) {
+  auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": " + what); };
+  if (cache == nullptr || batch == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, std::string(op) + ": NULL cache or batch");
+  if (cache->page_size < 16 || cache->page_size > 1024 || (cache->page_size & (cache->page_size - 1)) != 0)
+    return bad("page_size is a power of two from 16 to 1024");
+  if (cache->head_dim < 1 || cache->head_dim > 256 || cache->kv_heads < 1 || cache->kv_heads > 65535 || cache->pages < 0 || cache->pages > 0x7fffffffll)
+    return bad("head_dim 1 to 256, kv_heads 1 to 65535, pages 0 to 2^31 - 1");
+  if (batch->sequences < 0 || batch->sequences > (1 << 24) || batch->tokens < 0 || batch->tokens > 0x7fffffffll || batch->table_width < 0 || batch->max_tokens < 0 ||
+      batch->max_len < 0)
+    return bad("sequences 0 to 2^24, tokens 0 to 2^31 - 1, and no negative table_width, max_tokens or max_len");
+  const long long room = static_cast<long long>(batch->table_width) * cache->page_size;
+  if (room > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, std::string(op) + ": a row of the table holds more than 2^30 positions");
+  if (batch->max_len > room) return bad("max_len is more than a row of the table holds");
+  if (batch->sequences > 0 && batch->tokens > 0) {
+    if (cache->k == nullptr || cache->v == nullptr || cache->k_steps == nullptr || cache->v_steps == nullptr || batch->lens == nullptr ||
+        (batch->table == nullptr && batch->table_width > 0))
+      return op_fail(NCNN_B200_STATUS_NULL_POINTER, std::string(op) + ": NULL array in the cache or the batch");
+    if (!op_starts(cache->k, 16) || !op_starts(cache->v, 16) || !op_starts(cache->k_steps, 16) || !op_starts(cache->v_steps, 16))
+      return bad("the cache's arrays start at multiples of 16 bytes");
+    if (!op_starts(batch->table, 4) || !op_starts(batch->lens, 4) || !op_starts(batch->starts, 4)) return bad("an array does not start at a multiple of its elements' size");
+    if (cache->k == cache->v || cache->k_steps == cache->v_steps) return bad("keys and values need memory of their own");
+  }
+  p->k = cache->k;
+  p->v = cache->v;
+  p->k_steps = cache->k_steps;
+  p->v_steps = cache->v_steps;
+  p->pages = cache->pages;
+  p->page_shift = 0;
+  while ((1 << p->page_shift) < cache->page_size) ++p->page_shift;
+  p->kv_heads = cache->kv_heads;
+  p->d = cache->head_dim;
+  p->row = (cache->head_dim + 15) / 16 * 16;
+  p->table = batch->table;
+  p->lens = batch->lens;
+  p->starts = batch->starts;
+  p->sequences = static_cast<int>(batch->sequences);
+  p->width = batch->table_width;
+  p->tokens = batch->tokens;
+  p->max_tokens = static_cast<int>(batch->max_tokens == 0 ? batch->tokens : std::min<int64_t>(batch->max_tokens, batch->tokens));
+  if (batch->starts == nullptr) p->max_tokens = std::min(p->max_tokens, 1);
+  p->max_len = static_cast<int>(batch->max_len == 0 ? room : batch->max_len);
+  return 0;
+}
+
+// {token, head} strides of an array of `heads` rows of d at each token; `written`: rows must not overlap.
+int row_strides(const char* op, const int64_t* given, long long tokens, int heads, int d, bool written, long long* token, long long* head) {
+  if (given == nullptr) {
+    *token = static_cast<long long>(heads) * d;
+    *head = d;
+    return 0;
+  }
+  *token = given[0];
+  *head = given[1];
+  for (int i = 0; i < 2; ++i) {
+    if (given[i] < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": a stride is negative");
+    if (given[i] > (1ll << 50) / std::max<int64_t>({tokens, heads, 1})) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, std::string(op) + ": a stride is too large");
+  }
+  if (written) {
+    std::array<std::pair<int64_t, int64_t>, 2> axes = {{{*token, tokens}, {*head, heads}}};
+    std::sort(axes.begin(), axes.end());
+    int64_t extent = d;
+    for (const auto& a : axes) {
+      if (a.second == 1) continue;
+      if (a.first < extent) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": the result's rows overlap");
+      extent = a.first * (a.second - 1) + extent;
+    }
+  }
+  return 0;
+}
+
+// Whether `count` elements can be moved at a time in all rows of an array.
+bool moves(const void* base, int count, int size, int d, long long tokens, long long token, int heads, long long head) {
+  return base == nullptr || (d % count == 0 && reinterpret_cast<uintptr_t>(base) % (count * size) == 0 && (tokens == 1 || token % count == 0) &&
+                             (heads == 1 || head % count == 0));
+}
+
+int cache_rows_call(const char* op, bool read, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, void* k, void* v, int32_t type,
+                    const int64_t* strides, void* stream) {
+  return op_guarded(op, [&]() -> int {
+    auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": " + what); };
+    if (!op_type_ok(type)) return bad("unknown element type");
+    CacheRowsParams p{};
+    if (const int e = cache_params(op, cache, batch, &p.c); e != 0) return e;
+    const int size = op_elem_bytes(type);
+    if (const int e = row_strides(op, strides, p.c.tokens, p.c.kv_heads, p.c.d, read && k != nullptr, &p.k_token, &p.k_head); e != 0) return e;
+    if (const int e = row_strides(op, strides == nullptr ? nullptr : strides + 2, p.c.tokens, p.c.kv_heads, p.c.d, read && v != nullptr, &p.v_token, &p.v_head); e != 0)
+      return e;
+    if (p.c.tokens * 2 * p.c.kv_heads > (1ll << 33)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, std::string(op) + ": more than 2^33 rows");
+    if (p.c.tokens == 0 || p.c.sequences == 0) return NCNN_B200_STATUS_SUCCESS;
+    if (read ? k == nullptr && v == nullptr : k == nullptr || v == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, std::string(op) + ": NULL argument");
+    if (!op_starts(k, size) || !op_starts(v, size)) return bad("an array does not start at a multiple of its elements' size");
+    for (const void* a : {static_cast<const void*>(k), static_cast<const void*>(v)})
+      if (a != nullptr && (a == p.c.k || a == p.c.v || a == p.c.k_steps || a == p.c.v_steps)) return bad("the arrays must not lie over the cache");
+    if (read && k == v) return bad("keys and values need memory of their own");
+    p.k = k;
+    p.v = v;
+    p.kinds = k != nullptr && v != nullptr ? 2 : 1;
+    std::string why;
+    const int device = op_common_device(op, {k, v, p.c.k, p.c.v, p.c.k_steps, p.c.v_steps, p.c.table, p.c.lens, p.c.starts}, &why);
+    if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
+    DeviceGuard guard(device);
+    const int count = 16 / size;
+    const bool wide = moves(k, count, size, p.c.d, p.c.tokens, p.k_token, p.c.kv_heads, p.k_head) &&
+                      moves(v, count, size, p.c.d, p.c.tokens, p.v_token, p.c.kv_heads, p.v_head);
+    return op_by_type(type, [&](auto t) {
+      using T = decltype(t);
+      const cudaStream_t st = static_cast<cudaStream_t>(stream);
+      return op_launched(op, read ? cache_rows<T, true>(p, wide, st) : cache_rows<T, false>(p, wide, st));
+    });
+  });
+}
+
+// ------------------------------------------------------------------ attention
+// How a call is split into ranges of keys.
+struct AttendCachePlan {
+  int prefix_ranges, prefix_chunk, own_ranges, own_chunk;
+  int ranges() const { return prefix_ranges + own_ranges; }
+};
+
+int up(long long x, int to) { return static_cast<int>((x + to - 1) / to * to); }
+
+AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long shared, int sms) {
+  AttendCachePlan plan{};
+  const int G = heads / c.kv_heads;
+  // as many ranges as give each SM four CTAs, of 256 keys at least and no more than 64 of them
+  auto split = [&](long long keys, long long tiles, int* chunk) {
+    if (keys <= 0) {
+      *chunk = 16;
+      return 0;
+    }
+    const long long most = std::max<long long>(1, std::min<long long>({64, (keys + 255) / 256, 4ll * sms / std::max<long long>(tiles, 1)}));
+    *chunk = up((keys + most - 1) / most, 64);
+    return static_cast<int>((keys + *chunk - 1) / *chunk);
+  };
+  const long long own_tiles = static_cast<long long>(c.sequences) * c.kv_heads * ((static_cast<long long>(c.max_tokens) * G + kCacheRows - 1) / kCacheRows);
+  const long long prefix_tiles = c.kv_heads * ((c.tokens * G + kCacheRows - 1) / kCacheRows);
+  const long long in_prefix = std::min<long long>(shared, c.max_len);
+  plan.prefix_ranges = split(in_prefix, prefix_tiles, &plan.prefix_chunk);
+  plan.own_ranges = split(c.max_len - in_prefix, own_tiles, &plan.own_chunk);
+  return plan;
+}
+
+long long attend_cache_workspace(const CacheParams& c, int heads, const AttendCachePlan& plan) {
+  if (plan.ranges() <= 1) return 0;
+  return plan.ranges() * c.tokens * heads * (c.row * 4ll + 8);
+}
+
+template <class T, int D, int WARPS, int STAGES, int BLOCKS>
+cudaError_t launch_cache_few(const AttendCacheParams& p, int ranges, int device, cudaStream_t st) {
+  constexpr int smem = sizeof(CacheFewShared<T, D, WARPS, STAGES>);
+  static std::atomic<uint64_t> granted{0};
+  const auto kernel = k_attend_cache_few<T, D, WARPS, STAGES, BLOCKS>;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device >= 64 || !(granted.load(std::memory_order_acquire) & bit)) {
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
+    if (device < 64) granted.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  const long long G = p.rows_a_head;
+  const long long tiles = p.prefix ? (p.c.tokens * G + kCacheRows - 1) / kCacheRows
+                                   : static_cast<long long>(p.c.sequences) * ((p.c.max_tokens * G + kCacheRows - 1) / kCacheRows);
+  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  return op_launch(kernel, dim3(static_cast<unsigned>(tiles), p.c.kv_heads, ranges), WARPS * 32, smem, st, 0, p);
+}
+
+template <class T>
+cudaError_t attend_cache_few(const AttendCacheParams& p, int ranges, int device, cudaStream_t st) {
+  if (p.c.d <= 64) return launch_cache_few<T, 64, 4, 4, 3>(p, ranges, device, st);
+  if (p.c.d <= 128) return launch_cache_few<T, 128, 4, 4, 2>(p, ranges, device, st);
+  return launch_cache_few<T, 256, 4, 3, 1>(p, ranges, device, st);
+}
+
+int attend_cache_args(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, int32_t heads, int64_t shared, CacheParams* c) {
+  if (const int e = cache_params(op, cache, batch, c); e != 0) return e;
+  auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": " + what); };
+  if (heads <= 0 || heads > 65535 || heads % c->kv_heads != 0) return bad("heads is a multiple of kv_heads up to 65535");
+  if (shared < 0 || shared % cache->page_size != 0 || shared > static_cast<long long>(c->width) * cache->page_size)
+    return bad("shared is a multiple of page_size, and no more than a row of the table holds");
+  if (c->tokens * heads > (1ll << 31)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, std::string(op) + ": more than 2^31 rows");
+  return 0;
+}
+
+}  // namespace
+}  // namespace nb
+
+extern "C" int ncnn_b200_op_cache_write(const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, const void* k, const void* v, int32_t type,
+                                        const int64_t* strides, void* stream) {
+  return nb::cache_rows_call("op_cache_write", false, cache, batch, const_cast<void*>(k), const_cast<void*>(v), type, strides, stream);
+}
+
+extern "C" int ncnn_b200_op_cache_read(const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, void* k, void* v, int32_t type,
+                                       const int64_t* strides, void* stream) {
+  return nb::cache_rows_call("op_cache_read", true, cache, batch, k, v, type, strides, stream);
+}
+
+extern "C" int64_t ncnn_b200_op_cache_attention_workspace(const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, int32_t heads, int64_t shared) {
+  using namespace nb;
+  static const char* kOp = "op_cache_attention_workspace";
+  int64_t bytes = -1;
+  op_guarded(kOp, [&]() -> int {
+    CacheParams c{};
+    if (const int e = attend_cache_args(kOp, cache, batch, heads, shared, &c); e != 0) return e;
+    if (c.tokens == 0 || c.sequences == 0) {
+      bytes = 0;
+      return 0;
+    }
+    std::string why;
+    const int device = op_common_device(kOp, {c.k}, &why);
+    if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
+    bytes = attend_cache_workspace(c, heads, attend_cache_plan(c, heads, shared, op_sm_count(device)));
+    return 0;
+  });
+  return bytes;
+}
+
+extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, const void* q, void* o, int32_t type, int32_t heads,
+                                            const int64_t* strides, int64_t shared, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace nb;
+  static const char* kOp = "op_cache_attention";
+  return op_guarded(kOp, [&]() -> int {
+    auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(kOp) + ": " + what); };
+    if (!op_type_ok(type)) return bad("unknown element type");
+    AttendCacheParams p{};
+    if (const int e = attend_cache_args(kOp, cache, batch, heads, shared, &p.c); e != 0) return e;
+    if (!(scale >= 0.0f) || std::isinf(scale * 1.44269504088896340736f)) return bad("scale must not be negative, and scale / ln 2 finite");
+    if (const int e = row_strides(kOp, strides, p.c.tokens, heads, p.c.d, false, &p.q_token, &p.q_head); e != 0) return e;
+    if (const int e = row_strides(kOp, strides == nullptr ? nullptr : strides + 2, p.c.tokens, heads, p.c.d, true, &p.o_token, &p.o_head); e != 0) return e;
+    if (p.c.tokens == 0 || p.c.sequences == 0) return NCNN_B200_STATUS_SUCCESS;
+    if (q == nullptr || o == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_cache_attention: NULL argument");
+    const int size = op_elem_bytes(type);
+    if (!op_starts(q, size) || !op_starts(o, size) || !op_starts(workspace, 16))
+      return bad("an array does not start at a multiple of its elements' size (workspace: of 16 bytes)");
+    for (const void* a : {static_cast<const void*>(p.c.k), static_cast<const void*>(p.c.v), static_cast<const void*>(p.c.k_steps),
+                          static_cast<const void*>(p.c.v_steps), q, static_cast<const void*>(workspace)})
+      if (a == o) return bad("the result must not lie over an input");
+    std::string why;
+    const int device = op_common_device(kOp, {q, o, p.c.k, p.c.v, p.c.k_steps, p.c.v_steps, p.c.table, p.c.lens, p.c.starts, workspace}, &why);
+    if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
+    DeviceGuard guard(device);
+    const AttendCachePlan plan = attend_cache_plan(p.c, heads, shared, op_sm_count(device));
+    const long long bytes = attend_cache_workspace(p.c, heads, plan);
+    if (bytes > 0 && workspace == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_cache_attention: this call needs a workspace");
+    if (bytes > workspace_bytes && bytes > 0) return op_fail(NCNN_B200_STATUS_OUTPUT_CAPACITY, "op_cache_attention: the workspace is too small");
+    p.q = q;
+    p.o = o;
+    p.heads = heads;
+    p.rows_a_head = heads / p.c.kv_heads;
+    p.scale_log2 = (scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(p.c.d)) : scale) * 1.44269504088896340736f;
+    p.shared = static_cast<int>(shared);
+    p.prefix_ranges = plan.prefix_ranges;
+    p.prefix_chunk = plan.prefix_chunk;
+    p.own_ranges = plan.own_ranges;
+    p.own_chunk = plan.own_chunk;
+    p.part_width = p.c.row;
+    if (bytes > 0) {
+      p.part = static_cast<float*>(workspace);
+      p.part_top = reinterpret_cast<float2*>(p.part + static_cast<long long>(plan.ranges()) * p.c.tokens * heads * p.part_width);
+    }
+    p.o_wide = moves(o, 4, size, p.c.d, p.c.tokens, p.o_token, heads, p.o_head) ? 1 : 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return op_by_type(type, [&](auto t) {
+      using T = decltype(t);
+      cudaError_t e = cudaSuccess;
+      if (plan.prefix_ranges > 0) {
+        AttendCacheParams first = p;
+        first.prefix = 1;
+        first.chunk = plan.prefix_chunk;
+        e = attend_cache_few<T>(first, plan.prefix_ranges, device, st);
+      }
+      // (without any keys there is still a result: zeros)
+      if (e == cudaSuccess && (plan.own_ranges > 0 || plan.prefix_ranges == 0)) {
+        AttendCacheParams own = p;
+        own.chunk = plan.own_chunk;
+        own.first_range = plan.prefix_ranges;
+        e = attend_cache_few<T>(own, std::max(plan.own_ranges, 1), device, st);
+      }
+      if (e == cudaSuccess && p.part != nullptr)
+        e = op_launch(k_attend_cache_join<T>, dim3(static_cast<unsigned>((p.c.tokens * heads + 7) / 8)), 256, 0, st, 0, p);
+      return op_launched(kOp, e);
+    });
+  });
+}

@@ -1,0 +1,238 @@
+// Rows of numbers to 8-bit integers (ncnn_b200_op_quantize_rows) and products of tokens with them
+// (ncnn_b200_op_inner_product_tokens).
+#include <cmath>
+
+#include "op_tokens.h"
+#include "row_int8.cuh"
+
+namespace nb {
+namespace {
+
+// ------------------------------------------------------------------ rows to integers
+// A row to WARPS warps, V elements to an access.  What a thread reads first it keeps (KEEP accesses: rows of up to 32 WARPS V KEEP
+// elements are read once); the rest is read again out of the caches.  Bound: HBM.
+template <class T, int V, int WARPS>
+__global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long rows, int columns, long long x_pitch, int8_t* q, long long q_pitch,
+                                                       float* steps) {
+  constexpr int KEEP = V > 1 ? 4 : 8, THREADS = WARPS * 32, ROWS = 256 / THREADS;
+  using Vec = OpVec<T, V>;
+  __shared__ uint32_t tops[8];
+  const int lane = threadIdx.x % THREADS, warp = threadIdx.x >> 5;
+  const long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / THREADS;
+  const bool there = row < rows;
+  const int count = there ? columns / V : 0;
+  const Vec* from = reinterpret_cast<const Vec*>(x + (there ? row : 0) * x_pitch);
+  Vec kept[KEEP];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (lane + i * THREADS < count) kept[i] = from[lane + i * THREADS];
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (lane + i * THREADS < count)
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = max(top, magnitude_bits(op_get(kept[i].e[e])));
+  for (int i = lane + KEEP * THREADS; i < count; i += THREADS) {
+    const Vec v = from[i];
+#pragma unroll
+    for (int e = 0; e < V; ++e) top = max(top, magnitude_bits(op_get(v.e[e])));
+  }
+  top = __reduce_max_sync(~0u, top);
+  if (WARPS > 1) {
+    if ((threadIdx.x & 31) == 0) tops[warp] = top;
+    __syncthreads();
+    top = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = max(top, tops[warp / WARPS * WARPS + w]);
+  }
+  if (!there) return;
+  const RowScale scale = row_scale<T>(top);
+  if (lane == 0) steps[row] = scale.step;
+  int8_t* to = q + row * q_pitch;
+  auto put = [&](int i, const Vec& v) {
+    if constexpr (V == 1) {
+      to[i] = static_cast<int8_t>(row_integer<T>(op_get(v.e[0]), scale));
+    } else {
+      uint32_t w[V / 4];
+#pragma unroll
+      for (int g = 0; g < V / 4; ++g)
+        w[g] = low_bytes(row_integer<T>(op_get(v.e[4 * g]), scale), row_integer<T>(op_get(v.e[4 * g + 1]), scale),
+                         row_integer<T>(op_get(v.e[4 * g + 2]), scale), row_integer<T>(op_get(v.e[4 * g + 3]), scale));
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(to + i * 8) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(to + i * 4) = w[0];
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i)
+    if (lane + i * THREADS < count) put(lane + i * THREADS, kept[i]);
+  for (int i = lane + KEEP * THREADS; i < count; i += THREADS) put(i, from[i]);
+}
+
+template <class T>
+cudaError_t quantize_rows(const T* x, long long rows, int columns, long long x_pitch, int8_t* q, long long q_pitch, float* steps, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = columns % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_pitch % V == 0) &&
+                    reinterpret_cast<uintptr_t>(q) % V == 0 && (rows == 1 || q_pitch % V == 0);
+  // a warp to rows that it can keep, unless there are too few of them to fill the device
+  const bool warps = wide && columns <= 32 * V * 4 && rows >= 1024;
+  const long long ctas = warps ? (rows + 7) / 8 : rows;
+  if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(ctas));
+  if (!wide) return op_launch(k_quantize_rows<T, 1, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+  if (warps) return op_launch(k_quantize_rows<T, V, 1>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+  return op_launch(k_quantize_rows<T, V, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+}
+
+// ------------------------------------------------------------------ products at any alignment
+// 64 x 64 results to a CTA, 32 bytes of every row a step, brought byte by byte where rows are not aligned; dp4a.
+template <class T>
+__global__ void __launch_bounds__(256) k_product_tokens(const TokensParams p) {
+  __shared__ uint32_t a[64][9], b[64][9];  // (nine words a row: columns of threads read all banks)
+  const long long t0 = static_cast<long long>(blockIdx.y) * 64;
+  const long long c0 = static_cast<long long>(blockIdx.x) * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  int sum[4][4] = {};
+  for (int k0 = 0; k0 < p.k; k0 += 32) {
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+      const int r = i >> 5, c = i & 31;
+      reinterpret_cast<int8_t*>(&a[r][0])[c] = t0 + r < p.tokens && k0 + c < p.k ? p.q[(t0 + r) * p.q_pitch + k0 + c] : 0;
+      reinterpret_cast<int8_t*>(&b[r][0])[c] = c0 + r < p.n && k0 + c < p.k ? p.weight[(c0 + r) * p.weight_pitch + k0 + c] : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      int x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = static_cast<int>(a[ty + 16 * i][w]);
+        y[i] = static_cast<int>(b[tx + 16 * i][w]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] = __dp4a(x[i], y[j], sum[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long t = t0 + ty + 16 * i, c = c0 + tx + 16 * j;
+      if (t < p.tokens && c < p.n)
+        static_cast<T*>(p.y)[t * p.y_pitch + c] =
+            op_put<T>(tokens_result<T>(sum[i][j], p.steps[t], p.weight_steps[c], p.bias == nullptr ? 0.0f : p.bias[c], p.act));
+    }
+}
+
+constexpr long long kTokensMost = 1ll << 31, kColumnsMost = 1 << 24, kSumMost = 131072;
+
+long long padded_row(int k) { return (static_cast<long long>(k) + 15) / 16 * 16; }
+// steps first, then the integers
+long long steps_bytes(long long tokens) { return (tokens * 4 + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace nb
+
+extern "C" int ncnn_b200_op_quantize_rows(const void* x, int32_t type, int64_t rows, int32_t columns, int64_t x_pitch, int8_t* q, int64_t q_pitch,
+                                          float* steps, void* stream) {
+  using namespace nb;
+  static const char* kOp = "op_quantize_rows";
+  return op_guarded(kOp, [&]() -> int {
+    if (!op_type_ok(type)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_quantize_rows: unknown element type");
+    if (rows < 0 || columns <= 0 || columns > kColumnsMost) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_quantize_rows: rows not below 0, columns 1 to 2^24");
+    if (x_pitch == 0) x_pitch = columns;
+    if (q_pitch == 0) q_pitch = columns;
+    if (x_pitch < columns || q_pitch < columns) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_quantize_rows: a pitch is smaller than a row");
+    if (rows > kTokensMost || x_pitch > (1ll << 50) / std::max<int64_t>(rows, 1) || q_pitch > (1ll << 50) / std::max<int64_t>(rows, 1))
+      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_quantize_rows: too many rows");
+    if (rows == 0) return NCNN_B200_STATUS_SUCCESS;
+    if (x == nullptr || q == nullptr || steps == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_quantize_rows: NULL argument");
+    if (!op_starts(x, op_elem_bytes(type)) || !op_starts(steps, 4))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_quantize_rows: an array does not start at a multiple of its elements' size");
+    if (static_cast<const void*>(q) == x || static_cast<const void*>(steps) == x || static_cast<const void*>(steps) == q)
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_quantize_rows: the results must not lie over the input or each other");
+    std::string why;
+    const int device = op_common_device(kOp, {x, q, steps}, &why);
+    if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
+    DeviceGuard guard(device);
+    return op_by_type(type, [&](auto t) {
+      using T = decltype(t);
+      return op_launched(kOp, quantize_rows<T>(static_cast<const T*>(x), rows, columns, x_pitch, q, q_pitch, steps, static_cast<cudaStream_t>(stream)));
+    });
+  });
+}
+
+extern "C" int64_t ncnn_b200_op_inner_product_tokens_workspace(int64_t tokens, int32_t k) {
+  using namespace nb;
+  if (tokens < 0 || tokens > kTokensMost || k <= 0 || k > kSumMost) return -1;
+  return steps_bytes(tokens) + tokens * padded_row(k);
+}
+
+extern "C" int ncnn_b200_op_inner_product_tokens(const void* x, void* y, int32_t type, int64_t tokens, int32_t k, int32_t n, int64_t x_pitch,
+                                                 int64_t y_pitch, const int8_t* weight, int64_t weight_pitch, const float* weight_steps,
+                                                 const float* bias, int32_t activation, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace nb;
+  static const char* kOp = "op_inner_product_tokens";
+  return op_guarded(kOp, [&]() -> int {
+    if (!op_type_ok(type)) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: unknown element type");
+    if (activation != NCNN_B200_ACT_NONE && activation != NCNN_B200_ACT_RELU && activation != NCNN_B200_ACT_SWISH && activation != NCNN_B200_ACT_GELU)
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: unknown activation");
+    if (tokens < 0 || k <= 0 || k > kSumMost || n <= 0 || n > kColumnsMost)
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: tokens not below 0, k 1 to 131072, n 1 to 2^24");
+    if (x_pitch == 0) x_pitch = k;
+    if (y_pitch == 0) y_pitch = n;
+    if (weight_pitch == 0) weight_pitch = k;
+    if (x_pitch < k || y_pitch < n || weight_pitch < k) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: a pitch is smaller than a row");
+    const int64_t most = std::max<int64_t>(tokens, 1);
+    if (tokens > kTokensMost || x_pitch > (1ll << 50) / most || y_pitch > (1ll << 50) / most || weight_pitch > (1ll << 50) / n)
+      return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens, or a pitch is too large");
+    if (tokens == 0) return NCNN_B200_STATUS_SUCCESS;
+    if (x == nullptr || y == nullptr || weight == nullptr || weight_steps == nullptr || workspace == nullptr)
+      return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_inner_product_tokens: NULL argument");
+    const int size = op_elem_bytes(type);
+    if (!op_starts(x, size) || !op_starts(y, size) || !op_starts(weight_steps, 4) || !op_starts(bias, 4) || !op_starts(workspace, 16))
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: an array does not start at a multiple of its elements' size (workspace: of 16 bytes)");
+    if (workspace_bytes < ncnn_b200_op_inner_product_tokens_workspace(tokens, k))
+      return op_fail(NCNN_B200_STATUS_OUTPUT_CAPACITY, "op_inner_product_tokens: the workspace is too small");
+    if (y == x || y == weight || y == workspace || x == workspace)
+      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: the result and the workspace must not lie over an input or each other");
+    std::string why;
+    const int device = op_common_device(kOp, {x, y, weight, weight_steps, bias, workspace}, &why);
+    if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
+    DeviceGuard guard(device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    TokensParams p{};
+    p.tokens = tokens;
+    p.k = k;
+    p.n = n;
+    p.q_pitch = padded_row(k);
+    p.weight_pitch = weight_pitch;
+    p.y_pitch = y_pitch;
+    float* steps = static_cast<float*>(workspace);
+    int8_t* q = static_cast<int8_t*>(workspace) + steps_bytes(tokens);
+    p.steps = steps;
+    p.q = q;
+    p.weight = weight;
+    p.weight_steps = weight_steps;
+    p.bias = bias;
+    p.y = y;
+    p.act = activation;
+    return op_by_type(type, [&](auto t) {
+      using T = decltype(t);
+      if (const cudaError_t e = quantize_rows<T>(static_cast<const T*>(x), tokens, k, x_pitch, q, p.q_pitch, steps, st); e != cudaSuccess) return op_launched(kOp, e);
+      const long long rows = (tokens + 63) / 64, columns = (n + 63ll) / 64;
+      // (a launch has at most 65535 rows of CTAs)
+      for (long long r = 0; r < rows; r += 65535) {
+        TokensParams part = p;
+        part.tokens = std::min<long long>(tokens - r * 64, 65535ll * 64);
+        part.q += r * 64 * p.q_pitch;
+        part.steps += r * 64;
+        part.y = static_cast<T*>(p.y) + r * 64 * p.y_pitch;
+        const dim3 grid(static_cast<unsigned>(columns), static_cast<unsigned>(std::min<long long>(rows - r, 65535)));
+        if (const cudaError_t e = op_launch(k_product_tokens<T>, grid, 256, 0, st, 0, part); e != cudaSuccess) return op_launched(kOp, e);
+      }
+      return static_cast<int>(NCNN_B200_STATUS_SUCCESS);
+    });
+  });
+}

@@ -80,6 +80,17 @@ def load_library():
                                            c_void_p, ctypes.c_double, c_int32, c_int32, c_void_p]
     L.ncnn_b200_op_cross_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_int32,
                                                c_int32, c_void_p, c_void_p, c_void_p, c_float, c_void_p]
+    L.ncnn_b200_op_quantize_rows.argtypes = [c_void_p, c_int32, c_int64, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_void_p]
+    L.ncnn_b200_op_inner_product_tokens_workspace.argtypes = [c_int64, c_int32]
+    L.ncnn_b200_op_inner_product_tokens_workspace.restype = c_int64
+    L.ncnn_b200_op_inner_product_tokens.argtypes = [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_int64, c_int64, c_void_p, c_int64,
+                                                    c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p]
+    L.ncnn_b200_op_cache_write.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]
+    L.ncnn_b200_op_cache_read.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]
+    L.ncnn_b200_op_cache_attention_workspace.argtypes = [c_void_p, c_void_p, c_int32, c_int64]
+    L.ncnn_b200_op_cache_attention_workspace.restype = c_int64
+    L.ncnn_b200_op_cache_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_float, c_void_p,
+                                               c_int64, c_void_p]
     L.ncnn_b200_op_check_status.argtypes = []
     L.ncnn_b200_op_test_hooks.argtypes = [c_int32, ctypes.c_uint64, c_int32]
     L.ncnn_b200_multi_load.argtypes = [c_char_p, c_char_p, POINTER(_Options), POINTER(c_int32), c_int32, POINTER(c_void_p)]
@@ -411,6 +422,102 @@ def op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, element, batch, lq, lk, heads
     st = L.ncnn_b200_op_cross_attention(q_ptr, k_ptr, v_ptr, o_ptr, _of(ELEMENT_TYPES, element, "element"), batch, lq, lk, heads, kv_heads,
                                         head_dim, None if strides is None else struct.pack("12q", *strides), kv_lens_ptr, key_mask_ptr,
                                         scale, stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_quantize_rows(x_ptr, element, rows, columns, q_ptr, steps_ptr, x_pitch=0, q_pitch=0, stream=0):
+    """Rows of "f32", "f16" or "bf16" elements as int8 with a step for each row, fp32 [rows] (ncnn_b200_op_quantize_rows)."""
+    L = load_library()
+    st = L.ncnn_b200_op_quantize_rows(x_ptr, _of(ELEMENT_TYPES, element, "element"), rows, columns, x_pitch, q_ptr, q_pitch, steps_ptr, stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def _workspace_bytes(L, bytes_needed):
+    if bytes_needed < 0:
+        raise ValueError("no call of these sizes is allowed")
+    return bytes_needed
+
+
+def op_inner_product_tokens_workspace(tokens, k):
+    """Bytes of device memory that op_inner_product_tokens passes a call's integers through."""
+    L = load_library()
+    return _workspace_bytes(L, L.ncnn_b200_op_inner_product_tokens_workspace(tokens, k))
+
+
+def op_inner_product_tokens(x_ptr, y_ptr, element, tokens, k, n, weight_ptr, weight_steps_ptr, workspace_ptr, workspace_bytes, bias_ptr=None,
+                            activation="none", x_pitch=0, y_pitch=0, weight_pitch=0, stream=0):
+    """int8 InnerProduct of x [tokens][k] with a scale for each token, found in it, and one for each of the n channels: weight is
+    int8 [n][weight_pitch or k], weight_steps fp32 [n], y [tokens][n] of x's type (ncnn_b200_op_inner_product_tokens)."""
+    L = load_library()
+    st = L.ncnn_b200_op_inner_product_tokens(x_ptr, y_ptr, _of(ELEMENT_TYPES, element, "element"), tokens, k, n, x_pitch, y_pitch, weight_ptr,
+                                             weight_pitch, weight_steps_ptr, bias_ptr, _of(OP_ACTIVATIONS, activation, "activation"),
+                                             workspace_ptr, workspace_bytes, stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+class Cache(ctypes.Structure):
+    """Keys and values in pages of 8-bit integers: device pointers and sizes (ncnn_b200_cache).  row_bytes is what a row takes."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_steps", c_void_p), ("v_steps", c_void_p), ("pages", c_int64), ("page_size", c_int32),
+                ("kv_heads", c_int32), ("head_dim", c_int32)]
+
+    @property
+    def row_bytes(self):
+        return (self.head_dim + 15) // 16 * 16
+
+
+class CacheBatch(ctypes.Structure):
+    """The last tokens of some sequences of a cache (ncnn_b200_cache_batch): table is int32 [sequences][table_width], lens int32
+    [sequences], starts int32 [sequences + 1] or None (one token to each), all on the device."""
+    _fields_ = [("table", c_void_p), ("lens", c_void_p), ("starts", c_void_p), ("sequences", c_int64), ("tokens", c_int64),
+                ("table_width", c_int32), ("max_tokens", c_int32), ("max_len", c_int64)]
+
+    def __init__(self, table, lens, starts, sequences, tokens, table_width, max_tokens=0, max_len=0):
+        super().__init__(table, lens, starts, sequences, tokens, table_width, max_tokens, max_len)
+
+
+def _four(strides, what):
+    if strides is None:
+        return None
+    if len(strides) != 4:
+        raise ValueError("strides are four numbers: token and head of %s" % what)
+    return struct.pack("4q", *strides)
+
+
+def op_cache_write(cache, batch, k_ptr, v_ptr, element, strides=None, stream=0):
+    """Quantises the batch's keys and values [tokens][kv_heads][head_dim] into their pages (ncnn_b200_op_cache_write)."""
+    L = load_library()
+    st = L.ncnn_b200_op_cache_write(byref(cache), byref(batch), k_ptr, v_ptr, _of(ELEMENT_TYPES, element, "element"),
+                                    _four(strides, "k and of v"), stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_cache_read(cache, batch, k_ptr, v_ptr, element, strides=None, stream=0):
+    """The values that the batch's tokens have in the cache; k_ptr or v_ptr may be None (ncnn_b200_op_cache_read)."""
+    L = load_library()
+    st = L.ncnn_b200_op_cache_read(byref(cache), byref(batch), k_ptr, v_ptr, _of(ELEMENT_TYPES, element, "element"),
+                                   _four(strides, "k and of v"), stream)
+    if st != 0:
+        _op_message(L, st)
+
+
+def op_cache_attention_workspace(cache, batch, heads, shared=0):
+    """Bytes of device memory that op_cache_attention needs for such a call (0: none)."""
+    L = load_library()
+    return _workspace_bytes(L, L.ncnn_b200_op_cache_attention_workspace(byref(cache), byref(batch), heads, shared))
+
+
+def op_cache_attention(cache, batch, q_ptr, o_ptr, element, heads, shared=0, scale=0.0, strides=None, workspace_ptr=None, workspace_bytes=0,
+                       stream=0):
+    """Causal attention of the batch's tokens, q [tokens][heads][head_dim], to their sequences' pages; `shared` first positions are
+    the table's first row's for all sequences (ncnn_b200_op_cache_attention)."""
+    L = load_library()
+    _stall_as_asked(L)
+    st = L.ncnn_b200_op_cache_attention(byref(cache), byref(batch), q_ptr, o_ptr, _of(ELEMENT_TYPES, element, "element"), heads,
+                                        _four(strides, "q and of o"), shared, scale, workspace_ptr, workspace_bytes, stream)
     if st != 0:
         _op_message(L, st)
 
