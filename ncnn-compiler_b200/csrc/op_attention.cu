@@ -24,25 +24,7 @@ struct {
 // The devices that calls on the tensor cores went to (as bits).
 std::atomic<uint64_t> g_waited_on{0};
 
-void will_wait_on(int device) {
-  const uint64_t bit = 1ull << (device & 63);
-  if (!(g_waited_on.load(std::memory_order_relaxed) & bit)) g_waited_on.fetch_or(bit, std::memory_order_relaxed);
-}
-
 // ------------------------------------------------------------------ tensor cores
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static const EncodeTiledFn fn = [] {
-    cudaDriverEntryPointQueryResult query;
-    void* f = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &query) != cudaSuccess || query != cudaDriverEntryPointSuccess) f = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
 // [sequence][head][row][component] as TMA sees it, boxes of 128 rows (results: 32) of 64 components.  An axis that all heads or sequences
 // share (stride 0) has one entry: `step` says what to multiply its index with.
 bool encode_rows(CUtensorMap* map, bool half, const void* base, int d, long long rows, long long row, int heads, long long head, int batch,
@@ -102,9 +84,8 @@ struct TcMaps {
 bool fill_tc(const AttendParams& a, bool half, TcAttendParams* p, TcMaps* m) {
   p->a = a;
   p->scale_log2 = a.scale * 1.44269504088896340736f;
-  p->wait_ns = kTcWaitLimitNs;
-  p->stall = g_hooks.stall.load(std::memory_order_relaxed);
-  if (const unsigned long long ns = g_hooks.wait_ns.load(std::memory_order_relaxed); ns != 0) p->wait_ns = ns;
+  p->wait_ns = op_wait_ns(kTcWaitLimitNs);
+  p->stall = op_stalled() ? 1 : 0;
   return encode_rows(&m->q, half, a.q, a.d, a.lq, a.q_row, a.heads, a.q_head, a.batch, a.q_batch, p->q_step) &&
          encode_rows(&m->k, half, a.k, a.d, a.lk, a.k_row, a.kv_heads, a.k_head, a.batch, a.k_batch, p->k_step) &&
          encode_rows(&m->v, half, a.v, a.d, a.lk, a.v_row, a.kv_heads, a.v_head, a.batch, a.v_batch, p->v_step) &&
@@ -128,7 +109,7 @@ int launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
   if (const cudaError_t e = grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
   p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
   p.tiles = p.row_tiles * a.heads * a.batch;
-  will_wait_on(device);
+  op_will_wait_on(device);
   return op_launched("op_cross_attention",
                      op_launch(tc_attend_short_kernel<T, D>, dim3(std::min(sms, p.tiles)), Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
@@ -143,7 +124,7 @@ int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   const int registers = Shape::kShareRegs ? Shape::kRegsLaunch : 0;
   if (const cudaError_t e = grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
-  will_wait_on(device);
+  op_will_wait_on(device);
   return op_launched("op_cross_attention", op_launch(tc_attend_kernel<T, D, TILES>, grid, Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
 }
 
@@ -281,6 +262,19 @@ bool tma_strides(const AttendParams& p) {
 }
 
 }  // namespace
+
+bool op_stalled() { return g_hooks.stall.load(std::memory_order_relaxed) != 0; }
+
+unsigned long long op_wait_ns(unsigned long long usual) {
+  const unsigned long long ns = g_hooks.wait_ns.load(std::memory_order_relaxed);
+  return ns != 0 ? ns : usual;
+}
+
+void op_will_wait_on(int device) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(g_waited_on.load(std::memory_order_relaxed) & bit)) g_waited_on.fetch_or(bit, std::memory_order_relaxed);
+}
+
 }  // namespace nb
 
 extern "C" int ncnn_b200_op_test_hooks(int32_t stall, uint64_t wait_ns, int32_t registers) {
@@ -303,8 +297,11 @@ extern "C" int ncnn_b200_op_check_status(void) {
     for (int d = 0; d < 64; ++d) {
       if (!(devices >> d & 1u)) continue;
       DeviceGuard guard(d);
-      unsigned count = 0;
-      if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&count, g_attend_gave_up, sizeof count) != cudaSuccess) return failed();
+      unsigned count = 0, tokens = 0, cache = 0;
+      if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&count, g_attend_gave_up, sizeof count) != cudaSuccess ||
+          tokens_gave_up(&tokens) != cudaSuccess || cache_gave_up(&cache) != cudaSuccess)
+        return failed();
+      count += tokens + cache;
       ran_out = ran_out || count != told[d];
       told[d] = count;
     }

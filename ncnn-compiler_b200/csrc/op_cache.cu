@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) k_cache_rows(const __grid_constant__ Cach
     uint32_t w[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g)
-      w[g] = low_bytes(row_integer<T>(x[4 * g], scale), row_integer<T>(x[4 * g + 1], scale), row_integer<T>(x[4 * g + 2], scale),
+      w[g] = scale.factor == 0.0f ? 0u : low_bytes(row_integer<T>(x[4 * g], scale), row_integer<T>(x[4 * g + 1], scale), row_integer<T>(x[4 * g + 2], scale),
                        row_integer<T>(x[4 * g + 3], scale));
     *reinterpret_cast<uint2*>(ints) = make_uint2(w[0], w[1]);
     if (lane == 0) *steps = scale.step;
@@ -260,11 +260,7 @@ cudaError_t launch_cache_few(const AttendCacheParams& p, int ranges, int device,
   constexpr int smem = sizeof(CacheFewShared<T, D, WARPS, STAGES>);
   static std::atomic<uint64_t> granted{0};
   const auto kernel = k_attend_cache_few<T, D, WARPS, STAGES, BLOCKS>;
-  const uint64_t bit = 1ull << (device & 63);
-  if (device >= 64 || !(granted.load(std::memory_order_acquire) & bit)) {
-    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return e;
-    if (device < 64) granted.fetch_or(bit, std::memory_order_acq_rel);
-  }
+  if (const cudaError_t e = op_grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return e;
   const long long G = p.rows_a_head;
   const long long tiles = p.prefix ? (p.c.tokens * G + kCacheRows - 1) / kCacheRows
                                    : static_cast<long long>(p.c.sequences) * ((p.c.max_tokens * G + kCacheRows - 1) / kCacheRows);
@@ -290,6 +286,12 @@ int attend_cache_args(const char* op, const ncnn_b200_cache* cache, const ncnn_b
 }
 
 }  // namespace
+
+cudaError_t cache_gave_up(unsigned* count) {
+  *count = 0;
+  return cudaSuccess;
+}
+
 }  // namespace nb
 
 extern "C" int ncnn_b200_op_cache_write(const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, const void* k, const void* v, int32_t type,

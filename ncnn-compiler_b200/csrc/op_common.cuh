@@ -21,6 +21,13 @@ namespace nb {
 
 void set_global_error(const std::string& message);  // c_api.cu
 
+// What tests asked of the kernels whose waits are bounded (ncnn_b200_op_test_hooks), and who reports such a wait (op_attention.cu).
+bool op_stalled();
+unsigned long long op_wait_ns(unsigned long long usual);
+void op_will_wait_on(int device);
+cudaError_t tokens_gave_up(unsigned* count);  // op_tokens.cu, on the current device
+cudaError_t cache_gave_up(unsigned* count);   // op_cache.cu
+
 // ------------------------------------------------------------------ elements
 // 16-bit elements become fp32 on the way in and are rounded once, to nearest even, on the way out.
 template <class T> __device__ __forceinline__ float op_get(T v);
@@ -94,6 +101,29 @@ inline int op_common_device(const char* op, std::initializer_list<const void*> a
   return device;
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_tiled() {
+  static const EncodeTiledFn fn = [] {
+    cudaDriverEntryPointQueryResult query;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &query) != cudaSuccess || query != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// Dynamic shared memory above 48 KB is granted to a kernel once per device.
+template <class K>
+inline cudaError_t op_grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (granted->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) granted->fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
+
 inline int op_sm_count(int device) {
   int n = 148;
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
@@ -108,21 +138,32 @@ inline int op_launched(const char* op, cudaError_t e) {
   return op_fail(NCNN_B200_STATUS_RUNTIME, std::string(op) + ": launch failed: " + cudaGetErrorString(e));
 }
 
-// CTAs of `cluster` along x, if any
+// CTAs of `cluster` along x, if any; `early`: may start while the kernel before it in the stream still runs
 template <class... P, class... A>
-inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, int cluster, const A&... args) {
+inline cudaError_t op_launch_early(bool early, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, int cluster, const A&... args) {
   cudaLaunchConfig_t c{};
   c.gridDim = grid;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = st;
-  cudaLaunchAttribute size{};
-  size.id = cudaLaunchAttributeClusterDimension;
-  size.val.clusterDim.x = cluster;
-  size.val.clusterDim.y = size.val.clusterDim.z = 1;
-  c.attrs = &size;
-  c.numAttrs = cluster > 0 ? 1 : 0;
+  cudaLaunchAttribute attrs[2] = {};
+  c.attrs = attrs;
+  if (cluster > 0) {
+    cudaLaunchAttribute& size = attrs[c.numAttrs++];
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = cluster;
+    size.val.clusterDim.y = size.val.clusterDim.z = 1;
+  }
+  if (early) {
+    cudaLaunchAttribute& serial = attrs[c.numAttrs++];
+    serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    serial.val.programmaticStreamSerializationAllowed = 1;
+  }
   return cudaLaunchKernelEx(&c, kernel, args...);
+}
+template <class... P, class... A>
+inline cudaError_t op_launch(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, int cluster, const A&... args) {
+  return op_launch_early(false, kernel, grid, threads, smem, st, cluster, args...);
 }
 
 // f(T{}) with the element type that `type` names

@@ -4,6 +4,7 @@
 
 #include "op_tokens.h"
 #include "row_int8.cuh"
+#include "tc_tokens.cuh"
 
 namespace nb {
 namespace {
@@ -14,8 +15,9 @@ namespace {
 template <class T, int V, int WARPS>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long rows, int columns, long long x_pitch, int8_t* q, long long q_pitch,
                                                        float* steps) {
-  constexpr int KEEP = V > 1 ? 4 : 8, THREADS = WARPS * 32, ROWS = 256 / THREADS;
+  constexpr int KEEP = WARPS == 1 ? 16 : 8, THREADS = WARPS * 32, ROWS = 256 / THREADS;
   using Vec = OpVec<T, V>;
+  ptx::grid_dependency_trigger();  // (the product's kernel may begin with its weights)
   __shared__ uint32_t tops[8];
   const int lane = threadIdx.x % THREADS, warp = threadIdx.x >> 5;
   const long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / THREADS;
@@ -29,15 +31,9 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long row
     if (lane + i * THREADS < count) kept[i] = from[lane + i * THREADS];
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
-    if (lane + i * THREADS < count)
-#pragma unroll
-      for (int e = 0; e < V; ++e) top = max(top, magnitude_bits(op_get(kept[i].e[e])));
-  for (int i = lane + KEEP * THREADS; i < count; i += THREADS) {
-    const Vec v = from[i];
-#pragma unroll
-    for (int e = 0; e < V; ++e) top = max(top, magnitude_bits(op_get(v.e[e])));
-  }
-  top = __reduce_max_sync(~0u, top);
+    if (lane + i * THREADS < count) top = row_top(kept[i], top);
+  for (int i = lane + KEEP * THREADS; i < count; i += THREADS) top = row_top(from[i], top);
+  top = __reduce_max_sync(~0u, row_top_bits<T>(top));
   if (WARPS > 1) {
     if ((threadIdx.x & 31) == 0) tops[warp] = top;
     __syncthreads();
@@ -62,6 +58,10 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long row
       else *reinterpret_cast<uint32_t*>(to + i * 4) = w[0];
     }
   };
+  if (scale.factor == 0.0f) {
+    for (int i = lane; i < count; i += THREADS) put(i, Vec{});
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
     if (lane + i * THREADS < count) put(lane + i * THREADS, kept[i]);
@@ -74,7 +74,7 @@ cudaError_t quantize_rows(const T* x, long long rows, int columns, long long x_p
   const bool wide = columns % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_pitch % V == 0) &&
                     reinterpret_cast<uintptr_t>(q) % V == 0 && (rows == 1 || q_pitch % V == 0);
   // a warp to rows that it can keep, unless there are too few of them to fill the device
-  const bool warps = wide && columns <= 32 * V * 4 && rows >= 1024;
+  const bool warps = wide && columns <= 32 * V * 16 && rows >= 2048;
   const long long ctas = warps ? (rows + 7) / 8 : rows;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(ctas));
@@ -114,15 +114,105 @@ __global__ void __launch_bounds__(256) k_product_tokens(const TokensParams p) {
     }
     __syncthreads();
   }
+  tokens_by_activation(p.act, [&](auto plain) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long t = t0 + ty + 16 * i, c = c0 + tx + 16 * j;
-      if (t < p.tokens && c < p.n)
-        static_cast<T*>(p.y)[t * p.y_pitch + c] =
-            op_put<T>(tokens_result<T>(sum[i][j], p.steps[t], p.weight_steps[c], p.bias == nullptr ? 0.0f : p.bias[c], p.act));
-    }
+      for (int j = 0; j < 4; ++j) {
+        const long long t = t0 + ty + 16 * i, c = c0 + tx + 16 * j;
+        if (t < p.tokens && c < p.n)
+          static_cast<T*>(p.y)[t * p.y_pitch + c] = tokens_result<T>(plain, sum[i][j], p.steps[t], p.weight_steps[c], p.bias == nullptr ? 0.0f : p.bias[c], p.act);
+      }
+  });
+}
+
+// ------------------------------------------------------------------ tensor cores
+// Rows of bytes as TMA sees them, boxes of 128 bytes of `box_rows` rows.
+bool encode_bytes(CUtensorMap* map, const void* base, long long columns, long long rows, long long pitch, int box_rows) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {rows == 1 ? static_cast<cuuint64_t>((columns + 15) / 16 * 16) : static_cast<cuuint64_t>(pitch)};  // (a stride that is never stepped)
+  const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)}, ones[2] = {1, 1};
+  return encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Results as TMA stores them: 32 rows of 128 bytes.
+template <class T>
+bool encode_results(CUtensorMap* map, void* base, long long columns, long long rows, long long pitch) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * sizeof(T)};
+  const cuuint32_t box[2] = {128 / sizeof(T), 32}, ones[2] = {1, 1};
+  const CUtensorMapDataType kind = sizeof(T) == 4                          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_tiled()(map, kind, 2, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int no_token_maps() { return op_fail(NCNN_B200_STATUS_RUNTIME, "op_inner_product_tokens: the tensor maps could not be made"); }
+
+template <class T>
+int product_few(TcTokensParams p, int device, int sms, cudaStream_t st) {
+  const TokensParams& t = p.t;
+  p.columns = t.tokens >= 128 ? 128 : static_cast<int>((t.tokens + 15) / 16 * 16);
+  p.tiles_t = static_cast<int>((t.tokens + p.columns - 1) / p.columns);
+  p.tiles_c = (t.n + 127) / 128;
+  const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_c;
+  int ranks = 1;
+  // (two CTAs to an SM have no room for the sums of more than 64 tokens)
+  while (ranks < 8 && tiles * ranks * 2 <= (p.columns <= 64 ? 2ll : 1ll) * sms && ranks * 2 <= p.k_blocks) ranks *= 2;
+  if (tiles * ranks > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens");
+  p.t.ranks = ranks;
+  p.stage_bytes = 16384 + p.columns * 128;
+  const int room = tiles * ranks <= sms ? 200 * 1024 : 110 * 1024;  // one CTA to an SM, or two
+  const int sums = ranks > 1 ? ranks * ((p.columns + ranks - 1) / ranks) * 512 : 0;
+  p.stages = std::max(2, std::min({kTokStagesMost, (room - sums) / p.stage_bytes, (p.k_blocks + ranks - 1) / ranks}));
+  const int smem = p.stages * p.stage_bytes + sums + 1024;
+  CUtensorMap map_w, map_q;
+  if (!encode_bytes(&map_w, t.weight, t.k, t.n, t.weight_pitch, 128) || !encode_bytes(&map_q, t.q, t.k, t.tokens, t.q_pitch, p.columns)) return no_token_maps();
+  static std::atomic<uint64_t> granted{0};
+  if (const cudaError_t e = op_grant_smem(tc_tokens_few_kernel<T>, 201 * 1024, device, &granted); e != cudaSuccess) return op_launched("op_inner_product_tokens", e);
+  op_will_wait_on(device);
+  return op_launched("op_inner_product_tokens", op_launch_early(true, tc_tokens_few_kernel<T>, dim3(static_cast<unsigned>(tiles * ranks)), kTokFewThreads, smem, st,
+                                                                ranks > 1 ? ranks : 0, p, map_w, map_q));
+}
+
+template <class T>
+int product_pair(TcTokensParams p, int columns, int device, int sms, cudaStream_t st) {
+  const TokensParams& t = p.t;
+  p.columns = columns;
+  p.tiles_t = static_cast<int>((t.tokens + 255) / 256);
+  p.tiles_c = (t.n + columns - 1) / columns;
+  const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_c;
+  if (tiles > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens");
+  p.stage_bytes = 16384 + columns / 2 * 128;
+  p.stages = std::min(kTokStagesMost, (192 * 1024) / p.stage_bytes);
+  p.stored = reinterpret_cast<uintptr_t>(t.y) % 16 == 0 && t.y_pitch * static_cast<long long>(sizeof(T)) % 16 == 0 && t.y_pitch < (1ll << 37) ? 1 : 0;
+  const int smem = p.stages * p.stage_bytes + 8 * 4096 + 1024;
+  CUtensorMap map_w, map_q, map_y{};
+  if (!encode_bytes(&map_w, t.weight, t.k, t.n, t.weight_pitch, columns / 2) || !encode_bytes(&map_q, t.q, t.k, t.tokens, t.q_pitch, 128)) return no_token_maps();
+  if (p.stored && !encode_results<T>(&map_y, t.y, t.n, t.tokens, t.y_pitch)) return no_token_maps();
+  static std::atomic<uint64_t> granted{0};
+  if (const cudaError_t e = op_grant_smem(tc_tokens_pair_kernel<T>, 226 * 1024, device, &granted); e != cudaSuccess) return op_launched("op_inner_product_tokens", e);
+  op_will_wait_on(device);
+  const int pairs = static_cast<int>(std::min<long long>(sms / 2, tiles));
+  return op_launched("op_inner_product_tokens",
+                     op_launch_early(true, tc_tokens_pair_kernel<T>, dim3(pairs * 2), kTokPairThreads, smem, st, 2, p, map_w, map_q, map_y));
+}
+
+template <class T>
+int product_tc(const TokensParams& t, int device, cudaStream_t st) {
+  TcTokensParams p{};
+  p.t = t;
+  p.k_blocks = (t.k + 127) / 128;
+  p.wait_ns = op_wait_ns(kTcWaitLimitNs);
+  p.stall = op_stalled() ? 1 : 0;
+  const int sms = op_sm_count(device);
+  p.t.aligned = reinterpret_cast<uintptr_t>(t.weight_steps) % 16 == 0 && reinterpret_cast<uintptr_t>(t.bias) % 16 == 0 ? 1 : 0;
+  const long long rows = (t.tokens + 255) / 256;
+  if (t.tokens > 128 && 2 * rows * ((t.n + 255) / 256) >= sms) return product_pair<T>(p, 256, device, sms, st);
+  if (t.tokens > 128 && 2 * rows * ((t.n + 127) / 128) >= sms) return product_pair<T>(p, 128, device, sms, st);
+  return product_few<T>(p, device, sms, st);
 }
 
 constexpr long long kTokensMost = 1ll << 31, kColumnsMost = 1 << 24, kSumMost = 131072;
@@ -132,6 +222,9 @@ long long padded_row(int k) { return (static_cast<long long>(k) + 15) / 16 * 16;
 long long steps_bytes(long long tokens) { return (tokens * 4 + 15) / 16 * 16; }
 
 }  // namespace
+
+cudaError_t tokens_gave_up(unsigned* count) { return cudaMemcpyFromSymbol(count, g_tokens_gave_up, sizeof *count); }
+
 }  // namespace nb
 
 extern "C" int ncnn_b200_op_quantize_rows(const void* x, int32_t type, int64_t rows, int32_t columns, int64_t x_pitch, int8_t* q, int64_t q_pitch,
@@ -221,6 +314,11 @@ extern "C" int ncnn_b200_op_inner_product_tokens(const void* x, void* y, int32_t
     return op_by_type(type, [&](auto t) {
       using T = decltype(t);
       if (const cudaError_t e = quantize_rows<T>(static_cast<const T*>(x), tokens, k, x_pitch, q, p.q_pitch, steps, st); e != cudaSuccess) return op_launched(kOp, e);
+      // (weights whose rows TMA cannot start at go through the CUDA cores)
+      if (reinterpret_cast<uintptr_t>(weight) % 16 == 0 && (n == 1 || (weight_pitch % 16 == 0 && weight_pitch < (1ll << 39)))) {
+        if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_inner_product_tokens: cuTensorMapEncodeTiled is not available from this driver");
+        return product_tc<T>(p, device, st);
+      }
       const long long rows = (tokens + 63) / 64, columns = (n + 63ll) / 64;
       // (a launch has at most 65535 rows of CTAs)
       for (long long r = 0; r < rows; r += 65535) {

@@ -1,6 +1,8 @@
 // What the kernels of ncnn_b200_op_inner_product_tokens share.
 #pragma once
 
+#include <type_traits>
+
 #include "op_common.cuh"
 
 namespace nb {
@@ -16,19 +18,32 @@ struct TokensParams {
   const float* bias;    // or null
   void* y;
   int act;
+  int ranks;    // CTAs that share out a tile's K blocks
+  int aligned;  // steps and bias of four channels can be read at a time
 };
 
+// A sum of integers (exact) before its activation: the sum and the product of the steps are rounded to fp32, then one fma.
+__device__ __forceinline__ float tokens_sum(int sum, float step, float weight_step, float bias) {
+  return fmaf(static_cast<float>(sum), step * weight_step, bias);
+}
+// Called, not inlined: results leave in unrolled loops, which a copy of these for every value makes too long for the instruction
+// cache (64 tokens through 4096 x 11008, no activation: 5400 of a tile's 28000 clocks went into the last 16 values of each thread).
 template <class T>
-__device__ __forceinline__ float tokens_activate(float t, int act) {
+__device__ __noinline__ float tokens_activate(float t, int act) {
   if (act == NCNN_B200_ACT_RELU) return t > 0.0f ? t : t == t ? 0.0f : t;  // (a NaN stays one)
   if (act == NCNN_B200_ACT_SWISH) return sizeof(T) == 4 ? t / (1.0f + expf(-t)) : __fdividef(t, 1.0f + __expf(-t));  // (16 bits: good to 2^-20)
-  if (act == NCNN_B200_ACT_GELU) return 0.5f * t * erfcf(t * -0.7071067811865476f);
-  return t;
+  return 0.5f * t * erfcf(t * -0.7071067811865476f);
 }
-// A sum of integers (exact) as the result: the sum and the product of the steps are rounded to fp32, then one fma.
-template <class T>
-__device__ __forceinline__ float tokens_result(int sum, float step, float weight_step, float bias, int act) {
-  return tokens_activate<T>(fmaf(static_cast<float>(sum), step * weight_step, bias), act);
+// f(true_type) where there is no activation, f(false_type) where there is one
+template <class F>
+__device__ __forceinline__ void tokens_by_activation(int act, F&& f) {
+  if (act == NCNN_B200_ACT_NONE) f(std::true_type{});
+  else f(std::false_type{});
+}
+template <class T, class PLAIN>
+__device__ __forceinline__ T tokens_result(PLAIN, int sum, float step, float weight_step, float bias, int act) {
+  const float t = tokens_sum(sum, step, weight_step, bias);
+  return op_put<T>(PLAIN::value ? t : tokens_activate<T>(t, act));
 }
 
 }  // namespace nb

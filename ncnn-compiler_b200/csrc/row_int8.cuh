@@ -21,6 +21,29 @@ constexpr float kRowMagic = 12582912.0f;             // 1.5 2^23
 // |x| as an integer that orders infinities and NaN above all numbers
 __device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+// The largest magnitude of some elements so far: 16-bit types as the larger of two halves' bits, which row_top_bits joins and
+// makes fp32's.
+template <class T, int V>
+__device__ __forceinline__ uint32_t row_top(const OpVec<T, V>& v, uint32_t top) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+  } else if constexpr (sizeof(T) == 2) {
+    top = __vmaxu2(top, *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max(top, magnitude_bits(op_get(v.e[i])));
+  }
+  return top;
+}
+template <class T>
+__device__ __forceinline__ uint32_t row_top_bits(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return top;
+  const unsigned short bits = static_cast<unsigned short>(max(top & 0xffffu, top >> 16));
+  return __float_as_uint(op_get(*reinterpret_cast<const T*>(&bits)));
+}
+
 struct RowScale {
   float factor;  // 127 / top, or 0
   float top;
@@ -43,7 +66,7 @@ static __device__ __noinline__ float row_round_near_half(float x, float top) {
   return kRowMagic + static_cast<float>(x < 0.0f ? -q : q);
 }
 
-// The integer in the low byte.  (A row that is held as zeros: its factor is 0, and what is not finite is left out.)
+// The integer in the low byte, for rows whose factor is not 0 (the others are zeros, whatever is in them).
 template <class T>
 __device__ __forceinline__ uint32_t row_integer(float x, const RowScale& r) {
   float v = fmaf(x, r.factor, kRowMagic);
@@ -51,7 +74,7 @@ __device__ __forceinline__ uint32_t row_integer(float x, const RowScale& r) {
     const float rest = fmaf(x, r.factor, -(v - kRowMagic));
     if (fabsf(rest) > 0.4999f) v = row_round_near_half(x, r.top);
   }
-  return __float_as_uint(r.factor == 0.0f ? 0.0f : v);
+  return __float_as_uint(v);
 }
 
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
