@@ -17,7 +17,10 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long row
                                                        float* steps) {
   constexpr int KEEP = WARPS == 1 ? 16 : 8, THREADS = WARPS * 32, ROWS = 256 / THREADS;
   using Vec = OpVec<T, V>;
-  ptx::grid_dependency_trigger();  // (the product's kernel may begin with its weights)
+  // Launched early, too, where a product follows: the trigger lets that one ask for its weights, which the kernel before this one may
+  // have written, so it comes after the wait.
+  ptx::grid_dependency_wait();
+  ptx::grid_dependency_trigger();
   __shared__ uint32_t tops[8];
   const int lane = threadIdx.x % THREADS, warp = threadIdx.x >> 5;
   const long long row = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / THREADS;
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* x, long long row
 }
 
 template <class T>
-cudaError_t quantize_rows(const T* x, long long rows, int columns, long long x_pitch, int8_t* q, long long q_pitch, float* steps, cudaStream_t st) {
+cudaError_t quantize_rows(bool early, const T* x, long long rows, int columns, long long x_pitch, int8_t* q, long long q_pitch, float* steps, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = columns % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (rows == 1 || x_pitch % V == 0) &&
                     reinterpret_cast<uintptr_t>(q) % V == 0 && (rows == 1 || q_pitch % V == 0);
@@ -78,9 +81,9 @@ cudaError_t quantize_rows(const T* x, long long rows, int columns, long long x_p
   const long long ctas = warps ? (rows + 7) / 8 : rows;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(ctas));
-  if (!wide) return op_launch(k_quantize_rows<T, 1, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
-  if (warps) return op_launch(k_quantize_rows<T, V, 1>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
-  return op_launch(k_quantize_rows<T, V, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+  if (!wide) return op_launch_early(early, k_quantize_rows<T, 1, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+  if (warps) return op_launch_early(early, k_quantize_rows<T, V, 1>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
+  return op_launch_early(early, k_quantize_rows<T, V, 8>, grid, 256, 0, st, 0, x, rows, columns, x_pitch, q, q_pitch, steps);
 }
 
 // ------------------------------------------------------------------ products at any alignment
@@ -114,16 +117,130 @@ __global__ void __launch_bounds__(256) k_product_tokens(const TokensParams p) {
     }
     __syncthreads();
   }
-  tokens_by_activation(p.act, [&](auto plain) {
+  tokens_by_activation<T>(p.act, [&](auto loop) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long long t = t0 + ty + 16 * i, c = c0 + tx + 16 * j;
         if (t < p.tokens && c < p.n)
-          static_cast<T*>(p.y)[t * p.y_pitch + c] = tokens_result<T>(plain, sum[i][j], p.steps[t], p.weight_steps[c], p.bias == nullptr ? 0.0f : p.bias[c], p.act);
+          static_cast<T*>(p.y)[t * p.y_pitch + c] = tokens_result<T>(loop, sum[i][j], p.steps[t], p.weight_steps[c], p.bias == nullptr ? 0.0f : p.bias[c], p.act);
       }
   });
+}
+
+// ------------------------------------------------------------------ single tokens
+// One or two tokens in one launch: a pass over the weights, a warp to a channel, 16 bytes to a lane and access, dp4a.  What bounds it is
+// the weights' way from HBM and the time until the first of them are there; meanwhile every CTA quantises the tokens for itself (their
+// bytes are few, and out of L2).  Nothing goes through the workspace.
+constexpr int kOneThreads = 512, kOneAhead = 8;
+constexpr int kOneSmem = 46 * 1024;
+
+// fewer than 16 bytes, zeros behind them
+__device__ __noinline__ uint4 last_bytes(const int8_t* from, int count) {
+  uint32_t w[4] = {};
+  for (int i = 0; i < count; ++i) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(from[i])) << (8 * (i % 4));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class T, int M>
+__global__ void __launch_bounds__(kOneThreads, 2) k_product_one(const T* x, long long x_pitch, const __grid_constant__ TokensParams p, int wide) {
+  constexpr int WARPS = kOneThreads / 32, V = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint8_t one_smem[];  // [M] rows of integers, zeros up to a multiple of 512
+  __shared__ uint32_t tops[M][WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pieces = (p.k + 15) / 16, row = (p.k + 511) / 512 * 512;
+  const int step = gridDim.x * WARPS;
+  ptx::grid_dependency_wait();
+  ptx::grid_dependency_trigger();
+  // the first channel's weights.  A row's last piece may reach behind the row, as far as the pitch, where zeros stand in the tokens; the
+  // last row need not have a pitch's bytes: its last piece is taken byte by byte.
+  uint4 w[kOneAhead];
+  auto ask = [&](int c, int i0) {
+    const uint4* from = reinterpret_cast<const uint4*>(p.weight + c * p.weight_pitch) + lane;
+#pragma unroll
+    for (int i = 0; i < kOneAhead; ++i) {
+      const int at = i0 + i * 32;
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (c >= p.n || at + lane >= pieces) continue;
+      if (c + 1 < p.n || (at + lane + 1) * 16 <= p.k) w[i] = __ldcs(from + at);
+      else w[i] = last_bytes(p.weight + c * p.weight_pitch + (at + lane) * 16, p.k - (at + lane) * 16);
+    }
+  };
+  int c = blockIdx.x * WARPS + warp;
+  ask(c, 0);
+  RowScale scale[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const T* from = x + (m < p.tokens ? m : 0) * x_pitch;
+    uint32_t top = 0;
+    if (wide) {
+      for (int i = threadIdx.x; i < p.k / V; i += kOneThreads) top = row_top(reinterpret_cast<const OpVec<T, V>*>(from)[i], top);
+    } else {
+      for (int i = threadIdx.x; i < p.k; i += kOneThreads) top = row_top(reinterpret_cast<const OpVec<T, 1>*>(from)[i], top);
+    }
+    top = __reduce_max_sync(~0u, row_top_bits<T>(top));
+    if (lane == 0) tops[m][warp] = top;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    scale[m] = row_scale<T>(__reduce_max_sync(~0u, lane < WARPS ? tops[m][lane] : 0u));
+    const T* from = x + (m < p.tokens ? m : 0) * x_pitch;
+    uint8_t* to = one_smem + m * row;
+    const bool zeros = scale[m].factor == 0.0f;
+    for (int i = threadIdx.x; i < row / V; i += kOneThreads) {
+      uint32_t q[V];
+      if (wide) {
+        OpVec<T, V> v{};
+        if (i * V < p.k) v = reinterpret_cast<const OpVec<T, V>*>(from)[i];
+#pragma unroll
+        for (int e = 0; e < V; ++e) q[e] = zeros ? 0u : row_integer<T>(op_get(v.e[e]), scale[m]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) q[e] = zeros || i * V + e >= p.k ? 0u : row_integer<T>(op_get(from[i * V + e]), scale[m]);
+      }
+#pragma unroll
+      for (int g = 0; g < V / 4; ++g) reinterpret_cast<uint32_t*>(to + i * V)[g] = low_bytes(q[4 * g], q[4 * g + 1], q[4 * g + 2], q[4 * g + 3]);
+    }
+  }
+  __syncthreads();
+  const uint4* ints = reinterpret_cast<const uint4*>(one_smem);
+  for (; c < p.n; c += step) {
+    int sum[M] = {};
+    for (int i0 = 0; i0 < pieces; i0 += 32 * kOneAhead) {
+#pragma unroll
+      for (int i = 0; i < kOneAhead; ++i) {
+        const int at = i0 + i * 32 + lane;
+        if (i0 + i * 32 >= pieces) break;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const uint4 a = ints[m * (row / 16) + at];
+          sum[m] = __dp4a(static_cast<int>(a.x), static_cast<int>(w[i].x), sum[m]);
+          sum[m] = __dp4a(static_cast<int>(a.y), static_cast<int>(w[i].y), sum[m]);
+          sum[m] = __dp4a(static_cast<int>(a.z), static_cast<int>(w[i].z), sum[m]);
+          sum[m] = __dp4a(static_cast<int>(a.w), static_cast<int>(w[i].w), sum[m]);
+        }
+      }
+      if (i0 + 32 * kOneAhead < pieces) ask(c, i0 + 32 * kOneAhead);
+      else ask(c + step, 0);
+    }
+#pragma unroll
+    for (int m = 0; m < M; ++m) sum[m] = __reduce_add_sync(~0u, sum[m]);
+    // lane m finishes token m
+    int mine = sum[0];
+    float token_step = scale[0].step;
+#pragma unroll
+    for (int m = 1; m < M; ++m) {
+      mine = lane == m ? sum[m] : mine;
+      token_step = lane == m ? scale[m].step : token_step;
+    }
+    if (lane < M && lane < p.tokens) {
+      T* y = static_cast<T*>(p.y) + lane * p.y_pitch + c;
+      const float ws = __ldg(p.weight_steps + c), bias = p.bias == nullptr ? 0.0f : __ldg(p.bias + c);
+      tokens_by_activation<T>(p.act, [&](auto loop) { *y = tokens_result<T>(loop, mine, token_step, ws, bias, p.act); });
+    }
+  }
 }
 
 // ------------------------------------------------------------------ tensor cores
@@ -159,8 +276,8 @@ int product_few(TcTokensParams p, int device, int sms, cudaStream_t st) {
   p.tiles_c = (t.n + 127) / 128;
   const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_c;
   int ranks = 1;
-  // (two CTAs to an SM have no room for the sums of more than 64 tokens)
-  while (ranks < 8 && tiles * ranks * 2 <= (p.columns <= 64 ? 2ll : 1ll) * sms && ranks * 2 <= p.k_blocks) ranks *= 2;
+  // one CTA to an SM with a deep ring, while there are few tiles (64 tokens through 4096 x 11008: 86 CTAs 16.1 us, 172 on 148 SMs 17.1)
+  while (ranks < 8 && tiles * ranks * 2 <= sms && ranks * 2 <= p.k_blocks) ranks *= 2;
   if (tiles * ranks > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens");
   p.t.ranks = ranks;
   p.stage_bytes = 16384 + p.columns * 128;
@@ -199,6 +316,19 @@ int product_pair(TcTokensParams p, int columns, int device, int sms, cudaStream_
   return op_launched("op_inner_product_tokens",
                      op_launch_early(true, tc_tokens_pair_kernel<T>, dim3(pairs * 2), kTokPairThreads, smem, st, 2, p, map_w, map_q, map_y));
 }
+
+template <class T>
+cudaError_t product_one(const T* x, long long x_pitch, const TokensParams& t, int sms, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const int wide = t.k % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (t.tokens == 1 || x_pitch % V == 0) ? 1 : 0;
+  const dim3 grid(std::min(2 * sms, (t.n + kOneThreads / 32 - 1) / (kOneThreads / 32)));
+  const int row = (t.k + 511) / 512 * 512;
+  if (t.tokens == 1) return op_launch_early(true, k_product_one<T, 1>, grid, kOneThreads, row, st, 0, x, x_pitch, t, wide);
+  return op_launch_early(true, k_product_one<T, 2>, grid, kOneThreads, 2 * row, st, 0, x, x_pitch, t, wide);
+}
+// Whether a call takes k_product_one: its integers fit in shared memory without asking for more.  (Four tokens through 4096 x 4096: 10.2 us,
+// 9.3 on the tensor cores; one: 5.8 and 9.1.)
+bool one_fits(long long tokens, int k) { return tokens <= 2 && tokens * ((k + 511ll) / 512 * 512) <= kOneSmem; }
 
 template <class T>
 int product_tc(const TokensParams& t, int device, cudaStream_t st) {
@@ -251,7 +381,7 @@ extern "C" int ncnn_b200_op_quantize_rows(const void* x, int32_t type, int64_t r
     DeviceGuard guard(device);
     return op_by_type(type, [&](auto t) {
       using T = decltype(t);
-      return op_launched(kOp, quantize_rows<T>(static_cast<const T*>(x), rows, columns, x_pitch, q, q_pitch, steps, static_cast<cudaStream_t>(stream)));
+      return op_launched(kOp, quantize_rows<T>(false, static_cast<const T*>(x), rows, columns, x_pitch, q, q_pitch, steps, static_cast<cudaStream_t>(stream)));
     });
   });
 }
@@ -313,9 +443,11 @@ extern "C" int ncnn_b200_op_inner_product_tokens(const void* x, void* y, int32_t
     p.act = activation;
     return op_by_type(type, [&](auto t) {
       using T = decltype(t);
-      if (const cudaError_t e = quantize_rows<T>(static_cast<const T*>(x), tokens, k, x_pitch, q, p.q_pitch, steps, st); e != cudaSuccess) return op_launched(kOp, e);
+      const bool aligned = reinterpret_cast<uintptr_t>(weight) % 16 == 0 && (n == 1 || (weight_pitch % 16 == 0 && weight_pitch < (1ll << 39)));
+      if (aligned && one_fits(tokens, k)) return op_launched(kOp, product_one<T>(static_cast<const T*>(x), x_pitch, p, op_sm_count(device), st));
+      if (const cudaError_t e = quantize_rows<T>(true, static_cast<const T*>(x), tokens, k, x_pitch, q, p.q_pitch, steps, st); e != cudaSuccess) return op_launched(kOp, e);
       // (weights whose rows TMA cannot start at go through the CUDA cores)
-      if (reinterpret_cast<uintptr_t>(weight) % 16 == 0 && (n == 1 || (weight_pitch % 16 == 0 && weight_pitch < (1ll << 39)))) {
+      if (aligned) {
         if (encode_tiled() == nullptr) return op_fail(NCNN_B200_STATUS_RUNTIME, "op_inner_product_tokens: cuTensorMapEncodeTiled is not available from this driver");
         return product_tc<T>(p, device, st);
       }

@@ -31,19 +31,23 @@ __device__ __forceinline__ float tokens_sum(int sum, float step, float weight_st
 template <class T>
 __device__ __noinline__ float tokens_activate(float t, int act) {
   if (act == NCNN_B200_ACT_RELU) return t > 0.0f ? t : t == t ? 0.0f : t;  // (a NaN stays one)
-  if (act == NCNN_B200_ACT_SWISH) return sizeof(T) == 4 ? t / (1.0f + expf(-t)) : __fdividef(t, 1.0f + __expf(-t));  // (16 bits: good to 2^-20)
+  if (act == NCNN_B200_ACT_SWISH) return t / (1.0f + expf(-t));
   return 0.5f * t * erfcf(t * -0.7071067811865476f);
 }
-// f(true_type) where there is no activation, f(false_type) where there is one
-template <class F>
+// f is given what kind of loop it is: one without an activation, one with the Swish of 16-bit results in line, or one that calls.
+enum class Loop { kPlain, kSwish, kCalls };
+template <class T, class F>
 __device__ __forceinline__ void tokens_by_activation(int act, F&& f) {
-  if (act == NCNN_B200_ACT_NONE) f(std::true_type{});
-  else f(std::false_type{});
+  if (act == NCNN_B200_ACT_NONE) f(std::integral_constant<Loop, Loop::kPlain>{});
+  else if (sizeof(T) == 2 && act == NCNN_B200_ACT_SWISH) f(std::integral_constant<Loop, Loop::kSwish>{});
+  else f(std::integral_constant<Loop, Loop::kCalls>{});
 }
-template <class T, class PLAIN>
-__device__ __forceinline__ T tokens_result(PLAIN, int sum, float step, float weight_step, float bias, int act) {
+template <class T, class LOOP>
+__device__ __forceinline__ T tokens_result(LOOP, int sum, float step, float weight_step, float bias, int act) {
   const float t = tokens_sum(sum, step, weight_step, bias);
-  return op_put<T>(PLAIN::value ? t : tokens_activate<T>(t, act));
+  if constexpr (LOOP::value == Loop::kPlain) return op_put<T>(t);
+  else if constexpr (LOOP::value == Loop::kSwish) return op_put<T>(__fdividef(t, 1.0f + __expf(-t)));  // (good to 2^-20)
+  else return op_put<T>(tokens_activate<T>(t, act));
 }
 
 }  // namespace nb

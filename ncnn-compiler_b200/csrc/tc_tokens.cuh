@@ -161,7 +161,7 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
   // (few warps do this, each a long way: what counts is instructions, so that addresses are stepped and not computed)
   if (ranks == 1) {
     if (warp >= 2 && ok)
-      tokens_by_activation(p.t.act, [&](auto plain) {
+      tokens_by_activation<T>(p.t.act, [&](auto loop) {
 #pragma unroll 1
         for (int at = group * 16; at < left; at += 32) {
           uint32_t v[16];
@@ -170,7 +170,7 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
           T* to = y + at * p.t.y_pitch;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            if (there && at + j < left) *to = tokens_result<T>(plain, static_cast<int>(v[j]), steps[at + j], ws, bias, p.t.act);
+            if (there && at + j < left) *to = tokens_result<T>(loop, static_cast<int>(v[j]), steps[at + j], ws, bias, p.t.act);
             to += p.t.y_pitch;
           }
         }
@@ -201,7 +201,7 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
     cluster_sync_all();
     if (warp >= 2 && ok) {
       const int first = rank * share, mine = min(share, left - first);
-      tokens_by_activation(p.t.act, [&](auto plain) {
+      tokens_by_activation<T>(p.t.act, [&](auto loop) {
 #pragma unroll 1
         for (int i0 = group; i0 < mine; i0 += 8) {
           // four tokens at a time: their loads are under way together
@@ -217,7 +217,7 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
           T* to = y + (first + i0) * p.t.y_pitch;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (there && i0 + 2 * j < mine) *to = tokens_result<T>(plain, sum[j], steps[first + i0 + 2 * j], ws, bias, p.t.act);
+            if (there && i0 + 2 * j < mine) *to = tokens_result<T>(loop, sum[j], steps[first + i0 + 2 * j], ws, bias, p.t.act);
             to += 2 * p.t.y_pitch;
           }
         }
@@ -386,7 +386,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
       if (!ok) break;
       tc_fence_after_sync();
       const uint32_t at_tmem = tmem + (lanes << 16) + static_cast<uint32_t>(acc) * 256u + static_cast<uint32_t>(group * half);
-      tokens_by_activation(p.t.act, [&](auto plain) {
+      tokens_by_activation<T>(p.t.act, [&](auto loop) {
 #pragma unroll 1
       for (int at = 0; at < half; at += WIDE) {
         if (p.stored) {
@@ -405,16 +405,16 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
             for (int j = 0; j < 16; j += 4) {
               const float4 ws = __ldg(reinterpret_cast<const float4*>(p.t.weight_steps + c + j));
               const float4 b = p.t.bias == nullptr ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : __ldg(reinterpret_cast<const float4*>(p.t.bias + c + j));
-              y[j] = tokens_result<T>(plain, static_cast<int>(v[j]), step, ws.x, b.x, p.t.act);
-              y[j + 1] = tokens_result<T>(plain, static_cast<int>(v[j + 1]), step, ws.y, b.y, p.t.act);
-              y[j + 2] = tokens_result<T>(plain, static_cast<int>(v[j + 2]), step, ws.z, b.z, p.t.act);
-              y[j + 3] = tokens_result<T>(plain, static_cast<int>(v[j + 3]), step, ws.w, b.w, p.t.act);
+              y[j] = tokens_result<T>(loop, static_cast<int>(v[j]), step, ws.x, b.x, p.t.act);
+              y[j + 1] = tokens_result<T>(loop, static_cast<int>(v[j + 1]), step, ws.y, b.y, p.t.act);
+              y[j + 2] = tokens_result<T>(loop, static_cast<int>(v[j + 2]), step, ws.z, b.z, p.t.act);
+              y[j + 3] = tokens_result<T>(loop, static_cast<int>(v[j + 3]), step, ws.w, b.w, p.t.act);
             }
           } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const bool there = c + j < p.t.n;
-              y[j] = tokens_result<T>(plain, static_cast<int>(v[j]), step, there ? __ldg(p.t.weight_steps + c + j) : 0.0f,
+              y[j] = tokens_result<T>(loop, static_cast<int>(v[j]), step, there ? __ldg(p.t.weight_steps + c + j) : 0.0f,
                                       there && p.t.bias != nullptr ? __ldg(p.t.bias + c + j) : 0.0f, p.t.act);
             }
           }

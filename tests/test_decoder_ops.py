@@ -722,3 +722,33 @@ def test_a_decoder_step(pkg, count):
     graph.replay()
     torch.cuda.synchronize()
     check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 5000), (1, 47000, 33), (1, 100, 7), (2, 12000, 300), (3, 1003, 257), (4, 11264, 4800), (4, 13000, 100), (2, 17, 1)])
+def test_inner_product_of_single_tokens(pkg, element, m, k, n):
+    pitch = (k + 15) // 16 * 16
+    check_product(pkg, element, m, k, n, "none", w_pitch=pitch)
+    check_product(pkg, element, m, k, n, "gelu", x_pitch=k + 3, w_pitch=pitch + 32, w_shift=32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3, 40, 300])
+def test_weights_written_just_before_a_product(pkg, m):
+    """The product's kernels begin early with their weights: what the call before writes has to be there."""
+    k, n = 4096, 2048
+    g = gen(m)
+    x = normal(g, m, k).bfloat16()
+    full = [normal(g, n, k) for _ in range(4)]
+    w, ws = torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda")
+    y = [torch.zeros(m, n, device="cuda", dtype=torch.bfloat16) for _ in full]
+    space = torch.empty(pkg.op_inner_product_tokens_workspace(m, k), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    for f, out in zip(full, y):
+        pkg.op_quantize_rows(f.data_ptr(), "f32", n, k, w.data_ptr(), ws.data_ptr())
+        pkg.op_inner_product_tokens(x.data_ptr(), out.data_ptr(), "bf16", m, k, n, w.data_ptr(), ws.data_ptr(), space.data_ptr(), space.numel())
+    pkg.op_check_status()
+    for f, out in zip(full, y):
+        want, bound = product_want(*quantised(x), *quantised(f), None, "none", "bf16")
+        assert_within(out, want, bound)
