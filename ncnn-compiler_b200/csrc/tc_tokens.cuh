@@ -105,9 +105,10 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
       if (p.stall == 0) {
         grid_dependency_wait();
         for (int i = 0; i < ahead; ++i) tma_load_2d(ring + i * stage_bytes + 16384u, &map_q, smem_u32(&full[i]), (kb0 + i) * 128, t0);
+        int s = 0;
+        uint32_t ph = 0;
         for (int i = ahead; i < count; ++i) {
-          const int s = i % S;
-          if (!mbar_wait_bounded(smem_u32(&empty[s]), (i / S - 1) & 1, abort_ptr, p.wait_ns)) {
+          if (!mbar_wait_bounded(smem_u32(&empty[s]), ph, abort_ptr, p.wait_ns)) {
             gave_up();
             break;
           }
@@ -115,6 +116,10 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
           tma_load_2d(ring + s * stage_bytes, &map_w, smem_u32(&full[s]), (kb0 + i) * 128, c0);
           tma_load_2d(ring + s * stage_bytes + 16384u, &map_q, smem_u32(&full[s]), (kb0 + i) * 128, t0);
           issued = i + 1;
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
       }
       ring_landed(full, S, issued);
@@ -122,16 +127,21 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = instr_desc(2u, 1u, 128u, static_cast<uint32_t>(p.columns));
-      bool ok = true;
+      bool ok = true, full_seen = false;  // (tested before a commit: see tc_gemm_common.cuh)
+      int s = 0;
+      uint32_t ph = 0;
       for (int i = 0; i < count; ++i) {
-        const int s = i % S;
-        ok = mbar_wait_bounded(smem_u32(&full[s]), (i / S) & 1, abort_ptr, p.wait_ns);
+        ok = full_seen || mbar_wait_bounded(smem_u32(&full[s]), ph, abort_ptr, p.wait_ns);
         if (!ok) break;
         tc_fence_after_sync();
         const uint64_t a = smem_desc_kmajor(ring + s * stage_bytes, 128), b = smem_desc_kmajor(ring + s * stage_bytes + 16384u, 128);
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_i8(tmem, a + 2u * k, b + 2u * k, idesc, i > 0 || k > 0);
+        const int next = s + 1 == S ? 0 : s + 1;
+        if (next == 0) ph ^= 1u;
+        full_seen = i + 1 < count && mbar_test_wait(smem_u32(&full[next]), ph);
         tc_commit(smem_u32(&empty[s]));
+        s = next;
       }
       if (!ok) gave_up();
       tc_commit(smem_u32(&done));  // (also where a wait ran out: nor may MMAs be under way)
@@ -286,36 +296,54 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
     if (elect_one()) {
       const int half = p.columns / 2;
       int issued = 0;  // K blocks of all tiles
-      bool ok = p.stall == 0, waited = false;
-      int held = 0;    // blocks whose tokens wait for the kernel before
-      auto tokens_of = [&](int i) {
-        const int tile = pair + i / KB * pairs, kb = i % KB;
-        tma_load_2d_pair(ring + i % S * stage_bytes, &map_q, map_to_cta(smem_u32(&full[i % S]), 0u), kb * 128,
-                         tile % p.tiles_t * 256 + static_cast<int>(rank) * 128);
+      bool ok = p.stall == 0;
+      // (counters are stepped: a block's divisions took 900 clocks, its MMAs take 512)
+      int s = 0;
+      uint32_t ph = 0;
+      const uint32_t full0 = map_to_cta(smem_u32(&full[0]), 0u);
+      auto rows_of = [&](int tile, int* c0, int* t0) {
+        *c0 = tile / p.tiles_t * p.columns + static_cast<int>(rank) * half;
+        *t0 = tile % p.tiles_t * 256 + static_cast<int>(rank) * 128;
       };
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        const int c0 = tile / p.tiles_t * p.columns + static_cast<int>(rank) * half;
-        for (int kb = 0; kb < KB; ++kb) {
-          const int s = issued % S;
-          if (issued == S && !waited) {
-            grid_dependency_wait();
-            waited = true;
-            for (; held < issued; ++held) tokens_of(held);
+      // the first ring of weights, and when the kernel before has ended, its tokens
+      int tile = pair, kb = 0, c0 = 0, t0 = 0;
+      rows_of(tile, &c0, &t0);
+      for (int pass = 0; ok && pass < 2; ++pass) {
+        if (pass == 1) grid_dependency_wait();
+        tile = pair;
+        kb = 0;
+        rows_of(tile, &c0, &t0);
+        for (issued = 0; issued < S && tile < tiles; ++issued) {
+          if (pass == 0) {
+            if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[issued]), 2u * stage_bytes);
+            tma_load_2d_pair(ring + issued * stage_bytes + 16384u, &map_w, full0 + issued * 8u, kb * 128, c0);
+          } else {
+            tma_load_2d_pair(ring + issued * stage_bytes, &map_q, full0 + issued * 8u, kb * 128, t0);
           }
-          if (issued >= S && !mbar_wait_bounded(smem_u32(&empty[s]), (issued / S - 1) & 1, abort_ptr, p.wait_ns)) {
+          if (++kb == KB) {
+            kb = 0;
+            tile += pairs;
+            rows_of(tile, &c0, &t0);
+          }
+        }
+      }
+      for (; ok && tile < tiles; tile += pairs, kb = 0) {
+        rows_of(tile, &c0, &t0);
+        for (; kb < KB; ++kb) {
+          if (!mbar_wait_bounded(smem_u32(&empty[s]), ph, abort_ptr, p.wait_ns)) {
             ok = false;
             gave_up();
             break;
           }
           if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full[s]), 2u * stage_bytes);
-          tma_load_2d_pair(ring + s * stage_bytes + 16384u, &map_w, map_to_cta(smem_u32(&full[s]), 0u), kb * 128, c0);
-          if (waited) tokens_of(issued);
+          tma_load_2d_pair(ring + s * stage_bytes + 16384u, &map_w, full0 + s * 8u, kb * 128, c0);
+          tma_load_2d_pair(ring + s * stage_bytes, &map_q, full0 + s * 8u, kb * 128, t0);
           ++issued;
+          if (++s == S) {
+            s = 0;
+            ph ^= 1u;
+          }
         }
-      }
-      if (!waited) {
-        grid_dependency_wait();
-        for (; held < issued; ++held) tokens_of(held);
       }
       if (rank == 0) ring_landed(full, S, issued);  // (CTA 1's bytes are counted there too, and it waits for CTA 0 below)
     }
