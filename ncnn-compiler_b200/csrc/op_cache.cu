@@ -17,93 +17,124 @@ struct CacheRowsParams {
   int kinds;    // 2: keys and values; 1: those that are not null
 };
 
-// A row (keys or values of a token's head) to LANES lanes, eight components to each: what a lane reads is one or two accesses of 16
-// bytes (WIDE) or eight elements.  Bound: HBM for many tokens, the chain of loads (starts, lens, table, row) for few.
-template <class T, int LANES, bool WIDE, bool READ>
+// PER rows (keys or values of neighbouring heads of a token) to LANES lanes, eight components of each row to a lane: what a lane reads of
+// a row is one or two accesses of 16 bytes (WIDE) or eight elements.  Bound: HBM for many tokens, which wants several rows under way in
+// each lane and their place found once; the chain of loads (starts, lens, table, row) for few, which wants many lanes.
+template <class T, int LANES, int PER, bool WIDE, bool READ>
 __global__ void __launch_bounds__(256) k_cache_rows(const __grid_constant__ CacheRowsParams p) {
   const CacheParams& c = p.c;
-  constexpr int ROWS = 256 / LANES;
+  constexpr int GROUPS = 256 / LANES, V = 16 / sizeof(T);
   const int lane = threadIdx.x % LANES;
-  const long long rows = c.tokens * p.kinds * c.kv_heads;
-  const long long line = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / LANES;
-  const bool there = line < rows;
-  const long long rest = (there ? line : 0) / c.kv_heads, token = rest / p.kinds;
-  const int head = static_cast<int>((there ? line : 0) - rest * c.kv_heads);
+  const int chunks = (c.kv_heads + PER - 1) / PER;
+  const long long groups = c.tokens * p.kinds * chunks;
+  const long long group = static_cast<long long>(blockIdx.x) * GROUPS + threadIdx.x / LANES;
+  const bool there = group < groups;
+  const long long rest = (there ? group : 0) / chunks, token = rest / p.kinds;
+  const int head0 = static_cast<int>((there ? group : 0) - rest * chunks) * PER;
+  const int rows = there ? min(PER, c.kv_heads - head0) : 0;
   const bool value = p.kinds == 2 ? rest % 2 == 1 : p.k == nullptr;
-  T* row = static_cast<T*>(value ? p.v : p.k) + token * (value ? p.v_token : p.k_token) + head * (value ? p.v_head : p.k_head);
+  const long long head_step = value ? p.v_head : p.k_head;
   const int at = lane * 8;
-  float x[8];
-  uint32_t top = 0;
+  T* row = static_cast<T*>(value ? p.v : p.k) + token * (value ? p.v_token : p.k_token) + head0 * head_step + at;
+  OpVec<T, V> x[PER][8 / V];
   if constexpr (!READ) {
-    // (asked for before the row's place is known)
-    constexpr int V = 16 / sizeof(T);
+    // (asked for before the rows' place is known)
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      if constexpr (WIDE) {
-        OpVec<T, V> w{};
-        if (there && at + i < c.d) w = *reinterpret_cast<const OpVec<T, V>*>(row + at + i);
+    for (int r = 0; r < PER; ++r)
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[i + e] = at + i < c.d ? op_get(w.e[e]) : 0.0f;
-      } else {
+      for (int i = 0; i < 8 / V; ++i) {
+        x[r][i] = {};
+        if constexpr (WIDE) {
+          if (r < rows && at + i * V < c.d) x[r][i] = *reinterpret_cast<const OpVec<T, V>*>(row + r * head_step + i * V);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[i + e] = there && at + i + e < c.d ? op_get(row[at + i + e]) : 0.0f;
+          for (int e = 0; e < V; ++e)
+            if (r < rows && at + i * V + e < c.d) x[r][i].e[e] = row[r * head_step + i * V + e];
+        }
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(x[e]));
-#pragma unroll
-    for (int w = LANES / 2; w > 0; w >>= 1) top = max(top, __shfl_xor_sync(~0u, top, w));
   }
-  if (!there) return;
-  const CachePlace place = cache_place(c, token);
-  if (place.sequence < 0) return;
-  const int page = place.position < 0 ? -1 : cache_page(c, place.sequence, place.position);
-  const long long slot = (((page < 0 ? 0ll : page) * c.kv_heads + head) << c.page_shift) + (place.position & ((1 << c.page_shift) - 1));
+  const CachePlace place = there ? cache_place(c, token) : CachePlace{-1, -1};
+  const int page = place.sequence < 0 || place.position < 0 ? -1 : cache_page(c, place.sequence, place.position);
+  const long long slot = (((page < 0 ? 0ll : page) * c.kv_heads + head0) << c.page_shift) + (place.position & ((1 << c.page_shift) - 1));
   int8_t* ints = (value ? c.v : c.k) + slot * c.row + at;
   float* steps = (value ? c.v_steps : c.k_steps) + slot;
+  const long long line = 1ll << c.page_shift;  // rows from a head to the next
   if constexpr (READ) {
-    OpVec<T, 8> out{};
-    if (page >= 0 && at < c.row) {
-      const float step = *steps;
-      const uint2 w = *reinterpret_cast<const uint2*>(ints);
+    uint2 w[PER];
+    float step[PER];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out.e[e] = op_put<T>(static_cast<float>(static_cast<int8_t>((e < 4 ? w.x : w.y) >> (8 * (e % 4)))) * step);
+    for (int r = 0; r < PER; ++r) {
+      w[r] = make_uint2(0u, 0u);
+      step[r] = 0.0f;
+      if (r < rows && page >= 0 && at < c.row) {
+        w[r] = *reinterpret_cast<const uint2*>(ints + r * line * c.row);
+        step[r] = steps[r * line];
+      }
     }
-    constexpr int V = 16 / sizeof(T);
+    if (place.sequence < 0) return;
 #pragma unroll
-    for (int i = 0; i < 8; i += V) {
-      if constexpr (WIDE) {
-        if (at + i < c.d) *reinterpret_cast<OpVec<T, V>*>(row + at + i) = *reinterpret_cast<const OpVec<T, V>*>(&out.e[i]);
-      } else {
+    for (int r = 0; r < PER; ++r) {
+      if (r >= rows) break;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (at + i + e < c.d) row[at + i + e] = out.e[i + e];
+      for (int i = 0; i < 8 / V; ++i) {
+        OpVec<T, V> out;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int n = i * V + e;
+          out.e[e] = op_put<T>(static_cast<float>(static_cast<int8_t>((n < 4 ? w[r].x : w[r].y) >> (8 * (n % 4)))) * step[r]);
+        }
+        if constexpr (WIDE) {
+          if (at + i * V < c.d) *reinterpret_cast<OpVec<T, V>*>(row + r * head_step + i * V) = out;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (at + i * V + e < c.d) row[r * head_step + i * V + e] = out.e[e];
+        }
       }
     }
   } else {
-    if (page < 0 || at >= c.row) return;
-    const RowScale scale = row_scale<T>(top);
-    uint32_t w[2];
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
-      w[g] = scale.factor == 0.0f ? 0u : low_bytes(row_integer<T>(x[4 * g], scale), row_integer<T>(x[4 * g + 1], scale), row_integer<T>(x[4 * g + 2], scale),
-                       row_integer<T>(x[4 * g + 3], scale));
-    *reinterpret_cast<uint2*>(ints) = make_uint2(w[0], w[1]);
-    if (lane == 0) *steps = scale.step;
+    for (int r = 0; r < PER; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8 / V; ++i) top = row_top(x[r][i], top);
+      top = row_top_bits<T>(top);
+#pragma unroll
+      for (int w = LANES / 2; w > 0; w >>= 1) top = max(top, __shfl_xor_sync(~0u, top, w));
+      if (r >= rows || page < 0 || at >= c.row) continue;
+      const RowScale scale = row_scale<T>(top);
+      uint32_t w[2] = {0u, 0u};
+      if (scale.factor != 0.0f) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t b[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[e] = row_integer<T>(op_get(x[r][(4 * g + e) / V].e[(4 * g + e) % V]), scale);
+          w[g] = low_bytes(b[0], b[1], b[2], b[3]);
+        }
+      }
+      *reinterpret_cast<uint2*>(ints + r * line * c.row) = make_uint2(w[0], w[1]);
+      if (lane == 0) steps[r * line] = scale.step;
+    }
   }
 }
 
 template <class T, bool READ>
-cudaError_t cache_rows(const CacheRowsParams& p, bool wide, cudaStream_t st) {
-  const long long rows = p.c.tokens * p.kinds * p.c.kv_heads;
+cudaError_t cache_rows(const CacheRowsParams& p, bool wide, int sms, cudaStream_t st) {
   const int pieces = p.c.row / 8;
-  auto go = [&](auto lanes) {
-    constexpr int LANES = decltype(lanes)::value;
-    const dim3 grid(static_cast<unsigned>((rows + 256 / LANES - 1) / (256 / LANES)));
-    return wide ? op_launch(k_cache_rows<T, LANES, true, READ>, grid, 256, 0, st, 0, p) : op_launch(k_cache_rows<T, LANES, false, READ>, grid, 256, 0, st, 0, p);
+  auto go = [&](auto lanes, auto per) {
+    constexpr int LANES = decltype(lanes)::value, PER = decltype(per)::value;
+    const long long groups = p.c.tokens * p.kinds * ((p.c.kv_heads + PER - 1) / PER);
+    const dim3 grid(static_cast<unsigned>((groups + 256 / LANES - 1) / (256 / LANES)));
+    return wide ? op_launch(k_cache_rows<T, LANES, PER, true, READ>, grid, 256, 0, st, 0, p) : op_launch(k_cache_rows<T, LANES, PER, false, READ>, grid, 256, 0, st, 0, p);
   };
-  if (pieces <= 8) return go(std::integral_constant<int, 8>{});
-  return pieces <= 16 ? go(std::integral_constant<int, 16>{}) : go(std::integral_constant<int, 32>{});
+  auto by_lanes = [&](auto per) {
+    if (pieces <= 8) return go(std::integral_constant<int, 8>{}, per);
+    return pieces <= 16 ? go(std::integral_constant<int, 16>{}, per) : go(std::integral_constant<int, 32>{}, per);
+  };
+  // four rows to a lane where there are enough of them for the whole device
+  const long long rows = p.c.tokens * p.kinds * p.c.kv_heads;
+  return p.c.kv_heads > 1 && rows * pieces >= 4096ll * sms ? by_lanes(std::integral_constant<int, 4>{}) : by_lanes(std::integral_constant<int, 1>{});
 }
 
 // ------------------------------------------------------------------ arguments
@@ -215,7 +246,8 @@ int cache_rows_call(const char* op, bool read, const ncnn_b200_cache* cache, con
     return op_by_type(type, [&](auto t) {
       using T = decltype(t);
       const cudaStream_t st = static_cast<cudaStream_t>(stream);
-      return op_launched(op, read ? cache_rows<T, true>(p, wide, st) : cache_rows<T, false>(p, wide, st));
+      const int sms = op_sm_count(device);
+      return op_launched(op, read ? cache_rows<T, true>(p, wide, sms, st) : cache_rows<T, false>(p, wide, sms, st));
     });
   });
 }

@@ -272,11 +272,16 @@ template <class T>
 int product_few(TcTokensParams p, int device, int sms, cudaStream_t st) {
   const TokensParams& t = p.t;
   p.columns = t.tokens >= 128 ? 128 : static_cast<int>((t.tokens + 15) / 16 * 16);
-  p.tiles_t = static_cast<int>((t.tokens + p.columns - 1) / p.columns);
   p.tiles_c = (t.n + 127) / 128;
-  const long long tiles = static_cast<long long>(p.tiles_t) * p.tiles_c;
+  auto tiles_of = [&](int columns) { return (t.tokens + columns - 1) / columns * p.tiles_c; };
+  // Narrower tiles, down to 32 tokens, and then shares of the K blocks, until the SMs have a CTA each with a deep ring.  Tiles and ranks
+  // of calls that leave SMs idle: 256 tokens through 4096 x 4096 64 x 1 13.5 us, 128 x 2 15.7; 333 through 1000 x 1234 32 x 1 10.0, 64 x 4
+  // 11.1, 128 x 4 12.7; 128 through 4096 x 4096 32 x 1 12.4, 128 x 4 12.9.  64 tokens go the other way: 4096 x 4096 64 x 4 10.4, 32 x 2 10.8;
+  // 4096 x 11008 64 x 1 14.5, 32 x 1 15.0, 64 x 2 (172 CTAs on 148 SMs) 16.8.
+  while (t.tokens > 64 && p.columns > 32 && 2 * tiles_of(p.columns) <= sms) p.columns = (p.columns / 2 + 15) / 16 * 16;
+  p.tiles_t = static_cast<int>((t.tokens + p.columns - 1) / p.columns);
+  const long long tiles = tiles_of(p.columns);
   int ranks = 1;
-  // one CTA to an SM with a deep ring, while there are few tiles (64 tokens through 4096 x 11008: 86 CTAs 16.1 us, 172 on 148 SMs 17.1)
   while (ranks < 8 && tiles * ranks * 2 <= sms && ranks * 2 <= p.k_blocks) ranks *= 2;
   if (tiles * ranks > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens");
   p.t.ranks = ranks;
@@ -339,10 +344,13 @@ int product_tc(const TokensParams& t, int device, cudaStream_t st) {
   p.stall = op_stalled() ? 1 : 0;
   const int sms = op_sm_count(device);
   p.t.aligned = reinterpret_cast<uintptr_t>(t.weight_steps) % 16 == 0 && reinterpret_cast<uintptr_t>(t.bias) % 16 == 0 ? 1 : 0;
-  const long long rows = (t.tokens + 255) / 256;
-  if (t.tokens > 128 && 2 * rows * ((t.n + 255) / 256) >= sms) return product_pair<T>(p, 256, device, sms, st);
-  if (t.tokens > 128 && 2 * rows * ((t.n + 127) / 128) >= sms) return product_pair<T>(p, 128, device, sms, st);
-  return product_few<T>(p, device, sms, st);
+  // Tiles of 128 x 128 while two of them to an SM hold the call (1024 tokens through 4096 x 4096 24.1 us, 24.0 in pairs; 160 through
+  // 4096 x 12288 22.2 and 22.6), otherwise pairs; their tiles' width by the columns that the busiest pair has (512 through
+  // 4096 x 11008: 3 tiles of 128 29.7 us, 2 of 256 31.6, 128 x 128 37.3; 300 through 4096 x 14336: 4 of 128 50, 2 of 256 35).
+  const long long rows = (t.tokens + 255) / 256, pairs = sms / 2;
+  if ((t.tokens + 127) / 128 * ((t.n + 127) / 128) <= 2ll * sms) return product_few<T>(p, device, sms, st);
+  auto busiest = [&](int columns) { return (rows * ((t.n + columns - 1) / columns) + pairs - 1) / pairs * columns; };
+  return product_pair<T>(p, busiest(128) < busiest(256) ? 128 : 256, device, sms, st);
 }
 
 constexpr long long kTokensMost = 1ll << 31, kColumnsMost = 1 << 24, kSumMost = 131072;

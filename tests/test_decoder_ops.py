@@ -233,7 +233,10 @@ def product_want(q, steps, w, weight_steps, bias, act, element):
     elif act == "gelu":
         y = t * torch.special.ndtr(t)
         # erfcf is off by 4 steps; its argument's two roundings count 2 z^2 + 2 times (z = t / sqrt 2: t^2 + 2)
-        off = 1.13 * off + y.abs() * F * (12 + 3 * (t.clamp_max(0) ** 2 + 2)) + 2.0 ** -118
+        # 16 bits: a fit of erfcx that is off by 2^-16.8, times an exponential of z^2 (which is F off, so the power z^2 F) by __expf, 2 +
+        # 1.173 z^2 steps of 2 F, and a quotient by 2 steps
+        own = F * (12 + 3 * (t.clamp_max(0) ** 2 + 2)) if element == "f32" else 2.0 ** -16.8 + F * (16 + 2 * t ** 2).clamp_max(2.0 ** 10)
+        off = 1.13 * off + y.abs() * own + 2.0 ** -118
     else:
         y = t
     return y, off + U[element] * (y.abs() + off) + TINY[element]
