@@ -1,14 +1,16 @@
 // Attention over a paged cache of 8-bit integers for few rows: a pass over the pages at HBM speed.
 //
-// A CTA has a tile of 16 rows that read one key head (a row is a token and one of the head's query heads) and a range of keys; its
-// warps take blocks of 16 keys in turn, each with a running maximum, sum and result.  The products are mma.sync m16n8k16: HBM is the
-// bound, not the tensor cores, and tcgen05 would want 128 rows.
+// A CTA has a tile of 8, 16 or 32 rows that read one key head (a row is a token and one of the head's query heads) and a range of keys;
+// its warps take blocks of 16 keys in turn, each with a running maximum, sum and result.  The products are mma.sync m16n8k16 with the
+// keys, and then the values' components, as the 16 and the rows as the 8: a decoding step has 4 to 8 rows, and the other way half of
+// every instruction would be for rows that are not there.  HBM is the bound, not the tensor cores; tcgen05 would want 128 rows.
 //
 // Integers are exact in either 16-bit type (|q| is at most 127), so the steps stay out of the products: a key's multiplies its scores,
 // a value's its probabilities.  No integer is exchanged between lanes.  The contraction's order is free: a lane takes 16 neighbouring
-// bytes of "its" keys as the operands of four products, and the queries are permuted to match; for values it takes the same
+// bytes of "its" two keys as the operands of four products, and the queries are permuted to match; for values it takes the same
 // components of four keys and picks one byte of each.  So a lane copies (cp.async) only what it reads itself, into a queue
 // of its own in shared memory: no barriers, and every access of shared memory takes neighbouring 16 bytes for neighbouring lanes.
+// Scores come out as [key][row] and probabilities go in as [row][key]: movmatrix turns them.
 //
 // Roundings: scores of 16-bit queries are exact products (f32 queries: three bf16 terms, 24 bits); probabilities times steps are
 // split into two bf16 terms (16 bits), f32 three.
@@ -18,11 +20,10 @@
 #pragma once
 
 #include "attend_few.cuh"
+#include "ptx_sm100.cuh"
 #include "op_cache.h"
 
 namespace nb {
-
-constexpr int kCacheRows = 16;
 
 struct AttendCacheParams {
   CacheParams c;
@@ -83,55 +84,64 @@ __device__ __forceinline__ uint2 lds_8(uint32_t at) {
   return v;
 }
 
-template <class T, int D, int WARPS, int STAGES>
+__device__ __forceinline__ uint32_t turn_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// NT: eights of rows
+template <class T, int D, int NT, int WARPS, int STAGES>
 struct CacheFewShared {
+  static constexpr int kRows = 8 * NT;
   static constexpr int kQTerms = sizeof(T) == 4 ? 3 : 1;
   static constexpr int kValueBytes = D / 8;                    // of a key that a lane takes
   static constexpr int kKeyBytes = 2 * (D / 64) * 512;         // of a block, a warp
   static constexpr int kValues = 4 * kValueBytes * 32;
-  static constexpr int kStage = kKeyBytes + kValues + 4 * 256;  // and the steps
-  uint4 q[kQTerms][D / 16][32];                                // fragments by lane
+  static constexpr int kStage = kKeyBytes + kValues + 2 * 256;  // and the steps
+  uint2 q[kQTerms][D / 16][NT][32];                            // fragments by lane
   union {
     uint8_t ring[WARPS][STAGES][kStage];
     struct {
-      float part[WARPS][kCacheRows][D + 4];
-      float top[WARPS][kCacheRows], total[WARPS][kCacheRows];
+      float part[WARPS][kRows][D + 4];
+      float top[WARPS][kRows], total[WARPS][kRows];
     };
   };
 };
 
-template <class T, int D, int WARPS, int STAGES, int BLOCKS>
+template <class T, int D, int NT, int WARPS, int STAGES, int BLOCKS>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const __grid_constant__ AttendCacheParams p) {
-  using Shared = CacheFewShared<T, D, WARPS, STAGES>;
+  using Shared = CacheFewShared<T, D, NT, WARPS, STAGES>;
   using KT = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
   using VT = __nv_bfloat16;
-  constexpr int STEPS = D / 16, QTERMS = Shared::kQTerms, PTERMS = sizeof(T) == 4 ? 3 : 2;
+  constexpr int STEPS = D / 16, QTERMS = Shared::kQTerms, PTERMS = sizeof(T) == 4 ? 3 : 2, ROWS = Shared::kRows;
   constexpr int VB = Shared::kValueBytes;
+  constexpr bool KEEP_Q = NT == 1 && QTERMS == 1 && D <= 128;  // queries in registers
   extern __shared__ __align__(128) uint8_t cache_few_smem[];
   Shared& sh = *reinterpret_cast<Shared*>(cache_few_smem);
   const CacheParams& c = p.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane >> 2, quad = lane & 3;
   const int range = blockIdx.z, kv_head = blockIdx.y, G = p.rows_a_head;
-  // rows of this tile: 16 from row0 on, of a sequence or of all
+  ptx::grid_dependency_trigger();  // (whoever joins the ranges may be there, waiting)
+  // rows of this tile: ROWS from row0 on, of a sequence or of all
   int sequence = 0;
-  long long row0 = static_cast<long long>(blockIdx.x) * kCacheRows, first = 0, rows;
+  long long row0 = static_cast<long long>(blockIdx.x) * ROWS, first = 0, rows;
   int before = 0;  // position of a sequence's first row
   if (p.prefix) {
     rows = c.tokens * G;
   } else {
-    const int tiles = static_cast<int>((static_cast<long long>(c.max_tokens) * G + kCacheRows - 1) / kCacheRows);
+    const int tiles = static_cast<int>((static_cast<long long>(c.max_tokens) * G + ROWS - 1) / ROWS);
     sequence = blockIdx.x / tiles;
-    row0 = static_cast<long long>(blockIdx.x % tiles) * kCacheRows;
+    row0 = static_cast<long long>(blockIdx.x % tiles) * ROWS;
     first = cache_start(c, sequence);
     const long long count = max(cache_start(c, sequence + 1) - first, 0ll);
     rows = min(count, static_cast<long long>(c.max_tokens)) * G;
     before = static_cast<int>(max(cache_len(c, sequence) - count, -(1ll << 30)));
   }
-  if (row0 >= rows) return;
-  // a lane's row: its token and position (lanes 16 to 31 repeat lanes 0 to 15)
-  const long long my_row = row0 + (lane & 15);
-  int my_position = -2;  // -2: no row
-  if (my_row < rows) {
+  // a lane's row: its token and position (-2: no row)
+  const long long my_row = row0 + lane;
+  int my_position = -2;
+  if (lane < ROWS && my_row < rows) {
     if (p.prefix) {
       const CachePlace place = cache_place(c, my_row / G);
       my_position = place.sequence < 0 ? -2 : place.position;
@@ -144,62 +154,63 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
   const int from = p.prefix ? range * p.chunk : p.shared + range * p.chunk;
   const int end = p.prefix ? min(p.shared, last + 1) : last + 1;
   const int to = min(from + p.chunk, end);
-  if (from >= to && p.part != nullptr) return;  // (whoever joins knows)
-  int position[2];
+  // nothing to do (whoever joins knows), and before that the kernel that this one may have overtaken: its end is waited for through
+  // this one's
+  if (last == -2 || (from >= to && p.part != nullptr)) {
+    ptx::grid_dependency_wait();
+    return;
+  }
+  int position[NT][2];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) position[r] = __shfl_sync(~0u, my_position, group + 8 * r);
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) position[t][e] = __shfl_sync(~0u, my_position, 8 * t + 2 * quad + e);
 
-  const long long table_row = p.prefix ? 0 : sequence;
+  const int table_row = p.prefix ? 0 : sequence;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.ring[warp][0][0])) + lane * 16;
   const uint32_t ring8 = ring - lane * 8;
   // pages of this warp's next 32 blocks, one to a lane
   int ahead = 0;
-  auto look_ahead = [&](int i) {
-    const int key = from + (warp + (i + lane) * WARPS) * 16;
-    ahead = key < to ? cache_page(c, static_cast<int>(table_row), key) : -1;
-  };
   uint32_t held = 0;  // of the blocks under way, the last one lowest: whether their page is there
+  // this lane's bytes of a block's keys 2 group and 2 group + 1, and of the values 4 quad to 4 quad + 3
+  const int k_byte = quad * 16, v_byte = group * VB;
+  const long long k_from = static_cast<long long>(2 * group) * c.row + k_byte, v_from = static_cast<long long>(4 * quad) * c.row + v_byte;
   auto request = [&](int stage, int i) {
-    if ((i & 31) == 0) look_ahead(i);
     const int key = from + (warp + i * WARPS) * 16;
+    if ((i & 31) == 0) {
+      const int mine = key + lane * WARPS * 16;
+      ahead = mine < to ? cache_page(c, table_row, mine) : -1;
+    }
     const int page = __shfl_sync(~0u, ahead, i & 31);
-    held = held << 1 | (page >= 0 ? 1u : 0u);
+    const bool take = page >= 0;
+    held = held << 1 | (take ? 1u : 0u);
     if (key < to) {
-      const bool take = page >= 0;
-      const int in_page = key & ((1 << c.page_shift) - 1);
-      const long long line = ((take ? static_cast<long long>(page) * c.kv_heads + kv_head : 0) << c.page_shift) + (take ? in_page : 0);
-      const int8_t* k = c.k + line * c.row;
-      const int8_t* v = c.v + line * c.row;
-      const uint32_t at = ring + stage * Shared::kStage;
+      const long long line = take ? ((static_cast<long long>(page) * c.kv_heads + kv_head) << c.page_shift) + (key & ((1 << c.page_shift) - 1)) : 0;
+      const int8_t* k = c.k + (take ? line * c.row + k_from : 0);
+      const int8_t* v = c.v + (take ? line * c.row + v_from : 0);
+      const uint32_t at = ring + stage * Shared::kStage, at8 = ring8 + stage * Shared::kStage + Shared::kKeyBytes;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int cc = 0; cc < D / 64; ++cc) {
-          const int byte = cc * 64 + quad * 16;
-          const bool use = take && byte < c.row;
-          queue_16(at + (n * (D / 64) + cc) * 512, k + (use ? (group + 8 * n) * c.row + byte : 0), use);
+          const bool use = take && cc * 64 + k_byte < c.row;
+          queue_16(at + (n * (D / 64) + cc) * 512, use ? k + n * c.row + cc * 64 : c.k, use);
         }
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int key_of = 2 * quad + (n & 1) + 8 * (n >> 1);
         if constexpr (VB == 8) {
-          const bool use = take && group * 8 < c.row;
-          queue_8(ring8 + stage * Shared::kStage + Shared::kKeyBytes + n * 256, v + (use ? key_of * c.row + group * 8 : 0), use);
+          const bool use = take && v_byte < c.row;
+          queue_8(at8 + n * 256, use ? v + n * c.row : c.v, use);
         } else {
 #pragma unroll
           for (int h = 0; h < VB / 16; ++h) {
-            const int byte = group * VB + h * 16;
-            const bool use = take && byte < c.row;
-            queue_16(at + Shared::kKeyBytes + (n * (VB / 16) + h) * 512, v + (use ? key_of * c.row + byte : 0), use);
+            const bool use = take && v_byte + h * 16 < c.row;
+            queue_16(at + Shared::kKeyBytes + (n * (VB / 16) + h) * 512, use ? v + n * c.row + h * 16 : c.v, use);
           }
         }
       }
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t steps_at = ring8 + stage * Shared::kStage + Shared::kKeyBytes + Shared::kValues + n * 256;
-        queue_8(steps_at, c.k_steps + line + (take ? 2 * quad + 8 * n : 0), take);
-        queue_8(steps_at + 512, c.v_steps + line + (take ? 2 * quad + 8 * n : 0), take);
-      }
+      queue_8(at8 + Shared::kValues, c.k_steps + (take ? line + 2 * group : 0), take);
+      queue_8(at8 + Shared::kValues + 256, c.v_steps + (take ? line + 2 * group : 0), take);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -207,38 +218,43 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
 #pragma unroll
   for (int n = 0; n < STAGES - 1; ++n) request(n, n);
 
-  // the queries as A fragments in the order of the keys' bytes: a warp makes every WARPS-th product's
-  for (int s = warp; s < STEPS; s += WARPS) {
-    uint32_t f[QTERMS][4];
+  // the queries as B fragments in the order of the keys' bytes: a warp makes every WARPS-th product's
+  for (int s = warp; s < STEPS * NT; s += WARPS) {
+    const int step = s / NT, t = s % NT;
+    const int where = __shfl_sync(~0u, my_position, 8 * t + group);
+    const long long row = row0 + 8 * t + group;
+    const long long token = first + row / G;
+    const int head = kv_head * G + static_cast<int>(row % G);
+    const T* q = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
+    uint32_t f[QTERMS][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const long long row = row0 + group + 8 * r;
-      const long long token = first + row / G;
-      const int head = kv_head * G + static_cast<int>(row % G);
-      const T* q = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int at = (s / 4) * 64 + quad * 16 + (s % 4) * 4 + 2 * e;
-        const float x = position[r] > -2 && at < c.d ? op_get(q[at]) : 0.0f, y = position[r] > -2 && at + 1 < c.d ? op_get(q[at + 1]) : 0.0f;
-        if constexpr (QTERMS == 1) {
-          const OpVec<KT, 2> pair{{op_put<KT>(x), op_put<KT>(y)}};
-          f[0][r + 2 * e] = *reinterpret_cast<const uint32_t*>(&pair);
-        } else {
-          uint32_t rest;
-          split_pair<__nv_bfloat16>(x, y, f[0][r + 2 * e], rest);
-          const float x1 = x - __bfloat162float(op_put<__nv_bfloat16>(x)), y1 = y - __bfloat162float(op_put<__nv_bfloat16>(y));
-          split_pair<__nv_bfloat16>(x1, y1, f[1][r + 2 * e], f[2][r + 2 * e]);
-        }
+    for (int e = 0; e < 2; ++e) {
+      const int at = (step / 4) * 64 + quad * 16 + (step % 4) * 4 + 2 * e;
+      const float x = where > -2 && at < c.d ? op_get(q[at]) : 0.0f, y = where > -2 && at + 1 < c.d ? op_get(q[at + 1]) : 0.0f;
+      if constexpr (QTERMS == 1) {
+        const OpVec<KT, 2> pair{{op_put<KT>(x), op_put<KT>(y)}};
+        f[0][e] = *reinterpret_cast<const uint32_t*>(&pair);
+      } else {
+        uint32_t rest;
+        split_pair<__nv_bfloat16>(x, y, f[0][e], rest);
+        const float x1 = x - __bfloat162float(op_put<__nv_bfloat16>(x)), y1 = y - __bfloat162float(op_put<__nv_bfloat16>(y));
+        split_pair<__nv_bfloat16>(x1, y1, f[1][e], f[2][e]);
       }
     }
 #pragma unroll
-    for (int t = 0; t < QTERMS; ++t) sh.q[t][s][lane] = make_uint4(f[t][0], f[t][1], f[t][2], f[t][3]);
+    for (int w = 0; w < QTERMS; ++w) sh.q[w][step][t][lane] = make_uint2(f[w][0], f[w][1]);
   }
   __syncthreads();
+  const uint32_t q_at = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.q[0][0][0][0])) + lane * 8;
+  uint2 q_held[KEEP_Q ? STEPS : 1];
+  if constexpr (KEEP_Q)
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) q_held[s] = lds_8(q_at + s * 256);
 
-  float o[D / 8][4] = {};
-  float base[2] = {-INFINITY, -INFINITY}, total[2] = {0.0f, 0.0f};
-  const uint32_t q_at = static_cast<uint32_t>(__cvta_generic_to_shared(&sh.q[0][0][0])) + lane * 16;
+  float o[NT][STEPS][4] = {};
+  float base[NT][2], total[NT][2] = {};
+#pragma unroll
+  for (int t = 0; t < NT; ++t) base[t][0] = base[t][1] = -INFINITY;
   int stage = 0;
   for (int i = 0; i < blocks; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
@@ -246,85 +262,86 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
     request(stage == 0 ? STAGES - 1 : stage - 1, i + STAGES - 1);
     const uint32_t at = ring + stage * Shared::kStage, at8 = ring8 + stage * Shared::kStage + Shared::kKeyBytes;
     const int key = from + (warp + i * WARPS) * 16;
-    float s[2][4] = {};
+    float s[NT][4] = {};
 #pragma unroll
     for (int cc = 0; cc < D / 64; ++cc) {
       const uint4 k0 = lds_16(at + cc * 512), k1 = lds_16(at + (D / 64 + cc) * 512);
       const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t b[4];
-        int8_quad<KT>(w0[j], b[0], b[1]);
-        int8_quad<KT>(w1[j], b[2], b[3]);
+        uint32_t a[4];
+        int8_quad<KT>(w0[j], a[0], a[2]);
+        int8_quad<KT>(w1[j], a[1], a[3]);
 #pragma unroll
-        for (int t = QTERMS - 1; t >= 0; --t) {  // (small terms first)
-          const uint4 f = lds_16(q_at + (t * STEPS + cc * 4 + j) * 512);
-          const uint32_t a[4] = {f.x, f.y, f.z, f.w};
-          mma_16x8x16<KT>(s[0], a, b[0], b[1]);
-          mma_16x8x16<KT>(s[1], a, b[2], b[3]);
-        }
+        for (int w = QTERMS - 1; w >= 0; --w)  // (small terms first)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint2 b = KEEP_Q ? q_held[cc * 4 + j] : lds_8(q_at + ((w * STEPS + cc * 4 + j) * NT + t) * 256);
+            mma_16x8x16<KT>(s[t], a, b.x, b.y);
+          }
       }
     }
-    // s[n][e]: row group + 8 (e / 2), key 8 n + 2 quad + e % 2
-    float x[2][4], m[2], value_step[2][2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const uint2 ks = lds_8(at8 + Shared::kValues + n * 256), vs = lds_8(at8 + Shared::kValues + 512 + n * 256);
-      const float f0 = __uint_as_float(ks.x) * p.scale_log2, f1 = __uint_as_float(ks.y) * p.scale_log2;
-      value_step[n][0] = __uint_as_float(vs.x);
-      value_step[n][1] = __uint_as_float(vs.y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] = s[n][e] * (e & 1 ? f1 : f0);
-    }
+    // s[t][e]: key 2 group + e / 2, row 8 t + 2 quad + e % 2
+    const uint2 ks = lds_8(at8 + Shared::kValues), vs = lds_8(at8 + Shared::kValues + 256);
+    const float k_step[2] = {__uint_as_float(ks.x) * p.scale_log2, __uint_as_float(ks.y) * p.scale_log2};
+    const float v_step[2] = {__uint_as_float(vs.x), __uint_as_float(vs.y)};
     const bool whole = there && key + 15 <= least && key + 15 < to;
-    if (!whole) {
+    bool above = false;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at_key = key + 8 * n + 2 * quad + (e & 1);
-          if (!there || at_key > position[e >> 1] || at_key >= to) x[n][e] = -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        s[t][e] *= k_step[e >> 1];
+        if (!whole) {
+          const int at_key = key + 2 * group + (e >> 1);
+          if (!there || at_key > position[t][e & 1] || at_key >= to) s[t][e] = -INFINITY;
         }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      m[r] = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
-      m[r] = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 1));
-      m[r] = fmaxf(m[r], __shfl_xor_sync(~0u, m[r], 2));
-    }
-    // the base of the exponentials follows the maximum when that is 2^8 or more above it
-    if (__any_sync(~0u, m[0] > base[0] + 8.0f || m[1] > base[1] + 8.0f)) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float next = fmaxf(base[r], m[r]);
-        const float keep = next == -INFINITY ? 1.0f : exp2_approx(base[r] - next);
-        base[r] = next;
-        total[r] *= keep;
-#pragma unroll
-        for (int t = 0; t < D / 8; ++t) {
-          o[t][2 * r] *= keep;
-          o[t][2 * r + 1] *= keep;
-        }
+        above = above || s[t][e] > base[t][e & 1] + 8.0f;
       }
-    }
-    uint32_t prob[PTERMS][4];
+    // the base of the exponentials follows the maximum when that is 2^8 or more above it
+    if (__any_sync(~0u, above)) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float zero = base[r] == -INFINITY ? 0.0f : base[r];
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(s[t][e], s[t][2 + e]);
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+          const float next = fmaxf(base[t][e], m);
+          const float keep = next == -INFINITY ? 1.0f : exp2_approx(base[t][e] - next);
+          base[t][e] = next;
+          total[t][e] *= keep;
+#pragma unroll
+          for (int n = 0; n < STEPS; ++n) {
+            o[t][n][e] *= keep;
+            o[t][n][2 + e] *= keep;
+          }
+        }
+    }
+    uint32_t prob[PTERMS][NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float zero[2] = {base[t][0] == -INFINITY ? 0.0f : base[t][0], base[t][1] == -INFINITY ? 0.0f : base[t][1]};
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const float e0 = exp2_approx(x[n][2 * r] - zero), e1 = exp2_approx(x[n][2 * r + 1] - zero);
-        total[r] += e0 + e1;
+        const float e0 = exp2_approx(s[t][2 * n] - zero[0]), e1 = exp2_approx(s[t][2 * n + 1] - zero[1]);
+        total[t][0] += e0;
+        total[t][1] += e1;
         // (the step of a key that takes no part may be anything)
-        const float y0 = !whole && x[n][2 * r] == -INFINITY ? 0.0f : e0 * value_step[n][0];
-        const float y1 = !whole && x[n][2 * r + 1] == -INFINITY ? 0.0f : e1 * value_step[n][1];
-        split_pair<VT>(y0, y1, prob[0][2 * n + r], prob[1][2 * n + r]);
+        const float y0 = !whole && s[t][2 * n] == -INFINITY ? 0.0f : e0 * v_step[n];
+        const float y1 = !whole && s[t][2 * n + 1] == -INFINITY ? 0.0f : e1 * v_step[n];
+        uint32_t term[PTERMS];
+        split_pair<VT>(y0, y1, term[0], term[1]);
         if constexpr (PTERMS == 3) {
           const float r0 = y0 - __bfloat162float(op_put<VT>(y0)), r1 = y1 - __bfloat162float(op_put<VT>(y1));
-          split_pair<VT>(r0, r1, prob[1][2 * n + r], prob[2][2 * n + r]);
+          split_pair<VT>(r0, r1, term[1], term[2]);
         }
+#pragma unroll
+        for (int w = 0; w < PTERMS; ++w) prob[w][t][n] = turn_8x8(term[w]);
       }
     }
+    // prob[.][t][n]: row 8 t + group, keys 4 quad + n and 4 quad + n + 2
     constexpr int WORDS = VB / 4;
     uint32_t v[4][WORDS];
 #pragma unroll
@@ -345,37 +362,42 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
       }
     }
 #pragma unroll
-    for (int t = 0; t < D / 8; ++t) {
-      // byte t % 4 of two keys' words, in bytes 0 and 2
-      const uint32_t b0 = int8_pair<VT>(__byte_perm(v[0][t / 4], v[1][t / 4], 0x0400u + (t % 4) * 0x0101u));
-      const uint32_t b1 = int8_pair<VT>(__byte_perm(v[2][t / 4], v[3][t / 4], 0x0400u + (t % 4) * 0x0101u));
+    for (int n = 0; n < STEPS; ++n) {
+      // bytes 2 n and 2 n + 1 of two keys' words, in bytes 0 and 2
+      const uint32_t even = 0x0400u + (2 * n % 4) * 0x0101u, odd = 0x0400u + ((2 * n + 1) % 4) * 0x0101u;
+      const uint32_t a[4] = {int8_pair<VT>(__byte_perm(v[0][n / 2], v[2][n / 2], even)), int8_pair<VT>(__byte_perm(v[0][n / 2], v[2][n / 2], odd)),
+                             int8_pair<VT>(__byte_perm(v[1][n / 2], v[3][n / 2], even)), int8_pair<VT>(__byte_perm(v[1][n / 2], v[3][n / 2], odd))};
 #pragma unroll
-      for (int w = PTERMS - 1; w >= 0; --w) mma_16x8x16<VT>(o[t], prob[w], b0, b1);
+      for (int w = PTERMS - 1; w >= 0; --w)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_16x8x16<VT>(o[t][n], a, prob[w][t][0], prob[w][t][1]);
     }
     stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // the results take the ring's place
+  // o[t][n][e]: component group (D / 8) + 2 n + e / 2, row 8 t + 2 quad + e % 2
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    total[r] += __shfl_xor_sync(~0u, total[r], 1);
-    total[r] += __shfl_xor_sync(~0u, total[r], 2);
-    if (quad == 0) {
-      sh.top[warp][group + 8 * r] = base[r];
-      sh.total[warp][group + 8 * r] = total[r];
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * t + 2 * quad + e;
+      float sum = total[t][e];
+      sum += __shfl_xor_sync(~0u, sum, 4);
+      sum += __shfl_xor_sync(~0u, sum, 8);
+      sum += __shfl_xor_sync(~0u, sum, 16);
+      if (group == 0) {
+        sh.top[warp][r] = base[t][e];
+        sh.total[warp][r] = sum;
+      }
+      if (position[t][e] > -2)
+#pragma unroll
+        for (int n = 0; n < STEPS; n += 2)
+          *reinterpret_cast<float4*>(&sh.part[warp][r][group * (D / 8) + 2 * n]) = make_float4(o[t][n][e], o[t][n][2 + e], o[t][n + 1][e], o[t][n + 1][2 + e]);
     }
-    // o[t][e]: row group + 8 (e / 2), component (2 quad + e % 2) (D / 8) + t
-    if (position[r] > -2)
-#pragma unroll
-      for (int t = 0; t < D / 8; t += 4)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<float4*>(&sh.part[warp][group + 8 * r][(2 * quad + e) * (D / 8) + t]) =
-              make_float4(o[t][2 * r + e], o[t + 1][2 * r + e], o[t + 2][2 * r + e], o[t + 3][2 * r + e]);
-  }
   __syncthreads();
   const long long all_rows = c.tokens * p.heads;
-  for (int i = threadIdx.x; i < kCacheRows * (D / 4); i += WARPS * 32) {
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += WARPS * 32) {
     const int r = i / (D / 4), at = i % (D / 4) * 4;
     const int where = __shfl_sync(~0u, my_position, r);
     if (where < -1 || at >= c.d) continue;
@@ -414,11 +436,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
       }
     }
   }
+  ptx::grid_dependency_wait();
 }
 
 // The ranges' results of a row, joined: a warp to a row, ranges in the order of the keys.
 template <class T>
 __global__ void __launch_bounds__(256) k_attend_cache_join(const __grid_constant__ AttendCacheParams p) {
+  ptx::grid_dependency_wait();  // (launched early)
   const CacheParams& c = p.c;
   const int lane = threadIdx.x & 31;
   const long long rows = c.tokens * p.heads, row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);

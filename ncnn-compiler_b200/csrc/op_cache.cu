@@ -259,23 +259,29 @@ struct AttendCachePlan {
   int ranges() const { return prefix_ranges + own_ranges; }
 };
 
+constexpr long long kRangeCtas = 8;  // CTAs to an SM that ranges are made for
+
 int up(long long x, int to) { return static_cast<int>((x + to - 1) / to * to); }
+
+// Rows of a tile: eights, sixteens or, of heads up to 128, thirty-twos.
+int few_rows(long long rows, int d) { return rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : 32; }
 
 AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long shared, int sms) {
   AttendCachePlan plan{};
   const int G = heads / c.kv_heads;
-  // as many ranges as give each SM four CTAs, of 256 keys at least and no more than 64 of them
+  // ranges of 256 keys at least and no more than 64 of them
   auto split = [&](long long keys, long long tiles, int* chunk) {
     if (keys <= 0) {
       *chunk = 16;
       return 0;
     }
-    const long long most = std::max<long long>(1, std::min<long long>({64, (keys + 255) / 256, 4ll * sms / std::max<long long>(tiles, 1)}));
+    const long long most = std::max<long long>(1, std::min<long long>({64, (keys + 255) / 256, kRangeCtas * sms / std::max<long long>(tiles, 1)}));
     *chunk = up((keys + most - 1) / most, 64);
     return static_cast<int>((keys + *chunk - 1) / *chunk);
   };
-  const long long own_tiles = static_cast<long long>(c.sequences) * c.kv_heads * ((static_cast<long long>(c.max_tokens) * G + kCacheRows - 1) / kCacheRows);
-  const long long prefix_tiles = c.kv_heads * ((c.tokens * G + kCacheRows - 1) / kCacheRows);
+  const long long own_rows = static_cast<long long>(c.max_tokens) * G, all_rows = c.tokens * G;
+  const long long own_tiles = static_cast<long long>(c.sequences) * c.kv_heads * ((own_rows + few_rows(own_rows, c.d) - 1) / few_rows(own_rows, c.d));
+  const long long prefix_tiles = c.kv_heads * ((all_rows + few_rows(all_rows, c.d) - 1) / few_rows(all_rows, c.d));
   const long long in_prefix = std::min<long long>(shared, c.max_len);
   plan.prefix_ranges = split(in_prefix, prefix_tiles, &plan.prefix_chunk);
   plan.own_ranges = split(c.max_len - in_prefix, own_tiles, &plan.own_chunk);
@@ -287,24 +293,31 @@ long long attend_cache_workspace(const CacheParams& c, int heads, const AttendCa
   return plan.ranges() * c.tokens * heads * (c.row * 4ll + 8);
 }
 
-template <class T, int D, int WARPS, int STAGES, int BLOCKS>
-cudaError_t launch_cache_few(const AttendCacheParams& p, int ranges, int device, cudaStream_t st) {
-  constexpr int smem = sizeof(CacheFewShared<T, D, WARPS, STAGES>);
+template <class T, int D, int NT, int WARPS, int STAGES, int BLOCKS>
+cudaError_t launch_cache_few(const AttendCacheParams& p, int ranges, bool early, int device, cudaStream_t st) {
+  constexpr int smem = sizeof(CacheFewShared<T, D, NT, WARPS, STAGES>), ROWS = 8 * NT;
+  static_assert(BLOCKS * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
   static std::atomic<uint64_t> granted{0};
-  const auto kernel = k_attend_cache_few<T, D, WARPS, STAGES, BLOCKS>;
+  const auto kernel = k_attend_cache_few<T, D, NT, WARPS, STAGES, BLOCKS>;
   if (const cudaError_t e = op_grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return e;
   const long long G = p.rows_a_head;
-  const long long tiles = p.prefix ? (p.c.tokens * G + kCacheRows - 1) / kCacheRows
-                                   : static_cast<long long>(p.c.sequences) * ((p.c.max_tokens * G + kCacheRows - 1) / kCacheRows);
+  const long long tiles = p.prefix ? (p.c.tokens * G + ROWS - 1) / ROWS : static_cast<long long>(p.c.sequences) * ((p.c.max_tokens * G + ROWS - 1) / ROWS);
   if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
-  return op_launch(kernel, dim3(static_cast<unsigned>(tiles), p.c.kv_heads, ranges), WARPS * 32, smem, st, 0, p);
+  return op_launch_early(early, kernel, dim3(static_cast<unsigned>(tiles), p.c.kv_heads, ranges), WARPS * 32, smem, st, 0, p);
 }
 
 template <class T>
-cudaError_t attend_cache_few(const AttendCacheParams& p, int ranges, int device, cudaStream_t st) {
-  if (p.c.d <= 64) return launch_cache_few<T, 64, 4, 4, 3>(p, ranges, device, st);
-  if (p.c.d <= 128) return launch_cache_few<T, 128, 4, 4, 2>(p, ranges, device, st);
-  return launch_cache_few<T, 256, 4, 3, 1>(p, ranges, device, st);
+cudaError_t attend_cache_few(const AttendCacheParams& p, int ranges, bool early, int device, cudaStream_t st) {
+  const int rows = few_rows((p.prefix ? p.c.tokens : p.c.max_tokens) * static_cast<long long>(p.rows_a_head), p.c.d);
+  if (p.c.d <= 64) {
+    if (rows == 8) return launch_cache_few<T, 64, 1, 4, 5, 4>(p, ranges, early, device, st);
+    return rows == 16 ? launch_cache_few<T, 64, 2, 4, 4, 4>(p, ranges, early, device, st) : launch_cache_few<T, 64, 4, 4, 4, 3>(p, ranges, early, device, st);
+  }
+  if (p.c.d <= 128) {
+    if (rows == 8) return launch_cache_few<T, 128, 1, 4, 3, 3>(p, ranges, early, device, st);
+    return rows == 16 ? launch_cache_few<T, 128, 2, 4, 4, 2>(p, ranges, early, device, st) : launch_cache_few<T, 128, 4, 4, 3, 2>(p, ranges, early, device, st);
+  }
+  return rows == 8 ? launch_cache_few<T, 256, 1, 4, 3, sizeof(T) == 4 ? 1 : 2>(p, ranges, early, device, st) : launch_cache_few<T, 256, 2, 4, 3, 1>(p, ranges, early, device, st);
 }
 
 int attend_cache_args(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, int32_t heads, int64_t shared, CacheParams* c) {
@@ -408,17 +421,18 @@ extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const 
         AttendCacheParams first = p;
         first.prefix = 1;
         first.chunk = plan.prefix_chunk;
-        e = attend_cache_few<T>(first, plan.prefix_ranges, device, st);
+        e = attend_cache_few<T>(first, plan.prefix_ranges, false, device, st);
       }
       // (without any keys there is still a result: zeros)
       if (e == cudaSuccess && (plan.own_ranges > 0 || plan.prefix_ranges == 0)) {
         AttendCacheParams own = p;
         own.chunk = plan.own_chunk;
         own.first_range = plan.prefix_ranges;
-        e = attend_cache_few<T>(own, std::max(plan.own_ranges, 1), device, st);
+        // (beside the prefix's: it waits for that one's end before its own)
+        e = attend_cache_few<T>(own, std::max(plan.own_ranges, 1), plan.prefix_ranges > 0, device, st);
       }
       if (e == cudaSuccess && p.part != nullptr)
-        e = op_launch(k_attend_cache_join<T>, dim3(static_cast<unsigned>((p.c.tokens * heads + 7) / 8)), 256, 0, st, 0, p);
+        e = op_launch_early(true, k_attend_cache_join<T>, dim3(static_cast<unsigned>((p.c.tokens * heads + 7) / 8)), 256, 0, st, 0, p);
       return op_launched(kOp, e);
     });
   });
