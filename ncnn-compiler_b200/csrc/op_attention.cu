@@ -59,24 +59,6 @@ bool rows_of(const AttendParams& p, int count, int size) {
          ok(p.o, {{p.o_batch, p.batch}, {p.o_row, p.lq}, {p.o_head, p.heads}});
 }
 
-// Dynamic shared memory above 48 KB is granted to a kernel once per device.  `registers`: what the kernel's roles share out
-// between them; compiled for fewer, their setmaxnreg would wait for ever.
-template <class K>
-cudaError_t grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted, int registers = 0) {
-  const uint64_t bit = 1ull << (device & 63);
-  const int as_if = registers > 0 ? g_hooks.registers.load(std::memory_order_relaxed) : 0;
-  if (as_if != 0 && as_if != registers) return cudaErrorInvalidKernelImage;
-  if (device < 64 && (granted->load(std::memory_order_acquire) & bit)) return cudaSuccess;
-  if (registers > 0) {
-    cudaFuncAttributes a{};
-    if (const cudaError_t e = cudaFuncGetAttributes(&a, kernel); e != cudaSuccess) return e;
-    if (a.numRegs != registers) return cudaErrorInvalidKernelImage;
-  }
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess && device < 64) granted->fetch_or(bit, std::memory_order_acq_rel);
-  return e;
-}
-
 struct TcMaps {
   alignas(64) CUtensorMap q, k, v, o;
 };
@@ -106,7 +88,7 @@ int launch_short(const AttendParams& a, int device, int sms, cudaStream_t st) {
   TcMaps m;
   if (!fill_tc(a, std::is_same<T, __half>::value, &p.t, &m)) return no_maps();
   static std::atomic<uint64_t> granted{0};
-  if (const cudaError_t e = grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
+  if (const cudaError_t e = op_grant_smem(tc_attend_short_kernel<T, D>, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return refused_kernel(e);
   p.row_tiles = (a.lq + kAttRows - 1) / kAttRows;
   p.tiles = p.row_tiles * a.heads * a.batch;
   op_will_wait_on(device);
@@ -122,7 +104,7 @@ int launch_tc(const AttendParams& a, int device, cudaStream_t st) {
   if (!fill_tc(a, std::is_same<T, __half>::value, &p, &m)) return no_maps();
   static std::atomic<uint64_t> granted{0};
   const int registers = Shape::kShareRegs ? Shape::kRegsLaunch : 0;
-  if (const cudaError_t e = grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
+  if (const cudaError_t e = op_grant_smem(tc_attend_kernel<T, D, TILES>, Shape::kSmem, device, &granted, registers); e != cudaSuccess) return refused_kernel(e);
   const dim3 grid((a.lq + kAttRows * TILES - 1) / (kAttRows * TILES), a.heads, a.batch);
   op_will_wait_on(device);
   return op_launched("op_cross_attention", op_launch(tc_attend_kernel<T, D, TILES>, grid, Shape::kThreads, Shape::kSmem, st, 0, p, m.q, m.k, m.v, m.o));
@@ -155,7 +137,7 @@ int launch_few(const AttendParams& a, int device, int ranks, cudaStream_t st) {
   constexpr int smem = sizeof(FewShared<T, D, WARPS, STAGES>);
   static std::atomic<uint64_t> granted{0};
   const auto kernel = k_attend_few<T, D, WARPS, STAGES, BLOCKS>;
-  if (const cudaError_t e = grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return refused_kernel(e);
+  if (const cudaError_t e = op_grant_smem(kernel, smem, device, &granted); e != cudaSuccess) return refused_kernel(e);
   if (ranks > 8)
     if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return refused_kernel(e);
   return op_launched("op_cross_attention", op_launch(kernel, dim3(ranks, a.kv_heads * p.row_tiles, a.batch), WARPS * 32, smem, st, ranks, p));
@@ -213,7 +195,7 @@ cudaError_t launch_tile(F32Params p, int device, int sms, cudaStream_t st) {
   using Shape = TileShape<D, TM, KEYS, THREADS>;
   static std::atomic<uint64_t> granted{0};
   auto kernel = k_attend_tile<T, D, TM, KEYS, THREADS, WIDE>;
-  if (const cudaError_t e = grant_smem(kernel, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
+  if (const cudaError_t e = op_grant_smem(kernel, Shape::kSmem, device, &granted); e != cudaSuccess) return e;
   const long long rows = static_cast<long long>(p.a.lq) * (p.a.heads / p.a.kv_heads);
   const long long row_tiles = (rows + Shape::kRows - 1) / Shape::kRows, tiles = row_tiles * p.a.kv_heads * p.a.batch;
   // CTAs to a tile: what the device holds at once, while each has a block of keys; no more than the blocks are dealt evenly to
@@ -269,6 +251,8 @@ unsigned long long op_wait_ns(unsigned long long usual) {
   const unsigned long long ns = g_hooks.wait_ns.load(std::memory_order_relaxed);
   return ns != 0 ? ns : usual;
 }
+
+int op_registers() { return g_hooks.registers.load(std::memory_order_relaxed); }
 
 void op_will_wait_on(int device) {
   const uint64_t bit = 1ull << (device & 63);

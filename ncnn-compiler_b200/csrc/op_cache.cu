@@ -6,6 +6,7 @@
 #include "attend_cache.cuh"
 #include "op_cache.h"
 #include "row_int8.cuh"
+#include "tc_attend_cache.cuh"
 
 namespace nb {
 namespace {
@@ -253,44 +254,71 @@ int cache_rows_call(const char* op, bool read, const ncnn_b200_cache* cache, con
 }
 
 // ------------------------------------------------------------------ attention
-// How a call is split into ranges of keys.
-struct AttendCachePlan {
-  int prefix_ranges, prefix_chunk, own_ranges, own_chunk;
-  int ranges() const { return prefix_ranges + own_ranges; }
+// How the keys of a call, of its shared prefix and of the sequences' own, are walked: by which kernel, and in ranges of how many.
+struct AttendCachePart {
+  int wide, ranges, chunk;
 };
-
-constexpr long long kRangeCtas = 8;  // CTAs to an SM that ranges are made for
+struct AttendCachePlan {
+  AttendCachePart prefix, own;
+  int ranges() const { return prefix.ranges + own.ranges; }
+};
 
 int up(long long x, int to) { return static_cast<int>((x + to - 1) / to * to); }
 
 // Rows of a tile: eights, sixteens or, of heads up to 128, thirty-twos.
 int few_rows(long long rows, int d) { return rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : 32; }
 
-AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long shared, int sms) {
-  AttendCachePlan plan{};
+constexpr int kWideRows = 64;  // rows of a key head from which tiles of 128 rows are taken
+constexpr long long kRangeCtas = 8;  // CTAs to an SM that ranges are made for
+
+AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long shared, int sms, bool halves) {
   const int G = heads / c.kv_heads;
-  // ranges of 256 keys at least and no more than 64 of them
-  auto split = [&](long long keys, long long tiles, int* chunk) {
-    if (keys <= 0) {
-      *chunk = 16;
-      return 0;
-    }
-    const long long most = std::max<long long>(1, std::min<long long>({64, (keys + 255) / 256, kRangeCtas * sms / std::max<long long>(tiles, 1)}));
-    *chunk = up((keys + most - 1) / most, 64);
-    return static_cast<int>((keys + *chunk - 1) / *chunk);
+  auto part = [&](long long keys, long long sequences, long long rows) {
+    AttendCachePart p{0, 0, 128};
+    if (keys <= 0) return p;
+    p.wide = halves && c.d <= 128 && rows > kWideRows ? 1 : 0;
+    const int height = p.wide ? 256 : few_rows(rows, c.d);
+    const long long tiles = std::max<long long>(1, sequences * c.kv_heads * ((rows + height - 1) / height));
+    // Ranges of 256 keys at least, in tiles of 128 rows 512, and no more than 64 of them.
+    const long long most = std::max<long long>(1, p.wide ? std::min<long long>({64, (keys + 511) / 512, sms / tiles})
+                                                         : std::min<long long>({64, (keys + 255) / 256, kRangeCtas * sms / tiles}));
+    p.chunk = up((keys + most - 1) / most, p.wide ? 128 : 64);
+    p.ranges = static_cast<int>((keys + p.chunk - 1) / p.chunk);
+    return p;
   };
-  const long long own_rows = static_cast<long long>(c.max_tokens) * G, all_rows = c.tokens * G;
-  const long long own_tiles = static_cast<long long>(c.sequences) * c.kv_heads * ((own_rows + few_rows(own_rows, c.d) - 1) / few_rows(own_rows, c.d));
-  const long long prefix_tiles = c.kv_heads * ((all_rows + few_rows(all_rows, c.d) - 1) / few_rows(all_rows, c.d));
+  AttendCachePlan plan{};
   const long long in_prefix = std::min<long long>(shared, c.max_len);
-  plan.prefix_ranges = split(in_prefix, prefix_tiles, &plan.prefix_chunk);
-  plan.own_ranges = split(c.max_len - in_prefix, own_tiles, &plan.own_chunk);
+  plan.prefix = part(in_prefix, 1, c.tokens * G);
+  plan.own = part(c.max_len - in_prefix, c.sequences, static_cast<long long>(c.max_tokens) * G);
   return plan;
 }
 
-long long attend_cache_workspace(const CacheParams& c, int heads, const AttendCachePlan& plan) {
+long long attend_cache_bytes(const CacheParams& c, int heads, const AttendCachePlan& plan) {
   if (plan.ranges() <= 1) return 0;
   return plan.ranges() * c.tokens * heads * (c.row * 4ll + 8);
+}
+// (for any type)
+long long attend_cache_workspace(const CacheParams& c, int heads, long long shared, int sms) {
+  return std::max(attend_cache_bytes(c, heads, attend_cache_plan(c, heads, shared, sms, true)),
+                  attend_cache_bytes(c, heads, attend_cache_plan(c, heads, shared, sms, false)));
+}
+
+template <class T, int D>
+cudaError_t launch_cache_wide(const AttendCacheParams& a, int ranges, bool early, bool q_wide, int device, cudaStream_t st) {
+  using Shape = TcCacheShape<D>;
+  TcCacheParams p{};
+  p.a = a;
+  p.q_wide = q_wide ? 1 : 0;
+  p.stall = op_stalled() ? 1 : 0;
+  p.wait_ns = op_wait_ns(kTcWaitLimitNs);
+  static std::atomic<uint64_t> granted{0};
+  const auto kernel = tc_attend_cache_kernel<T, D>;
+  if (const cudaError_t e = op_grant_smem(kernel, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return e;
+  const long long G = a.rows_a_head;
+  const long long tiles = a.prefix ? (a.c.tokens * G + 255) / 256 : static_cast<long long>(a.c.sequences) * ((a.c.max_tokens * G + 255) / 256);
+  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  op_will_wait_on(device);
+  return op_launch_early(early, kernel, dim3(static_cast<unsigned>(tiles), a.c.kv_heads, ranges), Shape::kThreads, Shape::kSmem, st, 0, p);
 }
 
 template <class T, int D, int NT, int WARPS, int STAGES, int BLOCKS>
@@ -320,6 +348,15 @@ cudaError_t attend_cache_few(const AttendCacheParams& p, int ranges, bool early,
   return rows == 8 ? launch_cache_few<T, 256, 1, 4, 3, sizeof(T) == 4 ? 1 : 2>(p, ranges, early, device, st) : launch_cache_few<T, 256, 2, 4, 3, 1>(p, ranges, early, device, st);
 }
 
+template <class T>
+cudaError_t attend_cache_part(AttendCacheParams p, const AttendCachePart& part, bool early, bool q_wide, int device, cudaStream_t st) {
+  p.chunk = part.chunk;
+  const int ranges = std::max(part.ranges, 1);
+  if constexpr (sizeof(T) == 2)
+    if (part.wide) return p.c.d <= 64 ? launch_cache_wide<T, 64>(p, ranges, early, q_wide, device, st) : launch_cache_wide<T, 128>(p, ranges, early, q_wide, device, st);
+  return attend_cache_few<T>(p, ranges, early, device, st);
+}
+
 int attend_cache_args(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, int32_t heads, int64_t shared, CacheParams* c) {
   if (const int e = cache_params(op, cache, batch, c); e != 0) return e;
   auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": " + what); };
@@ -333,8 +370,7 @@ int attend_cache_args(const char* op, const ncnn_b200_cache* cache, const ncnn_b
 }  // namespace
 
 cudaError_t cache_gave_up(unsigned* count) {
-  *count = 0;
-  return cudaSuccess;
+  return cudaMemcpyFromSymbol(count, g_cache_gave_up, sizeof *count);
 }
 
 }  // namespace nb
@@ -363,7 +399,7 @@ extern "C" int64_t ncnn_b200_op_cache_attention_workspace(const ncnn_b200_cache*
     std::string why;
     const int device = op_common_device(kOp, {c.k}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
-    bytes = attend_cache_workspace(c, heads, attend_cache_plan(c, heads, shared, op_sm_count(device)));
+    bytes = attend_cache_workspace(c, heads, shared, op_sm_count(device));
     return 0;
   });
   return bytes;
@@ -393,8 +429,9 @@ extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const 
     const int device = op_common_device(kOp, {q, o, p.c.k, p.c.v, p.c.k_steps, p.c.v_steps, p.c.table, p.c.lens, p.c.starts, workspace}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
     DeviceGuard guard(device);
-    const AttendCachePlan plan = attend_cache_plan(p.c, heads, shared, op_sm_count(device));
-    const long long bytes = attend_cache_workspace(p.c, heads, plan);
+    const int sms = op_sm_count(device);
+    const AttendCachePlan plan = attend_cache_plan(p.c, heads, shared, sms, type != NCNN_B200_F32);
+    const long long bytes = attend_cache_workspace(p.c, heads, shared, sms);
     if (bytes > 0 && workspace == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, "op_cache_attention: this call needs a workspace");
     if (bytes > workspace_bytes && bytes > 0) return op_fail(NCNN_B200_STATUS_OUTPUT_CAPACITY, "op_cache_attention: the workspace is too small");
     p.q = q;
@@ -403,12 +440,12 @@ extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const 
     p.rows_a_head = heads / p.c.kv_heads;
     p.scale_log2 = (scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(p.c.d)) : scale) * 1.44269504088896340736f;
     p.shared = static_cast<int>(shared);
-    p.prefix_ranges = plan.prefix_ranges;
-    p.prefix_chunk = plan.prefix_chunk;
-    p.own_ranges = plan.own_ranges;
-    p.own_chunk = plan.own_chunk;
+    p.prefix_ranges = plan.prefix.ranges;
+    p.prefix_chunk = plan.prefix.chunk;
+    p.own_ranges = plan.own.ranges;
+    p.own_chunk = plan.own.chunk;
     p.part_width = p.c.row;
-    if (bytes > 0) {
+    if (plan.ranges() > 1) {
       p.part = static_cast<float*>(workspace);
       p.part_top = reinterpret_cast<float2*>(p.part + static_cast<long long>(plan.ranges()) * p.c.tokens * heads * p.part_width);
     }
@@ -417,19 +454,18 @@ extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const 
     return op_by_type(type, [&](auto t) {
       using T = decltype(t);
       cudaError_t e = cudaSuccess;
-      if (plan.prefix_ranges > 0) {
+      const bool q_wide = moves(q, 16 / size, size, p.c.d, p.c.tokens, p.q_token, heads, p.q_head);
+      if (plan.prefix.ranges > 0) {
         AttendCacheParams first = p;
         first.prefix = 1;
-        first.chunk = plan.prefix_chunk;
-        e = attend_cache_few<T>(first, plan.prefix_ranges, false, device, st);
+        e = attend_cache_part<T>(first, plan.prefix, false, q_wide, device, st);
       }
-      // (without any keys there is still a result: zeros)
-      if (e == cudaSuccess && (plan.own_ranges > 0 || plan.prefix_ranges == 0)) {
+      // The sequences' own keys.  (Without any keys there is still a result: zeros.)  Beside the prefix's: the kernel waits for that one's
+      // end before its own.
+      if (e == cudaSuccess && (plan.own.ranges > 0 || plan.prefix.ranges == 0)) {
         AttendCacheParams own = p;
-        own.chunk = plan.own_chunk;
-        own.first_range = plan.prefix_ranges;
-        // (beside the prefix's: it waits for that one's end before its own)
-        e = attend_cache_few<T>(own, std::max(plan.own_ranges, 1), plan.prefix_ranges > 0, device, st);
+        own.first_range = plan.prefix.ranges;
+        e = attend_cache_part<T>(own, plan.own, plan.prefix.ranges > 0, q_wide, device, st);
       }
       if (e == cudaSuccess && p.part != nullptr)
         e = op_launch_early(true, k_attend_cache_join<T>, dim3(static_cast<unsigned>((p.c.tokens * heads + 7) / 8)), 256, 0, st, 0, p);

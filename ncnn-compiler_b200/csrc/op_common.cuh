@@ -24,6 +24,7 @@ void set_global_error(const std::string& message);  // c_api.cu
 // What tests asked of the kernels whose waits are bounded (ncnn_b200_op_test_hooks), and who reports such a wait (op_attention.cu).
 bool op_stalled();
 unsigned long long op_wait_ns(unsigned long long usual);
+int op_registers();
 void op_will_wait_on(int device);
 cudaError_t tokens_gave_up(unsigned* count);  // op_tokens.cu, on the current device
 cudaError_t cache_gave_up(unsigned* count);   // op_cache.cu
@@ -114,11 +115,18 @@ inline EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// Dynamic shared memory above 48 KB is granted to a kernel once per device.
+// Dynamic shared memory above 48 KB is granted to a kernel once per device.  `registers`: what the kernel's roles share out between them;
+// compiled for fewer, their setmaxnreg would wait for ever.
 template <class K>
-inline cudaError_t op_grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted) {
+inline cudaError_t op_grant_smem(K kernel, int bytes, int device, std::atomic<uint64_t>* granted, int registers = 0) {
   const uint64_t bit = 1ull << (device & 63);
+  if (registers > 0 && op_registers() != 0 && op_registers() != registers) return cudaErrorInvalidKernelImage;
   if (device < 64 && (granted->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  if (registers > 0) {
+    cudaFuncAttributes a{};
+    if (const cudaError_t e = cudaFuncGetAttributes(&a, kernel); e != cudaSuccess) return e;
+    if (a.numRegs != registers) return cudaErrorInvalidKernelImage;
+  }
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess && device < 64) granted->fetch_or(bit, std::memory_order_acq_rel);
   return e;

@@ -1,0 +1,508 @@
+// Attention over a paged cache of 8-bit integers for many rows, 16-bit types: tcgen05 MMAs over tiles that warps convert on their way.
+//
+// A CTA has two tiles of 128 rows that read one key head (a row is a token and one of the head's query heads; of one sequence, or, for
+// a shared prefix, of all) and walks a range of keys in blocks of 128 with a running maximum and sum, as tc_attend.cuh does:
+//   S = Q K^T, P = 2^(S ks c - m) vs over S in tensor memory, O += P V
+// Integers are exact in 16 bits, so that keys and values are converted as they are and the steps ks, vs of a key meet its column in the
+// softmax.  P is rounded to bf16, whose range holds any step; f16 results take a second bf16 term of P (16 bits) and a second product.
+//
+// Roles: warps 0 to 2 bring blocks (each lane with cp.async into a queue of its own, a block ahead and more), convert them (16 bytes to 32)
+// and store them as TMA would with a 128-byte swizzle, keys and values in turn in a ring of three tiles; warp 3 issues the MMAs; warps
+// 4 to 7 are tile 0's softmax, 8 to 11 tile 1's.  Converting takes some 2300 instructions a block, the softmaxes 4500, of the 8192 that
+// fit into the time of the block's MMAs (2048 clocks): 256 rows to a CTA make the conversion cheap.
+#pragma once
+
+#include "attend_cache.cuh"
+#include "tc_attend.cuh"
+
+namespace nb {
+
+__device__ unsigned g_cache_gave_up;  // CTAs in which a wait ran out, ever: ncnn_b200_op_check_status
+
+struct TcCacheParams {
+  AttendCacheParams a;
+  int q_wide;  // 16 bytes of q can be read at a time
+  int stall;   // tests of the time-out path: no block is ever brought
+  unsigned long long wait_ns;
+};
+
+template <int D>
+struct TcCacheShape {
+  static constexpr int kThreads = 384;
+  static constexpr int kPanel = 128 * 128;  // 128 rows of 64 components
+  static constexpr int kTile = kPanel * (D / 64);
+  static constexpr int kSlots = 3, kSteps = 8, kQueue = 3;
+  static constexpr int kUnits = 128 * D / 512;            // of 32 pieces of 16 bytes, in a block of keys or values
+  static constexpr int kUnitsAWarp = (kUnits + 2) / 3;
+  static constexpr int kQueueTile = kUnitsAWarp * 3 * 512;
+  static constexpr int kRegsLaunch = 168, kRegsControl = 72, kRegsSoftmax = 216;
+  static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "registers of the roles");
+  static constexpr uint32_t kTmemCols = 512;
+  static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + kQueue * kQueueTile + kSteps * 1024;
+};
+
+// one pair of columns: scores times the keys' steps
+__device__ __forceinline__ uint64_t f32x2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_kernel(const __grid_constant__ TcCacheParams p) {
+  using namespace ptx;
+  using Shape = TcCacheShape<D>;
+  constexpr int kTile = Shape::kTile, kPanel = Shape::kPanel, kSlots = Shape::kSlots, kSteps = Shape::kSteps;
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  extern __shared__ uint8_t cache_smem[];
+  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2], p_half[2], p_full[2], o_full[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag, pages_there[kSteps];
+  const AttendCacheParams& a = p.a;
+  const CacheParams& c = a.c;
+  const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int range = blockIdx.z, kv_head = blockIdx.y, G = a.rows_a_head;
+  grid_dependency_trigger();
+
+  // rows: 256 from row0 on (the last ones first: their walks are the longest)
+  int sequence = 0;
+  long long row0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * 256, first = 0, rows;
+  int before = 0;
+  if (a.prefix) {
+    rows = c.tokens * G;
+  } else {
+    const int at = static_cast<int>(gridDim.x - 1 - blockIdx.x);
+    sequence = at % c.sequences;
+    row0 = static_cast<long long>(at / c.sequences) * 256;
+    first = cache_start(c, sequence);
+    const long long count = max(cache_start(c, sequence + 1) - first, 0ll);
+    rows = min(count, static_cast<long long>(c.max_tokens)) * G;
+    before = static_cast<int>(max(cache_len(c, sequence) - count, -(1ll << 30)));
+  }
+  // the CTA's last position: of a sequence's rows it is the last one's; of all tokens' any may be the last
+  int last = -2;
+  if (row0 < rows) {
+    const long long end_row = min(rows, row0 + 256) - 1;
+    if (a.prefix) {
+      for (long long t = row0 / G + lane; t <= end_row / G; t += 32) {
+        const CachePlace place = cache_place(c, t);
+        if (place.sequence >= 0) last = max(last, place.position);
+      }
+      last = __reduce_max_sync(~0u, last);
+    } else {
+      last = max(before + static_cast<int>(end_row / G), -1);
+    }
+  }
+  const int from = a.prefix ? range * a.chunk : a.shared + range * a.chunk;
+  const int end = a.prefix ? min(a.shared, last + 1) : last + 1;
+  const int to = min(from + a.chunk, end);
+  if (last == -2 || (from >= to && a.part != nullptr)) {
+    grid_dependency_wait();
+    return;
+  }
+  const int blocks = from < to ? (to - from + 127) / 128 : 0;
+  const int tiles = row0 + 128 < rows ? 2 : 1;
+  const uint32_t smem = (smem_u32(cache_smem) + 1023u) & ~1023u;
+  const uint32_t q_at = smem, ring = smem + 2 * kTile, queue = ring + kSlots * kTile, steps_at = queue + Shape::kQueue * Shape::kQueueTile;
+  volatile int* abort_ptr = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    mbar_init(smem_u32(&q_full), 4u * tiles);
+    mbar_init(smem_u32(&drained), 1);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&full[i]), 3);
+      mbar_init(smem_u32(&empty[i]), 1);
+    }
+    for (int i = 0; i < kSteps; ++i) mbar_init(smem_u32(&steps_full[i]), 3);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&s_full[t]), 1);
+      mbar_init(smem_u32(&p_half[t]), 4);
+      mbar_init(smem_u32(&p_full[t]), 4);
+      mbar_init(smem_u32(&o_full[t]), 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 3) {
+    tmem_alloc(smem_u32(&tmem_slot), Shape::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
+  auto gave_up = [&] {
+    if (atomicCAS(&abort_flag, 0, 1) == 0) atomicAdd(&g_cache_gave_up, 1u);
+  };
+  auto s_of = [&](int t) { return tmem + 128u * t; };
+  auto o_of = [&](int t) { return tmem + 256u + static_cast<uint32_t>(D * t); };
+
+  if (warp < 4) {
+    reg_dealloc<Shape::kRegsControl>();
+    if (warp < 3) {
+      // ---- blocks of keys and values: brought, converted, stored
+      constexpr int PIECES = D / 16, UNIT_ROWS = 32 / PIECES, UNITS = Shape::kUnitsAWarp;
+      const int piece = lane % PIECES, row_in = lane / PIECES;
+      const bool used_piece = piece * 16 < c.row;
+      const uint32_t my_queue = queue + static_cast<uint32_t>(warp * UNITS) * 512u + lane * 16u;
+      const int table_row = a.prefix ? 0 : sequence;
+      // where this lane's pieces of unit 0 go: 16 bytes become 32, that is, pieces 2 piece and 2 piece + 1 of a row of components.
+      // The lanes of the second panel store them the other way round, so that eight neighbours reach all banks.
+      const uint32_t panel = static_cast<uint32_t>(piece / 4) * kPanel;
+      const int out = piece % 4 * 2, swap = D == 128 ? piece / 4 : 0;
+      // eight pages to a block of keys, looked up when its keys are asked for; its values take the same
+      int pages[2] = {-1, -1};  // lanes 0 to 7, of even and odd blocks
+      auto ask = [&](int u) {
+        if (u < 2 * blocks && p.stall == 0) {
+          const int j = u >> 1, key0 = from + j * 128;
+          const bool value = u & 1;
+          if (!value) {
+            const int key = key0 + (lane & 7) * 16;
+            const int found = key < to ? cache_page(c, table_row, key) : -1;
+            if (j & 1) pages[1] = found;
+            else pages[0] = found;
+          }
+          const int mine = j & 1 ? pages[1] : pages[0];
+          const int8_t* base = value ? c.v : c.k;
+          const uint32_t stage = my_queue + static_cast<uint32_t>(u % Shape::kQueue) * Shape::kQueueTile;
+#pragma unroll
+          for (int i = 0; i < UNITS; ++i) {
+            const int unit = warp + 3 * i, r = unit * UNIT_ROWS + row_in;
+            const int page = __shfl_sync(~0u, mine, (unit * UNIT_ROWS / 16) & 7);
+            const bool take = unit < Shape::kUnits && page >= 0 && used_piece;
+            const long long line = take ? ((static_cast<long long>(page) * c.kv_heads + kv_head) << c.page_shift) + ((key0 + r) & ((1 << c.page_shift) - 1)) : 0;
+            queue_16(stage + i * 512, take ? base + line * c.row + piece * 16 : base, take);
+          }
+          if (warp < 2 && (warp == 1) == value) {
+            // the steps: four keys to a lane, all of one page
+            const int page = __shfl_sync(~0u, mine, lane / 4);
+            const bool take = page >= 0;
+            const long long line = take ? ((static_cast<long long>(page) * c.kv_heads + kv_head) << c.page_shift) + ((key0 + lane * 4) & ((1 << c.page_shift) - 1)) : 0;
+            queue_16(steps_at + static_cast<uint32_t>(j % kSteps) * 1024u + (value ? 512u : 0u) + lane * 16u, (value ? c.v_steps : c.k_steps) + line, take);
+          }
+          if (warp == 2 && !value) {
+            const int there = __ballot_sync(~0u, lane < 8 && mine >= 0);
+            if (lane == 0) pages_there[j % kSteps] = there;
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      bool ok = p.stall == 0;
+      for (int u = 0; u < Shape::kQueue - 1; ++u) ask(u);
+      int slot = 0;
+      uint32_t ph = 1;
+      for (int u = 0; ok && u < 2 * blocks; ++u) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(Shape::kQueue - 2) : "memory");
+        ask(u + Shape::kQueue - 1);
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), ph, abort_ptr, p.wait_ns));
+        if (!ok) break;
+        const bool value = u & 1;
+        const uint32_t from_at = my_queue + static_cast<uint32_t>(u % Shape::kQueue) * Shape::kQueueTile;
+        const uint32_t to_at = ring + static_cast<uint32_t>(slot) * kTile + panel;
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+          const int unit = warp + 3 * i, r = unit * UNIT_ROWS + row_in;
+          if (unit >= Shape::kUnits) break;
+          const uint4 w = lds_16(from_at + i * 512);
+          uint32_t h[8];
+          if (HALF && !value) {
+            int8_quad<__half>(w.x, h[0], h[1]);
+            int8_quad<__half>(w.y, h[2], h[3]);
+            int8_quad<__half>(w.z, h[4], h[5]);
+            int8_quad<__half>(w.w, h[6], h[7]);
+          } else {
+            int8_quad<__nv_bfloat16>(w.x, h[0], h[1]);
+            int8_quad<__nv_bfloat16>(w.y, h[2], h[3]);
+            int8_quad<__nv_bfloat16>(w.z, h[4], h[5]);
+            int8_quad<__nv_bfloat16>(w.w, h[6], h[7]);
+          }
+          const uint32_t at = to_at + static_cast<uint32_t>(r) * 128u;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int which = n ^ swap;
+            const uint32_t x0 = which ? h[4] : h[0], x1 = which ? h[5] : h[1], x2 = which ? h[6] : h[2], x3 = which ? h[7] : h[3];
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((out + which) ^ (r & 7)) << 4)), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&full[slot]));
+          if (value) mbar_arrive(smem_u32(&steps_full[(u >> 1) % kSteps]));  // (keys' and values' steps, and which pages are there)
+        }
+        if (++slot == kSlots) {
+          slot = 0;
+          ph ^= 1u;
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (!ok && p.stall == 0 && lane == 0) gave_up();
+    } else if (blocks > 0) {
+      // ---- MMAs
+      if (elect_one()) {
+        constexpr uint32_t kBMnMajor = 1u << 16;
+        const uint32_t s_idesc = instr_desc(1, HALF ? 0u : 1u, 128, 128), pv_idesc = instr_desc(1, 1u, 128, D) | kBMnMajor;
+        bool ok = mbar_wait_bounded(smem_u32(&q_full), 0, abort_ptr, p.wait_ns);
+        auto wait_use = [&](int u) { return mbar_wait_bounded(smem_u32(&full[u % kSlots]), (u / kSlots) & 1, abort_ptr, p.wait_ns); };
+        auto scores = [&](int t, int j) {
+          const uint32_t k_at = ring + static_cast<uint32_t>((2 * j) % kSlots) * kTile, a_at = q_at + t * kTile;
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            const uint32_t off = (n / 4) * kPanel + (n % 4) * 32;
+            mma_f16(s_of(t), smem_desc_kmajor(a_at + off, 128), smem_desc_kmajor(k_at + off, 128), s_idesc, n > 0);
+          }
+        };
+        // four steps of 16 keys; f16's second terms lie 64 columns behind the first
+        auto products = [&](int t, int j, int at) {
+          const uint32_t v_at = ring + static_cast<uint32_t>((2 * j + 1) % kSlots) * kTile;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t v = smem_desc_mnmajor(v_at + (at + i) * 2048, kPanel, 1024);
+            mma_f16_ts(o_of(t), s_of(t) + 8u * (at + i), v, pv_idesc, j > 0 || at + i > 0);
+            if (HALF) mma_f16_ts(o_of(t), s_of(t) + 64u + 8u * (at + i), v, pv_idesc, 1u);
+          }
+        };
+        ok = ok && wait_use(0);
+        if (ok) {
+          tc_fence_after_sync();
+          for (int t = 0; t < tiles; ++t) {
+            scores(t, 0);
+            tc_commit(smem_u32(&s_full[t]));
+          }
+          tc_commit(smem_u32(&empty[0]));
+        }
+        for (int j = 0; ok && j < blocks; ++j) {
+          for (int t = 0; t < tiles; ++t) {
+            if (t == 0) ok = wait_use(2 * j + 1);
+            ok = ok && mbar_wait_bounded(smem_u32(&p_half[t]), j & 1, abort_ptr, p.wait_ns);
+            if (!ok) break;
+            tc_fence_after_sync();
+            products(t, j, 0);
+            ok = mbar_wait_bounded(smem_u32(&p_full[t]), j & 1, abort_ptr, p.wait_ns);
+            if (!ok) break;
+            tc_fence_after_sync();
+            products(t, j, 4);
+            if (t == tiles - 1) tc_commit(smem_u32(&empty[(2 * j + 1) % kSlots]));
+            if (j + 1 < blocks) {
+              if (t == 0) ok = wait_use(2 * j + 2);
+              if (!ok) break;
+              scores(t, j + 1);
+              tc_commit(smem_u32(&s_full[t]));
+              if (t == tiles - 1) tc_commit(smem_u32(&empty[(2 * j + 2) % kSlots]));
+            } else {
+              tc_commit(smem_u32(&o_full[t]));
+            }
+          }
+        }
+        if (!ok) {
+          gave_up();
+          tc_commit(smem_u32(&drained));  // nor may MMAs be under way
+          for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&drained), 0); ++tries) {
+          }
+        }
+      }
+    }
+  } else {
+    // ---- softmaxes
+    reg_alloc<Shape::kRegsSoftmax>();
+    const int t = (warp - 4) >> 2;
+    if (t < tiles) {
+      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes of tensor memory (lane in the upper half word)
+      const uint32_t s_at = s_of(t) + lanes, o_at = o_of(t) + lanes;
+      const int r = (warp & 3) * 32 + lane;  // row of the tile
+      const long long row = row0 + t * 128 + r, token = first + row / G;
+      const int head = kv_head * G + static_cast<int>(row % G);
+      int position = -2;
+      if (row < rows) {
+        if (a.prefix) {
+          const CachePlace place = cache_place(c, token);
+          position = place.sequence < 0 ? -2 : place.position;
+        } else {
+          position = max(before + static_cast<int>(row / G), -1);
+        }
+      }
+      const int least = __reduce_min_sync(~0u, position < -1 ? 0x7fffffff : position);
+      // the row's query into the tile, as TMA would with a 128-byte swizzle
+      const T* q = static_cast<const T*>(a.q) + token * a.q_token + head * a.q_head;
+#pragma unroll 4
+      for (int n = 0; n < D / 8; ++n) {
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (position > -2 && n * 8 < c.d) {
+          if (p.q_wide) {
+            w = __ldg(reinterpret_cast<const uint4*>(q + n * 8));
+          } else {
+            OpVec<T, 8> e{};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n * 8 + i < c.d) e.e[i] = q[n * 8 + i];
+            w = *reinterpret_cast<const uint4*>(&e);
+          }
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + t * kTile + (n / 8) * kPanel + r * 128 + (((n & 7) ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y),
+                     "r"(w.z), "r"(w.w)
+                     : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&q_full));
+
+      const float scale = a.scale_log2;
+      const uint64_t c2 = f32x2_make(__float_as_uint(scale), __float_as_uint(scale));
+      float base = -INFINITY;  // of the exponentials: the maximum so far, or one up to 2^8 smaller
+      float total = 0.0f;
+      bool ok = true;
+      for (int j = 0; j < blocks; ++j) {
+        const int key0 = from + j * 128;
+        const uint32_t steps = steps_at + static_cast<uint32_t>(j % kSteps) * 1024u;
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&s_full[t]), j & 1, abort_ptr, p.wait_ns) &&
+                                 mbar_wait_bounded(smem_u32(&steps_full[j % kSteps]), (j / kSteps) & 1, abort_ptr, p.wait_ns));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const int there = pages_there[j % kSteps];
+        const bool whole = there == 0xff && key0 + 127 <= least && key0 + 127 < to;
+        uint32_t s[128];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) tmem_ld32(s_at + 32u * w, s + 32 * w);
+        tmem_ld_wait();
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          const uint4 k = lds_16(steps + i * 4);
+          const float2 x = f32x2_get(f32x2_mul(f32x2_make(s[i], s[i + 1]), f32x2_make(k.x, k.y)));
+          const float2 y = f32x2_get(f32x2_mul(f32x2_make(s[i + 2], s[i + 3]), f32x2_make(k.z, k.w)));
+          s[i] = __float_as_uint(x.x);
+          s[i + 1] = __float_as_uint(x.y);
+          s[i + 2] = __float_as_uint(y.x);
+          s[i + 3] = __float_as_uint(y.y);
+          if (whole) {
+            m[i / 4 & 3] = max3(m[i / 4 & 3], x.x, x.y);
+            m[i / 4 & 3] = max3(m[i / 4 & 3], y.x, y.y);
+          }
+        }
+        if (!whole) {
+          const int seen = min(position, to - 1) - key0;  // the last key of the block that the row sees
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            if (i > seen || !(there >> (i / 16) & 1)) s[i] = 0xff800000u;  // -infinity
+            m[i & 3] = fmaxf(m[i & 3], __uint_as_float(s[i]));
+          }
+        }
+        const float top = max3(m[0], m[1], fmaxf(m[2], m[3])) * scale;
+        const bool raise = top > base + 8.0f;  // (true for the first keys of a row: its base is -infinity)
+        if (__any_sync(~0u, raise)) {
+          const float next = raise ? top : base;
+          const float keep = raise ? exp2_fast(base - next) : 1.0f;
+          base = next;
+          total *= keep;
+          if (j > 0) {
+#pragma unroll
+            for (int w = 0; w < D / 16; ++w) {
+              uint32_t o[16];
+              tmem_ld16(o_at + 16u * w, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st16(o_at + 16u * w, o);
+            }
+          }
+        }
+        const float zero = base == -INFINITY ? 0.0f : -base;
+        const uint64_t from2 = f32x2_make(__float_as_uint(zero), __float_as_uint(zero));
+        uint64_t sums[2] = {0, 0};
+        // P leaves in halves: the first one's products begin while the second one's exponentials are taken
+        auto half = [&](int h, auto all) {
+#pragma unroll
+          for (int w = 4 * h; w < 4 * h + 4; ++w) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              const int at = 16 * w + 2 * i;
+              const uint4 v = lds_16(steps + 512u + at * 4);
+              const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 x = f32x2_get(f32x2_fma3(f32x2_make(s[at + 2 * e], s[at + 2 * e + 1]), c2, from2));
+                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                const uint64_t both = f32x2_make(__float_as_uint(e0), __float_as_uint(e1));
+                f32x2_add(sums[e], sums[e], both);
+                float2 y = f32x2_get(f32x2_mul(both, f32x2_make(vs[2 * e], vs[2 * e + 1])));
+                if (!decltype(all)::value) {  // (the step of a key that takes no part may be anything)
+                  if (s[at + 2 * e] == 0xff800000u) y.x = 0.0f;
+                  if (s[at + 2 * e + 1] == 0xff800000u) y.y = 0.0f;
+                }
+                hi[i + e] = pack2<__nv_bfloat16>(y.x, y.y);
+                if (HALF) lo[i + e] = pack2<__nv_bfloat16>(y.x - __uint_as_float(hi[i + e] << 16), y.y - __uint_as_float(hi[i + e] & 0xffff0000u));
+              }
+            }
+            tmem_st8(s_at + 8u * w, hi);
+            if (HALF) tmem_st8(s_at + 64u + 8u * w, lo);
+          }
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(h == 0 ? &p_half[t] : &p_full[t]));
+        };
+        if (whole) {
+          half(0, std::true_type{});
+          half(1, std::true_type{});
+        } else {
+          half(0, std::false_type{});
+          half(1, std::false_type{});
+        }
+        f32x2_add(sums[0], sums[0], sums[1]);
+        const float2 sum = f32x2_get(sums[0]);
+        total += sum.x + sum.y;
+      }
+      if (ok && blocks > 0) {
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_full[t]), 0, abort_ptr, p.wait_ns));
+        tc_fence_after_sync();
+      }
+      if (!ok) {
+        if (lane == 0) gave_up();
+      } else {
+        const long long line = (a.first_range + range) * (c.tokens * a.heads) + token * a.heads + head;
+        const float norm = total == 0.0f ? 0.0f : 1.0f / total;
+        if (a.part != nullptr && position > -2) a.part_top[line] = make_float2(base, total);
+        T* out = static_cast<T*>(a.o) + token * a.o_token + head * a.o_head;
+#pragma unroll 1
+        for (int w = 0; w < D / 16; ++w) {
+          uint32_t o[16] = {};
+          if (blocks > 0) {
+            tmem_ld16(o_at + 16u * w, o);
+            tmem_ld_wait();
+          }
+          if (position < -1 || 16 * w >= c.d) continue;
+          if (a.part != nullptr) {
+            float4* to_part = reinterpret_cast<float4*>(a.part + line * a.part_width + 16 * w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to_part[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          } else {
+            OpVec<T, 4> y[4];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i / 4].e[i % 4] = op_put<T>(total == 0.0f ? 0.0f : __uint_as_float(o[i]) * norm);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (a.o_wide) {
+                if (16 * w + 4 * i < c.d) *reinterpret_cast<OpVec<T, 4>*>(out + 16 * w + 4 * i) = y[i];
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (16 * w + 4 * i + e < c.d) out[16 * w + 4 * i + e] = y[i].e[e];
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before_sync();
+    }
+  }
+  __syncthreads();
+  if (warp == 3) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, Shape::kTmemCols);
+  }
+  grid_dependency_wait();
+}
+
+}  // namespace nb
