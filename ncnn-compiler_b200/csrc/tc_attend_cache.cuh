@@ -3,12 +3,15 @@
 // A CTA has two tiles of 128 rows that read one key head (a row is a token and one of the head's query heads; of one sequence, or, for
 // a shared prefix, of all) and walks a range of keys in blocks of 128 with a running maximum and sum, as tc_attend.cuh does:
 //   S = Q K^T, P = 2^(S ks c - m) vs over S in tensor memory, O += P V
+// Scores of a block lie in two halves of 64 keys, each with barriers of its own: while the softmax has one half, the other half's
+// products and its scores of the next block are made, so that a softmax never waits for the MMAs (one buffer for whole blocks: 4420
+// clocks a block, 3290 of them in the softmax).
 // Integers are exact in 16 bits, so that keys and values are converted as they are and the steps ks, vs of a key meet its column in the
 // softmax.  P is rounded to bf16, whose range holds any step; f16 results take a second bf16 term of P (16 bits) and a second product.
 //
-// Roles: warps 0 to 2 bring blocks (each lane with cp.async into a queue of its own, a block ahead and more), convert them (16 bytes to 32)
-// and store them as TMA would with a 128-byte swizzle, keys and values in turn in a ring of three tiles; warp 3 issues the MMAs; warps
-// 4 to 7 are tile 0's softmax, 8 to 11 tile 1's.  Converting takes some 2300 instructions a block, the softmaxes 4500, of the 8192 that
+// Roles: warp 6 brings blocks, 16 keys of a page to a bulk copy, into a ring of three; warps 0 to 5 convert them (16 bytes to 32) and
+// store them as TMA would with a 128-byte swizzle, keys and values in turn, in a second ring of three; warp 7 issues the MMAs; warps
+// 8 to 11 are tile 0's softmax, 12 to 15 tile 1's.  Converting takes some 2300 instructions a block, the softmaxes 4500, of the 8192 that
 // fit into the time of the block's MMAs (2048 clocks): 256 rows to a CTA make the conversion cheap.
 #pragma once
 
@@ -28,15 +31,15 @@ struct TcCacheParams {
 
 template <int D>
 struct TcCacheShape {
-  static constexpr int kThreads = 384;
+  static constexpr int kThreads = 512, kConverters = 6;
   static constexpr int kPanel = 128 * 128;  // 128 rows of 64 components
   static constexpr int kTile = kPanel * (D / 64);
   static constexpr int kSlots = 3, kSteps = 8, kQueue = 3;
   static constexpr int kUnits = 128 * D / 512;            // of 32 pieces of 16 bytes, in a block of keys or values
-  static constexpr int kUnitsAWarp = (kUnits + 2) / 3;
-  static constexpr int kQueueTile = kUnitsAWarp * 3 * 512;
-  static constexpr int kRegsLaunch = 168, kRegsControl = 72, kRegsSoftmax = 216;
-  static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "registers of the roles");
+  static constexpr int kUnitsAWarp = (kUnits + kConverters - 1) / kConverters;
+  static constexpr int kQueueTile = 128 * D;
+  static constexpr int kRegsLaunch = 128, kRegsControl = 56, kRegsSoftmax = 200;
+  static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "registers of the roles");
   static constexpr uint32_t kTmemCols = 512;
   static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + kQueue * kQueueTile + kSteps * 1024;
 };
@@ -55,7 +58,8 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
   constexpr int kTile = Shape::kTile, kPanel = Shape::kPanel, kSlots = Shape::kSlots, kSteps = Shape::kSteps;
   constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ uint8_t cache_smem[];
-  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2], p_half[2], p_full[2], o_full[2], drained;
+  __shared__ __align__(8) uint64_t brought[Shape::kQueue], taken[Shape::kQueue];
+  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2][2], p_full[2][2], o_done[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, pages_there[kSteps];
   const AttendCacheParams& a = p.a;
@@ -112,19 +116,24 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
     mbar_init(smem_u32(&q_full), 4u * tiles);
     mbar_init(smem_u32(&drained), 1);
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(smem_u32(&full[i]), 3);
+      mbar_init(smem_u32(&full[i]), Shape::kConverters);
       mbar_init(smem_u32(&empty[i]), 1);
     }
-    for (int i = 0; i < kSteps; ++i) mbar_init(smem_u32(&steps_full[i]), 3);
+    for (int i = 0; i < Shape::kQueue; ++i) {
+      mbar_init(smem_u32(&brought[i]), 1);
+      mbar_init(smem_u32(&taken[i]), Shape::kConverters);
+    }
+    for (int i = 0; i < kSteps; ++i) mbar_init(smem_u32(&steps_full[i]), Shape::kConverters);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&s_full[t]), 1);
-      mbar_init(smem_u32(&p_half[t]), 4);
-      mbar_init(smem_u32(&p_full[t]), 4);
-      mbar_init(smem_u32(&o_full[t]), 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_u32(&s_full[t][h]), 1);
+        mbar_init(smem_u32(&p_full[t][h]), 4);
+      }
+      mbar_init(smem_u32(&o_done[t]), 1);
     }
     fence_mbar_init();
   }
-  if (warp == 3) {
+  if (warp == 7) {
     tmem_alloc(smem_u32(&tmem_slot), Shape::kTmemCols);
     tmem_relinquish();
   }
@@ -138,73 +147,40 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
   auto s_of = [&](int t) { return tmem + 128u * t; };
   auto o_of = [&](int t) { return tmem + 256u + static_cast<uint32_t>(D * t); };
 
-  if (warp < 4) {
+  if (warp < 8) {
     reg_dealloc<Shape::kRegsControl>();
-    if (warp < 3) {
-      // ---- blocks of keys and values: brought, converted, stored
+    if (warp < Shape::kConverters) {
+      // ---- blocks of keys and values converted: a unit is a lane's 16 bytes of each of some rows
       constexpr int PIECES = D / 16, UNIT_ROWS = 32 / PIECES, UNITS = Shape::kUnitsAWarp;
       const int piece = lane % PIECES, row_in = lane / PIECES;
       const bool used_piece = piece * 16 < c.row;
-      const uint32_t my_queue = queue + static_cast<uint32_t>(warp * UNITS) * 512u + lane * 16u;
-      const int table_row = a.prefix ? 0 : sequence;
-      // where this lane's pieces of unit 0 go: 16 bytes become 32, that is, pieces 2 piece and 2 piece + 1 of a row of components.
+      // where this lane's pieces go: 16 bytes become 32, that is, pieces 2 piece and 2 piece + 1 of a row of components.
       // The lanes of the second panel store them the other way round, so that eight neighbours reach all banks.
       const uint32_t panel = static_cast<uint32_t>(piece / 4) * kPanel;
       const int out = piece % 4 * 2, swap = D == 128 ? piece / 4 : 0;
-      // eight pages to a block of keys, looked up when its keys are asked for; its values take the same
-      int pages[2] = {-1, -1};  // lanes 0 to 7, of even and odd blocks
-      auto ask = [&](int u) {
-        if (u < 2 * blocks && p.stall == 0) {
-          const int j = u >> 1, key0 = from + j * 128;
-          const bool value = u & 1;
-          if (!value) {
-            const int key = key0 + (lane & 7) * 16;
-            const int found = key < to ? cache_page(c, table_row, key) : -1;
-            if (j & 1) pages[1] = found;
-            else pages[0] = found;
-          }
-          const int mine = j & 1 ? pages[1] : pages[0];
-          const int8_t* base = value ? c.v : c.k;
-          const uint32_t stage = my_queue + static_cast<uint32_t>(u % Shape::kQueue) * Shape::kQueueTile;
+      const uint32_t my_piece = queue + static_cast<uint32_t>((warp * UNIT_ROWS + row_in) * c.row + (used_piece ? piece * 16 : 0));
+      const uint32_t unit_step = static_cast<uint32_t>(Shape::kConverters * UNIT_ROWS * c.row);
+      bool ok = true;
+      int slot = 0, in = 0;
+      uint32_t ph = 1, in_ph = 0;
+      for (int u = 0; u < 2 * blocks; ++u) {
+        const bool value = u & 1;
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&brought[in]), in_ph, abort_ptr, p.wait_ns));
+        if (!ok) break;
+        uint4 held[UNITS];
 #pragma unroll
-          for (int i = 0; i < UNITS; ++i) {
-            const int unit = warp + 3 * i, r = unit * UNIT_ROWS + row_in;
-            const int page = __shfl_sync(~0u, mine, (unit * UNIT_ROWS / 16) & 7);
-            const bool take = unit < Shape::kUnits && page >= 0 && used_piece;
-            const long long line = take ? ((static_cast<long long>(page) * c.kv_heads + kv_head) << c.page_shift) + ((key0 + r) & ((1 << c.page_shift) - 1)) : 0;
-            queue_16(stage + i * 512, take ? base + line * c.row + piece * 16 : base, take);
-          }
-          if (warp < 2 && (warp == 1) == value) {
-            // the steps: four keys to a lane, all of one page
-            const int page = __shfl_sync(~0u, mine, lane / 4);
-            const bool take = page >= 0;
-            const long long line = take ? ((static_cast<long long>(page) * c.kv_heads + kv_head) << c.page_shift) + ((key0 + lane * 4) & ((1 << c.page_shift) - 1)) : 0;
-            queue_16(steps_at + static_cast<uint32_t>(j % kSteps) * 1024u + (value ? 512u : 0u) + lane * 16u, (value ? c.v_steps : c.k_steps) + line, take);
-          }
-          if (warp == 2 && !value) {
-            const int there = __ballot_sync(~0u, lane < 8 && mine >= 0);
-            if (lane == 0) pages_there[j % kSteps] = there;
-          }
+        for (int i = 0; i < UNITS; ++i) {
+          held[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (warp + Shape::kConverters * i < Shape::kUnits && used_piece) held[i] = lds_16(my_piece + static_cast<uint32_t>(in) * Shape::kQueueTile + i * unit_step);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-      bool ok = p.stall == 0;
-      for (int u = 0; u < Shape::kQueue - 1; ++u) ask(u);
-      int slot = 0;
-      uint32_t ph = 1;
-      for (int u = 0; ok && u < 2 * blocks; ++u) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(Shape::kQueue - 2) : "memory");
-        ask(u + Shape::kQueue - 1);
         ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&empty[slot]), ph, abort_ptr, p.wait_ns));
         if (!ok) break;
-        const bool value = u & 1;
-        const uint32_t from_at = my_queue + static_cast<uint32_t>(u % Shape::kQueue) * Shape::kQueueTile;
         const uint32_t to_at = ring + static_cast<uint32_t>(slot) * kTile + panel;
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-          const int unit = warp + 3 * i, r = unit * UNIT_ROWS + row_in;
+          const int unit = warp + Shape::kConverters * i, r = unit * UNIT_ROWS + row_in;
           if (unit >= Shape::kUnits) break;
-          const uint4 w = lds_16(from_at + i * 512);
+          const uint4 w = held[i];
           uint32_t h[8];
           if (HALF && !value) {
             int8_quad<__half>(w.x, h[0], h[1]);
@@ -229,71 +205,127 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(smem_u32(&full[slot]));
+          mbar_arrive(smem_u32(&taken[in]));
           if (value) mbar_arrive(smem_u32(&steps_full[(u >> 1) % kSteps]));  // (keys' and values' steps, and which pages are there)
         }
         if (++slot == kSlots) {
           slot = 0;
           ph ^= 1u;
         }
+        if (++in == Shape::kQueue) {
+          in = 0;
+          in_ph ^= 1u;
+        }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (!ok && lane == 0) gave_up();
+    } else if (warp == 6) {
+      // ---- blocks brought: lanes 0 to 7 sixteen keys' rows each, lanes 8 to 15 their steps
+      const int table_row = a.prefix ? 0 : sequence;
+      const long long page_rows = static_cast<long long>(c.kv_heads) << c.page_shift, head_rows = static_cast<long long>(kv_head) << c.page_shift;
+      const int in_page = (1 << c.page_shift) - 1;
+      const uint32_t rows_bytes = 16u * c.row;
+      // eight pages to a block, four blocks to the lanes, looked up while the four blocks before are asked for
+      auto look_up = [&](int j0) {
+        const int key = from + j0 * 128 + lane * 16;
+        return key < to ? cache_page(c, table_row, key) : -1;
+      };
+      int pages = -1, next_pages = look_up(0);
+      int issued = 0, in = 0;
+      uint32_t ph = 1;
+      bool ok = p.stall == 0;
+      for (int u = 0; ok && u < 2 * blocks; ++u) {
+        const int j = u >> 1;
+        const bool value = u & 1;
+        if (!value && (j & 3) == 0) {
+          pages = next_pages;
+          next_pages = look_up(j + 4);
+        }
+        const int page = __shfl_sync(~0u, pages, (j & 3) * 8 + (lane & 7));
+        const uint32_t there = __ballot_sync(~0u, page >= 0) & 0xffu;
+        const long long line = page_rows * page + head_rows + ((from + j * 128 + (lane & 7) * 16) & in_page);
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&taken[in]), ph, abort_ptr, p.wait_ns));
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&brought[in]);
+        if (lane == 0) {
+          if (!value) pages_there[j % kSteps] = static_cast<int>(there);
+          mbar_arrive_expect_tx(bar, __popc(there) * (rows_bytes + 64u));
+        }
+        __syncwarp();
+        if (page >= 0 && lane < 8) bulk_load(queue + static_cast<uint32_t>(in) * Shape::kQueueTile + lane * rows_bytes, (value ? c.v : c.k) + line * c.row, rows_bytes, bar);
+        if (page >= 0 && lane >= 8 && lane < 16)
+          bulk_load(steps_at + static_cast<uint32_t>(j % kSteps) * 1024u + (value ? 512u : 0u) + (lane & 7) * 64u, (value ? c.v_steps : c.k_steps) + line, 64u, bar);
+        issued = u + 1;
+        if (++in == Shape::kQueue) {
+          in = 0;
+          ph ^= 1u;
+        }
+      }
       if (!ok && p.stall == 0 && lane == 0) gave_up();
+      // no copy may be under way when the CTA's shared memory is given back
+      if (lane == 0) {
+        const int before_last = issued > Shape::kQueue ? issued - Shape::kQueue : 0;
+        for (int u = before_last; u < issued; ++u)
+          for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&brought[u % Shape::kQueue]), (u / Shape::kQueue) & 1); ++tries) {
+          }
+      }
     } else if (blocks > 0) {
       // ---- MMAs
       if (elect_one()) {
         constexpr uint32_t kBMnMajor = 1u << 16;
-        const uint32_t s_idesc = instr_desc(1, HALF ? 0u : 1u, 128, 128), pv_idesc = instr_desc(1, 1u, 128, D) | kBMnMajor;
+        const uint32_t s_idesc = instr_desc(1, HALF ? 0u : 1u, 128, 64), pv_idesc = instr_desc(1, 1u, 128, D) | kBMnMajor;
         bool ok = mbar_wait_bounded(smem_u32(&q_full), 0, abort_ptr, p.wait_ns);
-        auto wait_use = [&](int u) { return mbar_wait_bounded(smem_u32(&full[u % kSlots]), (u / kSlots) & 1, abort_ptr, p.wait_ns); };
-        auto scores = [&](int t, int j) {
-          const uint32_t k_at = ring + static_cast<uint32_t>((2 * j) % kSlots) * kTile, a_at = q_at + t * kTile;
+        // (a block's keys are use 2 j of the ring, its values use 2 j + 1)
+        auto wait_use = [&](int slot, uint32_t ph) { return mbar_wait_bounded(smem_u32(&full[slot]), ph, abort_ptr, p.wait_ns); };
+        auto scores = [&](int t, int slot, int h) {
+          const uint32_t k_at = ring + static_cast<uint32_t>(slot) * kTile + h * 8192, a_at = q_at + t * kTile;
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
             const uint32_t off = (n / 4) * kPanel + (n % 4) * 32;
-            mma_f16(s_of(t), smem_desc_kmajor(a_at + off, 128), smem_desc_kmajor(k_at + off, 128), s_idesc, n > 0);
+            mma_f16(s_of(t) + 64u * h, smem_desc_kmajor(a_at + off, 128), smem_desc_kmajor(k_at + off, 128), s_idesc, n > 0);
           }
+          tc_commit(smem_u32(&s_full[t][h]));
         };
-        // four steps of 16 keys; f16's second terms lie 64 columns behind the first
-        auto products = [&](int t, int j, int at) {
-          const uint32_t v_at = ring + static_cast<uint32_t>((2 * j + 1) % kSlots) * kTile;
+        // four steps of 16 keys; f16's second terms lie 32 columns behind the first
+        auto products = [&](int t, int slot, int h, bool first_ones) {
+          const uint32_t v_at = ring + static_cast<uint32_t>(slot) * kTile + h * 8192;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint64_t v = smem_desc_mnmajor(v_at + (at + i) * 2048, kPanel, 1024);
-            mma_f16_ts(o_of(t), s_of(t) + 8u * (at + i), v, pv_idesc, j > 0 || at + i > 0);
-            if (HALF) mma_f16_ts(o_of(t), s_of(t) + 64u + 8u * (at + i), v, pv_idesc, 1u);
+            const uint64_t v = smem_desc_mnmajor(v_at + i * 2048, kPanel, 1024);
+            mma_f16_ts(o_of(t), s_of(t) + 64u * h + 8u * i, v, pv_idesc, !first_ones || i > 0);
+            if (HALF) mma_f16_ts(o_of(t), s_of(t) + 64u * h + 32u + 8u * i, v, pv_idesc, 1u);
           }
+          tc_commit(smem_u32(&o_done[t]));
         };
-        ok = ok && wait_use(0);
+        ok = ok && wait_use(0, 0);
         if (ok) {
           tc_fence_after_sync();
-          for (int t = 0; t < tiles; ++t) {
-            scores(t, 0);
-            tc_commit(smem_u32(&s_full[t]));
-          }
+          for (int h = 0; h < 2; ++h)
+            for (int t = 0; t < tiles; ++t) scores(t, 0, h);
           tc_commit(smem_u32(&empty[0]));
         }
+        int v_slot = 1;
+        uint32_t v_ph = 0;
         for (int j = 0; ok && j < blocks; ++j) {
-          for (int t = 0; t < tiles; ++t) {
-            if (t == 0) ok = wait_use(2 * j + 1);
-            ok = ok && mbar_wait_bounded(smem_u32(&p_half[t]), j & 1, abort_ptr, p.wait_ns);
-            if (!ok) break;
-            tc_fence_after_sync();
-            products(t, j, 0);
-            ok = mbar_wait_bounded(smem_u32(&p_full[t]), j & 1, abort_ptr, p.wait_ns);
-            if (!ok) break;
-            tc_fence_after_sync();
-            products(t, j, 4);
-            if (t == tiles - 1) tc_commit(smem_u32(&empty[(2 * j + 1) % kSlots]));
-            if (j + 1 < blocks) {
-              if (t == 0) ok = wait_use(2 * j + 2);
+          const int k_slot = v_slot == kSlots - 1 ? 0 : v_slot + 1;
+          const uint32_t k_ph = k_slot == 0 ? v_ph ^ 1u : v_ph;
+          const bool more = j + 1 < blocks;
+          ok = wait_use(v_slot, v_ph);
+          for (int h = 0; ok && h < 2; ++h)
+            for (int t = 0; t < tiles; ++t) {
+              ok = mbar_wait_bounded(smem_u32(&p_full[t][h]), j & 1, abort_ptr, p.wait_ns);
               if (!ok) break;
-              scores(t, j + 1);
-              tc_commit(smem_u32(&s_full[t]));
-              if (t == tiles - 1) tc_commit(smem_u32(&empty[(2 * j + 2) % kSlots]));
-            } else {
-              tc_commit(smem_u32(&o_full[t]));
+              tc_fence_after_sync();
+              products(t, v_slot, h, j == 0 && h == 0);
+              if (h == 1 && t == tiles - 1) tc_commit(smem_u32(&empty[v_slot]));
+              if (more) {
+                if (h == 0 && t == 0) ok = wait_use(k_slot, k_ph);
+                if (!ok) break;
+                scores(t, k_slot, h);
+                if (h == 1 && t == tiles - 1) tc_commit(smem_u32(&empty[k_slot]));
+              }
             }
-          }
+          v_slot = k_slot == kSlots - 1 ? 0 : k_slot + 1;
+          v_ph = v_slot == 0 ? k_ph ^ 1u : k_ph;
         }
         if (!ok) {
           gave_up();
@@ -306,7 +338,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
   } else {
     // ---- softmaxes
     reg_alloc<Shape::kRegsSoftmax>();
-    const int t = (warp - 4) >> 2;
+    const int t = (warp - 8) >> 2;
     if (t < tiles) {
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes of tensor memory (lane in the upper half word)
       const uint32_t s_at = s_of(t) + lanes, o_at = o_of(t) + lanes;
@@ -352,41 +384,35 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
       float base = -INFINITY;  // of the exponentials: the maximum so far, or one up to 2^8 smaller
       float total = 0.0f;
       bool ok = true;
-      for (int j = 0; j < blocks; ++j) {
-        const int key0 = from + j * 128;
-        const uint32_t steps = steps_at + static_cast<uint32_t>(j % kSteps) * 1024u;
-        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&s_full[t]), j & 1, abort_ptr, p.wait_ns) &&
-                                 mbar_wait_bounded(smem_u32(&steps_full[j % kSteps]), (j / kSteps) & 1, abort_ptr, p.wait_ns));
-        if (!ok) break;
-        tc_fence_after_sync();
-        const int there = pages_there[j % kSteps];
-        const bool whole = there == 0xff && key0 + 127 <= least && key0 + 127 < to;
-        uint32_t s[128];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) tmem_ld32(s_at + 32u * w, s + 32 * w);
+      // a half block: its 64 scores, and P in their place.  ALL: every row of the warp sees every key of it.
+      auto half = [&](int j, int h, auto all, int there) {
+        constexpr bool ALL = decltype(all)::value;
+        const uint32_t steps = steps_at + static_cast<uint32_t>(j % kSteps) * 1024u + h * 256u, s_half = s_at + 64u * h;
+        const int key0 = from + j * 128 + h * 64;
+        uint32_t s[64];
+        tmem_ld32(s_half, s);
+        tmem_ld32(s_half + 32u, s + 32);
         tmem_ld_wait();
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const int seen = min(position, to - 1) - key0;  // the last key of the half that the row sees
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
+        for (int i = 0; i < 64; i += 4) {
           const uint4 k = lds_16(steps + i * 4);
-          const float2 x = f32x2_get(f32x2_mul(f32x2_make(s[i], s[i + 1]), f32x2_make(k.x, k.y)));
-          const float2 y = f32x2_get(f32x2_mul(f32x2_make(s[i + 2], s[i + 3]), f32x2_make(k.z, k.w)));
+          float2 x = f32x2_get(f32x2_mul(f32x2_make(s[i], s[i + 1]), f32x2_make(k.x, k.y)));
+          float2 y = f32x2_get(f32x2_mul(f32x2_make(s[i + 2], s[i + 3]), f32x2_make(k.z, k.w)));
+          if (!ALL) {
+            const bool page = there >> (4 * h + i / 16) & 1;
+            if (!page || i > seen) x.x = -INFINITY;
+            if (!page || i + 1 > seen) x.y = -INFINITY;
+            if (!page || i + 2 > seen) y.x = -INFINITY;
+            if (!page || i + 3 > seen) y.y = -INFINITY;
+          }
           s[i] = __float_as_uint(x.x);
           s[i + 1] = __float_as_uint(x.y);
           s[i + 2] = __float_as_uint(y.x);
           s[i + 3] = __float_as_uint(y.y);
-          if (whole) {
-            m[i / 4 & 3] = max3(m[i / 4 & 3], x.x, x.y);
-            m[i / 4 & 3] = max3(m[i / 4 & 3], y.x, y.y);
-          }
-        }
-        if (!whole) {
-          const int seen = min(position, to - 1) - key0;  // the last key of the block that the row sees
-#pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            if (i > seen || !(there >> (i / 16) & 1)) s[i] = 0xff800000u;  // -infinity
-            m[i & 3] = fmaxf(m[i & 3], __uint_as_float(s[i]));
-          }
+          m[i / 4 & 3] = max3(m[i / 4 & 3], x.x, x.y);
+          m[i / 4 & 3] = max3(m[i / 4 & 3], y.x, y.y);
         }
         const float top = max3(m[0], m[1], fmaxf(m[2], m[3])) * scale;
         const bool raise = top > base + 8.0f;  // (true for the first keys of a row: its base is -infinity)
@@ -395,7 +421,12 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
           const float keep = raise ? exp2_fast(base - next) : 1.0f;
           base = next;
           total *= keep;
-          if (j > 0) {
+          if (j > 0 || h > 0) {
+            // The products of all halves before this one are in O.  (Those of the half before the last one are, since these scores came
+            // after them: the barrier is in the last one's phase, or past it.)
+            ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_done[t]), (h ^ 1) & 1, abort_ptr, p.wait_ns));
+            if (!ok) return;
+            tc_fence_after_sync();
 #pragma unroll
             for (int w = 0; w < D / 16; ++w) {
               uint32_t o[16];
@@ -410,52 +441,60 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         const float zero = base == -INFINITY ? 0.0f : -base;
         const uint64_t from2 = f32x2_make(__float_as_uint(zero), __float_as_uint(zero));
         uint64_t sums[2] = {0, 0};
-        // P leaves in halves: the first one's products begin while the second one's exponentials are taken
-        auto half = [&](int h, auto all) {
 #pragma unroll
-          for (int w = 4 * h; w < 4 * h + 4; ++w) {
-            uint32_t hi[8], lo[8];
+        for (int w = 0; w < 4; ++w) {
+          uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              const int at = 16 * w + 2 * i;
-              const uint4 v = lds_16(steps + 512u + at * 4);
-              const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
+          for (int i = 0; i < 8; i += 2) {
+            const int at = 16 * w + 2 * i;
+            const uint4 v = lds_16(steps + 512u + at * 4);
+            const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 2; ++e) {
+              uint64_t both;
+              if (ALL && !HALF && (i + e) % 4 == 3) {  // every fourth pair on the FMA pipe: see tc_attend.cuh
+                both = exp_pair_fma_value<__nv_bfloat16>(s[at + 2 * e], s[at + 2 * e + 1], c2, from2);
+              } else {
                 const float2 x = f32x2_get(f32x2_fma3(f32x2_make(s[at + 2 * e], s[at + 2 * e + 1]), c2, from2));
-                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-                const uint64_t both = f32x2_make(__float_as_uint(e0), __float_as_uint(e1));
-                f32x2_add(sums[e], sums[e], both);
-                float2 y = f32x2_get(f32x2_mul(both, f32x2_make(vs[2 * e], vs[2 * e + 1])));
-                if (!decltype(all)::value) {  // (the step of a key that takes no part may be anything)
-                  if (s[at + 2 * e] == 0xff800000u) y.x = 0.0f;
-                  if (s[at + 2 * e + 1] == 0xff800000u) y.y = 0.0f;
-                }
-                hi[i + e] = pack2<__nv_bfloat16>(y.x, y.y);
-                if (HALF) lo[i + e] = pack2<__nv_bfloat16>(y.x - __uint_as_float(hi[i + e] << 16), y.y - __uint_as_float(hi[i + e] & 0xffff0000u));
+                both = f32x2_make(__float_as_uint(exp2_fast(x.x)), __float_as_uint(exp2_fast(x.y)));
               }
+              f32x2_add(sums[e], sums[e], both);
+              float2 y = f32x2_get(f32x2_mul(both, f32x2_make(vs[2 * e], vs[2 * e + 1])));
+              if (!ALL) {  // (the step of a key that takes no part may be anything)
+                if (s[at + 2 * e] == 0xff800000u) y.x = 0.0f;
+                if (s[at + 2 * e + 1] == 0xff800000u) y.y = 0.0f;
+              }
+              hi[i + e] = pack2<__nv_bfloat16>(y.x, y.y);
+              if (HALF) lo[i + e] = pack2<__nv_bfloat16>(y.x - __uint_as_float(hi[i + e] << 16), y.y - __uint_as_float(hi[i + e] & 0xffff0000u));
             }
-            tmem_st8(s_at + 8u * w, hi);
-            if (HALF) tmem_st8(s_at + 64u + 8u * w, lo);
           }
-          tmem_st_wait();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(h == 0 ? &p_half[t] : &p_full[t]));
-        };
-        if (whole) {
-          half(0, std::true_type{});
-          half(1, std::true_type{});
-        } else {
-          half(0, std::false_type{});
-          half(1, std::false_type{});
+          tmem_st8(s_half + 8u * w, hi);
+          if (HALF) tmem_st8(s_half + 32u + 8u * w, lo);
         }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[t][h]));
         f32x2_add(sums[0], sums[0], sums[1]);
         const float2 sum = f32x2_get(sums[0]);
         total += sum.x + sum.y;
+      };
+      for (int j = 0; ok && j < blocks; ++j) {
+        const int key0 = from + j * 128;
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&steps_full[j % kSteps]), (j / kSteps) & 1, abort_ptr, p.wait_ns));
+        const int there = ok ? pages_there[j % kSteps] : 0;
+        const bool whole = there == 0xff && key0 + 127 <= least && key0 + 127 < to;
+        for (int h = 0; ok && h < 2; ++h) {
+          ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&s_full[t][h]), j & 1, abort_ptr, p.wait_ns));
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (whole) half(j, h, std::true_type{}, there);
+          else half(j, h, std::false_type{}, there);
+        }
       }
       if (ok && blocks > 0) {
-        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_full[t]), 0, abort_ptr, p.wait_ns));
+        // the last two halves' products, one after the other: a barrier can be asked for the phase that it is in, not for the one after
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_done[t]), 0, abort_ptr, p.wait_ns) && mbar_wait_bounded(smem_u32(&o_done[t]), 1, abort_ptr, p.wait_ns));
         tc_fence_after_sync();
       }
       if (!ok) {
@@ -498,7 +537,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
     }
   }
   __syncthreads();
-  if (warp == 3) {
+  if (warp == 7) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, Shape::kTmemCols);
   }
