@@ -43,27 +43,34 @@ struct AttendCacheParams {
   int o_wide;              // four components of o can be stored at a time
 };
 
-// four int8 as two pairs of T (the first in the lower half)
-template <class T> __device__ __forceinline__ uint32_t int8_pair(uint32_t spread);  // integers in bytes 0 and 2
-template <> __device__ __forceinline__ uint32_t int8_pair<__nv_bfloat16>(uint32_t x) {
-  // 128 + the low seven bits, less 128 or 256
-  uint32_t a, b, r;
-  asm("lop3.b32 %0, %1, 0x007f007f, 0x43004300, 0xea;" : "=r"(a) : "r"(x));
-  asm("lop3.b32 %0, %1, 0x00800080, 0x43004300, 0xea;" : "=r"(b) : "r"(x));
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+// Integers as 16-bit floating point.  bf16 whose upper byte is 0 are u 2^-133 for every lower byte u: 0 to 127 as subnormal numbers, 128
+// to 255 with the smallest exponent.  So a byte q + 128 becomes q / 64 in one fma, (q + 128) 2^-133 2^127 - 2, exactly; the 64 is made good
+// for in the factor of the scores and in the results.  (Three instructions and a subtraction to a pair before: 147 us for 64 ragged
+// sequences of up to 8192 keys, ALU-bound.)
+constexpr float kBf16Integers = 64.0f;
+__device__ __forceinline__ uint32_t biased_pair(uint32_t x) {  // q + 128 in bytes 0 and 2, zeros in 1 and 3
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0x7f007f00u), "r"(0xc000c000u));
   return r;
 }
+// integers in bytes 0 and 2, anything in 1 and 3
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t x) {
+  uint32_t u;
+  asm("lop3.b32 %0, %1, 0x00ff00ff, 0x00800080, 0x6a;" : "=r"(u) : "r"(x));  // (x & mask) ^ bias
+  return biased_pair(u);
+}
+// four integers as two pairs of T (the first in the lower half): fp16's as they are, bf16's over 64
 template <class T>
 __device__ __forceinline__ void int8_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
   if constexpr (std::is_same<T, __half>::value) {
     // 1024 + (q + 128), less 1152
-    const uint32_t u = w ^ 0x80808080u;
     const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
   } else {
-    lo = int8_pair<__nv_bfloat16>(__byte_perm(w, 0u, 0x4140));
-    hi = int8_pair<__nv_bfloat16>(__byte_perm(w, 0u, 0x4342));
+    lo = biased_pair(__byte_perm(u, 0u, 0x4140));
+    hi = biased_pair(__byte_perm(u, 0u, 0x4342));
   }
 }
 
@@ -251,6 +258,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) q_held[s] = lds_8(q_at + s * 256);
 
+  const float scale = p.scale_log2 * (std::is_same<KT, __half>::value ? 1.0f : kBf16Integers);
   float o[NT][STEPS][4] = {};
   float base[NT][2], total[NT][2] = {};
 #pragma unroll
@@ -283,7 +291,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
     }
     // s[t][e]: key 2 group + e / 2, row 8 t + 2 quad + e % 2
     const uint2 ks = lds_8(at8 + Shared::kValues), vs = lds_8(at8 + Shared::kValues + 256);
-    const float k_step[2] = {__uint_as_float(ks.x) * p.scale_log2, __uint_as_float(ks.y) * p.scale_log2};
+    const float k_step[2] = {__uint_as_float(ks.x) * scale, __uint_as_float(ks.y) * scale};
     const float v_step[2] = {__uint_as_float(vs.x), __uint_as_float(vs.y)};
     const bool whole = there && key + 15 <= least && key + 15 < to;
     bool above = false;
@@ -365,8 +373,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
     for (int n = 0; n < STEPS; ++n) {
       // bytes 2 n and 2 n + 1 of two keys' words, in bytes 0 and 2
       const uint32_t even = 0x0400u + (2 * n % 4) * 0x0101u, odd = 0x0400u + ((2 * n + 1) % 4) * 0x0101u;
-      const uint32_t a[4] = {int8_pair<VT>(__byte_perm(v[0][n / 2], v[2][n / 2], even)), int8_pair<VT>(__byte_perm(v[0][n / 2], v[2][n / 2], odd)),
-                             int8_pair<VT>(__byte_perm(v[1][n / 2], v[3][n / 2], even)), int8_pair<VT>(__byte_perm(v[1][n / 2], v[3][n / 2], odd))};
+      const uint32_t a[4] = {bf16_pair(__byte_perm(v[0][n / 2], v[2][n / 2], even)), bf16_pair(__byte_perm(v[0][n / 2], v[2][n / 2], odd)),
+                             bf16_pair(__byte_perm(v[1][n / 2], v[3][n / 2], even)), bf16_pair(__byte_perm(v[1][n / 2], v[3][n / 2], odd))};
 #pragma unroll
       for (int w = PTERMS - 1; w >= 0; --w)
 #pragma unroll
@@ -414,6 +422,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS) k_attend_cache_few(const _
       sum = make_float4(fmaf(f, y.x, sum.x), fmaf(f, y.y, sum.y), fmaf(f, y.z, sum.z), fmaf(f, y.w, sum.w));
       all = fmaf(f, sh.total[w][r], all);
     }
+    sum = make_float4(sum.x * kBf16Integers, sum.y * kBf16Integers, sum.z * kBf16Integers, sum.w * kBf16Integers);
     const long long row = row0 + r, token = first + row / G;
     const int head = kv_head * G + static_cast<int>(row % G);
     if (p.part != nullptr) {

@@ -316,9 +316,9 @@ cudaError_t launch_cache_wide(const AttendCacheParams& a, int ranges, bool early
   if (const cudaError_t e = op_grant_smem(kernel, Shape::kSmem, device, &granted, Shape::kRegsLaunch); e != cudaSuccess) return e;
   const long long G = a.rows_a_head;
   const long long tiles = a.prefix ? (a.c.tokens * G + 255) / 256 : static_cast<long long>(a.c.sequences) * ((a.c.max_tokens * G + 255) / 256);
-  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (tiles * a.c.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
   op_will_wait_on(device);
-  return op_launch_early(early, kernel, dim3(static_cast<unsigned>(tiles), a.c.kv_heads, ranges), Shape::kThreads, Shape::kSmem, st, 0, p);
+  return op_launch_early(early, kernel, dim3(static_cast<unsigned>(tiles * a.c.kv_heads), ranges), Shape::kThreads, Shape::kSmem, st, 0, p);
 }
 
 template <class T, int D, int NT, int WARPS, int STAGES, int BLOCKS>

@@ -59,24 +59,24 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
   constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ uint8_t cache_smem[];
   __shared__ __align__(8) uint64_t brought[Shape::kQueue], taken[Shape::kQueue];
-  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2][2], p_full[2][2], o_done[2], drained;
+  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, pages_there[kSteps];
   const AttendCacheParams& a = p.a;
   const CacheParams& c = a.c;
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int range = blockIdx.z, kv_head = blockIdx.y, G = a.rows_a_head;
+  const int range = blockIdx.y, kv_head = static_cast<int>(blockIdx.x % c.kv_heads), G = a.rows_a_head;
   grid_dependency_trigger();
 
-  // rows: 256 from row0 on (the last ones first: their walks are the longest)
+  // rows: 256 from row0 on (the last ones of all heads first: their walks are the longest)
+  const int at = static_cast<int>((gridDim.x - 1 - blockIdx.x) / c.kv_heads);
   int sequence = 0;
-  long long row0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * 256, first = 0, rows;
+  long long row0 = static_cast<long long>(at) * 256, first = 0, rows;
   int before = 0;
   if (a.prefix) {
     rows = c.tokens * G;
   } else {
-    const int at = static_cast<int>(gridDim.x - 1 - blockIdx.x);
     sequence = at % c.sequences;
     row0 = static_cast<long long>(at / c.sequences) * 256;
     first = cache_start(c, sequence);
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         mbar_init(smem_u32(&p_full[t][h]), 4);
       }
       mbar_init(smem_u32(&o_done[t]), 1);
+      mbar_init(smem_u32(&o_full[t]), 1);
     }
     fence_mbar_init();
   }
@@ -317,6 +318,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
               tc_fence_after_sync();
               products(t, v_slot, h, j == 0 && h == 0);
               if (h == 1 && t == tiles - 1) tc_commit(smem_u32(&empty[v_slot]));
+              if (!more && h == 1) tc_commit(smem_u32(&o_full[t]));
               if (more) {
                 if (h == 0 && t == 0) ok = wait_use(k_slot, k_ph);
                 if (!ok) break;
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&q_full));
 
-      const float scale = a.scale_log2;
+      const float scale = a.scale_log2 * (HALF ? 1.0f : kBf16Integers);
       const uint64_t c2 = f32x2_make(__float_as_uint(scale), __float_as_uint(scale));
       float base = -INFINITY;  // of the exponentials: the maximum so far, or one up to 2^8 smaller
       float total = 0.0f;
@@ -493,15 +495,15 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         }
       }
       if (ok && blocks > 0) {
-        // the last two halves' products, one after the other: a barrier can be asked for the phase that it is in, not for the one after
-        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_done[t]), 0, abort_ptr, p.wait_ns) && mbar_wait_bounded(smem_u32(&o_done[t]), 1, abort_ptr, p.wait_ns));
+        // (not o_done: by now that may be in the phase after the last, which nothing ends)
+        ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_full[t]), 0, abort_ptr, p.wait_ns));
         tc_fence_after_sync();
       }
       if (!ok) {
         if (lane == 0) gave_up();
       } else {
         const long long line = (a.first_range + range) * (c.tokens * a.heads) + token * a.heads + head;
-        const float norm = total == 0.0f ? 0.0f : 1.0f / total;
+        const float norm = a.part != nullptr ? kBf16Integers : total == 0.0f ? 0.0f : kBf16Integers / total;
         if (a.part != nullptr && position > -2) a.part_top[line] = make_float2(base, total);
         T* out = static_cast<T*>(a.o) + token * a.o_token + head * a.o_head;
 #pragma unroll 1
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
           if (a.part != nullptr) {
             float4* to_part = reinterpret_cast<float4*>(a.part + line * a.part_width + 16 * w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to_part[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            for (int i = 0; i < 4; ++i) to_part[i] = make_float4(__uint_as_float(o[4 * i]) * norm, __uint_as_float(o[4 * i + 1]) * norm, __uint_as_float(o[4 * i + 2]) * norm, __uint_as_float(o[4 * i + 3]) * norm);
           } else {
             OpVec<T, 4> y[4];
 #pragma unroll
