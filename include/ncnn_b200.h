@@ -339,15 +339,16 @@ int ncnn_b200_op_cache_attention(const ncnn_b200_cache *cache, const ncnn_b200_c
                                  int32_t type, int32_t heads, const int64_t *strides, int64_t shared, float scale,
                                  void *workspace, int64_t workspace_bytes, void *stream);
 
-/* The tensor-core kernels of ncnn_b200_op_cross_attention bound their waits (2 s each).  This waits for the current device and
- * for every device that such a call went to, and returns 7, once to each thread, when one of the waits ran out, on any of them and
- * in any thread's call, since that thread's last such call (its first: since the library was loaded); 0 otherwise. */
+/* The tensor-core kernels of ncnn_b200_op_cross_attention, _op_inner_product_tokens and _op_cache_attention bound their waits (2 s
+ * each).  This waits for the current device and for every device that such a call went to, and returns 7, once to each thread, when one
+ * of the waits ran out, on any of them and in any thread's call, since that thread's last such call (its first: since the library was
+ * loaded); 0 otherwise. */
 int ncnn_b200_op_check_status(void);
 
-/* For tests of failures, not for production: what later calls of ncnn_b200_op_cross_attention on the tensor cores do, in all
- * threads.  stall 1: their first block of keys never arrives, so that their waits run out.  wait_ns: the limit of a wait (0 = the
- * usual one).  registers: as if the kernels had been compiled for so many (0 = as they are); other than the count that their roles
- * share out, a call is refused.  All 0: as usual. */
+/* For tests of failures, not for production: what later calls of those operators on the tensor cores do, in all threads.  stall 1: their
+ * first block of keys (or of weights) never arrives, so that their waits run out.  wait_ns: the limit of a wait (0 = the usual one).
+ * registers: as if the kernels whose roles share out registers had been compiled for so many (0 = as they are); other than the count
+ * that is shared out, a call is refused.  All 0: as usual. */
 int ncnn_b200_op_test_hooks(int32_t stall, uint64_t wait_ns, int32_t registers);
 
 /* ---- One model on several GPUs of one box (batch sharding).

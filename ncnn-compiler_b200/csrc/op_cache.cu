@@ -268,8 +268,9 @@ int up(long long x, int to) { return static_cast<int>((x + to - 1) / to * to); }
 // Rows of a tile: eights, sixteens or, of heads up to 128, thirty-twos.
 int few_rows(long long rows, int d) { return rows <= 8 ? 8 : rows <= 16 || d > 128 ? 16 : 32; }
 
-constexpr int kWideRows = 64;  // rows of a key head from which tiles of 128 rows are taken
-constexpr long long kRangeCtas = 8;  // CTAs to an SM that ranges are made for
+// More rows to a key head than this go through tiles of 128 rows (32 heads over 8 key heads of 128, one sequence of 16000 keys: 68 rows
+// 32 us, 64 rows in thirty-twos 47; 16 sequences of 2000: 96 rows 40, 64 rows in thirty-twos 47).
+constexpr int kWideRows = 32;
 
 AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long shared, int sms, bool halves) {
   const int G = heads / c.kv_heads;
@@ -279,9 +280,13 @@ AttendCachePlan attend_cache_plan(const CacheParams& c, int heads, long long sha
     p.wide = halves && c.d <= 128 && rows > kWideRows ? 1 : 0;
     const int height = p.wide ? 256 : few_rows(rows, c.d);
     const long long tiles = std::max<long long>(1, sequences * c.kv_heads * ((rows + height - 1) / height));
-    // Ranges of 256 keys at least, in tiles of 128 rows 512, and no more than 64 of them.
-    const long long most = std::max<long long>(1, p.wide ? std::min<long long>({64, (keys + 511) / 512, sms / tiles})
-                                                         : std::min<long long>({64, (keys + 255) / 256, kRangeCtas * sms / tiles}));
+    // Ranges, 64 at most.  Tiles of 128 rows: as many as give each SM a CTA, of 512 keys or more.  Few rows: where there are no more tiles
+    // than SMs, as many as fill the device once (two CTAs to an SM), of 256 keys or more: a CTA has 3 to 4 us of its own (8 sequences of
+    // 8192 keys, 64 tiles: 4 ranges 40 us, 9 46, 18 54; one of 60001: 37 ranges 45, 64 57).  Otherwise up to eight CTAs to an SM, of
+    // 1024 keys or more, which evens out sequences of different lengths (64 of up to 8192, 512 tiles: 1 range 156 us, 2 140, 9 155).
+    const long long most = std::max<long long>(1, p.wide          ? std::min<long long>({64, (keys + 511) / 512, sms / tiles})
+                                                  : tiles <= sms ? std::min<long long>({64, (keys + 255) / 256, 2ll * sms / tiles})
+                                                                 : std::min<long long>({64, (keys + 1023) / 1024, 8ll * sms / tiles}));
     p.chunk = up((keys + most - 1) / most, p.wide ? 128 : 64);
     p.ranges = static_cast<int>((keys + p.chunk - 1) / p.chunk);
     return p;
@@ -342,7 +347,7 @@ cudaError_t attend_cache_few(const AttendCacheParams& p, int ranges, bool early,
     return rows == 16 ? launch_cache_few<T, 64, 2, 4, 4, 4>(p, ranges, early, device, st) : launch_cache_few<T, 64, 4, 4, 4, 3>(p, ranges, early, device, st);
   }
   if (p.c.d <= 128) {
-    if (rows == 8) return launch_cache_few<T, 128, 1, 4, 3, 3>(p, ranges, early, device, st);
+    if (rows == 8) return launch_cache_few<T, 128, 1, 8, 3, sizeof(T) == 4 ? 1 : 2>(p, ranges, early, device, st);
     return rows == 16 ? launch_cache_few<T, 128, 2, 4, 4, 2>(p, ranges, early, device, st) : launch_cache_few<T, 128, 4, 4, 3, 2>(p, ranges, early, device, st);
   }
   return rows == 8 ? launch_cache_few<T, 256, 1, 4, 3, sizeof(T) == 4 ? 1 : 2>(p, ranges, early, device, st) : launch_cache_few<T, 256, 2, 4, 3, 1>(p, ranges, early, device, st);

@@ -451,6 +451,7 @@ def op_inner_product_tokens(x_ptr, y_ptr, element, tokens, k, n, weight_ptr, wei
     """int8 InnerProduct of x [tokens][k] with a scale for each token, found in it, and one for each of the n channels: weight is
     int8 [n][weight_pitch or k], weight_steps fp32 [n], y [tokens][n] of x's type (ncnn_b200_op_inner_product_tokens)."""
     L = load_library()
+    _stall_as_asked(L)
     st = L.ncnn_b200_op_inner_product_tokens(x_ptr, y_ptr, _of(ELEMENT_TYPES, element, "element"), tokens, k, n, x_pitch, y_pitch, weight_ptr,
                                              weight_pitch, weight_steps_ptr, bias_ptr, _of(OP_ACTIVATIONS, activation, "activation"),
                                              workspace_ptr, workspace_bytes, stream)
