@@ -7,7 +7,7 @@
 // * 16-bit elements: x = X 2^e with X below 2^11, top = A 2^f.  127 x / top differs from every half that it does not equal by
 //   1 / (2 A 2^(f - e)) = |127 x / top| / (254 X) or more: 2^-19 of itself.  The factor 127 / top is taken 2^-21 too large (its two
 //   roundings are 2^-23): halves go up, away from zero on either side, and nothing else passes one.
-// * fp32 elements: the product is good to 127 2^-22 < 2^-14; where it is that near to a half, the quotient is taken in 64 bits.
+// * fp32 elements: the product is good to 127 2^-24 < 2^-17; where it is that near to a half, the quotient is taken in 64 bits.
 //   (Halves are 2^-33 of a quotient away or more: 127 x is exact in 64 bits, and the quotient's rounding 2^-53.)
 #pragma once
 
