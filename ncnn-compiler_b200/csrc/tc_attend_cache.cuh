@@ -268,9 +268,8 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
       // no copy may be under way when the CTA's shared memory is given back
       if (lane == 0) {
         const int before_last = issued > Shape::kQueue ? issued - Shape::kQueue : 0;
-        for (int u = before_last; u < issued; ++u)
-          for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&brought[u % Shape::kQueue]), (u / Shape::kQueue) & 1); ++tries) {
-          }
+        int nobody = 0;
+        for (int u = before_last; u < issued; ++u) mbar_wait_bounded(smem_u32(&brought[u % Shape::kQueue]), (u / Shape::kQueue) & 1, &nobody, 200000000ull);
       }
     } else if (blocks > 0) {
       // ---- MMAs

@@ -41,9 +41,9 @@ constexpr int kTokFewThreads = 320;  // warps: 0 loads, 1 MMAs, 2 to 5 and 6 to 
 
 // Loads in flight at a ring's end: none may be when the CTA's shared memory is given back.
 __device__ __forceinline__ void ring_landed(const uint64_t* full, int stages, int issued) {
+  int nobody = 0;  // (whoever gave up: these are waited for, 0.2 s at most)
   for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
-    for (int tries = 0; tries < 1 << 20 && !ptx::mbar_try_wait(ptx::smem_u32(full + j % stages), (j / stages) & 1); ++tries) {
-    }
+    ptx::mbar_wait_bounded(ptx::smem_u32(full + j % stages), (j / stages) & 1, &nobody, 200000000ull);
 }
 
 __device__ __forceinline__ void store_cluster(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
