@@ -330,7 +330,8 @@ int ncnn_b200_op_cache_read(const ncnn_b200_cache *cache, const ncnn_b200_cache_
  * kv_heads and query head h reads key head h / (heads / kv_heads); scale 0 = 1 / sqrt(head_dim); strides as above, of q and of o.
  * shared: the first `shared` positions (a multiple of page_size) of every sequence lie in the pages that the table's first row names;
  * they are read once for all sequences.  0: none.  A token that has no key gets zeros.  Results do not depend on which other
- * sequences are in the batch beyond the order of sums.  Values of tokens should be below 2^110.
+ * sequences are in the batch, nor on `shared`, beyond the order of sums: 16-bit types hold probabilities in 16 bits whatever the
+ * batch, f32 in 24.  Values of tokens should be below 2^110.
  * workspace: device memory at a multiple of 16 bytes, of as many bytes as ncnn_b200_op_cache_attention_workspace says for the same
  * cache, batch, heads and shared (0: none is needed; negative: the call would be refused); calls that may overlap need one each. */
 int64_t ncnn_b200_op_cache_attention_workspace(const ncnn_b200_cache *cache, const ncnn_b200_cache_batch *batch, int32_t heads,

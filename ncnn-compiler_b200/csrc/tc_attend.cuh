@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t exp_pair(uint32_t x, uint32_t y, uint64_t c2
 // eighteenth of bf16's half step, degree 4 to 2^-18.  x is held to -127, where the exponent's bits are 0 and the term is exactly 0,
 // as ex2 has it for a term below 2^-126: keys of score minus infinity add nothing, and a row of them has the sum 0.  A NaN stays one.
 template <class T>
-__device__ __forceinline__ uint64_t exp_pair_fma_value(uint32_t x, uint32_t y, uint64_t c2, uint64_t from2) {
+__device__ __forceinline__ uint32_t exp_pair_fma(uint32_t x, uint32_t y, uint64_t c2, uint64_t from2, uint64_t& sums) {
   auto both = [](float v) { return f32x2_make(__float_as_uint(v), __float_as_uint(v)); };
   float2 t = f32x2_get(f32x2_fma3(f32x2_make(x, y), c2, from2));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.x) : "f"(-127.0f));
@@ -155,11 +155,6 @@ __device__ __forceinline__ uint64_t exp_pair_fma_value(uint32_t x, uint32_t y, u
   const uint64_t power = f32x2_make((__float_as_uint(w.x) << 23) + 0x3f800000u, (__float_as_uint(w.y) << 23) + 0x3f800000u);
   uint64_t e;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(e) : "l"(p), "l"(power));
-  return e;
-}
-template <class T>
-__device__ __forceinline__ uint32_t exp_pair_fma(uint32_t x, uint32_t y, uint64_t c2, uint64_t from2, uint64_t& sums) {
-  const uint64_t e = exp_pair_fma_value<T>(x, y, c2, from2);
   f32x2_add(sums, sums, e);
   const float2 r = f32x2_get(e);
   return pack2<T>(r.x, r.y);

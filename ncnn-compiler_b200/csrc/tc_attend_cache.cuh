@@ -7,15 +7,18 @@
 // products and its scores of the next block are made, so that a softmax never waits for the MMAs (one buffer for whole blocks: 4420
 // clocks a block, 3290 of them in the softmax).
 // Integers are exact in 16 bits, so that keys and values are converted as they are and the steps ks, vs of a key meet its column in the
-// softmax.  P is rounded to bf16, whose range holds any step; f16 results take a second bf16 term of P (16 bits) and a second product.
+// softmax.  P goes in as two bf16 terms (16 bits, and a range that holds any step) and two products, as in the kernel for few rows: which of
+// the two a call takes, by the largest number of rows in its batch or by a shared prefix, does not show in its results.
 //
 // Roles: warp 6 brings blocks, 16 keys of a page to a bulk copy, into a ring of three; warps 0 to 5 convert them (16 bytes to 32) and
 // store them as TMA would with a 128-byte swizzle, keys and values in turn, in a second ring of three; warp 7 issues the MMAs; warps
 // 8 to 11 are tile 0's softmax, 12 to 15 tile 1's.  256 rows to a CTA share a conversion.
 //
-// Bound: shared memory.  A block's MMAs (two tiles, 2048 clocks) read 256 KB of operands, converting moves 128 KB and every softmax warp
-// reads the steps: some 3600 clocks at 128 bytes a clock, 4400 to 5000 measured.  Pieces of up to 2048 tokens of 4 sequences behind up to
-// 4096, 32 heads on 8 of 128, bf16: 397 us, 682 TFLOP/s; f16, with its second term, 464.
+// Bound: shared memory.  A block's MMAs (two tiles, 3072 clocks) read 320 KB of operands, converting moves 128 KB and every softmax warp
+// reads the steps: some 4100 clocks at 128 bytes a clock.  Pieces of up to 2048 tokens of 4 sequences behind up to 4096, 32 heads on 8 of 128:
+// bf16 457 us, 592 TFLOP/s, f16 465, which is 111 blocks to an SM of some 7500 clocks, the ends of the longest CTAs among them (with P
+// rounded once to bf16 404 us, but results 2.3e-3 off where their own rounding makes 1.7e-3; with every eighth pair of exponentials on the FMA
+// pipe, as tc_attend.cuh has them, 463 and 471, every fourth 473 and 485).
 #pragma once
 
 #include "attend_cache.cuh"
@@ -288,14 +291,14 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
           }
           tc_commit(smem_u32(&s_full[t][h]));
         };
-        // four steps of 16 keys; f16's second terms lie 32 columns behind the first
+        // four steps of 16 keys; the second terms lie 32 columns behind the first
         auto products = [&](int t, int slot, int h, bool first_ones) {
           const uint32_t v_at = ring + static_cast<uint32_t>(slot) * kTile + h * 8192;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint64_t v = smem_desc_mnmajor(v_at + i * 2048, kPanel, 1024);
             mma_f16_ts(o_of(t), s_of(t) + 64u * h + 8u * i, v, pv_idesc, !first_ones || i > 0);
-            if (HALF) mma_f16_ts(o_of(t), s_of(t) + 64u * h + 32u + 8u * i, v, pv_idesc, 1u);
+            mma_f16_ts(o_of(t), s_of(t) + 64u * h + 32u + 8u * i, v, pv_idesc, 1u);
           }
           tc_commit(smem_u32(&o_done[t]));
         };
@@ -455,13 +458,8 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
             const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              uint64_t both;
-              if (ALL && !HALF && (i + e) % 4 == 3) {  // every fourth pair on the FMA pipe: see tc_attend.cuh
-                both = exp_pair_fma_value<__nv_bfloat16>(s[at + 2 * e], s[at + 2 * e + 1], c2, from2);
-              } else {
-                const float2 x = f32x2_get(f32x2_fma3(f32x2_make(s[at + 2 * e], s[at + 2 * e + 1]), c2, from2));
-                both = f32x2_make(__float_as_uint(exp2_fast(x.x)), __float_as_uint(exp2_fast(x.y)));
-              }
+              const float2 x = f32x2_get(f32x2_fma3(f32x2_make(s[at + 2 * e], s[at + 2 * e + 1]), c2, from2));
+              const uint64_t both = f32x2_make(__float_as_uint(exp2_fast(x.x)), __float_as_uint(exp2_fast(x.y)));
               f32x2_add(sums[e], sums[e], both);
               float2 y = f32x2_get(f32x2_mul(both, f32x2_make(vs[2 * e], vs[2 * e + 1])));
               if (!ALL) {  // (the step of a key that takes no part may be anything)
@@ -469,11 +467,11 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
                 if (s[at + 2 * e + 1] == 0xff800000u) y.y = 0.0f;
               }
               hi[i + e] = pack2<__nv_bfloat16>(y.x, y.y);
-              if (HALF) lo[i + e] = pack2<__nv_bfloat16>(y.x - __uint_as_float(hi[i + e] << 16), y.y - __uint_as_float(hi[i + e] & 0xffff0000u));
+              lo[i + e] = pack2<__nv_bfloat16>(y.x - __uint_as_float(hi[i + e] << 16), y.y - __uint_as_float(hi[i + e] & 0xffff0000u));
             }
           }
           tmem_st8(s_half + 8u * w, hi);
-          if (HALF) tmem_st8(s_half + 32u + 8u * w, lo);
+          tmem_st8(s_half + 32u + 8u * w, lo);
         }
         tmem_st_wait();
         tc_fence_before_sync();

@@ -1,0 +1,56 @@
+"""How exact the operators of a decoder in 8-bit integers are, whichever kernel a call takes: attention's probabilities."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_decoder_ops import KIND, TINY, U, Setup, assert_within, attend, cache_attend_want, gen, normal  # noqa: E402
+
+
+def close(s, q, o, element):
+    """16-bit types: probabilities in 16 bits (2^-16 of the spread, which is the tolerance of f16 without its own rounding), whatever is
+    in the batch; then one rounding to the type."""
+    want, bound = cache_attend_want(s, q, 1 / math.sqrt(s.d), "f16")
+    return want, bound + U[element] * (want.abs() + bound) + TINY[element]
+
+
+def run(pkg, s, q, element, shared=0):
+    o = torch.zeros_like(q)
+    attend(pkg, s, q, o, element, q.shape[1], shared)
+    pkg.op_check_status()
+    return o
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+@pytest.mark.parametrize("new,lens,heads,kv_heads,d,shared", [
+    ([1, 1, 1], [700, 33, 2000], 32, 8, 128, 0), ([150, 40], [900, 333], 8, 2, 128, 0), ([300], [1500], 4, 4, 64, 0), ([1] * 70, [600 + i for i in range(70)], 8, 1, 128, 512),
+    ([100, 1], [400, 3000], 16, 4, 72, 0), ([3], [800], 64, 1, 128, 0)])
+def test_probabilities_are_held_in_16_bits(pkg, element, new, lens, heads, kv_heads, d, shared):
+    s = Setup(pkg, new, lens, kv_heads, d, 16, shared=shared)
+    q = normal(gen(3), s.tokens, heads, d).to(KIND[element])
+    o = run(pkg, s, q, element, shared)
+    assert_within(o, *close(s, q, o, element))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+@pytest.mark.parametrize("shared", [0, 512])
+def test_a_step_is_as_exact_beside_a_prompt_or_behind_a_prefix(pkg, element, shared):
+    """The same decoding steps alone and beside a sequence of many new tokens, which takes the batch to the tiles of many rows."""
+    lens, heads, kv_heads, d = [900, 700, 2100], 16, 4, 128
+    q = normal(gen(5), 103, heads, d).to(KIND[element])
+    beside = Setup(pkg, [1, 1, 1, 100], lens + [760], kv_heads, d, 16, shared=shared, seed=7)
+    wide = run(pkg, beside, q, element, shared)
+    assert_within(wide, *close(beside, q, wide, element))
+    # the steps alone, over the same pages
+    alone = Setup(pkg, [1, 1, 1], lens, kv_heads, d, 16, seed=7)
+    alone.ints, alone.steps, alone.whole, alone.table, alone.pages = beside.ints, beside.steps, beside.whole[:3], beside.table[:3].contiguous(), beside.pages
+    alone.table[:, :shared // 16] = alone.table[0, :shared // 16]
+    alone.cache = beside.cache
+    alone.batch = pkg.CacheBatch(alone.table.data_ptr(), alone.len_t.data_ptr(), alone.starts.data_ptr(), 3, 3, alone.table.shape[1], 1, max(lens))
+    few = run(pkg, alone, q[:3].contiguous(), element)
+    want, bound = close(alone, q[:3], few, element)
+    assert_within(few, want, bound)
+    assert_within(wide[:3], want, bound)
