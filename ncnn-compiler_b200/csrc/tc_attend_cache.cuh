@@ -16,7 +16,7 @@
 //
 // Bound: shared memory.  A block's MMAs (two tiles, 3072 clocks) read 320 KB of operands, converting moves 128 KB and every softmax warp
 // reads the steps: some 4100 clocks at 128 bytes a clock.  Pieces of up to 2048 tokens of 4 sequences behind up to 4096, 32 heads on 8 of 128:
-// bf16 457 us, 592 TFLOP/s, f16 465, which is 111 blocks to an SM of some 7500 clocks, the ends of the longest CTAs among them (with P
+// bf16 460 us, 588 TFLOP/s, f16 471, which is 111 blocks to an SM of some 7500 clocks, the ends of the longest CTAs among them (with P
 // rounded once to bf16 404 us, but results 2.3e-3 off where their own rounding makes 1.7e-3; with every eighth pair of exponentials on the FMA
 // pipe, as tc_attend.cuh has them, 463 and 471, every fourth 473 and 485).
 #pragma once
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
   constexpr bool HALF = std::is_same<T, __half>::value;
   extern __shared__ uint8_t cache_smem[];
   __shared__ __align__(8) uint64_t brought[Shape::kQueue], taken[Shape::kQueue];
-  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2][2], p_full[2][2], o_done[2], o_full[2], drained;
+  __shared__ __align__(8) uint64_t q_full, full[kSlots], empty[kSlots], steps_full[kSteps], s_full[2][2], p_full[2][2], o_done[2][2], o_full[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag, pages_there[kSteps];
   const AttendCacheParams& a = p.a;
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
       for (int h = 0; h < 2; ++h) {
         mbar_init(smem_u32(&s_full[t][h]), 1);
         mbar_init(smem_u32(&p_full[t][h]), 4);
+        mbar_init(smem_u32(&o_done[t][h]), 1);
       }
-      mbar_init(smem_u32(&o_done[t]), 1);
       mbar_init(smem_u32(&o_full[t]), 1);
     }
     fence_mbar_init();
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
             mma_f16_ts(o_of(t), s_of(t) + 64u * h + 8u * i, v, pv_idesc, !first_ones || i > 0);
             mma_f16_ts(o_of(t), s_of(t) + 64u * h + 32u + 8u * i, v, pv_idesc, 1u);
           }
-          tc_commit(smem_u32(&o_done[t]));
+          tc_commit(smem_u32(&o_done[t][h]));
         };
         ok = ok && wait_use(0, 0);
         if (ok) {
@@ -429,9 +429,8 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
           base = next;
           total *= keep;
           if (j > 0 || h > 0) {
-            // The products of all halves before this one are in O.  (Those of the half before the last one are, since these scores came
-            // after them: the barrier is in the last one's phase, or past it.)
-            ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_done[t]), (h ^ 1) & 1, abort_ptr, p.wait_ns));
+            // the products of the half before this one are in O, and with them all others
+            ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_done[t][h ^ 1]), (j + h + 1) & 1, abort_ptr, p.wait_ns));
             if (!ok) return;
             tc_fence_after_sync();
 #pragma unroll
@@ -487,7 +486,10 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         const int there = ok ? pages_there[j % kSteps] : 0;
         const bool whole = there == 0xff && key0 + 127 <= least && key0 + 127 < to;
         for (int h = 0; ok && h < 2; ++h) {
-          ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&s_full[t][h]), j & 1, abort_ptr, p.wait_ns));
+          // The products before these scores have ended, too; asked for so that no phase of their barrier is passed over: a parity
+          // says only which of two neighbouring phases it is in.
+          ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&s_full[t][h]), j & 1, abort_ptr, p.wait_ns) &&
+                                   (j == 0 || mbar_wait_bounded(smem_u32(&o_done[t][h]), (j - 1) & 1, abort_ptr, p.wait_ns)));
           if (!ok) break;
           tc_fence_after_sync();
           if (whole) half(j, h, std::true_type{}, there);
@@ -495,7 +497,6 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
         }
       }
       if (ok && blocks > 0) {
-        // (not o_done: by now that may be in the phase after the last, which nothing ends)
         ok = __all_sync(~0u, mbar_wait_bounded(smem_u32(&o_full[t]), 0, abort_ptr, p.wait_ns));
         tc_fence_after_sync();
       }

@@ -54,3 +54,21 @@ def test_a_step_is_as_exact_beside_a_prompt_or_behind_a_prefix(pkg, element, sha
     want, bound = close(alone, q[:3], few, element)
     assert_within(few, want, bound)
     assert_within(wide[:3], want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("count,shared", [(100, 0), (300, 0), (90, 1024)])
+def test_maxima_that_rise_with_every_key(pkg, element, d, count, shared):
+    """The results so far are scaled down before every half block: behind the products that are under way, each time."""
+    s = Setup(pkg, [count] * 3, [1500, 1400, 1300 + count], 2, d, 16, shared=shared)
+    s.ints["k"].fill_(100)
+    for i, n in enumerate(s.lens):
+        keys = torch.arange(n, device="cuda")
+        # a score of 10 more with every 64 keys (2^14 in the probability), for the smallest query
+        s.steps["k"][s.whole[i].long()[keys // 16], :, keys % 16] = (10 / 64 * keys / (100 * math.sqrt(d)))[:, None]
+    q = (1 + normal(gen(6), s.tokens, 8, 1).abs() / 4).expand(-1, -1, d).contiguous().to(KIND[element])
+    first = run(pkg, s, q, element, shared)
+    assert_within(first, *close(s, q, first, element))
+    assert all(torch.equal(first, run(pkg, s, q, element, shared)) for _ in range(20))
