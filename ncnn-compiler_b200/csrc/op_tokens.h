@@ -29,13 +29,23 @@ __device__ __forceinline__ float tokens_sum(int sum, float step, float weight_st
 }
 // Called, not inlined: results leave in unrolled loops, which a copy of these for every value makes too long for the instruction
 // cache (64 tokens through 4096 x 11008, no activation: 5400 of a tile's 28000 clocks went into the last 16 values of each thread).
-template <class T>
+// Swish by the exponential of -|t|: that of -t passes fp32's largest number where t e^t is still far from its smallest.
 __device__ __noinline__ float tokens_activate(float t, int act) {
-  if (act == NCNN_B200_ACT_SWISH) return t / (1.0f + expf(-t));
+  if (act == NCNN_B200_ACT_SWISH) {
+    const float e = expf(-fabsf(t));
+    return t * ((t < 0.0f ? e : 1.0f) / (1.0f + e));
+  }
   return 0.5f * t * erfcf(t * -0.7071067811865476f);
 }
+// Swish for 16-bit results: good to (5 + 1.2 |t|) 2^-23, most of it the fast exponential's, whose error grows with its argument; 2^-16
+// where results pass fp32's smallest number.
+__device__ __forceinline__ float tokens_swish16(float t) {
+  const float e = __expf(-fabsf(t));
+  return t * __fdividef(t < 0.0f ? e : 1.0f, 1.0f + e);
+}
 // GELU for 16-bit results: erfc(z) = exp(-z^2) u P(u) with u = 1 / (1 + 0.65 z), P of degree 5 fitted to erfcx in equal relative
-// error over z from 0 to 9.6 (2^-16.8; with the exponential and the reciprocal, 2^-16), where erfc(z) passes fp32's smallest number.
+// error over z from 0 to 9.6 (2^-16.8; with the exponential, whose error grows with z^2, and the reciprocal, 2^-16 down to t = -10 and 2^-15
+// below), where erfc(z) passes fp32's smallest number.
 __device__ __forceinline__ float tokens_gelu16(float t) {
   const float z = fabsf(t) * 0.7071067811865476f;
   const float u = __fdividef(1.0f, fmaf(0.65f, z, 1.0f));
@@ -64,9 +74,9 @@ __device__ __forceinline__ T tokens_result(LOOP, int sum, float step, float weig
     const float least = act == NCNN_B200_ACT_RELU ? 0.0f : -INFINITY;
     return op_put<T>(t < least ? least : t);  // (a NaN stays one)
   }
-  if constexpr (LOOP::value == Loop::kSwish) return op_put<T>(__fdividef(t, 1.0f + __expf(-t)));  // (good to 2^-20)
+  if constexpr (LOOP::value == Loop::kSwish) return op_put<T>(tokens_swish16(t));
   if constexpr (LOOP::value == Loop::kGelu) return op_put<T>(tokens_gelu16(t));
-  return op_put<T>(tokens_activate<T>(t, act));
+  return op_put<T>(tokens_activate(t, act));
 }
 
 }  // namespace nb

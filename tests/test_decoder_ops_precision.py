@@ -72,3 +72,29 @@ def test_maxima_that_rise_with_every_key(pkg, element, d, count, shared):
     first = run(pkg, s, q, element, shared)
     assert_within(first, *close(s, q, first, element))
     assert all(torch.equal(first, run(pkg, s, q, element, shared)) for _ in range(20))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_swish_of_numbers_far_below_zero(pkg, element, m):
+    """Sums from 0 to -104: the results are numbers of their type down to its smallest one.  A sum of one product is known to the bit, so that
+    what is off is the activation alone: fp32's exponential by a step and three roundings (8 F as elsewhere), the fast one by 2 + 1.173 |t|
+    steps of 2 F, its quotient by 2; of what is below fp32's smallest normal number a step, twice, times |t|."""
+    F, k, n = 2.0 ** -24, 16, 64
+    x = torch.zeros(m, k, device="cuda")
+    x[:, 0] = 1.0
+    w = torch.zeros(n, k, dtype=torch.int8, device="cuda")
+    w[:, 0] = -127
+    for top in (104.0, 10.0, 1.0):
+        ws = torch.linspace(0.0, top / 127, n, device="cuda")
+        y = torch.full((m, n), 5.0, device="cuda").to(KIND[element])
+        space = torch.empty(pkg.op_inner_product_tokens_workspace(m, k), dtype=torch.uint8, device="cuda")
+        pkg.op_inner_product_tokens(x.to(KIND[element]).data_ptr(), y.data_ptr(), element, m, k, n, w.data_ptr(), ws.data_ptr(), space.data_ptr(), space.numel(),
+                                    activation="swish")
+        torch.cuda.synchronize()
+        step = torch.ones(1, device="cuda") / 127
+        t = (torch.tensor(-127.0 * 127.0, device="cuda") * (step * ws)).double()
+        want = t * torch.sigmoid(t)
+        off = want.abs() * 2 * F * (4 if element == "f32" else 5 + 1.2 * t.abs()) + 2 * t.abs() * 2.0 ** -149
+        assert_within(y, want.expand(m, n), (off + U[element] * (want.abs() + off) + TINY[element]).expand(m, n))
