@@ -52,6 +52,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
                : "memory");
 }
 
+// `bytes` that a barrier expects and nobody will bring
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -104,6 +109,20 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
       else if (now - t0 > limit_ns) return false;
     }
   }
+}
+
+// Waits for the last phases of a ring of `slots` barriers of which `uses` are under way or past, 0.2 s at most for all of them together:
+// no copy may be in flight when a CTA's shared memory is given back, whoever gave up.
+__device__ __forceinline__ void ring_landed(const uint64_t* full, int slots, int uses) {
+  uint64_t t0 = 0;
+  uint32_t polls = 0;
+  for (int u = uses > slots ? uses - slots : 0; u < uses; ++u)
+    while (!mbar_try_wait(smem_u32(full + u % slots), (u / slots) & 1)) {
+      if ((++polls & 0x3ffu) != 0) continue;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 200000000ull) return;
+    }
 }
 
 // --------------------------------------------------------------------- TMA

@@ -269,11 +269,7 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
       }
       if (!ok && p.stall == 0 && lane == 0) gave_up();
       // no copy may be under way when the CTA's shared memory is given back
-      if (lane == 0) {
-        const int before_last = issued > Shape::kQueue ? issued - Shape::kQueue : 0;
-        int nobody = 0;
-        for (int u = before_last; u < issued; ++u) mbar_wait_bounded(smem_u32(&brought[u % Shape::kQueue]), (u / Shape::kQueue) & 1, &nobody, 200000000ull);
-      }
+      if (lane == 0) ring_landed(brought, Shape::kQueue, issued);
     } else if (blocks > 0) {
       // ---- MMAs
       if (elect_one()) {

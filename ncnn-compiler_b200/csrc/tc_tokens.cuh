@@ -33,18 +33,11 @@ struct TcTokensParams {
   int tiles_t, tiles_c;
   int stage_bytes;
   int stored;       // pair: results leave through TMA
-  int stall;        // tests of the time-out path: nothing is ever loaded
+  int stall;        // tests of the time-out path: nothing is ever loaded (pair: by one of the CTAs, and one ring by the other)
   unsigned long long wait_ns;
 };
 
 constexpr int kTokFewThreads = 320;  // warps: 0 loads, 1 MMAs, 2 to 5 and 6 to 9 results of every second 16 tokens
-
-// Loads in flight at a ring's end: none may be when the CTA's shared memory is given back.
-__device__ __forceinline__ void ring_landed(const uint64_t* full, int stages, int issued) {
-  int nobody = 0;  // (whoever gave up: these are waited for, 0.2 s at most)
-  for (int j = issued > stages ? issued - stages : 0; j < issued; ++j)
-    ptx::mbar_wait_bounded(ptx::smem_u32(full + j % stages), (j / stages) & 1, &nobody, 200000000ull);
-}
 
 __device__ __forceinline__ void store_cluster(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -247,6 +240,15 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
 
 constexpr int kTokPairThreads = 320;  // warps: 0 loads, 1 MMAs, 2 to 9 results
 
+// A pair's copies in flight after one of its CTAs gave up.  They are counted on CTA 0's barriers, for both CTAs: of K blocks that only one
+// of the two asked for, the other's part is made good, or the barrier's phase would never end.  (In a slot of the ring that can only be
+// the last use: the one before has ended when either CTA goes on.)
+__device__ __forceinline__ void pair_landed(const uint64_t* full, int stages, uint32_t stage_bytes, int uses0, int uses1) {
+  for (int u = uses0; u < uses1; ++u) ptx::mbar_arrive_expect_tx(ptx::smem_u32(full + u % stages), stage_bytes);
+  for (int u = uses1; u < uses0; ++u) ptx::mbar_complete_tx(ptx::smem_u32(full + u % stages), stage_bytes);
+  ptx::ring_landed(full, stages, max(uses0, uses1));
+}
+
 template <class T>
 __global__ void __launch_bounds__(kTokPairThreads, 1)
 tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
@@ -259,6 +261,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
   __shared__ __align__(8) uint64_t drained[2];             // CTA 0's: both CTAs have read it
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ int asked, ends[2];  // K blocks that this CTA has asked for; both CTAs', less than 0 (~blocks) where one gave up
   const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -300,6 +303,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
       const int half = p.columns / 2;
       int issued = 0;  // K blocks of all tiles
       bool ok = p.stall == 0;
+      const bool begins = ok || static_cast<uint32_t>(pair & 1) == rank;
       // (counters are stepped: a block's divisions took 900 clocks, its MMAs take 512)
       int s = 0;
       uint32_t ph = 0;
@@ -311,7 +315,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
       // the first ring of weights, and when the kernel before has ended, its tokens
       int tile = pair, kb = 0, c0 = 0, t0 = 0;
       rows_of(tile, &c0, &t0);
-      for (int pass = 0; ok && pass < 2; ++pass) {
+      for (int pass = 0; begins && pass < 2; ++pass) {
         if (pass == 1) grid_dependency_wait();
         tile = pair;
         kb = 0;
@@ -348,7 +352,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
           }
         }
       }
-      if (rank == 0) ring_landed(full, S, issued);  // (CTA 1's bytes are counted there too, and it waits for CTA 0 below)
+      asked = issued;
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -486,11 +490,23 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
     if (!ok && lane == 0) gave_up();
     if (p.stored && lane == 0) bulk_wait_read();
   }
-  // Neither CTA leaves while the other may signal its barriers or read its shared memory.
+  // Neither CTA leaves while the other may signal its barriers or read its shared memory, or while copies are in flight: where nobody gave up
+  // the MMAs have waited for all of them.
   tc_fence_before_sync();
   __syncthreads();
+  if (threadIdx.x == 0) {
+    const int mine = abort_flag != 0 ? ~asked : asked;
+    ends[rank] = mine;
+    store_cluster(map_to_cta(smem_u32(&ends[rank]), rank ^ 1u), static_cast<uint32_t>(mine));
+  }
+  __syncwarp();
   cluster_sync_all();
   tc_fence_after_sync();
+  if (ends[0] < 0 || ends[1] < 0) {
+    if (rank == 0 && threadIdx.x == 0) pair_landed(full, S, stage_bytes, ends[0] < 0 ? ~ends[0] : ends[0], ends[1] < 0 ? ~ends[1] : ends[1]);
+    __syncwarp();
+    cluster_sync_all();
+  }
   if (warp == 1) tmem_dealloc_pair(tmem, 512u);
 }
 
