@@ -112,7 +112,7 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
 }
 
 // Waits for the last phases of a ring of `slots` barriers of which `uses` are under way or past, 0.2 s at most for all of them together:
-// no copy may be in flight when a CTA's shared memory is given back, whoever gave up.
+// no copy (or MMA, of a ring that MMAs signal) may be under way when a CTA's memory is given back, whoever gave up.
 __device__ __forceinline__ void ring_landed(const uint64_t* full, int slots, int uses) {
   uint64_t t0 = 0;
   uint32_t polls = 0;

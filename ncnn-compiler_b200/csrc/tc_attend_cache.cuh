@@ -330,12 +330,10 @@ __global__ void __launch_bounds__(TcCacheShape<D>::kThreads, 1) tc_attend_cache_
           v_slot = k_slot == kSlots - 1 ? 0 : k_slot + 1;
           v_ph = v_slot == 0 ? k_ph ^ 1u : k_ph;
         }
-        if (!ok) {
-          gave_up();
-          tc_commit(smem_u32(&drained));  // nor may MMAs be under way
-          for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&drained), 0); ++tries) {
-          }
-        }
+        if (!ok) gave_up();
+        // MMAs under way are done before the CTA leaves, whoever gave up
+        tc_commit(smem_u32(&drained));
+        ring_landed(&drained, 1, 1);
       }
     }
   } else {

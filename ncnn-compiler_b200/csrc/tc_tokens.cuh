@@ -140,7 +140,8 @@ tc_tokens_few_kernel(const __grid_constant__ TcTokensParams p, const __grid_cons
         s = next;
       }
       if (!ok) gave_up();
-      tc_commit(smem_u32(&done));  // (also where a wait ran out: nor may MMAs be under way)
+      tc_commit(smem_u32(&done));
+      ring_landed(&done, 1, 1);  // (whoever gave up: nor may MMAs be under way when the CTA gives its memory back)
     }
   }
   __syncwarp();
@@ -259,6 +260,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
   __shared__ __align__(8) uint64_t empty[kTokStagesMost];  // in each CTA
   __shared__ __align__(8) uint64_t summed[2];              // in each CTA: an accumulator is complete
   __shared__ __align__(8) uint64_t drained[2];             // CTA 0's: both CTAs have read it
+  __shared__ __align__(8) uint64_t last;                   // CTA 0's: no MMA is under way any more
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int asked, ends[2];  // K blocks that this CTA has asked for; both CTAs', less than 0 (~blocks) where one gave up
@@ -281,6 +283,7 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
       mbar_init(smem_u32(&summed[i]), 1);
       mbar_init(smem_u32(&drained[i]), 16);
     }
+    mbar_init(smem_u32(&last), 1);
     fence_mbar_init();
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_q);
@@ -391,16 +394,10 @@ tc_tokens_pair_kernel(const __grid_constant__ TcTokensParams p, const __grid_con
         acc ^= 1;
         if (acc == 0) acc_ph ^= 1u;
       }
-      if (!ok) {
-        gave_up();
-        // MMAs under way are done before the CTAs leave
-        __shared__ __align__(8) uint64_t last;
-        mbar_init(smem_u32(&last), 1);
-        fence_mbar_init();
-        tc_commit_pair(smem_u32(&last), 1);
-        for (int tries = 0; tries < 1 << 20 && !mbar_try_wait(smem_u32(&last), 0); ++tries) {
-        }
-      }
+      if (!ok) gave_up();
+      // MMAs under way are done before the CTAs leave, whoever gave up
+      tc_commit_pair(smem_u32(&last), 1);
+      ring_landed(&last, 1, 1);
     }
   } else {
     grid_dependency_wait();
