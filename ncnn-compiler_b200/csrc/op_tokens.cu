@@ -309,7 +309,11 @@ int product_pair(TcTokensParams p, int columns, int device, int sms, cudaStream_
   if (tiles > (1 << 30)) return op_fail(NCNN_B200_STATUS_SHAPE_OVERFLOW, "op_inner_product_tokens: too many tokens");
   p.stage_bytes = 16384 + columns / 2 * 128;
   p.stages = std::min(kTokStagesMost, (192 * 1024) / p.stage_bytes);
-  p.stored = reinterpret_cast<uintptr_t>(t.y) % 16 == 0 && t.y_pitch * static_cast<long long>(sizeof(T)) % 16 == 0 && t.y_pitch < (1ll << 37) ? 1 : 0;
+  // (rows whose ends are no multiple of 16 bytes: TMA stores fill the last 16 with what lies in the box behind the row)
+  p.stored = reinterpret_cast<uintptr_t>(t.y) % 16 == 0 && t.n * static_cast<long long>(sizeof(T)) % 16 == 0 &&
+                     t.y_pitch * static_cast<long long>(sizeof(T)) % 16 == 0 && t.y_pitch < (1ll << 37)
+                 ? 1
+                 : 0;
   const int smem = p.stages * p.stage_bytes + 8 * 4096 + 1024;
   CUtensorMap map_w, map_q, map_y{};
   if (!encode_bytes(&map_w, t.weight, t.k, t.n, t.weight_pitch, columns / 2) || !encode_bytes(&map_q, t.q, t.k, t.tokens, t.q_pitch, 128)) return no_token_maps();

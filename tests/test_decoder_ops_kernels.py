@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decoder_ops import KIND, Setup, assert_within, check_product, check_rows, gen, normal, product_want, quantised, strided  # noqa: E402
+from test_decoder_ops import KIND, assert_within, check_product, gen, normal, product_want, quantised  # noqa: E402
 
 
 def up(a, b):
@@ -58,3 +58,66 @@ def test_a_wait_that_runs_out_in_each_kernel(pkg, monkeypatch, element, kernel, 
     monkeypatch.delenv("NCNN_B200_TEST_STALL")
     check_product(pkg, element, m, k, n)
     assert status(pkg) == 0
+
+
+def check(pkg, element, m, k, n, act="none", bias=True, y_pitch=0, shift=0, aligned=True):
+    """A product against the formula: results `shift` elements into their array, steps and bias at multiples of 16 bytes or not."""
+    g = gen(m + k + n)
+    yp, size = y_pitch or n, KIND[element].itemsize
+    x = normal(g, m, k).to(KIND[element])
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    y = torch.full((m * yp + shift,), 5.0, device="cuda", dtype=KIND[element])
+    at = 0 if aligned else 1
+    ws = ((normal(g, n + 1).abs() + 0.2) / (40 * k ** 0.5))[at:at + n]
+    b = normal(g, n + 1)[at:at + n] if bias else None
+    space = torch.empty(pkg.op_inner_product_tokens_workspace(m, k), dtype=torch.uint8, device="cuda")
+    pkg.op_inner_product_tokens(x.data_ptr(), y.data_ptr() + shift * size, element, m, k, n, w.data_ptr(), ws.data_ptr(), space.data_ptr(), space.numel(),
+                                None if b is None else b.data_ptr(), act, y_pitch=yp)
+    assert status(pkg) == 0
+    q, steps = quantised(x)
+    want, bound = product_want(q, steps, w, ws, b, act, element)
+    assert_within(torch.as_strided(y, (m, n), (yp, 1), shift), want, bound)
+    if yp > n:
+        assert bool((torch.as_strided(y, (m - 1, yp - n), (yp, 1), shift + n) == 5.0).all())
+    assert bool((y[:shift] == 5.0).all())
+
+
+SIZES = [(("pair", 128), 2100, 144, 4100), (("pair", 128), 2048, 2064, 3000), (("pair", 256), 3000, 272, 3000), (("pair", 256), 3000, 1040, 2960),
+         (("few", 128, 1), 1024, 272, 4096), (("few", 128, 1), 1000, 1040, 4000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "swish", "gelu"])
+@pytest.mark.parametrize("kernel,m,k,n", SIZES)
+def test_large_products(pkg, element, act, kernel, m, k, n):
+    took = product_kernel(m, k, n)
+    assert took[:len(kernel)] == kernel and (kernel[0] == "pair" or took[3] > torch.cuda.get_device_properties(0).multi_processor_count)  # (two CTAs to an SM)
+    check(pkg, element, m, k, n, act, bias=act != "none")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kernel,m,k,n", SIZES)
+def test_large_products_in_other_layouts(pkg, element, kernel, m, k, n):
+    assert product_kernel(m, k, n)[:len(kernel)] == kernel
+    check(pkg, element, m, k, n, "swish", y_pitch=n + 1)                       # (no row but the first where TMA could store it)
+    check(pkg, element, m, k, n, "gelu", y_pitch=n + (-n) % 8 + 24)            # (TMA stores into the pitch's rows, not between them)
+    check(pkg, element, m, k, n, "none", shift=1)
+    check(pkg, element, m, k, n, "relu", aligned=False)
+    check(pkg, element, m, k, n, "none", y_pitch=n + 3, shift=3, aligned=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel,m,k,n", SIZES)
+def test_large_products_of_tokens_that_are_no_numbers(pkg, kernel, m, k, n):
+    x = normal(gen(m), m, k).bfloat16()
+    bad = [0, 127, 128, 255, 256, m - 1]
+    x[bad, 3] = float("inf")
+    w, ws = torch.randint(-127, 128, (n, k), generator=gen(1), device="cuda", dtype=torch.int8), torch.full((n,), 1e-3, device="cuda")
+    y, space = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16), torch.empty(pkg.op_inner_product_tokens_workspace(m, k), dtype=torch.uint8, device="cuda")
+    for act in ("none", "relu", "swish", "gelu"):
+        pkg.op_inner_product_tokens(x.data_ptr(), y.data_ptr(), "bf16", m, k, n, w.data_ptr(), ws.data_ptr(), space.data_ptr(), space.numel(), activation=act)
+        assert status(pkg) == 0
+        rows = torch.isnan(y)
+        assert bool(rows[bad].all()) and int(rows.any(1).sum()) == len(bad)
