@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decoder_ops import KIND, assert_within, check_product, gen, normal, product_want, quantised  # noqa: E402
+from test_decoder_ops import KIND, Setup, assert_within, check_product, check_rows, gen, normal, product_want, quantised, strided  # noqa: E402
 
 
 def up(a, b):
@@ -121,3 +121,76 @@ def test_large_products_of_tokens_that_are_no_numbers(pkg, kernel, m, k, n):
         assert status(pkg) == 0
         rows = torch.isnan(y)
         assert bool(rows[bad].all()) and int(rows.any(1).sum()) == len(bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,columns", [(2048, 8), (2049, 4096), (5000, 1000), (3001, 2048), (2050, 4104), (2048, 520)])
+def test_many_rows_to_integers(pkg, element, rows, columns):
+    """From 2048 rows on a warp takes a row that it can keep (4096 columns, 2048 of f32)."""
+    g = gen(rows + columns)
+    x = (normal(g, rows, columns) * normal(g, columns).abs()).to(KIND[element])
+    x[5], x[rows - 1, 0], x[rows - 2, columns - 1], x[7, 0] = 0.0, float("nan"), float("-inf"), torch.finfo(KIND[element]).max
+    check_rows(pkg, x, element)
+    check_rows(pkg, x, element, columns + 24, 8)
+
+
+def places(s):
+    """Row, page (-1: none) and row of the page of every token, as tensors."""
+    rows, pages, at = [], [], []
+    for i, count in enumerate(s.new):
+        j = torch.arange(count, device="cuda")
+        position = s.lens[i] - count + j
+        page = s.whole[i].long()[(position // s.page).clamp_min(0)]
+        rows.append(s.firsts[i] + j)
+        pages.append(torch.where((position >= 0) & (page >= 0) & (page < s.pages), page, -1))
+        at.append(position % s.page)
+    return torch.cat(rows), torch.cat(pages), torch.cat(at)
+
+
+def check_many_rows(pkg, element, s, strides=None, shift=0):
+    g = gen(1)
+    kind, size = KIND[element], KIND[element].itemsize
+    four = None if strides is None else (*strides, *strides)
+    rows, pages, at = places(s)
+    there = pages >= 0
+    src = {n: strided(g, kind, s.tokens, s.kv_heads, s.d, strides, shift) for n in "kv"}
+    want = {n: (s.ints[n].clone(), s.steps[n].clone()) for n in "kv"}
+    for n in "kv":
+        q, steps = quantised(src[n][1][rows[there]])
+        want[n][0][pages[there], :, at[there]] = torch.nn.functional.pad(q, (0, s.row - s.d))
+        want[n][1][pages[there], :, at[there]] = steps
+    pkg.op_cache_write(s.cache, s.batch, src["k"][0].data_ptr() + shift * size, src["v"][0].data_ptr() + shift * size, element, four)
+    torch.cuda.synchronize()
+    for n in "kv":
+        assert torch.equal(s.ints[n], want[n][0]) and torch.equal(torch.nan_to_num(s.steps[n], nan=-1.0), torch.nan_to_num(want[n][1], nan=-1.0))
+    for names in ("kv", "k", "v"):
+        out = {n: strided(g, kind, s.tokens, s.kv_heads, s.d, strides, shift) for n in names}
+        for n in names:
+            view = torch.as_strided(want_out := out[n][0].clone(), out[n][1].shape, out[n][1].stride(), shift)
+            view[rows] = torch.where(there[:, None, None], (s.ints[n][pages, :, at, :s.d].float() * s.steps[n][pages, :, at][..., None]).to(kind), 0.0)
+            out[n] = (*out[n], want_out)
+        pkg.op_cache_read(s.cache, s.batch, *((out[n][0].data_ptr() + shift * size if n in out else None) for n in "kv"), element, four)
+        torch.cuda.synchronize()
+        for n in names:
+            assert torch.equal(out[n][0], out[n][2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kv_heads,d,page,strides,shift", [(8, 128, 64, None, 0), (3, 72, 16, None, 0), (6, 64, 32, (400, 64), 8), (5, 200, 16, None, 0), (7, 33, 16, None, 1),
+                                                          (2, 128, 128, (300, 137), 3), (6, 40, 16, (40, 40 * 30000), 0)])
+def test_many_rows_of_a_cache(pkg, element, kv_heads, d, page, strides, shift):
+    """Four heads to a lane, where keys or values alone fill the device: the ends of heads, tokens, pages and pieces of rows."""
+    row = (d + 15) // 16 * 16
+    most = 4096 * torch.cuda.get_device_properties(0).multi_processor_count
+    tokens = up(most, kv_heads * row // 8) + 77
+    new = [tokens // 2, 0, 1, tokens // 3, tokens - tokens // 2 - tokens // 3 - 1]
+    lens = [new[0] + 1000, 5, 40, new[3] - 20, new[4] + 3]  # (one has more rows than tokens: the first 20 have no place)
+    s = Setup(pkg, new, lens, kv_heads, d, page, behind=5, lead=3, fill=False)
+    assert tokens * kv_heads * (row // 8) >= most
+    for bad in (-1, s.pages, 1 << 30):
+        page_of = (1000 + new[0] // 2) // page
+        s.whole[0, page_of] = s.table[0, page_of] = bad
+        s.whole[3, 0] = s.table[3, 0] = bad
+        check_many_rows(pkg, element, s, strides, shift)
