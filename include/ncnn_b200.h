@@ -260,7 +260,8 @@ int ncnn_b200_op_cross_attention(const void *q, const void *k, const void *v, vo
 
 /* ---- A decoder in 8-bit integers: products whose activations are quantised token by token, a paged cache of keys and values, and
  * attention over it.  (The reference quantises with scales known ahead; these find them in the data.)  What is said above of arrays,
- * streams and refusals holds here too.
+ * streams and refusals holds here too.  What a call writes (results, integers and steps, the workspace) must not overlap what it reads, nor
+ * each other; arrays that start at one address are refused.
  *
  * A row of numbers becomes 8-bit integers and a step:  top = max |x|, step = top / 127, q = 127 x / top rounded to the nearest whole
  * number, halves away from zero (exactly: the integers are those of real arithmetic).  A row whose top is below 2^-100 is held as

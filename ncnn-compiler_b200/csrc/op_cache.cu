@@ -140,7 +140,7 @@ cudaError_t cache_rows(const CacheRowsParams& p, bool wide, int sms, cudaStream_
 }
 
 // ------------------------------------------------------------------ arguments
-// What a cache and a batch say, checked: 0, or a status (the message is set).  `device`: -1 asks for no check of memory.
+// What a cache and a batch say, checked: 0, or a status (the message is set).
 int cache_params(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_cache_batch* batch, CacheParams* p) {
   auto bad = [&](const char* what) { return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, std::string(op) + ": " + what); };
   if (cache == nullptr || batch == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, std::string(op) + ": NULL cache or batch");
@@ -161,6 +161,8 @@ int cache_params(const char* op, const ncnn_b200_cache* cache, const ncnn_b200_c
     if (!op_starts(cache->k, 16) || !op_starts(cache->v, 16) || !op_starts(cache->k_steps, 16) || !op_starts(cache->v_steps, 16))
       return bad("the cache's arrays start at multiples of 16 bytes");
     if (!op_starts(batch->table, 4) || !op_starts(batch->lens, 4) || !op_starts(batch->starts, 4)) return bad("an array does not start at a multiple of its elements' size");
+    for (const void* ints : {cache->k, cache->v})
+      if (ints == cache->k_steps || ints == cache->v_steps) return bad("integers and steps need memory of their own");
     if (cache->k == cache->v || cache->k_steps == cache->v_steps) return bad("keys and values need memory of their own");
   }
   p->k = cache->k;
@@ -232,8 +234,11 @@ int cache_rows_call(const char* op, bool read, const ncnn_b200_cache* cache, con
     if (p.c.tokens == 0 || p.c.sequences == 0) return NCNN_B200_STATUS_SUCCESS;
     if (read ? k == nullptr && v == nullptr : k == nullptr || v == nullptr) return op_fail(NCNN_B200_STATUS_NULL_POINTER, std::string(op) + ": NULL argument");
     if (!op_starts(k, size) || !op_starts(v, size)) return bad("an array does not start at a multiple of its elements' size");
-    for (const void* a : {static_cast<const void*>(k), static_cast<const void*>(v)})
-      if (a != nullptr && (a == p.c.k || a == p.c.v || a == p.c.k_steps || a == p.c.v_steps)) return bad("the arrays must not lie over the cache");
+    for (const void* a : {static_cast<const void*>(k), static_cast<const void*>(v)}) {
+      if (a == nullptr) continue;
+      if (a == p.c.k || a == p.c.v || a == p.c.k_steps || a == p.c.v_steps) return bad("the arrays must not lie over the cache");
+      if (a == p.c.table || a == p.c.lens || a == p.c.starts) return bad("the arrays must not lie over the batch's");
+    }
     if (read && k == v) return bad("keys and values need memory of their own");
     p.k = k;
     p.v = v;
@@ -429,8 +434,10 @@ extern "C" int ncnn_b200_op_cache_attention(const ncnn_b200_cache* cache, const 
     if (!op_starts(q, size) || !op_starts(o, size) || !op_starts(workspace, 16))
       return bad("an array does not start at a multiple of its elements' size (workspace: of 16 bytes)");
     for (const void* a : {static_cast<const void*>(p.c.k), static_cast<const void*>(p.c.v), static_cast<const void*>(p.c.k_steps),
-                          static_cast<const void*>(p.c.v_steps), q, static_cast<const void*>(workspace)})
-      if (a == o) return bad("the result must not lie over an input");
+                          static_cast<const void*>(p.c.v_steps), static_cast<const void*>(p.c.table), static_cast<const void*>(p.c.lens),
+                          static_cast<const void*>(p.c.starts), q})
+      if (a != nullptr && (a == o || a == workspace)) return bad("the result and the workspace must not lie over an input");
+    if (o == workspace) return bad("the result and the workspace must not lie over each other");
     std::string why;
     const int device = op_common_device(kOp, {q, o, p.c.k, p.c.v, p.c.k_steps, p.c.v_steps, p.c.table, p.c.lens, p.c.starts, workspace}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);

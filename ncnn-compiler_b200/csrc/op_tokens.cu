@@ -430,8 +430,9 @@ extern "C" int ncnn_b200_op_inner_product_tokens(const void* x, void* y, int32_t
       return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: an array does not start at a multiple of its elements' size (workspace: of 16 bytes)");
     if (workspace_bytes < ncnn_b200_op_inner_product_tokens_workspace(tokens, k))
       return op_fail(NCNN_B200_STATUS_OUTPUT_CAPACITY, "op_inner_product_tokens: the workspace is too small");
-    if (y == x || y == weight || y == workspace || x == workspace)
-      return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: the result and the workspace must not lie over an input or each other");
+    for (const void* a : {x, static_cast<const void*>(weight), static_cast<const void*>(weight_steps), static_cast<const void*>(bias)})
+      if (a == y || a == workspace || y == workspace)
+        return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, "op_inner_product_tokens: the result and the workspace must not lie over an input or each other");
     std::string why;
     const int device = op_common_device(kOp, {x, y, weight, weight_steps, bias, workspace}, &why);
     if (device < 0) return op_fail(NCNN_B200_STATUS_INVALID_SHAPE, why);
