@@ -6,7 +6,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decoder_ops import KIND, Setup, assert_within, check_product, check_rows, gen, normal, product_want, quantised, strided  # noqa: E402
+from test_decoder_ops import (KIND, Setup, assert_within, attend, cache_attend_want, check_product, check_rows, gen, normal, product_want,  # noqa: E402
+                              quantised, strided)
 
 
 def up(a, b):
@@ -194,3 +195,66 @@ def test_many_rows_of_a_cache(pkg, element, kv_heads, d, page, strides, shift):
         s.whole[0, page_of] = s.table[0, page_of] = bad
         s.whole[3, 0] = s.table[3, 0] = bad
         check_many_rows(pkg, element, s, strides, shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kernel,m,n", [(("pair", 128), 2100, 4100), (("pair", 256), 3000, 3000), (("few", 128, 1), 1024, 4096)])
+def test_large_products_of_rows_that_end_inside_16_bytes(pkg, element, kernel, m, n):
+    """Anything may lie behind a row of weights, and in the workspace behind a token's integers."""
+    for k, pitch in ((100, 112), (1, 16), (129, 176)):
+        assert product_kernel(m, k, n)[:2] == kernel[:2]
+        check_product(pkg, element, m, k, n, "none", w_pitch=pitch, x_pitch=k + 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,y_pitch", [(16384, 16400), (16399, 16400)])
+def test_results_past_32_bits(pkg, n, y_pitch):
+    """More than 2^32 results, through TMA and without it."""
+    m, k = 270000, 48
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("not enough device memory")
+    g = gen(2)
+    x = normal(g, m, k).bfloat16()
+    w, ws = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8), normal(g, n).abs()
+    y = torch.full((m, y_pitch), 5.0, device="cuda", dtype=torch.bfloat16)
+    space = torch.empty(pkg.op_inner_product_tokens_workspace(m, k), dtype=torch.uint8, device="cuda")
+    pkg.op_inner_product_tokens(x.data_ptr(), y.data_ptr(), "bf16", m, k, n, w.data_ptr(), ws.data_ptr(), space.data_ptr(), space.numel(), y_pitch=y_pitch)
+    assert status(pkg) == 0
+    for rows in (slice(0, 300), slice(261000, 263000), slice(m - 700, m)):
+        want, bound = product_want(*quantised(x[rows]), w, ws, None, "none", "bf16")
+        assert_within(y[rows, :n], want, bound)
+        assert bool((y[rows, n:] == 5.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("element", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,shared", [(4, 0), (4, 64), (64, 0), (64, 64)])
+def test_one_row_to_a_sequence_and_more_rows_or_sequences_than_the_other(pkg, element, heads, shared):
+    """Without starts, row s is sequence s's: sequences behind the last row have none, rows behind the last sequence are left alone."""
+    kv_heads, d, lens = 1, 64, [90, 70, 200, 65, 333]
+    for rows, sequences in ((3, 5), (5, 3), (9, 5)):
+        s = Setup(pkg, [1] * 5, lens, kv_heads, d, 16, shared=shared, starts=False)
+        s.batch = pkg.CacheBatch(s.table.data_ptr(), s.len_t.data_ptr(), None, sequences, rows, s.width, 0, 0)
+        used = min(rows, sequences)
+        q = normal(gen(1), rows, heads, d).to(KIND[element])
+        o = torch.full_like(q, 5.0)
+        attend(pkg, s, q, o, element, heads, shared)
+        assert status(pkg) == 0
+        s.new, s.lens, s.firsts = [1] * used, lens[:used], list(range(used + 1))
+        want, bound = cache_attend_want(s, q[:used], d ** -0.5, element)
+        assert_within(o[:used], want, bound)
+        assert bool((o[used:] == 5.0).all())
+        k = normal(gen(2), rows, kv_heads, d).to(KIND[element])
+        back = torch.full_like(k, 5.0)
+        before = {n: s.ints[n].clone() for n in "kv"}
+        pkg.op_cache_write(s.cache, s.batch, k.data_ptr(), k.data_ptr(), element)
+        pkg.op_cache_read(s.cache, s.batch, back.data_ptr(), None, element)
+        torch.cuda.synchronize()
+        integers, steps = quantised(k[:used])
+        assert torch.equal(back[:used], (integers.float() * steps[..., None]).to(KIND[element])) and bool((back[used:] == 5.0).all())
+        for n in "kv":
+            page = [int(s.whole[i, (lens[i] - 1) // 16]) for i in range(used)]
+            for i in range(used):
+                before[n][page[i], :, (lens[i] - 1) % 16, :d] = integers[i]
+            assert torch.equal(s.ints[n][..., :d], before[n][..., :d])
