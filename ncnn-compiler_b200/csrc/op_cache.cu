@@ -19,9 +19,10 @@ struct CacheRowsParams {
 };
 
 // PER rows (keys or values of neighbouring heads of a token) to LANES lanes, eight components of each row to a lane: what a lane reads of
-// a row is one or two accesses of 16 bytes (WIDE) or eight elements.  Bound: HBM for many tokens, which wants several rows under way in
-// each lane and their place found once; the chain of loads (starts, lens, table, row) for few, which wants many lanes.  36864 tokens of
-// 8 heads of 128, f16: written in 64 us (3.6 TB/s), read in 47 (4.8); a row to a group of lanes 136 and 112.
+// a row is one or two accesses of 16 bytes (WIDE) or eight elements.  Bound: instructions for many tokens (83 % of the issue slots when
+// writing, 75 % when reading; HBM at 36 and 43 %), which wants several rows under way in each lane and their place found once; the chain of
+// loads (starts, lens, table, row) for few, which wants many lanes.  36864 tokens of 8 heads of 128, f16: written in 64 us (3.6 TB/s),
+// read in 47 (4.8); a row to a group of lanes 136 and 112.
 template <class T, int LANES, int PER, bool WIDE, bool READ>
 __global__ void __launch_bounds__(256) k_cache_rows(const __grid_constant__ CacheRowsParams p) {
   const CacheParams& c = p.c;
