@@ -14,9 +14,10 @@
 // store them as TMA would with a 128-byte swizzle, keys and values in turn, in a second ring of three; warp 7 issues the MMAs; warps
 // 8 to 11 are tile 0's softmax, 12 to 15 tile 1's.  256 rows to a CTA share a conversion.
 //
-// Bound: the chain of a block, scores - softmax - products, which two tiles and two halves hide in part.  A block's MMAs (two tiles, 3072
-// clocks) read 320 KB of operands, converting moves 128 KB and every softmax warp reads the steps, some 4100 clocks at 128 bytes a clock;
-// a block takes 5200, with the tensor pipe active for 51 % of them, shared memory's banks for 63 % and the issue slots for 58 %.
+// Bound: the chain of a block, scores - softmax - products, which two tiles and two halves hide in part.  A block's MMAs (two tiles: 1024
+// clocks for the scores, as many for each term of P) read 320 KB of operands, converting moves 128 KB and every softmax warp reads the
+// steps, some 4100 clocks at 128 bytes a clock; a block takes 5200, with the tensor pipe active for 51 % of them, shared memory's banks
+// for 63 % and the issue slots for 58 %.
 // Pieces of up to 2048 tokens of 4 sequences behind up to 4096, 32 heads on 8 of 128: bf16 460 us, 588 TFLOP/s, f16 471 (with P rounded
 // once to bf16 404 us, but results 2.3e-3 off where their own rounding makes 1.7e-3; with every eighth pair of exponentials on the FMA pipe,
 // as tc_attend.cuh has them, 463 and 471, every fourth 473 and 485).
